@@ -381,6 +381,31 @@ int trx_attn_fwd_dropout(const void* q, const void* k, const void* v, void* out,
                          uint32_t offset, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Attention over packed sequences: q (Tq, Hq, D), k / v (Tk, Hk, D), out (Tq, Hq, D), D contiguous, D in
+ * {64, 128}, strides (row, head) in elements. Sequence s of n_seq has the rows cu_q[s] .. cu_q[s + 1] - 1
+ * and the keys cu_k[s] .. cu_k[s + 1] - 1 (device memory, n_seq + 1 ascending values each, the first 0;
+ * a value out of range or out of order is cut to what the tensors hold: such a call's results are
+ * undefined, its accesses are not). With Sq rows and Sk keys, query i stands at key position
+ * i + Sk - Sq: causal, window and ALiBi of trx_attn_fwd are relative to that, so a whole prompt
+ * (Sq == Sk), a piece of one behind cached keys and a single token (Sq == 1) need nothing else. A row
+ * without a visible key returns 0 (LSE -inf).
+ *   lse_or_null: fp32 (Hq, Tq);
+ *   max_sq: no sequence has more rows (0: unknown). Up to 16 selects the kernel for few rows, which leaves
+ *     rows beyond it unwritten;
+ *   zero_rest: rows behind cu_q[n_seq] are written as rows without a visible key; otherwise not touched.
+ * Keys outside a sequence are never used, whatever their values (NaN among them).
+ * `workspace` as for trx_attn_fwd. No counterpart in the reference, whose attention takes one batch of
+ * equal lengths (trinix/kernels/attention_kernel.py:498-664) and has prompts of different lengths padded.
+ */
+int trx_attn_fwd_packed(const void* q, const void* k, const void* v, void* out, float* lse_or_null,
+                        const float* slopes_or_null, const int32_t* cu_q, const int32_t* cu_k,
+                        int64_t n_seq, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                        const int64_t q_strides[2], const int64_t k_strides[2],
+                        const int64_t v_strides[2], const int64_t o_strides[2], float scale, int causal,
+                        int64_t window_left, int64_t window_right, int64_t max_sq, int zero_rest,
+                        int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Status word of an attention workspace, read without synchronising. `host_word` is host
  * memory the caller keeps alive across calls (pinned memory keeps the copy asynchronous),
  * zero before the first call. If *host_word — as copied there by an earlier call — is already

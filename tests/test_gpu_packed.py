@@ -1,0 +1,190 @@
+"""Attention over packed sequences against the definition in 64 bits, one sequence at a time."""
+import itertools
+
+import pytest
+import torch
+
+import trinix_b200 as T
+from tests.ragged_ref import assert_within, attend64
+
+pytestmark = pytest.mark.gpu
+
+
+def starts(sizes, dev, dtype=torch.int32):
+    return torch.tensor([0, *itertools.accumulate(sizes)], dtype=dtype, device=dev)
+
+
+def make(seed, dev, dtype, *shape):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return torch.randn(*shape, generator=g, device=dev).to(dtype)
+
+
+def slopes_of(heads, dev):
+    return 2.0 ** (-8.0 * torch.arange(1, heads + 1, device=dev) / heads)
+
+
+def check(out, lse, q, k, v, len_q, len_k, **how):
+    """Every sequence of a packed call, and the rows behind the last one."""
+    row = key = 0
+    for s, (n, m) in enumerate(zip(len_q, len_k)):
+        want, want_lse, allowed, allowed_lse = attend64(q[row:row + n], k[key:key + m], v[key:key + m],
+                                                        **how)
+        assert_within(out[row:row + n], want, allowed, f"sequence {s} ({n}, {m})")
+        if lse is not None:
+            assert_within(lse[:, row:row + n], want_lse, allowed_lse, f"lse of sequence {s}")
+        row, key = row + n, key + m
+    assert not out[row:].any()
+    if lse is not None:
+        assert torch.equal(lse[:, row:], torch.full_like(lse[:, row:], float("-inf")))
+
+
+LENGTHS = [
+    ([1], None), ([17], None), ([128], None), ([129], None), ([257], None), ([700], None),
+    ([0], None), ([0, 5, 0, 1, 0], None), ([127, 128, 129, 1, 31, 33, 64, 200], None),
+    ([3] * 40, None), ([1, 2, 600, 1, 4], None),
+    # behind cached keys; single tokens; no keys at all; fewer keys than queries
+    ([1, 1, 1], [1, 300, 129]), ([5, 130, 1], [5 + 250, 130 + 1, 128]), ([4, 0, 7], [0, 9, 0]),
+    ([9, 140], [3, 20]), ([260], [1000]),
+]
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 1), (8, 2), (6, 2), (5, 5)])
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+@pytest.mark.parametrize("causal", [True, False])
+def test_lengths(cuda, lengths, heads, kv, causal):
+    len_q, len_k = lengths[0], lengths[1] or lengths[0]
+    dtype, dim = (torch.bfloat16, 128) if heads % 2 else (torch.float16, 64)
+    q = make(1, cuda, dtype, sum(len_q) + 3, heads, dim)
+    k, v = (make(i, cuda, dtype, sum(len_k), kv, dim) for i in (2, 3))
+    cu_q, cu_k = starts(len_q, cuda), starts(len_k, cuda)
+    out, lse = T.attention_packed(q, k, v, cu_q, None if lengths[1] is None else cu_k, causal=causal,
+                                  return_lse=True)
+    check(out, lse, q, k, v, len_q, len_k, causal=causal)
+
+
+# every group size that leaves a tile of another shape: 1 head, all of them, some of them
+@pytest.mark.parametrize("heads,kv", [(2, 1), (3, 1), (7, 1), (10, 2), (16, 1), (24, 1), (32, 8), (48, 1),
+                                      (71, 1), (128, 1), (130, 1)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_groups(cuda, heads, kv, dtype):
+    lens = [200, 3, 64, 65]
+    q = make(4, cuda, dtype, sum(lens), heads, 64)
+    k, v = (make(i, cuda, dtype, sum(lens), kv, 64) for i in (5, 6))
+    out, lse = T.attention_packed(q, k, v, starts(lens, cuda), causal=True, return_lse=True)
+    check(out, lse, q, k, v, lens, lens, causal=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 80, 16, 100])
+@pytest.mark.parametrize("how", [
+    dict(window=(40, 0)), dict(window=(0, 0)), dict(window=(130, 70)), dict(causal=True, window=(64, 64)),
+    dict(causal=True, alibi=True), dict(alibi=True), dict(window=(50, 0), alibi=True),
+    dict(causal=True, scale=0.3), dict(causal=True, scale=-0.05), dict(scale=0.0), dict(scale=-0.1, alibi=True),
+], ids=str)
+def test_masks_and_biases(cuda, how, dim):
+    how = dict(how)
+    len_q, len_k = [150, 1, 300, 20], [150, 200, 290, 160]
+    slopes = slopes_of(8, cuda) if how.pop("alibi", False) else None
+    q = make(7, cuda, torch.bfloat16, sum(len_q), 8, dim)
+    k, v = (make(i, cuda, torch.bfloat16, sum(len_k), 2, dim) for i in (8, 9))
+    out, lse = T.attention_packed(q, k, v, starts(len_q, cuda), starts(len_k, cuda), return_lse=True,
+                                  alibi_slopes=slopes, **how)
+    check(out, lse, q, k, v, len_q, len_k, slopes=slopes, **how)
+
+
+@pytest.mark.parametrize("alibi", [False, True])
+def test_several_items_per_cta(cuda, alibi):
+    """More work items than SMs: the items that a CTA takes behind its first one, skipped slots."""
+    lens = [1000, 1, 0, 333, 5, 5, 5, 2048, 64, 0, 0, 700]
+    slopes = slopes_of(32, cuda) if alibi else None
+    q = make(10, cuda, torch.bfloat16, sum(lens) + 40, 32, 128)
+    k, v = (make(i, cuda, torch.bfloat16, sum(lens), 8, 128) for i in (11, 12))
+    out, lse = T.attention_packed(q, k, v, starts(lens, cuda), causal=True, return_lse=True,
+                                  alibi_slopes=slopes)
+    check(out, lse, q, k, v, lens, lens, causal=True, slopes=slopes)
+
+
+def test_many_sequences(cuda):
+    """The search for a block's sequence: over 1024 of them, most of a few rows, many empty."""
+    g = torch.Generator().manual_seed(3)
+    lens = [int(n) for n in torch.randint(0, 9, (3000,), generator=g)]
+    q = make(13, cuda, torch.float16, sum(lens), 2, 64)
+    k, v = (make(i, cuda, torch.float16, sum(lens), 1, 64) for i in (14, 15))
+    out = T.attention_packed(q, k, v, starts(lens, cuda), causal=True)
+    # one sequence after the other would take minutes: a block-diagonal causal order instead
+    rows = torch.arange(sum(lens), device=cuda)
+    seq = torch.searchsorted(starts(lens, cuda)[1:].long(), rows, right=True)
+    for at in range(0, sum(lens), 2000):
+        r = slice(at, min(sum(lens), at + 2000))
+        hidden = (seq[r, None] != seq[None]) | (rows[None] > rows[r, None])
+        for h in range(2):
+            s = (q[r, h].double() @ k[:, 0].double().t() * 0.125).masked_fill(hidden, float("-inf"))
+            want = torch.softmax(s, -1) @ v[:, 0].double()
+            # at most 8 keys: |out| and A are below max|v|, weights are off by far less than a rounding
+            assert float((out[r, h].double() - want).abs().max()) <= 2.01 * 2 ** -11 * float(v.abs().max())
+
+
+def test_strided_views_and_out(cuda):
+    """q, k, v as views of one projection, and an output with rows that belong to no sequence."""
+    lens, hq, hk, d = [70, 200, 1], 8, 2, 128
+    qkv = make(16, cuda, torch.bfloat16, sum(lens) + 5, (hq + 2 * hk), d)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+    buf = make(17, cuda, torch.bfloat16, sum(lens) + 5, hq + 1, d)
+    held = buf.clone()
+    res, lse = T.attention_packed(q, k, v, starts(lens, cuda), causal=True, return_lse=True, out=buf[:, 1:])
+    assert res.data_ptr() == buf[:, 1:].data_ptr()
+    n = sum(lens)
+    check(buf[:n, 1:], lse[:, :n], q, k, v, lens, lens, causal=True)
+    assert torch.equal(buf[n:], held[n:]) and torch.equal(buf[:, 0], held[:, 0])
+    assert torch.equal(lse[:, n:], torch.full_like(lse[:, n:], float("-inf")))
+    # a layout that the kernel cannot take as it is: head dim 40 at an odd offset, expanded kv heads
+    odd = make(18, cuda, torch.bfloat16, n + 5, hq, 43)[..., 3:]
+    one = make(19, cuda, torch.bfloat16, n, 1, 40)
+    kx = one.expand(-1, 4, -1)
+    out2 = make(20, cuda, torch.bfloat16, n + 5, hq, 41)
+    held = out2.clone()
+    T.attention_packed(odd, kx, kx, starts(lens, cuda), out=out2[..., :40])
+    check(out2[:n, :, :40], None, odd, kx, kx, lens, lens)
+    assert torch.equal(out2[n:], held[n:]) and torch.equal(out2[..., 40:], held[..., 40:])
+
+
+@pytest.mark.parametrize("max_q", [None, 4])
+def test_neighbours_and_rest_never_matter(cuda, max_q):
+    """What lies behind a sequence's last key is NaN or infinite: the next sequence, or nothing."""
+    len_q, len_k = [4, 3, 1, 4], [140, 33, 260, 17]
+    q = make(21, cuda, torch.bfloat16, sum(len_q), 4, 128)
+    k, v = (make(i, cuda, torch.bfloat16, sum(len_k) + 90, 2, 128) for i in (22, 23))
+    cu_q, cu_k = starts(len_q, cuda), starts(len_k, cuda)
+    want = T.attention_packed(q, k, v, cu_q, cu_k, causal=True, max_seqlen_q=max_q)
+    check(want, None, q, k, v, len_q, len_k, causal=True)
+    for s in range(4):
+        for bad in (float("nan"), float("inf")):
+            kk, vv = k.clone(), v.clone()
+            lo, hi = int(cu_k[s]), int(cu_k[s + 1])
+            for t in (kk, vv):
+                t[:lo], t[hi:] = bad, bad
+            got = T.attention_packed(q, kk, vv, cu_q, cu_k, causal=True, max_seqlen_q=max_q)
+            a, b = int(cu_q[s]), int(cu_q[s + 1])
+            assert torch.equal(got[a:b], want[a:b])
+
+
+def test_long_offsets(cuda):
+    """Element offsets beyond 32 bits in the keys and in the output."""
+    rows, hk, d = 2_200_000, 8, 128
+    kv = torch.zeros(rows, hk, d, dtype=torch.bfloat16, device=cuda)  # 4.5 GB
+    kv[-500:] = make(24, cuda, torch.bfloat16, 500, hk, d)
+    q = make(25, cuda, torch.bfloat16, 9, hk, d)
+    cu_q = torch.tensor([0, 1, 9], dtype=torch.int32, device=cuda)
+    cu_k = torch.tensor([0, rows - 300, rows], dtype=torch.int32, device=cuda)
+    for most in (None, 8):
+        got = T.attention_packed(q[1:], kv, kv, cu_q[1:] - 1, cu_k[1:], max_seqlen_q=most)
+        check(got, None, q[1:], kv[-300:], kv[-300:], [8], [300])
+    del kv
+    hq, rows = 32, 540_000
+    q = torch.zeros(rows, hq, d, dtype=torch.bfloat16, device=cuda)  # 4.4 GB
+    q[-70:] = make(26, cuda, torch.bfloat16, 70, hq, d)
+    k = make(27, cuda, torch.bfloat16, 70, hk, d)
+    cu_q = torch.tensor([0, rows - 70, rows], dtype=torch.int32, device=cuda)
+    cu_k = torch.tensor([0, 0, 70], dtype=torch.int32, device=cuda)
+    got = T.attention_packed(q, k, k, cu_q, cu_k, causal=True)
+    assert not got[:rows - 70].any()
+    check(got[rows - 70:], None, q[rows - 70:], k, k, [70], [70], causal=True)

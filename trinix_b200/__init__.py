@@ -38,6 +38,7 @@ from .layers import (
 )
 from .ops import (
     attention,
+    attention_packed,
     attention_status,
     dequantize_rowwise,
     glu,

@@ -811,53 +811,6 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
 // ------------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;  // host threads that race on the first call all see the result
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) ==
-            cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
-  return fn;
-}
-
-// (D, S, H, B) view of a (B, S, H, D) tensor with element strides (b, s, h); box = 64 x box_rows.
-// Dims with stride 0 (broadcast) are collapsed to size 1 by the caller.
-static int make_map(CUtensorMap* tm, const void* base, int is_bf16, int64_t D, int64_t S,
-                    int64_t H, int64_t B, int64_t sb, int64_t ss, int64_t sh, int box_rows) {
-  EncodeTiledFn enc = get_encode_fn();
-  if (!enc) return TRX_ERR_CUDA;
-  if (!aligned_to(base, 16)) return TRX_ERR_ALIGNMENT;
-  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S),
-                        static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(B)};
-  // size-1 dims may carry any stride; give them a legal one
-  if (S == 1) ss = D;
-  if (H == 1) sh = ss * S;
-  if (B == 1) sb = (sh * H > ss * S) ? sh * H : ss * S;
-  if (ss < D || sh <= 0 || sb <= 0) return TRX_ERR_STRIDE;
-  if ((ss * 2) % 16 || (sh * 2) % 16 || (sb * 2) % 16) return TRX_ERR_ALIGNMENT;
-  cuuint64_t strides[3] = {static_cast<cuuint64_t>(ss * 2), static_cast<cuuint64_t>(sh * 2),
-                           static_cast<cuuint64_t>(sb * 2)};
-  for (int i = 0; i < 3; ++i)
-    if (strides[i] >= (1ull << 40)) return TRX_ERR_STRIDE;
-  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(tm, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                   4, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? TRX_OK : TRX_ERR_CUDA;
-}
-
 template <int D, bool BF16, int FEATURE>
 static int launch_attn_feature(const AttnParams& p, cudaStream_t stream) {
   // The attribute is set once per device; host threads that race on the first call each set

@@ -25,7 +25,11 @@ enum AttnStatus : unsigned {
   ATT_ST_DRAIN = 8u,
 };
 
+// How the rows and keys of a launch are laid out (attention_plain.cuh).
+enum AttnForm { ATT_BATCH = 0, ATT_PACKED = 1, ATT_SHARED = 2, ATT_PREFIX = 3 };
+
 struct AttnParams {
+  static constexpr int FORM = ATT_BATCH;
   CUtensorMap tm_q;
   CUtensorMap tm_k;
   CUtensorMap tm_v;
@@ -152,6 +156,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
       " [%0], [%1, {%3, %4, %5, %6}], [%2];"
       :
       : "r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* tm, uint32_t bar,
+                                            int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      :
+      : "r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() {
@@ -316,6 +329,15 @@ __host__ __device__ constexpr uint32_t make_idesc(int is_bf16, int m, int n, int
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// Visits count an item's KV tiles in visiting order: visit r is KV tile first + r * step. Q tile t
+// takes part in visits [lo[t], hi[t]); its rows are m0 + t * t_rows .. of query head h + t * t_head.
+struct PlainItem {
+  int valid, b, h, m0;
+  int n, first;
+  int lo[ATT_NQ], hi[ATT_NQ];
+};
+static_assert(sizeof(PlainItem) <= 64, "shared memory slot");
+
 struct TileRange {
   int jlo, jhi;  // KV tiles [jlo, jhi)
 };
@@ -333,6 +355,53 @@ __device__ __forceinline__ TileRange tile_range(const AttnParams& p, int row0) {
   r.jlo = lo / ATT_BN;
   r.jhi = hi / ATT_BN + 1;
   return r;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn get_encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;  // host threads that race on the first call all see the result
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) ==
+            cudaSuccess &&
+        qres == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// (D, S, H, B) view of a (B, S, H, D) tensor with element strides (b, s, h); box = 64 x box_rows.
+// Dims with stride 0 (broadcast) are collapsed to size 1 by the caller.
+inline int make_map(CUtensorMap* tm, const void* base, int is_bf16, int64_t D, int64_t S,
+                    int64_t H, int64_t B, int64_t sb, int64_t ss, int64_t sh, int box_rows) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return TRX_ERR_CUDA;
+  if (!aligned_to(base, 16)) return TRX_ERR_ALIGNMENT;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S),
+                        static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(B)};
+  // size-1 dims may carry any stride; give them a legal one
+  if (S == 1) ss = D;
+  if (H == 1) sh = ss * S;
+  if (B == 1) sb = (sh * H > ss * S) ? sh * H : ss * S;
+  if (ss < D || sh <= 0 || sb <= 0) return TRX_ERR_STRIDE;
+  if ((ss * 2) % 16 || (sh * 2) % 16 || (sb * 2) % 16) return TRX_ERR_ALIGNMENT;
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(ss * 2), static_cast<cuuint64_t>(sh * 2),
+                           static_cast<cuuint64_t>(sb * 2)};
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] >= (1ull << 40)) return TRX_ERR_STRIDE;
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(tm, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                   4, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TRX_OK : TRX_ERR_CUDA;
 }
 
 // Calls without a dense mask and without dropout (attention_plain.cu).

@@ -1,0 +1,275 @@
+// Rows and keys that are not one batch of equal lengths: what attention_plain.cuh's kernel and the decode
+// kernel need to know of them.
+//
+//   ATT_PACKED  sequences of any lengths one after the other in q and in k / v, bounded by cu_q and cu_k
+//               (device memory: the host knows only the totals);
+//   ATT_SHARED  a batch whose sequences all have the keys of one prefix in front of their own, which lie in
+//               a cache of fixed capacity of which lengths[b] are in use;
+//   ATT_PREFIX  the prefix alone, the rows of the whole batch as one run, its keys split over CTAs; fp32
+//               results that the decode kernel merges with those of the sequences' own keys.
+//
+// Query i of a sequence of Sq queries and Sk keys stands at key position i + Sk - Sq, the last query at the
+// last key: a whole prompt, a piece of one behind cached keys and a single token are the same case.
+//
+// Query tiles: `tile_heads` query heads of one kv head times `tile_tokens` tokens, heads running faster, at
+// most 128 rows. All heads of a group share a tile, so a short sequence fills it with heads where a tile of
+// one head would be padding, and a CTA's two tiles see almost the same keys.
+//
+// Key tiles are not cut to a sequence: what follows its last key in memory belongs to another one, or is
+// stale, and may be NaN. Scores there are masked as any others; in V, where a probability of 0 would not
+// hide it (0 * NaN), the rows behind the last key are zeroed in shared memory (attention_plain.cuh).
+#pragma once
+
+#include "attention_common.cuh"
+
+namespace trx {
+
+struct RaggedParams : AttnParams {
+  CUtensorMap tm_pk, tm_pv;  // the shared prefix
+  const int* cu_q;           // packed: [n_cu + 1] first rows; the last is the end
+  const int* cu_k;
+  const int* lengths;        // shared: own keys in use; null: all
+  int n_cu;                  // sequences of cu_q
+  int n_seq;                 // and one more, without keys, if rows behind the last are to be zeroed
+  int rows, keys;            // of the whole packed q and k / v; shared: keys a sequence's cache holds
+  int tile_heads, tile_tokens;
+  int slots_first;           // packed: the grid's x counts slots (and not heads)
+  int seq;                   // shared: queries per sequence
+  int prefix, prefix_tiles;  // keys of the prefix, in KV tiles
+  int split_tiles;           // KV tiles of one split of the prefix
+};
+template <int F>
+struct RaggedParamsOf : RaggedParams {
+  static constexpr int FORM = F;
+};
+
+struct RaggedItem : PlainItem {
+  int q0, sq, k0, sk;  // first row and rows, first key and keys of the item's sequence
+};
+
+__device__ __forceinline__ int ragged_tokens(const RaggedParams& p) { return p.tile_tokens; }
+__device__ __forceinline__ uint32_t ragged_q_bytes(const RaggedParams& p) {  // of 64 columns of a Q tile
+  return 128u * p.tile_heads * p.tile_tokens;
+}
+__device__ __forceinline__ int ragged_tokens(const AttnParams&) { return 0; }
+__device__ __forceinline__ uint32_t ragged_q_bytes(const AttnParams&) { return 0; }
+
+// Bounds that are out of range or out of order are cut to what the tensors hold.
+__device__ __forceinline__ int ragged_row(const RaggedParams& p, int i) {  // first row of sequence i
+  return i > p.n_cu ? p.rows : min(max(p.cu_q[i], 0), p.rows);
+}
+__device__ __forceinline__ int ragged_key(const RaggedParams& p, int i) {
+  return min(max(p.cu_k[i], 0), p.keys);
+}
+__device__ __forceinline__ int ragged_length(const RaggedParams& p, int b) {
+  return p.lengths ? min(max(p.lengths[b], 0), p.keys) : p.keys;
+}
+// Position, behind the prefix, of row r of the batch.
+__device__ __forceinline__ int ragged_position(const RaggedParams& p, int r) {
+  const int b = r / p.seq;
+  return p.prefix + ragged_length(p, b) - p.seq + (r - b * p.seq);
+}
+__device__ __forceinline__ int ragged_position(const AttnParams&, int) { return 0; }
+
+// Packed rows: which sequence a block works on. The host knows the rows and the number of sequences but not
+// where they end, and a table of blocks would cost a launch in front. So each sequence has the slots from
+// floor(first row / R) + its index to the next one's, R rows being a block's: at least as many as it has
+// blocks, on average half a slot too many, which are passed over, and found by a search in cu_q alone.
+struct RaggedCursor {
+  int s, slot, slot0, next;  // sequence, the slot looked for, first slots of this and the next sequence
+  int q0, sq, k0, sk;
+
+  static __device__ __forceinline__ int first_slot(const RaggedParams& p, int i) {
+    return ragged_row(p, i) / (ATT_NQ * p.tile_tokens) + i;
+  }
+  __device__ __forceinline__ void load(const RaggedParams& p) {
+    const int step = ATT_NQ * p.tile_tokens;
+    q0 = ragged_row(p, s);
+    const int q1 = ragged_row(p, s + 1);
+    slot0 = q0 / step + s;
+    next = q1 / step + s + 1;
+    sq = max(0, q1 - q0);
+    k0 = sk = 0;
+    if (s < p.n_cu) {
+      k0 = ragged_key(p, s);
+      sk = max(0, ragged_key(p, s + 1) - k0);
+    }
+  }
+  // The last sequence in [lo, hi) whose first slot is not behind `slot`; a whole warp, 32 probes at a time.
+  __device__ __forceinline__ void seek(const RaggedParams& p, int at, int lane) {
+    slot = at;
+    int lo = 0, hi = p.n_seq;
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+      const unsigned not_behind = __ballot_sync(0xffffffffu, i < hi && first_slot(p, i) <= at);
+      const int n = __popc(not_behind);
+      lo += max(0, n - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    s = lo;
+    load(p);
+  }
+  // The same from where the cursor stands, by one thread: blocks are handed out in their order, so the next
+  // one is of this sequence or of one shortly behind it.
+  __device__ __forceinline__ void advance(const RaggedParams& p, int at) {
+    slot = at;
+    if (at >= slot0 && at < next) return;
+    int lo = at >= slot0 ? s : 0, hi = p.n_seq;
+    if (at >= slot0) {
+#pragma unroll 1
+      for (int i = 0; i < 3 && lo + 1 < hi; ++i) {
+        if (first_slot(p, lo + 1) > at) hi = lo + 1;
+        else ++lo;
+      }
+    }
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (first_slot(p, mid) <= at) lo = mid;
+      else hi = mid;
+    }
+    s = lo;
+    load(p);
+  }
+};
+
+__device__ __forceinline__ int ragged_slot(const RaggedParams& p, int x, int y) {
+  return p.slots_first ? x : y;
+}
+__device__ __forceinline__ bool ragged_has_rows(const RaggedItem& w) { return w.sq > 0; }
+__device__ __forceinline__ bool ragged_has_rows(const PlainItem&) { return true; }
+
+// KV tiles that the rows of a Q tile see, the first of them `row0` of its sequence. Shared form: the tiles
+// of the prefix, then those of the sequence's own keys.
+template <int FORM>
+__device__ __forceinline__ TileRange ragged_range(const RaggedParams& p, const RaggedItem& w, int row0) {
+  TileRange r{0, 0};
+  if (row0 >= w.sq) return r;
+  const int last = min(w.sq, row0 + p.tile_tokens) - 1;
+  if constexpr (FORM == ATT_PREFIX) {
+    r.jlo = w.b * p.split_tiles;
+    r.jhi = min(p.prefix_tiles, r.jlo + p.split_tiles);
+  } else if constexpr (FORM == ATT_SHARED) {
+    const int hi = last + w.sk - w.sq;  // of its own keys
+    if (hi >= 0) r.jhi = p.prefix_tiles + hi / ATT_BN + 1;
+    else if (p.prefix + hi >= 0) r.jhi = (p.prefix + hi) / ATT_BN + 1;
+  } else {
+    const int shift = w.sk - w.sq;
+    int hi = w.sk - 1, lo = 0;
+    if (p.causal) hi = min(hi, last + shift);
+    if (p.win_right >= 0) hi = min(hi, last + shift + p.win_right);
+    if (p.win_left >= 0) lo = max(0, row0 + shift - p.win_left);
+    if (hi < lo) return r;
+    r.jlo = lo / ATT_BN;
+    r.jhi = hi / ATT_BN + 1;
+  }
+  return r;
+}
+
+template <int FORM>
+__device__ __forceinline__ RaggedItem ragged_item(const RaggedParamsOf<FORM>& p, const RaggedCursor& c,
+                                                  int x, int y, int z) {
+  RaggedItem w;
+  const int step = ATT_NQ * p.tile_tokens;
+  w.valid = 1;
+  w.h = (FORM == ATT_PACKED && p.slots_first ? y : x) * p.tile_heads;
+  if constexpr (FORM == ATT_PACKED) {
+    w.b = 0;
+    w.q0 = c.q0;
+    w.sq = c.sq;
+    w.k0 = c.k0;
+    w.sk = c.sk;
+    const int blocks = (c.sq + step - 1) / step, i = c.slot - c.slot0;
+    if (i < 0 || i >= blocks) {  // the slot holds no rows
+      w.sq = w.m0 = 0;
+    } else {
+      w.m0 = (p.causal ? blocks - 1 - i : i) * step;  // heaviest first
+    }
+  } else {
+    w.b = z;  // sequence, or split of the prefix
+    w.q0 = w.k0 = 0;
+    w.sq = FORM == ATT_SHARED ? p.seq : p.rows;
+    w.sk = FORM == ATT_SHARED ? ragged_length(p, z) : 0;
+    w.m0 = static_cast<int>(gridDim.y - 1 - y) * step;
+  }
+  TileRange r[ATT_NQ];
+  int jlo = 1 << 30, jhi = 0;
+#pragma unroll
+  for (int t = 0; t < ATT_NQ; ++t) {
+    r[t] = ragged_range<FORM>(p, w, w.m0 + t * p.tile_tokens);
+    if (r[t].jhi > r[t].jlo) {
+      jlo = min(jlo, r[t].jlo);
+      jhi = max(jhi, r[t].jhi);
+    }
+  }
+  w.n = max(0, jhi - jlo);
+  w.first = p.reverse_kv ? jhi - 1 : jlo;
+#pragma unroll
+  for (int t = 0; t < ATT_NQ; ++t) {
+    const bool any = r[t].jhi > r[t].jlo;
+    w.lo[t] = !any ? 0 : p.reverse_kv ? jhi - r[t].jhi : r[t].jlo - jlo;
+    w.hi[t] = !any ? 0 : w.lo[t] + r[t].jhi - r[t].jlo;
+  }
+  return w;
+}
+
+// Where KV tile j of an item starts, and how many of its rows are the sequence's; `edge`: the others are
+// inside the tensor (behind its end the copy fills with zeros).
+struct RaggedTile {
+  int row, b, rows;
+  bool prefix, edge;
+};
+template <int BN, int FORM>
+__device__ __forceinline__ RaggedTile ragged_tile(const RaggedParamsOf<FORM>& p, const RaggedItem& w, int j) {
+  RaggedTile r;
+  r.prefix = FORM == ATT_PREFIX || (FORM == ATT_SHARED && j < p.prefix_tiles);
+  const int first = (FORM == ATT_SHARED && !r.prefix ? j - p.prefix_tiles : j) * BN;
+  const int keys = r.prefix ? p.prefix : w.sk;
+  r.row = w.k0 + first;
+  r.b = FORM == ATT_SHARED && !r.prefix ? w.b : 0;
+  r.rows = keys - first;
+  r.edge = r.rows < BN && w.k0 + keys < (r.prefix ? p.prefix : p.keys);
+  return r;
+}
+
+// ------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------
+// (B, rows, H, D) queries for tiles of `heads` heads x `tokens` rows: dims D, head in tile, row, tile of
+// heads, B.
+inline int make_ragged_q_map(CUtensorMap* tm, const void* base, int is_bf16, int64_t D, int64_t rows, int64_t H,
+                             int64_t B, int64_t sb, int64_t ss, int64_t sh, int heads, int tokens) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return TRX_ERR_CUDA;
+  if (!aligned_to(base, 16)) return TRX_ERR_ALIGNMENT;
+  if (rows == 1) ss = D;
+  if (H == 1) sh = D;
+  if (B == 1) sb = D;
+  if (ss < D || sh < D || sb < D) return TRX_ERR_STRIDE;
+  if (ss % 8 || sh % 8 || sb % 8) return TRX_ERR_ALIGNMENT;
+  if (ss >= (1ll << 38) || sh >= (1ll << 30) || sb >= (1ll << 38)) return TRX_ERR_STRIDE;
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(H / heads),
+                              static_cast<cuuint64_t>(B)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(ss) * 2,
+                                 static_cast<cuuint64_t>(sh) * heads * 2, static_cast<cuuint64_t>(sb) * 2};
+  const cuuint32_t tile[5] = {64, static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(tokens), 1, 1},
+                   step[5] = {1, 1, 1, 1, 1};
+  const CUresult r = enc(tm, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                         const_cast<void*>(base), dims, strides, tile, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TRX_OK : TRX_ERR_CUDA;
+}
+
+// Query heads of one tile, and tokens: as many heads of the group as leave at most a tenth of a tile's 128
+// rows unused. (A group of 71 heads is none but 1 and 71, and 71 would leave 57 rows.)
+inline void choose_tile(RaggedParams& p) {
+  p.tile_heads = 1;
+  for (int h = 2; h <= p.group && h <= ATT_BM; ++h)
+    if (p.group % h == 0 && ATT_BM / h * h * 10 >= ATT_BM * 9) p.tile_heads = h;
+  p.tile_tokens = ATT_BM / p.tile_heads;
+}
+
+}  // namespace trx

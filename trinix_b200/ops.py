@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import I64x3
+from ._lib import I64x2, I64x3
 
 _DTYPE_CODE = {torch.float32: _lib.TRX_F32, torch.float16: _lib.TRX_F16,
                torch.bfloat16: _lib.TRX_BF16}
@@ -679,3 +679,114 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     else:
         _launch("trx_attn_fwd", dev, *head, *problem, *work)
     return (out, lse) if return_lse else out
+
+
+def _packed_view(t: torch.Tensor) -> torch.Tensor:
+    """A view whose last dim is dense, whose base is 16-byte aligned and whose other strides are
+    multiples of 8 elements and at least a row apart, as the tensor maps of the packed and shared
+    kernels want it; anything else (expanded heads, a slice along D at an odd offset) is
+    materialised once."""
+    if t.numel() == 0:
+        return t
+    d = t.shape[-1]
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        t.shape[i] == 1 or (t.stride(i) % 8 == 0 and t.stride(i) >= d) for i in range(t.dim() - 1))
+    return t if ok else t.contiguous()
+
+
+def _check_attention_types(*ts: torch.Tensor) -> None:
+    if any(t.dtype != ts[0].dtype for t in ts) or ts[0].dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("attention needs queries, keys and values of one dtype, bfloat16 or float16")
+
+
+def _slopes(alibi_slopes: Optional[torch.Tensor], heads: int) -> Optional[torch.Tensor]:
+    if alibi_slopes is None:
+        return None
+    slopes = alibi_slopes.detach().reshape(-1).to(torch.float32).contiguous()
+    if slopes.numel() != heads:
+        raise ValueError(f"alibi_slopes must have {heads} entries")
+    return slopes
+
+
+def _padded_dim(d: int) -> int:
+    """The head dim that the kernels run `d` as: zero columns are appended to anything else."""
+    if not 0 < d <= 128:
+        raise ValueError(f"head_dim must be in 1 .. 128, got {d}")
+    return 64 if d <= 64 else 128
+
+
+def _pad(t: torch.Tensor, d: int) -> torch.Tensor:
+    return t if t.shape[-1] == d else torch.nn.functional.pad(t, (0, d - t.shape[-1]))
+
+
+def _cu_seqlens(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() == 0:
+        raise ValueError(f"{name} must be a one-dimensional int32 tensor of sequences + 1 entries")
+    return t.contiguous()
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                     cu_seqlens_k: Optional[torch.Tensor] = None, *, causal: bool = False,
+                     scale: Optional[float] = None, window: Optional[Tuple[int, int]] = None,
+                     alibi_slopes: Optional[torch.Tensor] = None, return_lse: bool = False,
+                     max_seqlen_q: Optional[int] = None, out: Optional[torch.Tensor] = None):
+    """Attention over sequences of different lengths packed one after the other, without padding.
+
+    q (Tq, Hq, D), k / v (Tk, Hk, D), Hq % Hk == 0. Sequence s has the rows cu_seqlens_q[s] ..
+    cu_seqlens_q[s + 1] - 1 and the keys of cu_seqlens_k (default: the same) likewise; both are int32
+    tensors on the device, ascending from 0, and are not looked at by the host. With Sq rows and
+    Sk keys, query i stands at key position p = i + Sk - Sq, the last query at the last key: causal
+    shows it keys j <= p, window = (left, right) keys p - left <= j <= p + right, alibi_slopes (Hq,)
+    add -slope * |p - j|. So a prompt, a piece of one behind cached keys and a single token are one
+    call. A row that sees nothing is 0.
+
+    max_seqlen_q, if given, promises that no sequence has more rows; up to 16 selects the kernel for
+    decoding, which leaves rows beyond it unwritten. Rows behind cu_seqlens_q[-1] are 0 in a new
+    output; in `out`, if given (it then is the result), they stay what they were. With return_lse
+    also the fp32 (Hq, Tq) log-sum-exp, -inf for rows without a key and rows behind the last.
+    """
+    dev = _need_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, alibi_slopes, out)
+    _check_attention_types(q, k, v)
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"expected (rows, heads, head_dim) tensors, got q {tuple(q.shape)}, "
+                         f"k {tuple(k.shape)}, v {tuple(v.shape)}")
+    Tq, Hq, d = q.shape
+    Tk, Hk, _ = k.shape
+    if k.shape[2] != d or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError(f"query heads ({Hq}) must be a multiple of kv heads ({Hk})")
+    cu_q = _cu_seqlens(cu_seqlens_q, "cu_seqlens_q")
+    cu_k = cu_q if cu_seqlens_k is None else _cu_seqlens(cu_seqlens_k, "cu_seqlens_k")
+    if cu_q.numel() != cu_k.numel():
+        raise ValueError(f"{cu_q.numel() - 1} sequences of queries and {cu_k.numel() - 1} of keys")
+    wl, wr = (-1, -1) if window is None else (int(window[0]), int(window[1]))
+    if window is not None and (wl < 0 or wr < 0):
+        raise ValueError("window sizes must be >= 0")
+    if max_seqlen_q is not None and max_seqlen_q < 0:
+        raise ValueError("max_seqlen_q must be >= 0")
+    slopes = _slopes(alibi_slopes, Hq)
+    scale = d ** -0.5 if scale is None else float(scale)
+    dp = _padded_dim(d)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+        raise ValueError("out must have the shape and dtype of q")
+    q, k, v = (_packed_view(_pad(t, dp)) for t in (q, k, v))
+    if out is None:
+        o = _empty(q, (Tq, Hq, dp))
+    else:
+        o = _packed_view(_pad(out, dp))  # a copy where the kernel cannot write into it
+    lse = _empty(q, (Hq, Tq), dtype=torch.float32) if return_lse else None
+    if lse is not None and out is not None:
+        lse.fill_(float("-inf"))  # rows behind the last sequence are not touched
+    ws = _workspace(dev)
+    _raise_if_failed("trx_attn_fwd_packed", dev)  # of an earlier launch, before more work is queued
+    _launch("trx_attn_fwd_packed", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse),
+            _ptr(slopes), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, Tq, Tk, Hq, Hk, dp,
+            I64x2(*q.stride()[:2]), I64x2(*k.stride()[:2]), I64x2(*v.stride()[:2]),
+            I64x2(*o.stride()[:2]), scale, int(bool(causal)), wl, wr, int(max_seqlen_q or 0),
+            int(out is None), _code(q), ws.data_ptr(), ws.numel())
+    if out is None:
+        o = o if dp == d else o[..., :d].contiguous()
+    elif o is not out:
+        o = out.copy_(o[..., :d])
+    return (o, lse) if return_lse else o
