@@ -406,6 +406,30 @@ int trx_attn_fwd_packed(const void* q, const void* k, const void* v, void* out, 
                         int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Attention for a batch that shares a prefix: the prefix's keys and values (P, Hk, D), strides (row, head),
+ * are those of every sequence, in front of its own (B, S, Hk, D), strides (batch, row, head), of which
+ * lengths[b] (device memory, cut to 0 .. S; NULL: S) are in use; the others are never used, whatever their
+ * values (NaN among them). q, out (B, Sq, Hq, D): the last Sq tokens of each sequence. Over the P + lengths[b]
+ * keys of the concatenation this is causal attention of trx_attn_fwd_packed: query i stands at
+ * P + lengths[b] - Sq + i and sees the keys up to there; slopes_or_null (ALiBi) counts from there.
+ * scale > 0. lse_or_null: fp32 (B, Hq, Sq).
+ * With few rows (Sq <= 16) the prefix is read and computed once for all sequences, its keys split over the
+ * GPU; the splits' results need `parts`: trx_attn_shared_bytes(...) bytes of device memory, 16-byte aligned
+ * (0: none, parts may be NULL), contents on entry irrelevant, nothing kept between calls.
+ * `workspace` as for trx_attn_fwd. No counterpart in the reference, whose attention takes one batch
+ * (trinix/kernels/attention_kernel.py:498-664) and has the prefix repeated for every sequence.
+ */
+size_t trx_attn_shared_bytes(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int64_t Hk, int64_t D);
+int trx_attn_fwd_shared(const void* q, const void* prefix_k, const void* prefix_v, const void* k,
+                        const void* v, void* out, float* lse_or_null, const float* slopes_or_null,
+                        const int32_t* lengths_or_null, int64_t B, int64_t Sq, int64_t P, int64_t S,
+                        int64_t Hq, int64_t Hk, int64_t D, const int64_t q_strides[3],
+                        const int64_t pk_strides[2], const int64_t pv_strides[2],
+                        const int64_t k_strides[3], const int64_t v_strides[3],
+                        const int64_t o_strides[3], float scale, int dtype, void* parts,
+                        size_t parts_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Status word of an attention workspace, read without synchronising. `host_word` is host
  * memory the caller keeps alive across calls (pinned memory keeps the copy asynchronous),
  * zero before the first call. If *host_word — as copied there by an earlier call — is already

@@ -43,3 +43,52 @@ def test_cpu_tensors_are_refused():
     q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):
         T.attention_packed(q, q, q, torch.tensor([0, 4], dtype=torch.int32))
+
+
+I64x3 = _lib.I64x3
+
+
+def shared(lib, **change):
+    a = dict(q=ONE, pk=ONE, pv=ONE, k=ONE, v=ONE, out=ONE, lse=None, slopes=None, lengths=None, b=2, sq=1,
+             p=100, s=20, hq=4, hk=2, d=128, qs=I64x3(512, 512, 128), pks=I64x2(256, 128),
+             pvs=I64x2(256, 128), ks=I64x3(5120, 256, 128), vs=I64x3(5120, 256, 128),
+             os=I64x3(512, 512, 128), scale=1.0, dtype=2, parts=ONE, pb=1 << 30, ws=ONE, wsb=256, stream=None)
+    assert set(change) <= set(a)
+    a.update(change)
+    return lib.trx_attn_fwd_shared(*a.values())
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(dtype=0), -2), (dict(hk=3), -3), (dict(b=-1), -3), (dict(p=-1), -3), (dict(s=-1), -3),
+    (dict(d=96), -6), (dict(scale=0.0), -6), (dict(scale=float("nan")), -6), (dict(q=None), -1),
+    (dict(pk=None), -1), (dict(pv=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(out=None), -1),
+    (dict(ws=None), -9), (dict(parts=None), -9), (dict(parts=ctypes.c_void_p(4104)), -9), (dict(pb=16), -9),
+    (dict(b=1 << 17), -3), (dict(p=1 << 29), -3), (dict(s=1 << 29), -3), (dict(sq=1 << 30), -3),
+    (dict(lengths=ctypes.c_void_p(4098)), -4), (dict(out=ctypes.c_void_p(4104)), -4),
+    (dict(os=I64x3(512, 516, 128)), -4), (dict(qs=I64x3(-8, 512, 128)), -5), (dict(pks=I64x2(256, -8)), -5),
+], ids=str)
+def test_shared_entry_refuses(lib, change, code):
+    assert shared(lib, **change) == code
+
+
+def test_shared_entry_has_nothing_to_do(lib):
+    assert shared(lib, b=0) == 0
+    assert shared(lib, sq=0) == 0
+
+
+def test_shared_bytes(lib):
+    """Space for the results of the prefix's splits: none without a prefix, none with many rows."""
+    size = lib.trx_attn_shared_bytes
+    assert size(64, 1, 0, 32, 8, 128) == 0 and size(4, 17, 5000, 32, 8, 128) == 0
+    row = 64 * 32 * 129 * 4
+    n = size(64, 1, 8192, 32, 8, 128)
+    assert n >= row and n % row == 0
+    assert size(64, 1, 100, 32, 8, 128) == row  # a single tile of keys cannot be split
+    for bad in ((0, 1, 5, 4, 2, 64), (1, 1, -1, 4, 2, 64), (1, 1, 5, 4, 3, 64), (1 << 20, 1, 5, 4, 2, 64)):
+        assert size(*bad) == 0
+
+
+def test_cpu_tensors_are_refused_behind_a_prefix():
+    q, pk = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16), torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        T.attention_shared_prefix(q, pk, pk, q, q)

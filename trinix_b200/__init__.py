@@ -39,6 +39,7 @@ from .layers import (
 from .ops import (
     attention,
     attention_packed,
+    attention_shared_prefix,
     attention_status,
     dequantize_rowwise,
     glu,

@@ -998,14 +998,7 @@ static int attn_fwd_prepare(AttnParams& p, bool* nothing_to_do, const void* q, c
 
 static int attn_fwd_launch(AttnParams& p, int64_t D, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p.decode) {
-    const bool wide = p.group * p.Sq > 16;
-    if (D == 128)
-      return p.is_bf16 ? (wide ? launch_decode<128, true, 2>(p, s) : launch_decode<128, true, 1>(p, s))
-                       : (wide ? launch_decode<128, false, 2>(p, s) : launch_decode<128, false, 1>(p, s));
-    return p.is_bf16 ? (wide ? launch_decode<64, true, 2>(p, s) : launch_decode<64, true, 1>(p, s))
-                     : (wide ? launch_decode<64, false, 2>(p, s) : launch_decode<64, false, 1>(p, s));
-  }
+  if (p.decode) return launch_decode_rows(p, D, s);
   if (p.plain && !is_short(p)) return launch_attn_plain(p, D, s);
   if (D == 128) return p.is_bf16 ? launch_attn<128, true>(p, s) : launch_attn<128, false>(p, s);
   return p.is_bf16 ? launch_attn<64, true>(p, s) : launch_attn<64, false>(p, s);

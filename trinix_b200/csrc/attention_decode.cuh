@@ -1,5 +1,5 @@
-// Attention forward for few query rows against many keys (decoding against a KV cache).
-// Included by attention.cu, whose parameter block, barrier and TMA wrappers it uses.
+// Attention forward for few query rows against many keys (decoding against a KV cache): of one batch, of
+// packed sequences, or of a batch whose shared prefix has been done (attention_ragged.cuh).
 //
 // The work is reading K and V once: per key and kv head 4 * D bytes and, with `group` query heads
 // of Sq rows on that kv head, only group * Sq rows of arithmetic. The tcgen05 kernel gives such a
@@ -24,6 +24,8 @@
 #pragma once
 
 #include <cooperative_groups.h>
+
+#include "attention_ragged.cuh"
 
 namespace trx {
 
@@ -77,12 +79,30 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Grid (splits, kv units * row tiles, B), clusters of all the splits of one row tile. Packed row r
+// Rows behind the last packed sequence: 0, LSE -inf.
+template <int D>
+__device__ __forceinline__ void zero_rest(const RaggedParams& p) {
+  const int row0 = ragged_row(p, p.n_cu);
+  const long long n = static_cast<long long>(p.rows - row0) * p.Hq * (D / 8);
+  const long long step = static_cast<long long>(gridDim.x) * gridDim.y * DEC_THREADS;
+  for (long long i = static_cast<long long>(blockIdx.y * gridDim.x + blockIdx.x) * DEC_THREADS + threadIdx.x;
+       i < n; i += step) {
+    const long long rh = i / (D / 8);
+    const int c = static_cast<int>(i - rh * (D / 8)), h = static_cast<int>(rh % p.Hq);
+    const long long row = row0 + rh / p.Hq;
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + row * p.o_stride_s + h * p.o_stride_h +
+                              8 * c) = make_uint4(0u, 0u, 0u, 0u);
+    if (p.lse && c == 0) p.lse[h * p.lse_stride_h + row] = -INFINITY;
+  }
+}
+
+// Grid (splits, kv units * row tiles, sequences), clusters of all the splits of one row tile. Packed row r
 // of a kv unit is row r / group of query head unit * group + r % group.
-template <int D, bool BF16, int MT>
+template <int D, bool BF16, int MT, class P>
 __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
-    attn_decode_kernel(const __grid_constant__ AttnParams p) {
+    attn_decode_kernel(const __grid_constant__ P p) {
   using L = DecSmem<D, MT>;
+  constexpr int FORM = P::FORM;
   namespace cg = cooperative_groups;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -91,26 +111,44 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q4 = lane & 3, rl = lane >> 2;
   const int nsplit = gridDim.x, split = blockIdx.x, b = blockIdx.z;
-  const int group = p.group, rows = group * p.Sq;
-  const int row_tiles = (rows + L::ROWS - 1) / L::ROWS;
+  const int group = p.group;
+  const int row_tiles = (group * p.Sq + L::ROWS - 1) / L::ROWS;
   const int unit = blockIdx.y / row_tiles;
   const int r0 = (blockIdx.y - unit * row_tiles) * L::ROWS;
   const int h0 = unit * group;
+  // this sequence's rows and keys; `shift`: position of its first query
+  int q0 = 0, sq = p.Sq, k0 = 0, sk = p.Sk, shift = 0;
+  if constexpr (FORM == ATT_PACKED) {
+    if (b >= p.n_cu) {
+      zero_rest<D>(p);
+      return;
+    }
+    q0 = ragged_row(p, b);
+    sq = min(max(0, ragged_row(p, b + 1) - q0), p.Sq);
+    k0 = ragged_key(p, b);
+    sk = max(0, ragged_key(p, b + 1) - k0);
+  }
+  if constexpr (FORM == ATT_SHARED) sk = ragged_length(p, b);
+  if constexpr (FORM != ATT_BATCH) {
+    if (r0 >= group * sq) return;  // the whole cluster: a shorter sequence than the longest
+    shift = sk - sq;
+  }
+  const int rows = group * sq;
 
   // keys that any row of this tile sees, in tiles of 16, and this CTA's share of them
   const int s_min = r0 / group, s_max = min(rows - 1, r0 + L::ROWS - 1) / group;
-  int hi = p.Sk - 1, lo = 0, hi_min = p.Sk - 1, lo_max = 0;
+  int hi = sk - 1, lo = 0, hi_min = sk - 1, lo_max = 0;
   if (p.causal) {
-    hi = min(hi, s_max);
-    hi_min = min(hi_min, s_min);
+    hi = min(hi, s_max + shift);
+    hi_min = min(hi_min, s_min + shift);
   }
   if (p.win_right >= 0) {
-    hi = min(hi, s_max + p.win_right);
-    hi_min = min(hi_min, s_min + p.win_right);
+    hi = min(hi, s_max + shift + p.win_right);
+    hi_min = min(hi_min, s_min + shift + p.win_right);
   }
   if (p.win_left >= 0) {
-    lo = max(0, s_min - p.win_left);
-    lo_max = max(0, s_max - p.win_left);
+    lo = max(0, s_min + shift - p.win_left);
+    lo_max = max(0, s_max + shift - p.win_left);
   }
   const int t_lo = lo / DEC_KEYS, n_tiles = hi < lo ? 0 : hi / DEC_KEYS + 1 - t_lo;
   const int share = (n_tiles + nsplit - 1) / nsplit;
@@ -124,7 +162,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
   volatile int* abort_flag = no_result + warp;
   const int kh = h0 / p.k_hdiv, vh = h0 / p.v_hdiv, kb = b * p.k_bmul, vb = b * p.v_bmul;
   auto issue_fill = [&](int it) {  // one lane: K and V of the it-th tile of this warp
-    const int s = it % DEC_STAGES, key0 = (first + it * DEC_WARPS) * DEC_KEYS;
+    const int s = it % DEC_STAGES, key0 = k0 + (first + it * DEC_WARPS) * DEC_KEYS;
     mbar_expect_tx(bars + 8 * s, 2 * L::TILE_BYTES);
 #pragma unroll
     for (int c = 0; c < L::CHUNKS; ++c)
@@ -165,7 +203,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
       row_s[m][e] = s;
       slope2[m][e] = p.slopes ? p.slopes[h] * 1.4426950408889634f : 0.0f;
       const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + b * p.q_stride_b +
-                             s * p.q_stride_s + h * p.q_stride_h + 2 * q4;
+                             (q0 + s) * p.q_stride_s + h * p.q_stride_h + 2 * q4;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
@@ -229,8 +267,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int i = row_s[m][e];
-        int hi_i = p.Sk - 1, lo_i = 0;
+        const int i = row_s[m][e] + shift;
+        int hi_i = sk - 1, lo_i = 0;
         if (p.causal) hi_i = min(hi_i, i);
         if (p.win_right >= 0) hi_i = min(hi_i, i + p.win_right);
         if (p.win_left >= 0) lo_i = max(0, i - p.win_left);
@@ -267,11 +305,24 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
         pf[m][2 + e] = pack16<BF16>(x[2], x[3]);
       }
     }
+    // V behind the sequence's last key may be anything: keys 2 q4, 2 q4 + 1 of either half, if they are its
+    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+    if constexpr (FORM != ATT_BATCH) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int left = sk - c0 - 8 * n - 2 * q4;
+        keep[n] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+      }
+    }
 #pragma unroll
     for (int dn = 0; dn < D / 16; ++dn) {
       uint32_t vf[4];
       const int col = (dn % 4) * 2 + v_col;
       ldsm_x4_trans(vt + (dn / 4) * L::CHUNK_BYTES + v_key * 128 + ((col ^ (lane & 7)) << 4), vf);
+      if constexpr (FORM != ATT_BATCH) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) vf[n] &= keep[n & 1];
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         mma_16816<BF16>(o[m][2 * dn], pf[m], vf[0], vf[1]);
@@ -329,15 +380,35 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
   // out[row, 4 c4 ..] = acc / l, and the row's LSE
   auto emit = [&](int r, int c4, float4 acc, float mx, float l) {
     const int s = (r0 + r) / group, h = h0 + (r0 + r) % group;
+    if constexpr (FORM == ATT_SHARED) {  // with the parts of the prefix: their rows' O / l and log2 sums
+      const long long part = static_cast<long long>(p.B) * p.Sq * p.Hq;  // rows of a part
+      const long long at = (static_cast<long long>(b) * p.Sq + s) * p.Hq + h;
+      float top = mx;
+      for (int k = 0; k < p.parts; ++k) top = fmaxf(top, p.part_lse[k * part + at]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float f = fast_exp2(mx - ref);
+      acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+      l *= f;
+      for (int k = 0; k < p.parts; ++k) {
+        const float w = fast_exp2(p.part_lse[k * part + at] - ref);
+        const float4 o = *reinterpret_cast<const float4*>(p.part_o + (k * part + at) * D + 4 * c4);
+        l += w;
+        acc.x = fmaf(w, o.x, acc.x);
+        acc.y = fmaf(w, o.y, acc.y);
+        acc.z = fmaf(w, o.z, acc.z);
+        acc.w = fmaf(w, o.w, acc.w);
+      }
+      mx = ref;
+    }
     const float inv = l > 0.0f ? __fdividef(1.0f, l) : 0.0f;
     if (whole) {
       uint2 v;
       v.x = pack16<BF16>(acc.x * inv, acc.y * inv);
       v.y = pack16<BF16>(acc.z * inv, acc.w * inv);
       *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + b * p.o_stride_b +
-                                s * p.o_stride_s + h * p.o_stride_h + 4 * c4) = v;
+                                (q0 + s) * p.o_stride_s + h * p.o_stride_h + 4 * c4) = v;
       if (p.lse && c4 == 0)
-        p.lse[b * p.lse_stride_b + h * p.lse_stride_h + s] =
+        p.lse[b * p.lse_stride_b + h * p.lse_stride_h + q0 + s] =
             l > 0.0f ? (mx + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
   };
@@ -412,12 +483,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
 // single shapes (32 / 8 heads, head dim 128, that / this / the tcgen05 kernel): 24 x 256 keys, 16 rows
 // 40.6 / 23.7 / 28.6 us; 8 x 256 keys, 16 rows 14.8 / 11.2 / 10.8 us; 2 x 4096 keys, 1 row 18.2 / 12.6
 // / 69.5 us.
-static int decode_splits(const AttnParams& p, int64_t units, bool wide) {
-  int64_t keys = p.Sk;  // that some row sees
-  if (p.causal && p.Sq < keys) keys = p.Sq;
-  if (p.win_right >= 0 && static_cast<int64_t>(p.Sq) + p.win_right < keys) keys = p.Sq + p.win_right;
-  if (p.win_left >= 0 && static_cast<int64_t>(p.Sq) + p.win_left + p.win_right < keys)
-    keys = p.Sq + p.win_left + p.win_right;
+inline int decode_splits(int64_t keys, int64_t units, bool wide) {
   const int64_t sms = sm_count_of_current_device(), slots = sms * DEC_CTAS_PER_SM;
   const int64_t tiles = (keys + DEC_KEYS - 1) / DEC_KEYS;
   auto cost = [&](int64_t n) {
@@ -436,10 +502,23 @@ static int decode_splits(const AttnParams& p, int64_t units, bool wide) {
   return best;
 }
 
-template <int D, bool BF16, int MT>
-static int launch_decode(const AttnParams& p, cudaStream_t stream) {
+// Keys of a sequence that some row sees, as far as the host knows: those of the whole call, or for packed
+// sequences the mean, where p.Sk holds it.
+inline int64_t decode_keys(const AttnParams& p, bool ragged) {
+  int64_t keys = p.Sk;
+  if (!ragged && p.causal && p.Sq < keys) keys = p.Sq;
+  if (!ragged && p.win_right >= 0 && static_cast<int64_t>(p.Sq) + p.win_right < keys)
+    keys = p.Sq + p.win_right;
+  if (p.win_left >= 0 && static_cast<int64_t>(p.Sq) + p.win_left + p.win_right < keys)
+    keys = p.Sq + p.win_left + p.win_right;
+  return keys;
+}
+
+// p.Sq: rows of the longest sequence; p.B: sequences.
+template <int D, bool BF16, int MT, class P>
+static int launch_decode(const P& p, cudaStream_t stream) {
   using L = DecSmem<D, MT>;
-  auto kernel = attn_decode_kernel<D, BF16, MT>;
+  auto kernel = attn_decode_kernel<D, BF16, MT, P>;
   static std::atomic<bool> configured[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return TRX_ERR_CUDA;
@@ -456,7 +535,8 @@ static int launch_decode(const AttnParams& p, cudaStream_t stream) {
                         ((static_cast<int64_t>(p.group) * p.Sq + L::ROWS - 1) / L::ROWS);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
-  const unsigned n = static_cast<unsigned>(decode_splits(p, units * p.B, MT == 2));
+  const unsigned n = static_cast<unsigned>(
+      decode_splits(decode_keys(p, P::FORM != ATT_BATCH), units * p.B, MT == 2));
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = n;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
@@ -469,6 +549,16 @@ static int launch_decode(const AttnParams& p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
 }
 
+template <class P>
+static int launch_decode_rows(const P& p, int64_t D, cudaStream_t s) {
+  const bool wide = p.group * p.Sq > 16;
+  if (D == 128)
+    return p.is_bf16 ? (wide ? launch_decode<128, true, 2>(p, s) : launch_decode<128, true, 1>(p, s))
+                     : (wide ? launch_decode<128, false, 2>(p, s) : launch_decode<128, false, 1>(p, s));
+  return p.is_bf16 ? (wide ? launch_decode<64, true, 2>(p, s) : launch_decode<64, true, 1>(p, s))
+                   : (wide ? launch_decode<64, false, 2>(p, s) : launch_decode<64, false, 1>(p, s));
+}
+
 // Calls that take this kernel: up to 16 query rows. The tcgen05 kernels spend the same time on any
 // Sq up to 128 (they work on whole 128-row tiles), this one works on tiles of 16 packed rows. Measured
 // at 4096 keys, head dim 128, this / attention_plain.cu: Sq = 16, B = 16, 32 / 32 heads 160 / 198 us;
@@ -477,7 +567,7 @@ static int launch_decode(const AttnParams& p, cudaStream_t stream) {
 // that is nearly full, in one wave of CTAs, at head dim 128, against two row tiles per warp here: 97 to
 // 128 keys 8.4 to 8.7 / 7.3 to 7.8 us (96 keys 8.1 to 8.4 / 7.6 to 7.9, 64 keys 7.3 / 7.4; 129 keys 9.2 /
 // 10.0).
-static bool use_decode(const AttnParams& p, int64_t D) {
+inline bool use_decode(const AttnParams& p, int64_t D) {
   const int64_t rows = static_cast<int64_t>(p.Sq) * p.group;
   if (p.Sq > 16 || (p.Hq / p.group) * ((rows + 15) / 16) > 65535) return false;
   const int64_t ctas = static_cast<int64_t>(p.B) * (p.pair_heads ? p.Hq / 2 : p.Hq);

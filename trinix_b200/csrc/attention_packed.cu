@@ -1,5 +1,6 @@
-// Attention over packed sequences of different lengths: launches and C entry. The kernel is
-// attention_plain.cuh's in its packed form.
+// Attention over packed sequences of different lengths: launches and C entry. The kernels are those of
+// attention_plain.cuh and, for few rows, attention_decode.cuh in their packed form.
+#include "attention_decode.cuh"
 #include "attention_plain.cuh"
 
 namespace trx {
@@ -68,11 +69,15 @@ extern "C" int trx_attn_fwd_packed(const void* q, const void* k, const void* v, 
   int rc = make_ragged_q_map(&p.tm_q, q, is_bf16, D, Tq, Hq, 1, 0, q_strides[0], q_strides[1], p.tile_heads,
                              p.tile_tokens);
   if (rc != TRX_OK) return rc;
+  // few rows: see use_decode in attention_decode.cuh
+  const int64_t row_tiles = (p.group * max_sq + 15) / 16;
+  const bool decode = max_sq > 0 && max_sq <= 16 && n_seq > 0 && n_seq < 65535 && Hk * row_tiles <= 65535;
+  const int box = decode ? DEC_KEYS : ATT_BN;
   // without keys nothing is loaded: any legal map
   const void *kk = Tk > 0 ? k : q, *vv = Tk > 0 ? v : q;
-  rc = make_map(&p.tm_k, kk, is_bf16, D, Tk > 0 ? Tk : 1, Hk, 1, 0, k_strides[0], k_strides[1], ATT_BN);
+  rc = make_map(&p.tm_k, kk, is_bf16, D, Tk > 0 ? Tk : 1, Hk, 1, 0, k_strides[0], k_strides[1], box);
   if (rc != TRX_OK) return rc;
-  rc = make_map(&p.tm_v, vv, is_bf16, D, Tk > 0 ? Tk : 1, Hk, 1, 0, v_strides[0], v_strides[1], ATT_BN);
+  rc = make_map(&p.tm_v, vv, is_bf16, D, Tk > 0 ? Tk : 1, Hk, 1, 0, v_strides[0], v_strides[1], box);
   if (rc != TRX_OK) return rc;
   p.out = out;
   p.lse = lse_or_null;
@@ -95,11 +100,21 @@ extern "C" int trx_attn_fwd_packed(const void* q, const void* k, const void* v, 
   // ALiBi under a causal mask: backwards, see attention_plain.cuh
   p.reverse_kv = (slopes_or_null != nullptr && (causal || window_right == 0)) ? 1 : 0;
 
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (decode) {
+    p.q = q;
+    p.q_stride_s = q_strides[0];
+    p.q_stride_h = q_strides[1];
+    p.k_hdiv = p.v_hdiv = p.group;
+    p.B = p.n_seq;
+    p.Sq = static_cast<int>(max_sq);
+    p.Sk = static_cast<int>((Tk + n_seq - 1) / n_seq);
+    return launch_decode_rows(p, D, s);
+  }
   const int64_t slots = Tq / (ATT_NQ * p.tile_tokens) + p.n_seq, heads = Hq / p.tile_heads;
   p.slots_first = slots > 65535 ? 1 : 0;
   const dim3 grid = p.slots_first ? dim3(static_cast<unsigned>(slots), static_cast<unsigned>(heads))
                                   : dim3(static_cast<unsigned>(heads), static_cast<unsigned>(slots));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (D == 128)
     return is_bf16 ? launch_packed_items<128, true>(p, grid, s) : launch_packed_items<128, false>(p, grid, s);
   return is_bf16 ? launch_packed_items<64, true>(p, grid, s) : launch_packed_items<64, false>(p, grid, s);

@@ -37,6 +37,9 @@ struct RaggedParams : AttnParams {
   int seq;                   // shared: queries per sequence
   int prefix, prefix_tiles;  // keys of the prefix, in KV tiles
   int split_tiles;           // KV tiles of one split of the prefix
+  const float* part_o;       // shared, decode kernel: [parts][B * Sq][Hq][D] results of the prefix's splits
+  const float* part_lse;     // and their row sums' log2, [parts][B * Sq][Hq]
+  int parts;
 };
 template <int F>
 struct RaggedParamsOf : RaggedParams {

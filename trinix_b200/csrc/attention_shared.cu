@@ -1,0 +1,195 @@
+// Attention for a batch whose sequences share a prefix: launches and C entries. Two ways:
+//
+//   few rows (decoding)   the rows of the whole batch are one run of query rows against the prefix, whose
+//                         keys are split over the CTAs (attention_plain.cuh, ATT_PREFIX): the prefix is read
+//                         and multiplied once for all, at 128 rows to a tile where a sequence alone would
+//                         fill a few. The decode kernel then does the sequences' own keys and merges.
+//   many rows (prompts)   one pass over the prefix's tiles and the sequence's own (ATT_SHARED): its own rows
+//                         fill the tiles, and the prefix comes from L2.
+#include "attention_decode.cuh"
+#include "attention_plain.cuh"
+
+namespace trx {
+
+using SharedParams = RaggedParamsOf<ATT_SHARED>;
+using PrefixParams = RaggedParamsOf<ATT_PREFIX>;
+
+template <int D, bool BF16, int BIAS, bool SINGLE, class P>
+static int launch_form(const P& p, dim3 grid, cudaStream_t stream) {
+  const int rc = configure_plain<D, BF16, BIAS, SINGLE, P>();
+  if (rc != TRX_OK) return rc;
+  attn_plain_kernel<D, BF16, BIAS, SINGLE, P><<<grid, AP_THREADS, PlainSmem<D>::DYN_BYTES, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
+}
+template <int D, bool BF16, class P>
+static int launch_form_items(const P& p, dim3 grid, cudaStream_t s) {
+  // every visible key is at or before its query, the scale is positive
+  if (static_cast<int64_t>(grid.x) * grid.y * grid.z <= sm_count_of_current_device())
+    return p.slopes ? launch_form<D, BF16, AP_RAMP, true>(p, grid, s)
+                    : launch_form<D, BF16, AP_NONE, true>(p, grid, s);
+  return p.slopes ? launch_form<D, BF16, AP_RAMP, false>(p, grid, s)
+                  : launch_form<D, BF16, AP_NONE, false>(p, grid, s);
+}
+template <class P>
+static int launch_form_rows(const P& p, int64_t D, dim3 grid, cudaStream_t s) {
+  if (D == 128)
+    return p.is_bf16 ? launch_form_items<128, true>(p, grid, s) : launch_form_items<128, false>(p, grid, s);
+  return p.is_bf16 ? launch_form_items<64, true>(p, grid, s) : launch_form_items<64, false>(p, grid, s);
+}
+
+struct SharedPlan {
+  RaggedParams tile;  // tile_heads, tile_tokens
+  bool few;
+  int parts, split_tiles;  // of the prefix, with few rows
+};
+static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int64_t Hk) {
+  SharedPlan s{};
+  s.tile.group = static_cast<int>(Hq / Hk);
+  choose_tile(s.tile);
+  const int64_t row_tiles = (s.tile.group * Sq + 15) / 16;
+  s.few = Sq <= 16 && Hk * row_tiles <= 65535;
+  if (!s.few || P == 0) return s;
+  const int64_t step = ATT_NQ * s.tile.tile_tokens;
+  const int64_t items = Hq / s.tile.tile_heads * ((B * Sq + step - 1) / step);
+  const int64_t tiles = (P + ATT_BN - 1) / ATT_BN;
+  int64_t parts = sm_count_of_current_device() / items;
+  parts = parts < 1 ? 1 : parts > tiles ? tiles : parts;
+  s.split_tiles = static_cast<int>((tiles + parts - 1) / parts);
+  s.parts = static_cast<int>((tiles + s.split_tiles - 1) / s.split_tiles);
+  return s;
+}
+
+}  // namespace trx
+
+using namespace trx;
+
+static size_t shared_bytes(const SharedPlan& s, int64_t B, int64_t Sq, int64_t Hq, int64_t D) {
+  return static_cast<size_t>(s.parts) * B * Sq * Hq * (D + 1) * sizeof(float);
+}
+
+extern "C" size_t trx_attn_shared_bytes(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int64_t Hk, int64_t D) {
+  if (B <= 0 || Sq <= 0 || P < 0 || Hq <= 0 || Hk <= 0 || D <= 0 || Hq % Hk || B > 65535 ||
+      Sq >= (1ll << 30) || P >= (1ll << 30) || Hq > 65535)
+    return 0;
+  return shared_bytes(shared_plan(B, Sq, P, Hq, Hk), B, Sq, Hq, D);
+}
+
+extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const void* prefix_v, const void* k,
+                                   const void* v, void* out, float* lse_or_null, const float* slopes_or_null,
+                                   const int32_t* lengths_or_null, int64_t B, int64_t Sq, int64_t P, int64_t S,
+                                   int64_t Hq, int64_t Hk, int64_t D, const int64_t q_strides[3],
+                                   const int64_t pk_strides[2], const int64_t pv_strides[2],
+                                   const int64_t k_strides[3], const int64_t v_strides[3],
+                                   const int64_t o_strides[3], float scale, int dtype, void* parts,
+                                   size_t parts_bytes, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  if (dtype != TRX_BF16 && dtype != TRX_F16) return TRX_ERR_DTYPE;
+  if (B < 0 || Sq < 0 || P < 0 || S < 0 || Hq <= 0 || Hk <= 0 || D <= 0 || Hq % Hk != 0) return TRX_ERR_SHAPE;
+  if (D != 64 && D != 128) return TRX_ERR_UNSUPPORTED;
+  if (!(scale > 0.0f)) return TRX_ERR_UNSUPPORTED;
+  if (B == 0 || Sq == 0) return TRX_OK;
+  if (!q || !out || !q_strides || !pk_strides || !pv_strides || !k_strides || !v_strides || !o_strides)
+    return TRX_ERR_NULL_POINTER;
+  if ((P > 0 && (!prefix_k || !prefix_v)) || (S > 0 && (!k || !v))) return TRX_ERR_NULL_POINTER;
+  if (!workspace || workspace_bytes < trx_attn_workspace_bytes() || !aligned_to(workspace, 16))
+    return TRX_ERR_WORKSPACE;
+  if (B > 65535 || Sq >= (1ll << 30) || B * Sq >= (1ll << 30) || P >= (1ll << 29) || S >= (1ll << 29) ||
+      Hq > 65535)
+    return TRX_ERR_SHAPE;
+  if (lengths_or_null && !aligned_to(lengths_or_null, 4)) return TRX_ERR_ALIGNMENT;
+  if (!aligned_to(out, 16) || o_strides[0] % 8 || o_strides[1] % 8 || o_strides[2] % 8)
+    return TRX_ERR_ALIGNMENT;
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] < 0 || k_strides[i] < 0 || v_strides[i] < 0 || o_strides[i] < 0 ||
+        (i < 2 && (pk_strides[i] < 0 || pv_strides[i] < 0)))
+      return TRX_ERR_STRIDE;
+
+  SharedPlan plan = shared_plan(B, Sq, P, Hq, Hk);
+  // the rows of the batch as one run: what the prefix's launch wants
+  const int64_t row_stride = Sq == 1 ? q_strides[0] : q_strides[1];
+  if (plan.few && B > 1 && Sq > 1 && q_strides[0] != Sq * q_strides[1]) plan.few = false;
+  if (plan.few && plan.parts > 0 &&
+      (!parts || !aligned_to(parts, 16) || parts_bytes < shared_bytes(plan, B, Sq, Hq, D)))
+    return TRX_ERR_WORKSPACE;
+
+  SharedParams p{};
+  const int is_bf16 = dtype == TRX_BF16, tokens = plan.tile.tile_tokens, heads = plan.tile.tile_heads;
+  const int box = plan.few ? DEC_KEYS : ATT_BN;
+  // without keys nothing is loaded: any legal map
+  int rc = make_map(&p.tm_k, S > 0 ? k : q, is_bf16, D, S > 0 ? S : 1, Hk, B, k_strides[0], k_strides[1],
+                    k_strides[2], box);
+  if (rc != TRX_OK) return rc;
+  rc = make_map(&p.tm_v, S > 0 ? v : q, is_bf16, D, S > 0 ? S : 1, Hk, B, v_strides[0], v_strides[1],
+                v_strides[2], box);
+  if (rc != TRX_OK) return rc;
+  rc = make_map(&p.tm_pk, P > 0 ? prefix_k : q, is_bf16, D, P > 0 ? P : 1, Hk, 1, 0, pk_strides[0],
+                pk_strides[1], ATT_BN);
+  if (rc != TRX_OK) return rc;
+  rc = make_map(&p.tm_pv, P > 0 ? prefix_v : q, is_bf16, D, P > 0 ? P : 1, Hk, 1, 0, pv_strides[0],
+                pv_strides[1], ATT_BN);
+  if (rc != TRX_OK) return rc;
+  p.tile_heads = heads;
+  p.tile_tokens = tokens;
+  p.group = plan.tile.group;
+  p.k_hdiv = p.v_hdiv = p.group;
+  p.k_bmul = p.v_bmul = 1;
+  p.slopes = slopes_or_null;
+  p.status = reinterpret_cast<unsigned int*>(workspace);
+  p.lengths = lengths_or_null;
+  p.B = static_cast<int>(B);
+  p.Sq = p.seq = static_cast<int>(Sq);
+  p.Sk = p.keys = static_cast<int>(S);
+  p.Hq = static_cast<int>(Hq);
+  p.prefix = static_cast<int>(P);
+  p.prefix_tiles = static_cast<int>((P + ATT_BN - 1) / ATT_BN);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.causal = 1;
+  p.win_left = p.win_right = -1;
+  p.is_bf16 = is_bf16;
+  p.reverse_kv = slopes_or_null ? 1 : 0;  // ALiBi: backwards, see attention_plain.cuh
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t step = ATT_NQ * tokens, rows = plan.few ? B * Sq : Sq;
+  const int64_t blocks = (rows + step - 1) / step;
+  if (blocks > 65535) return TRX_ERR_SHAPE;
+  dim3 grid(static_cast<unsigned>(Hq / heads), static_cast<unsigned>(blocks), static_cast<unsigned>(B));
+
+  if (plan.few && plan.parts > 0) {
+    PrefixParams f{};
+    static_cast<RaggedParams&>(f) = p;
+    rc = make_ragged_q_map(&f.tm_q, q, is_bf16, D, B * Sq, Hq, 1, 0, row_stride, q_strides[2], heads, tokens);
+    if (rc != TRX_OK) return rc;
+    const int64_t n = B * Sq * Hq;
+    f.rows = static_cast<int>(B * Sq);
+    f.split_tiles = plan.split_tiles;
+    f.out = parts;
+    f.o_stride_b = n * D;
+    f.o_stride_s = Hq * D;
+    f.o_stride_h = D;
+    f.lse = static_cast<float*>(parts) + plan.parts * n * D;
+    f.lse_stride_b = n;
+    p.part_o = static_cast<float*>(parts);
+    p.part_lse = f.lse;
+    p.parts = plan.parts;
+    grid.z = plan.parts;
+    rc = launch_form_rows(f, D, grid, s);
+    if (rc != TRX_OK) return rc;
+  }
+  p.out = out;
+  p.o_stride_b = o_strides[0];
+  p.o_stride_s = o_strides[1];
+  p.o_stride_h = o_strides[2];
+  p.lse = lse_or_null;
+  p.lse_stride_b = Hq * Sq;
+  p.lse_stride_h = Sq;
+  if (plan.few) {
+    p.q = q;
+    p.q_stride_b = q_strides[0];
+    p.q_stride_s = q_strides[1];
+    p.q_stride_h = q_strides[2];
+    return launch_decode_rows(p, D, s);
+  }
+  rc = make_ragged_q_map(&p.tm_q, q, is_bf16, D, Sq, Hq, B, q_strides[0], q_strides[1], q_strides[2], heads,
+                         tokens);
+  if (rc != TRX_OK) return rc;
+  return launch_form_rows(p, D, grid, s);
+}

@@ -790,3 +790,64 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     elif o is not out:
         o = out.copy_(o[..., :d])
     return (o, lse) if return_lse else o
+
+
+def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
+                            k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor] = None, *,
+                            scale: Optional[float] = None, alibi_slopes: Optional[torch.Tensor] = None,
+                            return_lse: bool = False):
+    """Causal attention of a batch whose sequences all begin with the same keys, held and computed once.
+
+    q (B, Sq, Hq, D): the last Sq tokens of each sequence; prefix_k / prefix_v (P, Hk, D): the keys and
+    values that all of them begin with; k / v (B, S, Hk, D): each sequence's own behind them, of which the
+    first lengths[b] are in use (int32 on the device; None: all S), the new tokens' among them. The
+    others are never used, whatever they hold. Query i stands at key P + lengths[b] - Sq + i of the
+    concatenation and sees the keys up to there; alibi_slopes (Hq,) add -slope * distance. A query
+    without a key is 0. With return_lse also the fp32 (B, Hq, Sq) log-sum-exp.
+
+    Up to 16 tokens (decoding): the prefix is read once for the whole batch and multiplied with all its
+    rows together. More: one pass over both, the prefix from L2.
+    """
+    dev = _need_cuda(q, prefix_k, prefix_v, k, v, lengths, alibi_slopes)
+    _check_attention_types(q, prefix_k, prefix_v, k, v)
+    if q.dim() != 4 or k.dim() != 4 or prefix_k.dim() != 3:
+        raise ValueError(f"expected q (batch, rows, heads, head_dim), prefix_k (rows, heads, head_dim) and "
+                         f"k (batch, rows, heads, head_dim), got {tuple(q.shape)}, "
+                         f"{tuple(prefix_k.shape)}, {tuple(k.shape)}")
+    B, Sq, Hq, d = q.shape
+    P, Hk, _ = prefix_k.shape
+    S = k.shape[1]
+    if prefix_k.shape[2] != d or prefix_v.shape != prefix_k.shape:
+        raise ValueError(f"prefix_k {tuple(prefix_k.shape)} / prefix_v {tuple(prefix_v.shape)} do not match "
+                         f"q {tuple(q.shape)}")
+    if k.shape != (B, S, Hk, d) or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)} and "
+                         f"prefix_k {tuple(prefix_k.shape)}")
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError(f"query heads ({Hq}) must be a multiple of kv heads ({Hk})")
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or lengths.shape != (B,):
+            raise ValueError(f"lengths must be an int32 tensor of {B} entries")
+        lengths = lengths.contiguous()
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not scale > 0.0:
+        raise ValueError(f"scale must be positive, got {scale}")
+    slopes = _slopes(alibi_slopes, Hq)
+    dp = _padded_dim(d)
+    q, prefix_k, prefix_v, k, v = (_packed_view(_pad(t, dp)) for t in (q, prefix_k, prefix_v, k, v))
+    if B > 1 and Sq > 1 and q.stride(0) != Sq * q.stride(1) and Sq <= 16:
+        q = q.contiguous()  # the rows of the batch as one run
+    out = _empty(q, (B, Sq, Hq, dp))
+    lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
+    parts = _empty(q, _lib.load().trx_attn_shared_bytes(B, Sq, P, Hq, Hk, dp), dtype=torch.uint8)
+    ws = _workspace(dev)
+    _raise_if_failed("trx_attn_fwd_shared", dev)  # of an earlier launch, before more work is queued
+    _launch("trx_attn_fwd_shared", dev, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k.data_ptr(),
+            v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(slopes), _ptr(lengths), B, Sq, P, S, Hq, Hk, dp,
+            I64x3(*q.stride()[:3]), I64x2(*prefix_k.stride()[:2]), I64x2(*prefix_v.stride()[:2]),
+            I64x3(*k.stride()[:3]), I64x3(*v.stride()[:3]), I64x3(*out.stride()[:3]), scale, _code(q),
+            parts.data_ptr(), parts.numel(), ws.data_ptr(), ws.numel())
+    if parts.numel():
+        _count()  # the prefix is a launch of its own
+    out = out if dp == d else out[..., :d].contiguous()
+    return (out, lse) if return_lse else out
