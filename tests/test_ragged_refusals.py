@@ -8,7 +8,7 @@ import torch
 import trinix_b200 as T
 from trinix_b200 import _lib
 
-I64x2 = _lib.I64x2
+I64x2 = ctypes.c_int64 * 2
 ONE = ctypes.c_void_p(4096)
 
 

@@ -16,7 +16,6 @@ TRX_F32, TRX_F16, TRX_BF16 = 0, 1, 2
 GLU_SWIGLU, GLU_GEGLU_TANH, GLU_REGLU = 0, 1, 2
 TRX_ERR_DEVICE_STATUS = -8
 
-I64x2 = c_int64 * 2
 I64x3 = c_int64 * 3
 
 # name -> (restype, argtypes); mirrors include/trinix_b200.h one to one.
@@ -92,13 +91,12 @@ SIGNATURES = {
                                      c_size_t, c_void_p]),
     "trx_attn_fwd_packed": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
-                                    c_int64, I64x2, I64x2, I64x2, I64x2, c_float, c_int, c_int64,
+                                    c_int64, *[c_void_p] * 4, c_float, c_int, c_int64,
                                     c_int64, c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "trx_attn_shared_bytes": (c_size_t, [c_int64] * 6),
     "trx_attn_fwd_shared": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
-                                    c_int64, c_int64, c_int64, I64x3, I64x2, I64x2, I64x3, I64x3, I64x3,
-                                    c_float, c_int, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
+                                    c_int64, c_int64, c_int64, *[c_void_p] * 6, c_float, c_int, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
     "trx_attn_status": (c_int, [c_void_p, c_void_p, c_void_p]),
     "trx_attn_mirror": (c_int, [c_void_p, c_void_p, c_void_p]),
     "trx_attn_fwd_static_scratch": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

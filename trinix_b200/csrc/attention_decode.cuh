@@ -377,28 +377,47 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
 #pragma unroll
   for (int w = 0; w < DEC_WARPS; ++w) whole = whole && no_result[w] == 0;
 
+  // Behind the prefix's launch this one may have started beside it: from here on its results are read.
+  if constexpr (FORM == ATT_SHARED) asm volatile("griddepcontrol.wait;" ::: "memory");
+
   // out[row, 4 c4 ..] = acc / l, and the row's LSE
   auto emit = [&](int r, int c4, float4 acc, float mx, float l) {
     const int s = (r0 + r) / group, h = h0 + (r0 + r) % group;
     if constexpr (FORM == ATT_SHARED) {  // with the parts of the prefix: their rows' O / l and log2 sums
       const long long part = static_cast<long long>(p.B) * p.Sq * p.Hq;  // rows of a part
       const long long at = (static_cast<long long>(b) * p.Sq + s) * p.Hq + h;
-      float top = mx;
-      for (int k = 0; k < p.parts; ++k) top = fmaxf(top, p.part_lse[k * part + at]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      const float f = fast_exp2(mx - ref);
-      acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-      l *= f;
-      for (int k = 0; k < p.parts; ++k) {
-        const float w = fast_exp2(p.part_lse[k * part + at] - ref);
-        const float4 o = *reinterpret_cast<const float4*>(p.part_o + (k * part + at) * D + 4 * c4);
-        l += w;
-        acc.x = fmaf(w, o.x, acc.x);
-        acc.y = fmaf(w, o.y, acc.y);
-        acc.z = fmaf(w, o.z, acc.z);
-        acc.w = fmaf(w, o.w, acc.w);
+      // eight parts at a time, all their loads in flight: one after the other each costs an L2 latency
+      constexpr int N = 8;
+#pragma unroll 1
+      for (int k0 = 0; k0 < p.parts; k0 += N) {
+        float sum[N];
+        float4 o[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const bool there = k0 + i < p.parts;
+          const long long r = (k0 + i) * part + at;
+          sum[i] = there ? p.part_lse[r] : -INFINITY;
+          o[i] = there ? *reinterpret_cast<const float4*>(p.part_o + r * D + 4 * c4)
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float top = mx;
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = fmaxf(top, sum[i]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        const float f = fast_exp2(mx - ref);  // 0 when mx == -inf
+        mx = ref;
+        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float w = fast_exp2(sum[i] - ref);
+          l += w;
+          acc.x = fmaf(w, o[i].x, acc.x);
+          acc.y = fmaf(w, o[i].y, acc.y);
+          acc.z = fmaf(w, o[i].z, acc.z);
+          acc.w = fmaf(w, o[i].w, acc.w);
+        }
       }
-      mx = ref;
     }
     const float inv = l > 0.0f ? __fdividef(1.0f, l) : 0.0f;
     if (whole) {
@@ -514,9 +533,10 @@ inline int64_t decode_keys(const AttnParams& p, bool ragged) {
   return keys;
 }
 
-// p.Sq: rows of the longest sequence; p.B: sequences.
+// p.Sq: rows of the longest sequence; p.B: sequences. beside_last: it may start before the launch in front of
+// it is over (and waits for that before it reads that one's results).
 template <int D, bool BF16, int MT, class P>
-static int launch_decode(const P& p, cudaStream_t stream) {
+static int launch_decode(const P& p, bool beside_last, cudaStream_t stream) {
   using L = DecSmem<D, MT>;
   auto kernel = attn_decode_kernel<D, BF16, MT, P>;
   static std::atomic<bool> configured[64];
@@ -534,7 +554,8 @@ static int launch_decode(const P& p, cudaStream_t stream) {
   const int64_t units = static_cast<int64_t>(p.Hq / p.group) *
                         ((static_cast<int64_t>(p.group) * p.Sq + L::ROWS - 1) / L::ROWS);
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
+  cudaLaunchAttribute attrs[2] = {};
+  cudaLaunchAttribute& attr = attrs[0];
   const unsigned n = static_cast<unsigned>(
       decode_splits(decode_keys(p, P::FORM != ATT_BATCH), units * p.B, MT == 2));
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -544,19 +565,28 @@ static int launch_decode(const P& p, cudaStream_t stream) {
   cfg.blockDim = dim3(DEC_THREADS);
   cfg.dynamicSmemBytes = L::DYN_BYTES;
   cfg.stream = stream;
-  cfg.attrs = &attr;
+  cfg.attrs = attrs;
   cfg.numAttrs = 1;
+  if (beside_last) {
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
 }
 
 template <class P>
-static int launch_decode_rows(const P& p, int64_t D, cudaStream_t s) {
-  const bool wide = p.group * p.Sq > 16;
-  if (D == 128)
-    return p.is_bf16 ? (wide ? launch_decode<128, true, 2>(p, s) : launch_decode<128, true, 1>(p, s))
-                     : (wide ? launch_decode<128, false, 2>(p, s) : launch_decode<128, false, 1>(p, s));
-  return p.is_bf16 ? (wide ? launch_decode<64, true, 2>(p, s) : launch_decode<64, true, 1>(p, s))
-                   : (wide ? launch_decode<64, false, 2>(p, s) : launch_decode<64, false, 1>(p, s));
+static int launch_decode_rows(const P& p, int64_t D, cudaStream_t s, bool beside_last = false) {
+  auto launch = [&](auto dim, auto bf16) {
+    constexpr int DIM = decltype(dim)::value;
+    constexpr bool BF = decltype(bf16)::value;
+    return p.group * p.Sq > 16 ? launch_decode<DIM, BF, 2>(p, beside_last, s)
+                               : launch_decode<DIM, BF, 1>(p, beside_last, s);
+  };
+  using D128 = std::integral_constant<int, 128>;
+  using D64 = std::integral_constant<int, 64>;
+  if (D == 128) return p.is_bf16 ? launch(D128{}, std::true_type{}) : launch(D128{}, std::false_type{});
+  return p.is_bf16 ? launch(D64{}, std::true_type{}) : launch(D64{}, std::false_type{});
 }
 
 // Calls that take this kernel: up to 16 query rows. The tcgen05 kernels spend the same time on any

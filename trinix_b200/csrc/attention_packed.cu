@@ -12,7 +12,7 @@ static int launch_packed(const PackedParams& p, dim3 grid, cudaStream_t stream) 
   const int rc = configure_plain<D, BF16, BIAS, SINGLE, PackedParams>();
   if (rc != TRX_OK) return rc;
   attn_plain_kernel<D, BF16, BIAS, SINGLE, PackedParams>
-      <<<grid, AP_THREADS, PlainSmem<D>::DYN_BYTES, stream>>>(p);
+      <<<grid, AP_THREADS, plain_smem_bytes<D, SINGLE, PackedParams>(), stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
 }
 

@@ -120,6 +120,9 @@ struct PlainSmem {
   static constexpr int STAT_OFF = ITEM_OFF + 2 * 64;               // [2 tiles][sum, max][128]
   static constexpr int TOTAL = STAT_OFF + 2 * 2 * ATT_BM * 4;
   static constexpr int DYN_BYTES = TOTAL + 1024;  // slack for 1024-byte alignment
+  static constexpr int TABLE_OFF = TOTAL;         // packed form, several items per CTA: RaggedTable
+  static constexpr int TABLE_BYTES = sizeof(RaggedTable);
+  static_assert(TABLE_OFF % 4 == 0 && DYN_BYTES + TABLE_BYTES <= 232448, "shared memory");
   static_assert(DYN_BYTES <= 232448, "shared memory");
 };
 
@@ -461,11 +464,22 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     mbar_arrive(bar(B_ITEM + (q & 1)));
   };
 
+  // the decode kernel that merges these results may start on what does not depend on them
+  if constexpr (FORM == ATT_PREFIX) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Work first_item;  // of the producer
   RaggedCursor cursor;
+  RaggedTable* table = reinterpret_cast<RaggedTable*>(smem + L::TABLE_OFF);
+  bool use_table = false;
   if constexpr (FORM == ATT_PACKED) {
+    use_table = !SINGLE && p.n_seq <= RAGGED_TABLE;
+    if (use_table) {
+      ragged_fill(p, *table);
+      // blocks behind the last one with rows, if it is that late that they are launched at all
+      if (ragged_slot(p, blockIdx.x, blockIdx.y) >= table->first[p.n_seq]) return;
+    }
     if (warp == 12) {
-      cursor.seek(p, ragged_slot(p, blockIdx.x, blockIdx.y), lane);
+      if (use_table) cursor.look_up(p, *table, ragged_slot(p, blockIdx.x, blockIdx.y));
+      else cursor.seek(p, ragged_slot(p, blockIdx.x, blockIdx.y), lane);
       first_item = ragged_item(p, cursor, blockIdx.x, blockIdx.y, 0);
     }
   } else if constexpr (FORM != ATT_BATCH) {
@@ -621,6 +635,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         int start = min(STAGES, 2 * w.n);    // of this one, issued before the CTA-wide sync
         bool ok = true, asked = false;
         int q = 0, asks = 0;
+        auto ask = [&] {
+          mbar_expect_tx(bar(B_NEXT), 16);
+          request_block(sbase + L::NEXT_OFF, bar(B_NEXT));
+          asked = true;
+        };
         auto fill_one = [&](int fill) {
           const int g = base + fill;
           if (g >= STAGES) ok = wait(B_KVEMPTY + g % STAGES, ((g / STAGES) & 1) ^ 1);
@@ -637,12 +656,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if constexpr (SINGLE) break;  // no other item, and no answer to wait for
           // The next item is asked for when this one's last tiles have been: some visits before its
           // end, enough to hide the answer; earlier would take items from CTAs that are done sooner.
-          bool more = false;
+          bool more = false, rest = false;
 #pragma unroll 1
           do {  // a slot between two packed sequences may hold no rows: the next one then
-            mbar_expect_tx(bar(B_NEXT), 16);
-            request_block(sbase + L::NEXT_OFF, bar(B_NEXT));
-            asked = true;
+            ask();
             ok = wait(B_NEXT, asks & 1);
             if (!ok) break;
             asked = false;
@@ -654,19 +671,37 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               if constexpr (FORM == ATT_BATCH) {
                 w = plain_item(p, x, y, z);
               } else {
-                if constexpr (FORM == ATT_PACKED) cursor.advance(p, ragged_slot(p, x, y));
+                if constexpr (FORM == ATT_PACKED) {
+                  rest = use_table && ragged_slot(p, x, y) >= table->first[p.n_seq];
+                  if (use_table) cursor.look_up(p, *table, ragged_slot(p, x, y));
+                  else cursor.seek_alone(p, ragged_slot(p, x, y));
+                }
                 w = ragged_item(p, cursor, x, y, z);
               }
               kv_heads(w, kh, vh);
             } else {
               w.valid = 0;
             }
-          } while (FORM == ATT_PACKED && more && !ragged_has_rows(w));
+          } while (FORM == ATT_PACKED && more && !rest && !ragged_has_rows(w));
           if (!ok) break;
+          if (rest) {
+            more = false;
+            w.valid = 0;
+          }
           ++q;
           if (q >= 2) ok = wait(B_ITEMFREE + (q & 1), ((q >> 1) & 1) ^ 1);
           if (!ok) break;
           publish(w, q);
+          if (rest) {  // the blocks from here on have no rows: taken from the grid while the others finish
+            int x, y, z;
+            do {
+              ask();
+              ok = wait(B_NEXT, asks & 1);
+              if (!ok) break;
+              asked = false;
+              ++asks;
+            } while (requested_block(sbase + L::NEXT_OFF, x, y, z));
+          }
           if (!more) break;
           if (w.n > 0) {  // its first K tile need not wait for the Q tiles to be free
             fill_one(0);
@@ -1178,6 +1213,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   }
 }
 
+template <int D, bool SINGLE, class P>
+constexpr int plain_smem_bytes() {
+  return PlainSmem<D>::DYN_BYTES + (P::FORM == ATT_PACKED && !SINGLE ? PlainSmem<D>::TABLE_BYTES : 0);
+}
 template <int D, bool BF16, int BIAS, bool SINGLE, class P>
 static int configure_plain() {
   // The attribute is set once per device; host threads that race on the first call each set
@@ -1194,7 +1233,7 @@ static int configure_plain() {
     using Regs = PlainRegs<D, BIAS, SINGLE>;
     if (a.numRegs * 4 < 2 * Regs::SOFTMAX + Regs::EPILOGUE + Regs::OTHER) return TRX_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             PlainSmem<D>::DYN_BYTES) != cudaSuccess)
+                             plain_smem_bytes<D, SINGLE, P>()) != cudaSuccess)
       return TRX_ERR_CUDA;
     if (cacheable) configured[dev].store(true, std::memory_order_release);
   }

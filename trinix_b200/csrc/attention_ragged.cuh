@@ -75,9 +75,18 @@ __device__ __forceinline__ int ragged_position(const RaggedParams& p, int r) {
 __device__ __forceinline__ int ragged_position(const AttnParams&, int) { return 0; }
 
 // Packed rows: which sequence a block works on. The host knows the rows and the number of sequences but not
-// where they end, and a table of blocks would cost a launch in front. So each sequence has the slots from
-// floor(first row / R) + its index to the next one's, R rows being a block's: at least as many as it has
-// blocks, on average half a slot too many, which are passed over, and found by a search in cu_q alone.
+// where they end, and a table of blocks would cost a launch in front. A launch of several items per CTA with
+// up to RAGGED_TABLE sequences counts every sequence's blocks in shared memory when a CTA starts, and finds
+// a block by bisection there. Otherwise each sequence has the slots from floor(first row / R) + its index to
+// the next one's, R rows being a block's: at least as many as it has blocks, on average half a slot too
+// many, which are passed over, and found by a search in cu_q alone.
+constexpr int RAGGED_TABLE = 1024;
+struct RaggedTable {
+  int first[RAGGED_TABLE + 1];  // blocks before each sequence; the last: all
+  int row[RAGGED_TABLE + 1], key[RAGGED_TABLE + 1];
+  int warp_sum[16];
+};
+
 struct RaggedCursor {
   int s, slot, slot0, next;  // sequence, the slot looked for, first slots of this and the next sequence
   int q0, sq, k0, sk;
@@ -98,7 +107,7 @@ struct RaggedCursor {
       sk = max(0, ragged_key(p, s + 1) - k0);
     }
   }
-  // The last sequence in [lo, hi) whose first slot is not behind `slot`; a whole warp, 32 probes at a time.
+  // The last sequence whose first slot is not behind `at`; a whole warp, 32 probes at a time.
   __device__ __forceinline__ void seek(const RaggedParams& p, int at, int lane) {
     slot = at;
     int lo = 0, hi = p.n_seq;
@@ -113,29 +122,82 @@ struct RaggedCursor {
     s = lo;
     load(p);
   }
-  // The same from where the cursor stands, by one thread: blocks are handed out in their order, so the next
-  // one is of this sequence or of one shortly behind it.
-  __device__ __forceinline__ void advance(const RaggedParams& p, int at) {
+  // The same by one thread: 15 probes at a time, whose loads are in flight together where a bisection
+  // waits for each.
+  __device__ __forceinline__ void seek_alone(const RaggedParams& p, int at) {
     slot = at;
-    if (at >= slot0 && at < next) return;
-    int lo = at >= slot0 ? s : 0, hi = p.n_seq;
-    if (at >= slot0) {
-#pragma unroll 1
-      for (int i = 0; i < 3 && lo + 1 < hi; ++i) {
-        if (first_slot(p, lo + 1) > at) hi = lo + 1;
-        else ++lo;
-      }
-    }
+    constexpr int N = 15;
+    int lo = 0, hi = p.n_seq;
 #pragma unroll 1
     while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2;
-      if (first_slot(p, mid) <= at) lo = mid;
-      else hi = mid;
+      const int step = (hi - lo + N) / (N + 1);
+      int n = 0;
+#pragma unroll
+      for (int i = 1; i <= N; ++i) {
+        const int probe = lo + i * step;
+        n += probe < hi && first_slot(p, min(probe, hi - 1)) <= at ? 1 : 0;
+      }
+      lo += n * step;
+      if (n < N) hi = min(hi, lo + step);
     }
     s = lo;
     load(p);
   }
+  __device__ __forceinline__ void look_up(const RaggedParams& p, const RaggedTable& t, int at) {
+    slot = at;
+    int lo = 0, hi = p.n_seq;
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (t.first[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    s = lo;
+    slot0 = t.first[lo];
+    q0 = t.row[lo];
+    sq = max(0, t.row[lo + 1] - q0);
+    k0 = t.key[lo];
+    sk = lo < p.n_cu ? max(0, t.key[lo + 1] - k0) : 0;
+  }
 };
+// The whole CTA, 512 threads of two sequences each.
+__device__ __forceinline__ void ragged_fill(const RaggedParams& p, RaggedTable& t) {
+  static_assert(RAGGED_TABLE == 2 * 512, "two sequences per thread");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = 2 * threadIdx.x;
+  const int step = ATT_NQ * p.tile_tokens;
+  int row[3], blocks[2];
+#pragma unroll
+  for (int e = 0; e < 3; ++e) row[e] = i + e <= p.n_seq ? ragged_row(p, i + e) : 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    blocks[e] = i + e < p.n_seq ? (max(0, row[e + 1] - row[e]) + step - 1) / step : 0;
+  const int own = blocks[0] + blocks[1];
+  int sum = own;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int below = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += below;
+  }
+  if (lane == 31) t.warp_sum[warp] = sum;
+  __syncthreads();
+  int before = sum - own;
+  for (int w = 0; w < warp; ++w) before += t.warp_sum[w];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (i + e <= p.n_seq) {
+      t.first[i + e] = before;
+      t.row[i + e] = row[e];
+      t.key[i + e] = ragged_key(p, min(i + e, p.n_cu));
+    }
+    before += blocks[e];
+  }
+  if (i + 2 == p.n_seq && threadIdx.x == 511) {  // a full table: its end
+    t.first[i + 2] = before;
+    t.row[i + 2] = row[2];
+    t.key[i + 2] = ragged_key(p, min(i + 2, p.n_cu));
+  }
+  __syncthreads();
+}
 
 __device__ __forceinline__ int ragged_slot(const RaggedParams& p, int x, int y) {
   return p.slots_first ? x : y;

@@ -153,6 +153,7 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   if (blocks > 65535) return TRX_ERR_SHAPE;
   dim3 grid(static_cast<unsigned>(Hq / heads), static_cast<unsigned>(blocks), static_cast<unsigned>(B));
 
+  bool beside = false;
   if (plan.few && plan.parts > 0) {
     PrefixParams f{};
     static_cast<RaggedParams&>(f) = p;
@@ -171,6 +172,8 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
     p.part_lse = f.lse;
     p.parts = plan.parts;
     grid.z = plan.parts;
+    // the decode kernel beside the prefix's, where all of that one's CTAs are running
+    beside = static_cast<int64_t>(grid.x) * grid.y * grid.z <= sm_count_of_current_device();
     rc = launch_form_rows(f, D, grid, s);
     if (rc != TRX_OK) return rc;
   }
@@ -186,7 +189,7 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
     p.q_stride_b = q_strides[0];
     p.q_stride_s = q_strides[1];
     p.q_stride_h = q_strides[2];
-    return launch_decode_rows(p, D, s);
+    return launch_decode_rows(p, D, s, beside);
   }
   rc = make_ragged_q_map(&p.tm_q, q, is_bf16, D, Sq, Hq, B, q_strides[0], q_strides[1], q_strides[2], heads,
                          tokens);

@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import I64x2, I64x3
+from ._lib import I64x3
 
 _DTYPE_CODE = {torch.float32: _lib.TRX_F32, torch.float16: _lib.TRX_F16,
                torch.bfloat16: _lib.TRX_BF16}
@@ -681,22 +681,21 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     return (out, lse) if return_lse else out
 
 
-def _packed_view(t: torch.Tensor) -> torch.Tensor:
-    """A view whose last dim is dense, whose base is 16-byte aligned and whose other strides are
-    multiples of 8 elements and at least a row apart, as the tensor maps of the packed and shared
-    kernels want it; anything else (expanded heads, a slice along D at an odd offset) is
-    materialised once."""
-    if t.numel() == 0:
-        return t
-    d = t.shape[-1]
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        t.shape[i] == 1 or (t.stride(i) % 8 == 0 and t.stride(i) >= d) for i in range(t.dim() - 1))
-    return t if ok else t.contiguous()
-
-
-def _check_attention_types(*ts: torch.Tensor) -> None:
-    if any(t.dtype != ts[0].dtype for t in ts) or ts[0].dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError("attention needs queries, keys and values of one dtype, bfloat16 or float16")
+def _packed_view(t: torch.Tensor, d: int) -> torch.Tensor:
+    """A view with head dim d (zero columns are appended to fewer) whose last dim is dense, whose base
+    is 16-byte aligned and whose other strides are multiples of 8 elements and at least a row apart, as
+    the tensor maps of the packed and shared kernels want it; anything else (expanded heads, a slice
+    along D at an odd offset) is materialised once."""
+    n = t.shape[-1]
+    if n != d:
+        return torch.nn.functional.pad(t, (0, d - n))
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        if t.stride(-1) == 1 and all(size == 1 or (step % 8 == 0 and step >= d)
+                                     for size, step in zip(t.shape[:-1], t.stride())):
+            return t
+    return t.contiguous() if t.numel() else t
 
 
 def _slopes(alibi_slopes: Optional[torch.Tensor], heads: int) -> Optional[torch.Tensor]:
@@ -709,14 +708,15 @@ def _slopes(alibi_slopes: Optional[torch.Tensor], heads: int) -> Optional[torch.
 
 
 def _padded_dim(d: int) -> int:
-    """The head dim that the kernels run `d` as: zero columns are appended to anything else."""
+    """The head dim that the kernels run `d` as."""
     if not 0 < d <= 128:
         raise ValueError(f"head_dim must be in 1 .. 128, got {d}")
     return 64 if d <= 64 else 128
 
 
-def _pad(t: torch.Tensor, d: int) -> torch.Tensor:
-    return t if t.shape[-1] == d else torch.nn.functional.pad(t, (0, d - t.shape[-1]))
+# Element strides of an entry's tensors in one block, its parts passed by address: an array object for
+# each tensor costs the host 0.6 us.
+_I64x8, _I64x16 = ctypes.c_int64 * 8, ctypes.c_int64 * 16
 
 
 def _cu_seqlens(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -746,13 +746,15 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     also the fp32 (Hq, Tq) log-sum-exp, -inf for rows without a key and rows behind the last.
     """
     dev = _need_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, alibi_slopes, out)
-    _check_attention_types(q, k, v)
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+    dtype, shape = q.dtype, k.shape
+    if not (dtype == k.dtype == v.dtype) or dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("attention needs q, k, v of one dtype, bfloat16 or float16")
+    if q.dim() != 3 or len(shape) != 3:
         raise ValueError(f"expected (rows, heads, head_dim) tensors, got q {tuple(q.shape)}, "
-                         f"k {tuple(k.shape)}, v {tuple(v.shape)}")
+                         f"k {tuple(shape)}, v {tuple(v.shape)}")
     Tq, Hq, d = q.shape
-    Tk, Hk, _ = k.shape
-    if k.shape[2] != d or v.shape != k.shape:
+    Tk, Hk, _ = shape
+    if shape[2] != d or v.shape != shape:
         raise ValueError(f"k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
     if Hk == 0 or Hq == 0 or Hq % Hk:
         raise ValueError(f"query heads ({Hq}) must be a multiple of kv heads ({Hk})")
@@ -768,23 +770,24 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     slopes = _slopes(alibi_slopes, Hq)
     scale = d ** -0.5 if scale is None else float(scale)
     dp = _padded_dim(d)
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+    if out is not None and (out.shape != q.shape or out.dtype != dtype):
         raise ValueError("out must have the shape and dtype of q")
-    q, k, v = (_packed_view(_pad(t, dp)) for t in (q, k, v))
+    q, k, v = _packed_view(q, dp), _packed_view(k, dp), _packed_view(v, dp)
     if out is None:
         o = _empty(q, (Tq, Hq, dp))
     else:
-        o = _packed_view(_pad(out, dp))  # a copy where the kernel cannot write into it
+        o = _packed_view(out, dp)  # a copy where the kernel cannot write into it
     lse = _empty(q, (Hq, Tq), dtype=torch.float32) if return_lse else None
     if lse is not None and out is not None:
         lse.fill_(float("-inf"))  # rows behind the last sequence are not touched
     ws = _workspace(dev)
     _raise_if_failed("trx_attn_fwd_packed", dev)  # of an earlier launch, before more work is queued
+    strides = _I64x8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *o.stride()[:2])
+    at = ctypes.addressof(strides)
     _launch("trx_attn_fwd_packed", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse),
-            _ptr(slopes), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, Tq, Tk, Hq, Hk, dp,
-            I64x2(*q.stride()[:2]), I64x2(*k.stride()[:2]), I64x2(*v.stride()[:2]),
-            I64x2(*o.stride()[:2]), scale, int(bool(causal)), wl, wr, int(max_seqlen_q or 0),
-            int(out is None), _code(q), ws.data_ptr(), ws.numel())
+            _ptr(slopes), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, Tq, Tk, Hq, Hk, dp, at,
+            at + 16, at + 32, at + 48, scale, 1 if causal else 0, wl, wr, int(max_seqlen_q or 0),
+            1 if out is None else 0, _DTYPE_CODE[dtype], ws.data_ptr(), ws.numel())
     if out is None:
         o = o if dp == d else o[..., :d].contiguous()
     elif o is not out:
@@ -809,19 +812,22 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     rows together. More: one pass over both, the prefix from L2.
     """
     dev = _need_cuda(q, prefix_k, prefix_v, k, v, lengths, alibi_slopes)
-    _check_attention_types(q, prefix_k, prefix_v, k, v)
-    if q.dim() != 4 or k.dim() != 4 or prefix_k.dim() != 3:
+    dtype, own = q.dtype, k.shape
+    if (not (dtype == prefix_k.dtype == prefix_v.dtype == k.dtype == v.dtype)
+            or dtype not in (torch.bfloat16, torch.float16)):
+        raise TypeError("attention needs queries, keys and values of one dtype, bfloat16 or float16")
+    if q.dim() != 4 or len(own) != 4 or prefix_k.dim() != 3:
         raise ValueError(f"expected q (batch, rows, heads, head_dim), prefix_k (rows, heads, head_dim) and "
                          f"k (batch, rows, heads, head_dim), got {tuple(q.shape)}, "
-                         f"{tuple(prefix_k.shape)}, {tuple(k.shape)}")
+                         f"{tuple(prefix_k.shape)}, {tuple(own)}")
     B, Sq, Hq, d = q.shape
-    P, Hk, _ = prefix_k.shape
-    S = k.shape[1]
-    if prefix_k.shape[2] != d or prefix_v.shape != prefix_k.shape:
+    P, Hk, dim = prefix_k.shape
+    S = own[1]
+    if dim != d or prefix_v.shape != prefix_k.shape:
         raise ValueError(f"prefix_k {tuple(prefix_k.shape)} / prefix_v {tuple(prefix_v.shape)} do not match "
                          f"q {tuple(q.shape)}")
-    if k.shape != (B, S, Hk, d) or v.shape != k.shape:
-        raise ValueError(f"k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)} and "
+    if own != (B, S, Hk, d) or v.shape != own:
+        raise ValueError(f"k {tuple(own)} / v {tuple(v.shape)} do not match q {tuple(q.shape)} and "
                          f"prefix_k {tuple(prefix_k.shape)}")
     if Hk == 0 or Hq == 0 or Hq % Hk:
         raise ValueError(f"query heads ({Hq}) must be a multiple of kv heads ({Hk})")
@@ -834,19 +840,22 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
         raise ValueError(f"scale must be positive, got {scale}")
     slopes = _slopes(alibi_slopes, Hq)
     dp = _padded_dim(d)
-    q, prefix_k, prefix_v, k, v = (_packed_view(_pad(t, dp)) for t in (q, prefix_k, prefix_v, k, v))
-    if B > 1 and Sq > 1 and q.stride(0) != Sq * q.stride(1) and Sq <= 16:
+    q, prefix_k, prefix_v = _packed_view(q, dp), _packed_view(prefix_k, dp), _packed_view(prefix_v, dp)
+    k, v = _packed_view(k, dp), _packed_view(v, dp)
+    if B > 1 and 1 < Sq <= 16 and q.stride(0) != Sq * q.stride(1):
         q = q.contiguous()  # the rows of the batch as one run
     out = _empty(q, (B, Sq, Hq, dp))
     lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
     parts = _empty(q, _lib.load().trx_attn_shared_bytes(B, Sq, P, Hq, Hk, dp), dtype=torch.uint8)
     ws = _workspace(dev)
     _raise_if_failed("trx_attn_fwd_shared", dev)  # of an earlier launch, before more work is queued
+    strides = _I64x16(*q.stride()[:3], *prefix_k.stride()[:2], *prefix_v.stride()[:2], *k.stride()[:3],
+                      *v.stride()[:3], *out.stride()[:3])
+    at = ctypes.addressof(strides)
     _launch("trx_attn_fwd_shared", dev, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k.data_ptr(),
             v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(slopes), _ptr(lengths), B, Sq, P, S, Hq, Hk, dp,
-            I64x3(*q.stride()[:3]), I64x2(*prefix_k.stride()[:2]), I64x2(*prefix_v.stride()[:2]),
-            I64x3(*k.stride()[:3]), I64x3(*v.stride()[:3]), I64x3(*out.stride()[:3]), scale, _code(q),
-            parts.data_ptr(), parts.numel(), ws.data_ptr(), ws.numel())
+            at, at + 24, at + 40, at + 56, at + 80, at + 104, scale, _DTYPE_CODE[dtype], parts.data_ptr(),
+            parts.numel(), ws.data_ptr(), ws.numel())
     if parts.numel():
         _count()  # the prefix is a launch of its own
     out = out if dp == d else out[..., :d].contiguous()
