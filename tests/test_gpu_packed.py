@@ -188,3 +188,32 @@ def test_long_offsets(cuda):
     got = T.attention_packed(q, k, k, cu_q, cu_k, causal=True)
     assert not got[:rows - 70].any()
     check(got[rows - 70:], None, q[rows - 70:], k, k, [70], [70], causal=True)
+
+
+@pytest.mark.parametrize("few", [True, False])
+def test_more_blocks_than_a_grid_dimension_holds(cuda, few):
+    """Blocks counted along the grid's other dimension: a few long sequences, or 70000 of a row or two."""
+    if few:
+        lens = [100, 17_000_000, 300]
+        q = torch.zeros(sum(lens), 2, 64, dtype=torch.bfloat16, device=cuda)  # 4.4 GB
+        q[:100], q[-300:] = make(28, cuda, torch.bfloat16, 100, 2, 64), make(29, cuda, torch.bfloat16, 300, 2, 64)
+        len_k = [100, 1, 300]
+        k = make(30, cuda, torch.bfloat16, sum(len_k), 2, 64)
+        out = T.attention_packed(q, k, k, starts(lens, cuda), starts(len_k, cuda))
+        check(out[:100], None, q[:100], k[:100], k[:100], [100], [100])
+        middle = out[100:-300]
+        assert bool((middle == k[100]).all())  # a single key
+        check(out[-300:], None, q[-300:], k[101:], k[101:], [300], [300])
+        return
+    lens = [1 + (i * 7919) % 2 for i in range(70_000)]
+    q = make(31, cuda, torch.bfloat16, sum(lens), 1, 64)
+    k, v = make(32, cuda, torch.bfloat16, sum(lens), 1, 64), make(33, cuda, torch.bfloat16, sum(lens), 1, 64)
+    cu = starts(lens, cuda).long()
+    for most in (None, 2):
+        out = T.attention_packed(q, k, v, cu.int(), causal=True, max_seqlen_q=most)[:, 0]
+        assert torch.equal(out[cu[:-1]], v[cu[:-1], 0])  # the first token of each sees itself
+        two = cu[:-1][cu.diff() == 2]
+        s = (q[two + 1, 0].double()[:, None] * torch.stack((k[two, 0], k[two + 1, 0]), 1).double()).sum(-1) / 8
+        want = (torch.softmax(s, -1)[..., None] * torch.stack((v[two, 0], v[two + 1, 0]), 1).double()).sum(1)
+        # one rounding of each of two probabilities and one of the result, weights far closer
+        assert float((out[two + 1].double() - want).abs().max()) <= 2.01 * 2 ** -8 * float(v.abs().max())

@@ -672,7 +672,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 w = plain_item(p, x, y, z);
               } else {
                 if constexpr (FORM == ATT_PACKED) {
-                  rest = use_table && ragged_slot(p, x, y) >= table->first[p.n_seq];
+                  // (heads run faster than slots: no block behind this one has rows either)
+                  rest = use_table && !p.slots_first && y >= table->first[p.n_seq];
                   if (use_table) cursor.look_up(p, *table, ragged_slot(p, x, y));
                   else cursor.seek_alone(p, ragged_slot(p, x, y));
                 }
