@@ -79,6 +79,29 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The sequence that a grid's z works on: of every 128, the one with the most keys first. CTAs start in the
+// order of their index, and one that starts late on many keys ends the launch late.
+template <class P>
+__device__ __forceinline__ int by_keys(const P& p, int z) {
+  __shared__ int keys[DEC_THREADS];
+  __shared__ int found;
+  const int n = P::FORM == ATT_PACKED ? p.n_cu : p.B, first = z - z % DEC_THREADS;
+  const int s = first + static_cast<int>(threadIdx.x), count = min(DEC_THREADS, n - first);
+  int own = -1;
+  if (s < n) own = P::FORM == ATT_PACKED ? ragged_key(p, s + 1) - ragged_key(p, s) : ragged_length(p, s);
+  keys[threadIdx.x] = own;
+  __syncthreads();
+  int more = 0;  // sequences in front of this thread's
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) {
+    const int k = keys[i];
+    more += k > own || (k == own && i < static_cast<int>(threadIdx.x)) ? 1 : 0;
+  }
+  if (s < n && more == z - first) found = s;
+  __syncthreads();
+  return found;
+}
+
 // Rows behind the last packed sequence: 0, LSE -inf.
 template <int D>
 __device__ __forceinline__ void zero_rest(const RaggedParams& p) {
@@ -110,7 +133,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q4 = lane & 3, rl = lane >> 2;
-  const int nsplit = gridDim.x, split = blockIdx.x, b = blockIdx.z;
+  const int nsplit = gridDim.x, split = blockIdx.x;
+  int b = blockIdx.z;
   const int group = p.group;
   const int row_tiles = (group * p.Sq + L::ROWS - 1) / L::ROWS;
   const int unit = blockIdx.y / row_tiles;
@@ -123,12 +147,16 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
       zero_rest<D>(p);
       return;
     }
+    b = by_keys(p, b);
     q0 = ragged_row(p, b);
     sq = min(max(0, ragged_row(p, b + 1) - q0), p.Sq);
     k0 = ragged_key(p, b);
     sk = max(0, ragged_key(p, b + 1) - k0);
   }
-  if constexpr (FORM == ATT_SHARED) sk = ragged_length(p, b);
+  if constexpr (FORM == ATT_SHARED) {
+    if (p.lengths) b = by_keys(p, b);
+    sk = ragged_length(p, b);
+  }
   if constexpr (FORM != ATT_BATCH) {
     if (r0 >= group * sq) return;  // the whole cluster: a shorter sequence than the longest
     shift = sk - sq;
