@@ -81,8 +81,11 @@ __device__ __forceinline__ int ragged_position(const AttnParams&, int) { return 
 // the next one's, R rows being a block's: at least as many as it has blocks, on average half a slot too
 // many, which are passed over, and found by a search in cu_q alone.
 constexpr int RAGGED_TABLE = 1024;
+// The sequences of every 128 are taken in the order of their keys, the most first: a block of many keys
+// that starts late ends the launch late.
 struct RaggedTable {
-  int first[RAGGED_TABLE + 1];  // blocks before each sequence; the last: all
+  int first[RAGGED_TABLE + 1];  // blocks before each sequence, in that order; the last: all
+  int seq[RAGGED_TABLE];        // which one it is
   int row[RAGGED_TABLE + 1], key[RAGGED_TABLE + 1];
   int warp_sum[16];
 };
@@ -152,12 +155,12 @@ struct RaggedCursor {
       if (t.first[mid] <= at) lo = mid;
       else hi = mid;
     }
-    s = lo;
     slot0 = t.first[lo];
-    q0 = t.row[lo];
-    sq = max(0, t.row[lo + 1] - q0);
-    k0 = t.key[lo];
-    sk = lo < p.n_cu ? max(0, t.key[lo + 1] - k0) : 0;
+    s = t.seq[lo];
+    q0 = t.row[s];
+    sq = max(0, t.row[s + 1] - q0);
+    k0 = t.key[s];
+    sk = s < p.n_cu ? max(0, t.key[s + 1] - k0) : 0;
   }
 };
 // The whole CTA, 512 threads of two sequences each.
@@ -165,12 +168,36 @@ __device__ __forceinline__ void ragged_fill(const RaggedParams& p, RaggedTable& 
   static_assert(RAGGED_TABLE == 2 * 512, "two sequences per thread");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = 2 * threadIdx.x;
   const int step = ATT_NQ * p.tile_tokens;
-  int row[3], blocks[2];
+  for (int e = threadIdx.x; e <= p.n_seq; e += 512) {
+    t.row[e] = ragged_row(p, e);
+    t.key[e] = ragged_key(p, min(e, p.n_cu));
+  }
+  __syncthreads();
+  auto keys_of = [&](int s) { return t.key[s + 1] - t.key[s]; };
 #pragma unroll
-  for (int e = 0; e < 3; ++e) row[e] = i + e <= p.n_seq ? ragged_row(p, i + e) : 0;
+  for (int e = 0; e < 2; ++e) {
+    const int s = i + e;
+    if (s < p.n_seq) {
+      const int own = keys_of(s), from = s - s % 128, to = min(p.n_seq, from + 128);
+      int more = from;  // sequences in front of this one
+#pragma unroll 4
+      for (int o = from; o < to; ++o) {
+        const int k = keys_of(o);
+        more += k > own || (k == own && o < s) ? 1 : 0;
+      }
+      t.seq[more] = s;
+    }
+  }
+  __syncthreads();
+  int blocks[2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    blocks[e] = i + e < p.n_seq ? (max(0, row[e + 1] - row[e]) + step - 1) / step : 0;
+  for (int e = 0; e < 2; ++e) {
+    blocks[e] = 0;
+    if (i + e < p.n_seq) {
+      const int s = t.seq[i + e];
+      blocks[e] = (max(0, t.row[s + 1] - t.row[s]) + step - 1) / step;
+    }
+  }
   const int own = blocks[0] + blocks[1];
   int sum = own;
 #pragma unroll
@@ -184,17 +211,9 @@ __device__ __forceinline__ void ragged_fill(const RaggedParams& p, RaggedTable& 
   for (int w = 0; w < warp; ++w) before += t.warp_sum[w];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    if (i + e <= p.n_seq) {
-      t.first[i + e] = before;
-      t.row[i + e] = row[e];
-      t.key[i + e] = ragged_key(p, min(i + e, p.n_cu));
-    }
+    if (i + e < p.n_seq) t.first[i + e] = before;
     before += blocks[e];
-  }
-  if (i + 2 == p.n_seq && threadIdx.x == 511) {  // a full table: its end
-    t.first[i + 2] = before;
-    t.row[i + 2] = row[2];
-    t.key[i + 2] = ragged_key(p, min(i + 2, p.n_cu));
+    if (i + e == p.n_seq - 1) t.first[p.n_seq] = before;
   }
   __syncthreads();
 }
