@@ -9,7 +9,9 @@ from .functional import flash_attn_func, triton_attn_func
 from .fusion import FastFusedRMSNormInt8, RowwiseInt8Quant, fuse, register_fusion
 from .install import install, uninstall
 from .kernels import (
+    PackedAttentionKernel,
     RowwiseInt8Kernel,
+    SharedPrefixAttentionKernel,
     TritonAttentionKernel,
     TritonFusedResidualLayerNormKernel,
     TritonFusedResidualRMSNormKernel,

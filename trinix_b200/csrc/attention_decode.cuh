@@ -405,8 +405,17 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
 #pragma unroll
   for (int w = 0; w < DEC_WARPS; ++w) whole = whole && no_result[w] == 0;
 
-  // Behind the prefix's launch this one may have started beside it: from here on its results are read.
-  if constexpr (FORM == ATT_SHARED) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Behind the prefix's launch this one may have started beside it: from here on its results are read, if
+  // it has not given up.
+  if constexpr (FORM == ATT_SHARED) {
+    if (p.parts) {
+      __shared__ int prefix_done;
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (threadIdx.x == 0) prefix_done = *reinterpret_cast<volatile unsigned int*>(p.status) == 0u;
+      __syncthreads();
+      whole = whole && prefix_done;
+    }
+  }
 
   // out[row, 4 c4 ..] = acc / l, and the row's LSE
   auto emit = [&](int r, int c4, float4 acc, float mx, float l) {

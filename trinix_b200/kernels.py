@@ -352,6 +352,50 @@ class TritonAttentionKernel:
             q, k, v)
 
 
+class PackedAttentionKernel:
+    """Attention over sequences of different lengths packed one after the other (`ops.attention_packed`).
+    The reference has no such class, its attention takes one batch of equal lengths
+    (trinix/kernels/attention_kernel.py:498-664); arguments are named as TritonAttentionKernel's.
+    Forward only, as attention is."""
+
+    @staticmethod
+    def is_available() -> bool:
+        return _available()
+
+    @staticmethod
+    def apply(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+              cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = False,
+              scale: Optional[float] = None, window_size: Optional[tuple] = None,
+              alibi_slopes: Optional[torch.Tensor] = None,
+              max_seqlen_q: Optional[int] = None) -> torch.Tensor:
+        return _run(
+            lambda a, b, c: ops.attention_packed(a, b, c, cu_seqlens_q, cu_seqlens_k, causal=causal,
+                                                 scale=scale, window=window_size,
+                                                 alibi_slopes=alibi_slopes,
+                                                 max_seqlen_q=max_seqlen_q),
+            q, k, v)
+
+
+class SharedPrefixAttentionKernel:
+    """Causal attention of a batch whose sequences begin with the same keys
+    (`ops.attention_shared_prefix`). No counterpart in the reference, where the prefix is repeated for
+    every sequence. Forward only, as attention is."""
+
+    @staticmethod
+    def is_available() -> bool:
+        return _available()
+
+    @staticmethod
+    def apply(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
+              v: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+              scale: Optional[float] = None,
+              alibi_slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return _run(
+            lambda a, pk, pv, b, c: ops.attention_shared_prefix(a, pk, pv, b, c, lengths, scale=scale,
+                                                                alibi_slopes=alibi_slopes),
+            q, prefix_k, prefix_v, k, v)
+
+
 class RowwiseInt8Kernel:
     """Per-row symmetric int8 ops. The reference has no such class; the naming follows its
     kernel-class convention so the ops are reachable the same way."""

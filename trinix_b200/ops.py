@@ -846,7 +846,12 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
         q = q.contiguous()  # the rows of the batch as one run
     out = _empty(q, (B, Sq, Hq, dp))
     lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
-    parts = _empty(q, _lib.load().trx_attn_shared_bytes(B, Sq, P, Hq, Hk, dp), dtype=torch.uint8)
+    if dev.index == torch.cuda.current_device():
+        size = _lib.load().trx_attn_shared_bytes(B, Sq, P, Hq, Hk, dp)
+    else:  # the number of parts goes by the SMs of the current device
+        with torch.cuda.device(dev):
+            size = _lib.load().trx_attn_shared_bytes(B, Sq, P, Hq, Hk, dp)
+    parts = _empty(q, size, dtype=torch.uint8)
     ws = _workspace(dev)
     _raise_if_failed("trx_attn_fwd_shared", dev)  # of an earlier launch, before more work is queued
     strides = _I64x16(*q.stride()[:3], *prefix_k.stride()[:2], *prefix_v.stride()[:2], *k.stride()[:3],
