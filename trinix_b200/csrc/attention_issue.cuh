@@ -1,4 +1,4 @@
-// Order of work of an issuing warp of attention_plain.cu, without any CUDA, so that a model on the host
+// Order of work of an issuing warp of attention_plain.cuh, without any CUDA, so that a model on the host
 // can run it too.
 //
 // The work is the sequence of one Q tile's visits over all items of the CTA. The Q K^T run one visit
@@ -23,6 +23,18 @@ struct PlainCursor {
   int lo, hi, n, item, v;
 };
 
+// With mask 1 only every second of them, the others being the other Q tile's: the two tiles then work on
+// different K and V tiles at the same time, each released by the other at once.
+struct AltCursor : PlainCursor {
+  int mask;
+};
+TRX_ISSUE bool mine(const PlainCursor& c, int v) { return v >= c.lo && v < c.hi; }
+TRX_ISSUE bool mine(const AltCursor& c, int v) {
+  return v >= c.lo && v < c.hi && ((v - c.lo) & c.mask) == 0;
+}
+TRX_ISSUE bool alternates(const PlainCursor&) { return false; }
+TRX_ISSUE bool alternates(const AltCursor& c) { return c.mask != 0; }
+
 // What the order is made of. `open` reads an item and says whether there is one; `*_there` ask without
 // waiting; waits and `pv` return false when the CTA gives up.
 template <class Open, class ItemThere, class WaitFill, class FillThere, class FreeFill, class WaitQ,
@@ -45,7 +57,7 @@ template <class... F>
 PlainSteps(F...) -> PlainSteps<F...>;
 
 // All items; false: the CTA gives up.
-template <class Steps>
+template <class Cursor = PlainCursor, class Steps>
 TRX_ISSUE bool plain_issue(Steps& s) {
   bool ok = true;
   unsigned qpar = 0;    // parity of the next Q tile
@@ -66,24 +78,24 @@ TRX_ISSUE bool plain_issue(Steps& s) {
     ok = s.pv(vf, acc);
     s_busy = false;
   };
-  auto step_qk = [&](PlainCursor& c) {
+  auto step_qk = [&](Cursor& c) {
     const int v = c.v;
     wait_fill(kf);
     if (ok && v == c.lo && c.lo < c.hi) {
       ok = s.wait_q(qpar);
       qpar ^= 1u;
     }
-    if (ok && v >= c.lo && v < c.hi) qk();
+    if (ok && mine(c, v)) qk();
     if (ok && v == c.hi - 1 && c.lo < c.hi) s.q_done();
     free_fill(kf);
     kf += v == 0 && c.n > 1 ? 1 : 2;
     if (v + 1 == c.n) kf += c.n > 1 ? 1 : 0;
     c.v = v + 1;
   };
-  auto step_pv = [&](PlainCursor& c) {
+  auto step_pv = [&](Cursor& c) {
     const int v = c.v;
     wait_fill(vf);
-    if (ok && v >= c.lo && v < c.hi) {
+    if (ok && mine(c, v)) {
       // the epilogue is done with the last O (items without keys have none: it does not wait
       // for this warp there, so they must not count)
       if (v == c.lo && keyed++ > 0) ok = s.wait_o_free(keyed & 1);
@@ -95,7 +107,7 @@ TRX_ISSUE bool plain_issue(Steps& s) {
     c.v = v + 1;
   };
 
-  PlainCursor qc, pc, nc;  // of the Q K^T, of the P V, and the next item's
+  Cursor qc, pc, nc;  // of the Q K^T, of the P V, and the next item's
   bool more = s.open(qc, 0, ok);  // there may be another item
   pc = qc;
   vf = qc.n > 1 ? 2 : qc.n;  // V(0) comes behind K(1) of its item, if there is one
@@ -114,7 +126,8 @@ TRX_ISSUE bool plain_issue(Steps& s) {
         qc = nc;
         continue;
       }
-      if (s_busy) break;
+      // the other Q tile's K is released without waiting for this one's P
+      if (s_busy && !(alternates(qc) && !mine(qc, qc.v))) break;
       // `fill_there` compares one bit of a phase count, so it answers for this fill only if the one
       // before it in its stage has been waited for. Behind the P V that need not be so: the next item's
       // K(0) shares a stage with V(n - 3), for which nothing has waited if its visit is not this Q tile's.
@@ -125,7 +138,7 @@ TRX_ISSUE bool plain_issue(Steps& s) {
       step_qk(qc);
     }
     if (!ok) break;
-    if (qc.item == pc.item && qc.v == pc.v + 1 && s_busy && pc.v > pc.lo) {
+    if (qc.item == pc.item && qc.v == pc.v + 1 && s_busy && pc.v > pc.lo && !alternates(pc)) {
       const int last = pc.hi - 3;  // of the P V visits
 #pragma unroll 1
       while (pc.v <= last) {
