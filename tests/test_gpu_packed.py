@@ -103,6 +103,26 @@ def test_several_items_per_cta(cuda, alibi):
     check(out, lse, q, k, v, lens, lens, causal=True, slopes=slopes)
 
 
+# two tiles of heads of one item, each with the K and V tiles of its own kv head (or of the same one)
+@pytest.mark.parametrize("heads,kv", [(16, 16), (4, 2), (48, 1), (20, 4), (24, 2), (6, 2), (3, 3)])
+@pytest.mark.parametrize("how", [dict(causal=True), dict(), dict(window=(30, 0)), dict(causal=True, alibi=True)],
+                         ids=str)
+def test_short_sequences_of_two_heads(cuda, heads, kv, how):
+    how = dict(how)
+    slopes = slopes_of(heads, cuda) if how.pop("alibi", False) else None
+    g = torch.Generator().manual_seed(heads)
+    most = 128 // (heads // kv)
+    len_q = torch.randint(0, most + 1, (70,), generator=g).tolist() + [most + 1, 300, 1, most]
+    len_k = [n + m for n, m in zip(len_q, torch.randint(0, 400, (74,), generator=g).tolist())]
+    dtype, dim = (torch.bfloat16, 128) if heads % 3 else (torch.float16, 64)
+    q = make(40, cuda, dtype, sum(len_q) + 9, heads, dim)
+    k, v = (make(i, cuda, dtype, sum(len_k) + 100, kv, dim) for i in (41, 42))
+    k[sum(len_k):], v[sum(len_k):] = float("nan"), float("nan")
+    out, lse = T.attention_packed(q, k, v, starts(len_q, cuda), starts(len_k, cuda), return_lse=True,
+                                  alibi_slopes=slopes, **how)
+    check(out, lse, q, k, v, len_q, len_k, slopes=slopes, **how)
+
+
 def test_many_sequences(cuda):
     """The search for a block's sequence: over 1024 of them, most of a few rows, many empty."""
     g = torch.Generator().manual_seed(3)

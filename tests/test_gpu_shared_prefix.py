@@ -64,6 +64,19 @@ def test_biases(cuda, how, Sq, dim):
     check(out, lse, q, pk, pv, k, v, lens, slopes=slopes, **how)
 
 
+@pytest.mark.parametrize("P", [129, 600, 9000, 20_000])
+@pytest.mark.parametrize("heads,kv", [(4, 4), (32, 8), (5, 1)])
+@pytest.mark.parametrize("alibi", [False, True])
+def test_one_tile_of_rows(cuda, P, heads, kv, alibi):
+    """All rows in one Q tile: the two have every second tile of a split's keys, an odd number among them."""
+    slopes = slopes_of(heads, cuda) if alibi else None
+    lens = [1, 20, 64, 5, 33]
+    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 5, 2, P, 64, heads, kv, 128, seed=45)
+    out, lse = T.attention_shared_prefix(q, pk, pv, k, v, lengths(lens, cuda), return_lse=True,
+                                         alibi_slopes=slopes)
+    check(out, lse, q, pk, pv, k, v, lens, slopes=slopes)
+
+
 @pytest.mark.parametrize("Sq,B", [(1, 100), (5, 60), (300, 12)])
 @pytest.mark.parametrize("alibi", [False, True])
 def test_many_rows(cuda, Sq, B, alibi):

@@ -30,6 +30,7 @@ enum AttnForm { ATT_BATCH = 0, ATT_PACKED = 1, ATT_SHARED = 2, ATT_PREFIX = 3 };
 
 struct AttnParams {
   static constexpr int FORM = ATT_BATCH;
+  static constexpr bool ALT = false;
   CUtensorMap tm_q;
   CUtensorMap tm_k;
   CUtensorMap tm_v;

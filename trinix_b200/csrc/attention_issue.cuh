@@ -28,10 +28,9 @@ struct PlainCursor {
 struct AltCursor : PlainCursor {
   int mask;
 };
-TRX_ISSUE bool mine(const PlainCursor& c, int v) { return v >= c.lo && v < c.hi; }
-TRX_ISSUE bool mine(const AltCursor& c, int v) {
-  return v >= c.lo && v < c.hi && ((v - c.lo) & c.mask) == 0;
-}
+// Whether visit v of [lo, hi) is this Q tile's.
+TRX_ISSUE bool mine(const PlainCursor&, int) { return true; }
+TRX_ISSUE bool mine(const AltCursor& c, int v) { return ((v - c.lo) & c.mask) == 0; }
 TRX_ISSUE bool alternates(const PlainCursor&) { return false; }
 TRX_ISSUE bool alternates(const AltCursor& c) { return c.mask != 0; }
 
@@ -85,7 +84,7 @@ TRX_ISSUE bool plain_issue(Steps& s) {
       ok = s.wait_q(qpar);
       qpar ^= 1u;
     }
-    if (ok && mine(c, v)) qk();
+    if (ok && v >= c.lo && v < c.hi && mine(c, v)) qk();
     if (ok && v == c.hi - 1 && c.lo < c.hi) s.q_done();
     free_fill(kf);
     kf += v == 0 && c.n > 1 ? 1 : 2;
@@ -95,7 +94,7 @@ TRX_ISSUE bool plain_issue(Steps& s) {
   auto step_pv = [&](Cursor& c) {
     const int v = c.v;
     wait_fill(vf);
-    if (ok && mine(c, v)) {
+    if (ok && v >= c.lo && v < c.hi && mine(c, v)) {
       // the epilogue is done with the last O (items without keys have none: it does not wait
       // for this warp there, so they must not count)
       if (v == c.lo && keyed++ > 0) ok = s.wait_o_free(keyed & 1);
@@ -127,7 +126,7 @@ TRX_ISSUE bool plain_issue(Steps& s) {
         continue;
       }
       // the other Q tile's K is released without waiting for this one's P
-      if (s_busy && !(alternates(qc) && !mine(qc, qc.v))) break;
+      if (s_busy && !(alternates(qc) && (qc.v < qc.lo || qc.v >= qc.hi || !mine(qc, qc.v)))) break;
       // `fill_there` compares one bit of a phase count, so it answers for this fill only if the one
       // before it in its stage has been waited for. Behind the P V that need not be so: the next item's
       // K(0) shares a stage with V(n - 3), for which nothing has waited if its visit is not this Q tile's.

@@ -7,17 +7,17 @@ namespace trx {
 
 using PackedParams = RaggedParamsOf<ATT_PACKED>;
 
-template <int D, bool BF16, int BIAS, bool SINGLE>
-static int launch_packed(const PackedParams& p, dim3 grid, cudaStream_t stream) {
-  const int rc = configure_plain<D, BF16, BIAS, SINGLE, PackedParams>();
+template <int D, bool BF16, int BIAS, bool SINGLE, class P>
+static int launch_packed(const P& p, dim3 grid, cudaStream_t stream) {
+  const int rc = configure_plain<D, BF16, BIAS, SINGLE, P>();
   if (rc != TRX_OK) return rc;
-  attn_plain_kernel<D, BF16, BIAS, SINGLE, PackedParams>
-      <<<grid, AP_THREADS, plain_smem_bytes<D, SINGLE, PackedParams>(), stream>>>(p);
+  attn_plain_kernel<D, BF16, BIAS, SINGLE, P>
+      <<<grid, AP_THREADS, plain_smem_bytes<D, SINGLE, P>(), stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
 }
 
-template <int D, bool BF16, bool SINGLE>
-static int launch_packed_bias(const PackedParams& p, dim3 grid, cudaStream_t stream) {
+template <int D, bool BF16, bool SINGLE, class P>
+static int launch_packed_bias(const P& p, dim3 grid, cudaStream_t stream) {
   if (!(p.scale_log2 > 0.0f)) return launch_packed<D, BF16, AP_GENERAL, SINGLE>(p, grid, stream);
   if (!p.slopes) return launch_packed<D, BF16, AP_NONE, SINGLE>(p, grid, stream);
   // under a causal mask, or a window that ends at the query, every visible key is at or before it
@@ -26,10 +26,22 @@ static int launch_packed_bias(const PackedParams& p, dim3 grid, cudaStream_t str
 }
 
 template <int D, bool BF16>
-static int launch_packed_items(const PackedParams& p, dim3 grid, cudaStream_t stream) {
-  return static_cast<int64_t>(grid.x) * grid.y <= sm_count_of_current_device()
-             ? launch_packed_bias<D, BF16, true>(p, grid, stream)
-             : launch_packed_bias<D, BF16, false>(p, grid, stream);
+static int launch_packed_items(PackedParams& p, cudaStream_t stream) {
+  // slots: see RaggedCursor
+  const int64_t slots = p.rows / (ATT_NQ * p.tile_tokens) + static_cast<int64_t>(p.n_seq);
+  p.slots_first = slots > 65535 ? 1 : 0;
+  const unsigned heads = p.head_tiles, n = static_cast<unsigned>(slots);
+  const dim3 grid = p.slots_first ? dim3(n, heads) : dim3(heads, n);
+  if (slots * heads <= sm_count_of_current_device()) return launch_packed_bias<D, BF16, true>(p, grid, stream);
+  if (p.n_seq > RAGGED_TABLE) return launch_packed_bias<D, BF16, false>(p, grid, stream);
+  if (slots * heads >= (1ll << 31)) return TRX_ERR_SHAPE;
+  // sequences that fit one Q tile take two tiles of heads at a time, where they are most of the sequences
+  if (heads % 2 == 0 && static_cast<int64_t>(p.n_cu) * p.tile_tokens >= p.rows) {
+    RaggedParamsOf<ATT_PACKED, true> alt;
+    static_cast<RaggedParams&>(alt) = p;
+    return launch_packed_bias<D, BF16, false>(alt, dim3(n * heads), stream);
+  }
+  return launch_packed_bias<D, BF16, false>(p, dim3(n * heads), stream);
 }
 
 }  // namespace trx
@@ -111,11 +123,7 @@ extern "C" int trx_attn_fwd_packed(const void* q, const void* k, const void* v, 
     p.Sk = static_cast<int>((Tk + n_seq - 1) / n_seq);
     return launch_decode_rows(p, D, s);
   }
-  const int64_t slots = Tq / (ATT_NQ * p.tile_tokens) + p.n_seq, heads = Hq / p.tile_heads;
-  p.slots_first = slots > 65535 ? 1 : 0;
-  const dim3 grid = p.slots_first ? dim3(static_cast<unsigned>(slots), static_cast<unsigned>(heads))
-                                  : dim3(static_cast<unsigned>(heads), static_cast<unsigned>(slots));
   if (D == 128)
-    return is_bf16 ? launch_packed_items<128, true>(p, grid, s) : launch_packed_items<128, false>(p, grid, s);
-  return is_bf16 ? launch_packed_items<64, true>(p, grid, s) : launch_packed_items<64, false>(p, grid, s);
+    return is_bf16 ? launch_packed_items<128, true>(p, s) : launch_packed_items<128, false>(p, s);
+  return is_bf16 ? launch_packed_items<64, true>(p, s) : launch_packed_items<64, false>(p, s);
 }

@@ -328,6 +328,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     attn_plain_kernel(const __grid_constant__ P p) {
   using L = PlainSmem<D>;
   constexpr int FORM = P::FORM;
+  constexpr bool ALT = P::ALT;
+  constexpr bool TWO_HEADS = ALT && FORM == ATT_PACKED, HALVES = ALT && FORM == ATT_PREFIX;
   using Work = std::conditional_t<FORM == ATT_BATCH, PlainItem, RaggedItem>;
   static_assert(sizeof(Work) <= 64, "shared memory slot");
   constexpr int STAGES = AP_STAGES, BN = ATT_BN;
@@ -395,18 +397,24 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     const int s = g % STAGES;
     const bool is_k = fill == 0 || ((fill & 1) != 0 && fill != 2 * w.n - 1);
     const int v = is_k ? (fill + 1) >> 1 : fill == 2 * w.n - 1 ? w.n - 1 : (fill >> 1) - 1;
-    const int j = w.first + v * kv_step;
+    int second = 0, visit = v;  // whether it is of the item's second tile of heads
+    if constexpr (TWO_HEADS) {
+      second = v & w.alt;
+      visit = v >> w.alt;
+    }
+    const int j = w.first + visit * kv_step;
     if constexpr (FORM == ATT_BATCH) mbar_expect_tx(bar(B_KVFULL + s), L::TILE_BYTES);
     fills_issued[s] = g / STAGES + 1;
     const uint32_t dst = sbase + L::KV_OFF + s * L::TILE_BYTES;
-    const int hh = is_k ? kh : vh;
     if constexpr (FORM == ATT_BATCH) {
+      const int hh = is_k ? kh : vh;
       const CUtensorMap* tm = is_k ? &p.tm_k : &p.tm_v;
       const int bb = w.b * (is_k ? p.k_bmul : p.v_bmul);
 #pragma unroll
       for (int c = 0; c < L::CHUNKS; ++c)
         tma_load_4d(dst + c * L::CHUNK_BYTES, tm, bar(B_KVFULL + s), c * 64, j * BN, hh, bb);
     } else {
+      const int hh = second ? vh : kh;
       const RaggedTile r = ragged_tile<BN>(p, w, j);
       const CUtensorMap* tm = r.prefix ? (is_k ? &p.tm_pk : &p.tm_pv) : (is_k ? &p.tm_k : &p.tm_v);
       const uint32_t full = bar((!is_k && r.edge ? B_RAW : B_KVFULL) + s);
@@ -425,7 +433,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       kh = w.h / p.k_hdiv;
       vh = p.v_hdiv == p.k_hdiv ? kh : w.h / p.v_hdiv;
     } else {
-      kh = vh = w.h / p.group;
+      kh = w.h / p.group;
+      vh = TWO_HEADS ? (w.h + p.tile_heads) / p.group : kh;  // of an item's second tile of heads
     }
   };
   auto issue_q = [&](const Work& w, int t) {
@@ -437,8 +446,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       if constexpr (FORM == ATT_BATCH)
         tma_load_4d(dst, &p.tm_q, bar(B_QFULL + t), c * 64, w.m0 + t * t_rows, w.h + t * t_head, w.b);
       else
-        tma_load_5d(dst, &p.tm_q, bar(B_QFULL + t), c * 64, 0, w.q0 + w.m0 + t * t_rows,
-                    w.h / p.tile_heads, FORM == ATT_SHARED ? w.b : 0);
+        tma_load_5d(dst, &p.tm_q, bar(B_QFULL + t), c * 64, 0, w.q0 + w.m0 + (ALT && w.alt ? 0 : t * t_rows),
+                    w.h / p.tile_heads + (TWO_HEADS ? t * w.alt : 0), FORM == ATT_SHARED ? w.b : 0);
     }
   };
   auto publish = [&](const Work& w, int q) {  // item q, for the other roles
@@ -449,6 +458,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         o.q0 = w.q0;
         o.sq = w.sq;
         o.sk = w.sk;
+        if (ALT) o.alt = w.alt;
       }
       o.b = w.b;
       o.h = w.h;
@@ -473,14 +483,18 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   if constexpr (FORM == ATT_PACKED) {
     use_table = !SINGLE && p.n_seq <= RAGGED_TABLE;
     if (use_table) {
-      ragged_fill(p, *table);
-      // blocks behind the last one with rows, if it is that late that they are launched at all
-      if (ragged_slot(p, blockIdx.x, blockIdx.y) >= table->first[p.n_seq]) return;
+      ragged_fill<ALT>(p, *table);
+      // blocks behind the last item, if it is that late that they are launched at all
+      if (static_cast<int>(blockIdx.x) >= table->first[p.n_seq]) return;
     }
     if (warp == 12) {
-      if (use_table) cursor.look_up(p, *table, ragged_slot(p, blockIdx.x, blockIdx.y));
-      else cursor.seek(p, ragged_slot(p, blockIdx.x, blockIdx.y), lane);
-      first_item = ragged_item(p, cursor, blockIdx.x, blockIdx.y, 0);
+      if (use_table) {
+        cursor.template look_up<ALT>(p, *table, blockIdx.x);
+      } else {
+        cursor.seek(p, ragged_slot(p, blockIdx.x, blockIdx.y), lane);
+        cursor.head = ragged_head(p, blockIdx.x, blockIdx.y);
+      }
+      first_item = ragged_item(p, cursor, 0, 0, 0);
     }
   } else if constexpr (FORM != ATT_BATCH) {
     if (warp == 12) first_item = ragged_item(p, cursor, blockIdx.x, blockIdx.y, blockIdx.z);
@@ -672,10 +686,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 w = plain_item(p, x, y, z);
               } else {
                 if constexpr (FORM == ATT_PACKED) {
-                  // (heads run faster than slots: no block behind this one has rows either)
-                  rest = use_table && !p.slots_first && y >= table->first[p.n_seq];
-                  if (use_table) cursor.look_up(p, *table, ragged_slot(p, x, y));
-                  else cursor.seek_alone(p, ragged_slot(p, x, y));
+                  rest = use_table && x >= table->first[p.n_seq];  // as is every block behind it
+                  if (use_table) {
+                    cursor.template look_up<ALT>(p, *table, x);
+                  } else {
+                    cursor.seek_alone(p, ragged_slot(p, x, y));
+                    cursor.head = ragged_head(p, x, y);
+                  }
                 }
                 w = ragged_item(p, cursor, x, y, z);
               }
@@ -802,7 +819,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       };
       // Values that are the same in every lane, in a way the compiler knows.
       auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };
-      auto open = [&](PlainCursor& c, int item, bool& ok) -> bool {  // false: there is no such item
+      using Cursor = std::conditional_t<ALT, AltCursor, PlainCursor>;
+      auto open = [&](Cursor& c, int item, bool& ok) -> bool {  // false: there is no such item
         if (SINGLE && item > 0) return false;
         ok = wait(B_ITEM + (item & 1), (item >> 1) & 1);
         if (!ok) return false;
@@ -814,6 +832,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           c.n = uniform(w.n);
           c.item = item;
           c.v = 0;
+          if constexpr (ALT) c.mask = uniform(w.alt);
         }
         item_read(item);
         return valid;
@@ -831,7 +850,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           [&](uint32_t parity) { return wait(B_OFREE + t, parity); },
           pv,
           [&] { commit(B_ODONE + t); }};
-      const bool ok = plain_issue(steps);
+      const bool ok = plain_issue<Cursor>(steps);
       if (!ok && elect_one()) {
         // drain whatever was issued before giving up: a commit follows the MMAs of its own thread, and
         // which lane elect.sync takes is not specified
@@ -877,7 +896,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     struct Item {
       int q, b, h, m0;
       bool any0, any1;  // whether a Q tile has a key
-      int q0, sq;       // of the sequence
+      int q0, sq, alt;  // of a ragged item
     };
     auto finish = [&](const Item& w) -> bool {  // O and the row statistics of an item to global memory
       bool ok = true;
@@ -891,19 +910,22 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         }
         if (!ok) break;
         const float* stat = reinterpret_cast<const float*>(smem + L::STAT_OFF) + t * 2 * ATT_BM;
-        int hq = w.h + t * t_head, row = w.m0 + t * t_rows;
+        int hq = w.h + t * t_head, row = w.m0 + t * t_rows, b = w.b;
         bool live;
         if constexpr (FORM == ATT_BATCH) {
           row += r;
           live = row < p.Sq;
         } else {
           const int tok = r / p.tile_heads;
+          if (ALT && w.alt) row = w.m0;
           row += tok;
           hq += r - tok * p.tile_heads;
+          if (TWO_HEADS && w.alt) hq += t * p.tile_heads;
+          if (HALVES) b = 2 * w.b + t;  // parts of their own
           live = tok < t_rows && row < w.sq;
           row += w.q0;
         }
-        store_rows(t, any, stat[r], stat[ATT_BM + r], w.b, hq, row, live,
+        store_rows(t, any, stat[r], stat[ATT_BM + r], b, hq, row, live,
                    [&] {  // O and the statistics are read: the next item may write them
                      tc_fence_before();
                      __syncwarp();
@@ -924,6 +946,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       if constexpr (FORM != ATT_BATCH) {
         it.q0 = w.q0;
         it.sq = w.sq;
+        if (ALT) it.alt = w.alt;
       }
       it.q = q;
       it.b = w.b;
@@ -957,8 +980,12 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       volatile Work& w = items[q & 1];
       const bool valid = w.valid != 0;
       int row0 = w.m0 + t * t_rows;           // key position of the tile's first query
-      const int lo = w.lo[t], n_it = w.hi[t] - lo;
+      const int lo = w.lo[t], visits = w.hi[t] - lo;
+      int alt = 0;
+      if constexpr (ALT) alt = w.alt;
+      const int n_it = (visits + alt) >> alt;
       int c0 = (w.first + lo * kv_step) * BN;  // first key of the visit
+      if (TWO_HEADS && alt) c0 = w.first * BN;
       float slope2 = 0.0f;
       int row, row1, hi_i;                    // position of this row and of the tile's last; last key
       if constexpr (FORM == ATT_BATCH) {
@@ -969,8 +996,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         hi_i = p.Sk - 1;
       } else {
         const int tok = min(rl / p.tile_heads, t_rows - 1);
+        if (alt) row0 = w.m0;
         if (BIAS != AP_NONE && valid && p.slopes)
-          slope2 = p.slopes[w.h + rl % p.tile_heads] * 1.4426950408889634f;
+          slope2 = p.slopes[w.h + (TWO_HEADS && alt ? t * p.tile_heads : 0) + rl % p.tile_heads] *
+                   1.4426950408889634f;
         row1 = min(w.sq, row0 + t_rows) - 1;
         row = row0 + tok;
         if (FORM == ATT_PREFIX && valid) row = ragged_position(p, min(row, w.sq - 1));
@@ -1035,7 +1064,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         if (turn <= 0) turn = -1;
       }
 #pragma unroll 1
-      for (int itn = 0; itn < n_it; ++itn, c0 += kv_step * BN) {
+      for (int itn = 0; itn < n_it; ++itn, c0 += HALVES ? 2 * kv_step * BN : kv_step * BN) {
         if (FORM == ATT_SHARED && itn == turn) enter(kv_step < 0);
         ok = wait(B_SFULL + t, s_par);
         if (!ok) break;

@@ -15,6 +15,13 @@
 // most 128 rows. All heads of a group share a tile, so a short sequence fills it with heads where a tile of
 // one head would be padding, and a CTA's two tiles see almost the same keys.
 //
+// Where one Q tile holds all the rows, the CTA's two tiles take every second K and V tile each (`alt` of an
+// item), so that one tile's softmax runs under the other's MMAs: a packed sequence of up to `tile_tokens`
+// rows with two tiles of heads, a run of that few rows against a prefix with two halves of its keys. Such
+// launches have instantiations of their own (ALT): the test in the issuing warps' loop costs the others 3 to
+// 5 % (16 prompts of 32 to 2048 rows 111 us, so 114; 16 x 512, 32 / 8 heads x 128 93, so 97; of ALT, 64 x
+// 128, 16 heads x 64 36.9, so 28.6; 64 x 32, 32 / 8 heads x 128 31, so 25).
+//
 // Key tiles are not cut to a sequence: what follows its last key in memory belongs to another one, or is
 // stale, and may be NaN. Scores there are masked as any others; in V, where a probability of 0 would not
 // hide it (0 * NaN), the rows behind the last key are zeroed in shared memory (attention_plain.cuh).
@@ -33,7 +40,8 @@ struct RaggedParams : AttnParams {
   int n_seq;                 // and one more, without keys, if rows behind the last are to be zeroed
   int rows, keys;            // of the whole packed q and k / v; shared: keys a sequence's cache holds
   int tile_heads, tile_tokens;
-  int slots_first;           // packed: the grid's x counts slots (and not heads)
+  int head_tiles;            // query heads / tile_heads
+  int slots_first;           // packed without a table: the grid's x counts slots (and not heads)
   int seq;                   // shared: queries per sequence
   int prefix, prefix_tiles;  // keys of the prefix, in KV tiles
   int split_tiles;           // KV tiles of one split of the prefix
@@ -41,13 +49,15 @@ struct RaggedParams : AttnParams {
   const float* part_lse;     // and their row sums' log2, [parts][B * Sq][Hq]
   int parts;
 };
-template <int F>
+template <int F, bool A = false>
 struct RaggedParamsOf : RaggedParams {
   static constexpr int FORM = F;
+  static constexpr bool ALT = A;
 };
 
 struct RaggedItem : PlainItem {
   int q0, sq, k0, sk;  // first row and rows, first key and keys of the item's sequence
+  int alt;             // 1: visit v is Q tile v & 1's alone
 };
 
 __device__ __forceinline__ int ragged_tokens(const RaggedParams& p) { return p.tile_tokens; }
@@ -76,43 +86,48 @@ __device__ __forceinline__ int ragged_position(const AttnParams&, int) { return 
 
 // Packed rows: which sequence a block works on. The host knows the rows and the number of sequences but not
 // where they end, and a table of blocks would cost a launch in front. A launch of several items per CTA with
-// up to RAGGED_TABLE sequences counts every sequence's blocks in shared memory when a CTA starts, and finds
-// a block by bisection there. Otherwise each sequence has the slots from floor(first row / R) + its index to
+// up to RAGGED_TABLE sequences counts every sequence's items (blocks of rows times tiles of heads, or pairs
+// of these) in shared memory when a CTA starts, and finds an item by bisection there. Otherwise the grid is
+// tiles of heads times slots: each sequence has the slots from floor(first row / R) + its index to
 // the next one's, R rows being a block's: at least as many as it has blocks, on average half a slot too
 // many, which are passed over, and found by a search in cu_q alone.
 constexpr int RAGGED_TABLE = 1024;
 // The sequences of every 128 are taken in the order of their keys, the most first: a block of many keys
 // that starts late ends the launch late.
 struct RaggedTable {
-  int first[RAGGED_TABLE + 1];  // blocks before each sequence, in that order; the last: all
+  int first[RAGGED_TABLE + 1];  // items before each sequence, in that order; the last: all
   int seq[RAGGED_TABLE];        // which one it is
   int row[RAGGED_TABLE + 1], key[RAGGED_TABLE + 1];
   int warp_sum[16];
 };
 
+// Whether a sequence of sq rows has its tiles of heads (an even number of them) in pairs.
+template <bool ALT>
+__device__ __forceinline__ bool ragged_pairs(const RaggedParams& p, int sq) {
+  return ALT && sq <= p.tile_tokens;
+}
+
 struct RaggedCursor {
-  int s, slot, slot0, next;  // sequence, the slot looked for, first slots of this and the next sequence
-  int q0, sq, k0, sk;
+  int q0, sq, k0, sk;  // of the sequence
+  int block, head;     // of its blocks of rows; tile of heads
+  int alt;             // and the next tile of heads
 
   static __device__ __forceinline__ int first_slot(const RaggedParams& p, int i) {
     return ragged_row(p, i) / (ATT_NQ * p.tile_tokens) + i;
   }
-  __device__ __forceinline__ void load(const RaggedParams& p) {
-    const int step = ATT_NQ * p.tile_tokens;
+  __device__ __forceinline__ void load(const RaggedParams& p, int s, int slot) {
     q0 = ragged_row(p, s);
-    const int q1 = ragged_row(p, s + 1);
-    slot0 = q0 / step + s;
-    next = q1 / step + s + 1;
-    sq = max(0, q1 - q0);
+    sq = max(0, ragged_row(p, s + 1) - q0);
     k0 = sk = 0;
     if (s < p.n_cu) {
       k0 = ragged_key(p, s);
       sk = max(0, ragged_key(p, s + 1) - k0);
     }
+    block = slot - (q0 / (ATT_NQ * p.tile_tokens) + s);
+    alt = 0;
   }
   // The last sequence whose first slot is not behind `at`; a whole warp, 32 probes at a time.
   __device__ __forceinline__ void seek(const RaggedParams& p, int at, int lane) {
-    slot = at;
     int lo = 0, hi = p.n_seq;
 #pragma unroll 1
     while (hi - lo > 1) {
@@ -122,13 +137,11 @@ struct RaggedCursor {
       lo += max(0, n - 1) * step;
       hi = min(hi, lo + step);
     }
-    s = lo;
-    load(p);
+    load(p, lo, at);
   }
   // The same by one thread: 15 probes at a time, whose loads are in flight together where a bisection
   // waits for each.
   __device__ __forceinline__ void seek_alone(const RaggedParams& p, int at) {
-    slot = at;
     constexpr int N = 15;
     int lo = 0, hi = p.n_seq;
 #pragma unroll 1
@@ -143,11 +156,10 @@ struct RaggedCursor {
       lo += n * step;
       if (n < N) hi = min(hi, lo + step);
     }
-    s = lo;
-    load(p);
+    load(p, lo, at);
   }
+  template <bool ALT>
   __device__ __forceinline__ void look_up(const RaggedParams& p, const RaggedTable& t, int at) {
-    slot = at;
     int lo = 0, hi = p.n_seq;
 #pragma unroll 1
     while (hi - lo > 1) {
@@ -155,15 +167,19 @@ struct RaggedCursor {
       if (t.first[mid] <= at) lo = mid;
       else hi = mid;
     }
-    slot0 = t.first[lo];
-    s = t.seq[lo];
+    const int s = t.seq[lo], i = at - t.first[lo];
     q0 = t.row[s];
     sq = max(0, t.row[s + 1] - q0);
     k0 = t.key[s];
     sk = s < p.n_cu ? max(0, t.key[s + 1] - k0) : 0;
+    alt = ragged_pairs<ALT>(p, sq) ? 1 : 0;
+    const int heads = p.head_tiles >> alt;
+    block = i / heads;
+    head = (i - block * heads) << alt;
   }
 };
 // The whole CTA, 512 threads of two sequences each.
+template <bool ALT>
 __device__ __forceinline__ void ragged_fill(const RaggedParams& p, RaggedTable& t) {
   static_assert(RAGGED_TABLE == 2 * 512, "two sequences per thread");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = 2 * threadIdx.x;
@@ -195,7 +211,8 @@ __device__ __forceinline__ void ragged_fill(const RaggedParams& p, RaggedTable& 
     blocks[e] = 0;
     if (i + e < p.n_seq) {
       const int s = t.seq[i + e];
-      blocks[e] = (max(0, t.row[s + 1] - t.row[s]) + step - 1) / step;
+      const int rows = max(0, t.row[s + 1] - t.row[s]);
+      blocks[e] = (rows + step - 1) / step * (ragged_pairs<ALT>(p, rows) ? p.head_tiles / 2 : p.head_tiles);
     }
   }
   const int own = blocks[0] + blocks[1];
@@ -218,8 +235,12 @@ __device__ __forceinline__ void ragged_fill(const RaggedParams& p, RaggedTable& 
   __syncthreads();
 }
 
+// The cursor of a block of the grid without a table.
 __device__ __forceinline__ int ragged_slot(const RaggedParams& p, int x, int y) {
   return p.slots_first ? x : y;
+}
+__device__ __forceinline__ int ragged_head(const RaggedParams& p, int x, int y) {
+  return p.slots_first ? y : x;
 }
 __device__ __forceinline__ bool ragged_has_rows(const RaggedItem& w) { return w.sq > 0; }
 __device__ __forceinline__ bool ragged_has_rows(const PlainItem&) { return true; }
@@ -251,37 +272,40 @@ __device__ __forceinline__ TileRange ragged_range(const RaggedParams& p, const R
   return r;
 }
 
-template <int FORM>
-__device__ __forceinline__ RaggedItem ragged_item(const RaggedParamsOf<FORM>& p, const RaggedCursor& c,
+template <int FORM, bool ALT>
+__device__ __forceinline__ RaggedItem ragged_item(const RaggedParamsOf<FORM, ALT>& p, const RaggedCursor& c,
                                                   int x, int y, int z) {
   RaggedItem w;
   const int step = ATT_NQ * p.tile_tokens;
   w.valid = 1;
-  w.h = (FORM == ATT_PACKED && p.slots_first ? y : x) * p.tile_heads;
   if constexpr (FORM == ATT_PACKED) {
     w.b = 0;
+    w.h = c.head * p.tile_heads;
     w.q0 = c.q0;
     w.sq = c.sq;
     w.k0 = c.k0;
     w.sk = c.sk;
-    const int blocks = (c.sq + step - 1) / step, i = c.slot - c.slot0;
-    if (i < 0 || i >= blocks) {  // the slot holds no rows
+    w.alt = ALT ? c.alt : 0;
+    const int blocks = (c.sq + step - 1) / step;
+    if (c.block < 0 || c.block >= blocks) {  // the slot holds no rows
       w.sq = w.m0 = 0;
     } else {
-      w.m0 = (p.causal ? blocks - 1 - i : i) * step;  // heaviest first
+      w.m0 = (p.causal ? blocks - 1 - c.block : c.block) * step;  // heaviest first
     }
   } else {
     w.b = z;  // sequence, or split of the prefix
+    w.h = x * p.tile_heads;
     w.q0 = w.k0 = 0;
     w.sq = FORM == ATT_SHARED ? p.seq : p.rows;
     w.sk = FORM == ATT_SHARED ? ragged_length(p, z) : 0;
+    w.alt = ALT ? 1 : 0;
     w.m0 = static_cast<int>(gridDim.y - 1 - y) * step;
   }
   TileRange r[ATT_NQ];
   int jlo = 1 << 30, jhi = 0;
 #pragma unroll
   for (int t = 0; t < ATT_NQ; ++t) {
-    r[t] = ragged_range<FORM>(p, w, w.m0 + t * p.tile_tokens);
+    r[t] = ragged_range<FORM>(p, w, w.m0 + (w.alt ? 0 : t * p.tile_tokens));
     if (r[t].jhi > r[t].jlo) {
       jlo = min(jlo, r[t].jlo);
       jhi = max(jhi, r[t].jhi);
@@ -295,6 +319,15 @@ __device__ __forceinline__ RaggedItem ragged_item(const RaggedParamsOf<FORM>& p,
     w.lo[t] = !any ? 0 : p.reverse_kv ? jhi - r[t].jhi : r[t].jlo - jlo;
     w.hi[t] = !any ? 0 : w.lo[t] + r[t].jhi - r[t].jlo;
   }
+  if (ALT && w.alt) {  // both have the same range: every second visit each
+    if (FORM == ATT_PACKED) w.n *= 2;  // (of two heads)
+#pragma unroll
+    for (int t = 0; t < ATT_NQ; ++t) {
+      const int own = (w.n - t + 1) / 2;
+      w.lo[t] = own > 0 ? t : 0;
+      w.hi[t] = own > 0 ? t + 2 * own - 1 : 0;
+    }
+  }
   return w;
 }
 
@@ -304,8 +337,8 @@ struct RaggedTile {
   int row, b, rows;
   bool prefix, edge;
 };
-template <int BN, int FORM>
-__device__ __forceinline__ RaggedTile ragged_tile(const RaggedParamsOf<FORM>& p, const RaggedItem& w, int j) {
+template <int BN, int FORM, bool ALT>
+__device__ __forceinline__ RaggedTile ragged_tile(const RaggedParamsOf<FORM, ALT>& p, const RaggedItem& w, int j) {
   RaggedTile r;
   r.prefix = FORM == ATT_PREFIX || (FORM == ATT_SHARED && j < p.prefix_tiles);
   const int first = (FORM == ATT_SHARED && !r.prefix ? j - p.prefix_tiles : j) * BN;
@@ -349,11 +382,12 @@ inline int make_ragged_q_map(CUtensorMap* tm, const void* base, int is_bf16, int
 
 // Query heads of one tile, and tokens: as many heads of the group as leave at most a tenth of a tile's 128
 // rows unused. (A group of 71 heads is none but 1 and 71, and 71 would leave 57 rows.)
-inline void choose_tile(RaggedParams& p) {
+inline void choose_tile(RaggedParams& p) {  // from its Hq and group
   p.tile_heads = 1;
   for (int h = 2; h <= p.group && h <= ATT_BM; ++h)
     if (p.group % h == 0 && ATT_BM / h * h * 10 >= ATT_BM * 9) p.tile_heads = h;
   p.tile_tokens = ATT_BM / p.tile_heads;
+  p.head_tiles = p.Hq / p.tile_heads;
 }
 
 }  // namespace trx

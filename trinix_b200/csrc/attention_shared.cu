@@ -13,6 +13,7 @@ namespace trx {
 
 using SharedParams = RaggedParamsOf<ATT_SHARED>;
 using PrefixParams = RaggedParamsOf<ATT_PREFIX>;
+using HalvesParams = RaggedParamsOf<ATT_PREFIX, true>;
 
 template <int D, bool BF16, int BIAS, bool SINGLE, class P>
 static int launch_form(const P& p, dim3 grid, cudaStream_t stream) {
@@ -38,12 +39,15 @@ static int launch_form_rows(const P& p, int64_t D, dim3 grid, cudaStream_t s) {
 }
 
 struct SharedPlan {
-  RaggedParams tile;  // tile_heads, tile_tokens
+  RaggedParams tile;  // tile_heads, tile_tokens, head_tiles
   bool few;
-  int parts, split_tiles;  // of the prefix, with few rows
+  int splits, split_tiles;  // of the prefix, with few rows
+  bool halves;              // one Q tile holds all rows, and the two have halves of a split's keys
+  int parts;                // results of the splits, or halves
 };
 static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int64_t Hk) {
   SharedPlan s{};
+  s.tile.Hq = static_cast<int>(Hq);
   s.tile.group = static_cast<int>(Hq / Hk);
   choose_tile(s.tile);
   const int64_t row_tiles = (s.tile.group * Sq + 15) / 16;
@@ -55,7 +59,9 @@ static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int6
   int64_t parts = sm_count_of_current_device() / items;
   parts = parts < 1 ? 1 : parts > tiles ? tiles : parts;
   s.split_tiles = static_cast<int>((tiles + parts - 1) / parts);
-  s.parts = static_cast<int>((tiles + s.split_tiles - 1) / s.split_tiles);
+  s.splits = static_cast<int>((tiles + s.split_tiles - 1) / s.split_tiles);
+  s.halves = B * Sq <= s.tile.tile_tokens && s.split_tiles > 1;
+  s.parts = s.halves ? 2 * s.splits : s.splits;
   return s;
 }
 
@@ -130,6 +136,7 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   if (rc != TRX_OK) return rc;
   p.tile_heads = heads;
   p.tile_tokens = tokens;
+  p.head_tiles = plan.tile.head_tiles;
   p.group = plan.tile.group;
   p.k_hdiv = p.v_hdiv = p.group;
   p.k_bmul = p.v_bmul = 1;
@@ -171,10 +178,16 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
     p.part_o = static_cast<float*>(parts);
     p.part_lse = f.lse;
     p.parts = plan.parts;
-    grid.z = plan.parts;
+    grid.z = plan.splits;
     // the decode kernel beside the prefix's, where all of that one's CTAs are running
     beside = static_cast<int64_t>(grid.x) * grid.y * grid.z <= sm_count_of_current_device();
-    rc = launch_form_rows(f, D, grid, s);
+    if (plan.halves) {
+      HalvesParams two;
+      static_cast<RaggedParams&>(two) = f;
+      rc = launch_form_rows(two, D, grid, s);
+    } else {
+      rc = launch_form_rows(f, D, grid, s);
+    }
     if (rc != TRX_OK) return rc;
   }
   p.out = out;
