@@ -413,13 +413,16 @@ int trx_attn_fwd_packed(const void* q, const void* k, const void* v, void* out, 
  * keys of the concatenation this is causal attention of trx_attn_fwd_packed: query i stands at
  * P + lengths[b] - Sq + i and sees the keys up to there; slopes_or_null (ALiBi) counts from there.
  * scale > 0. lse_or_null: fp32 (B, Hq, Sq).
- * With few rows (Sq <= 16) the prefix is read and computed once for all sequences, its keys split over the
- * GPU; the splits' results need `parts`: trx_attn_shared_bytes(...) bytes of device memory, 16-byte aligned
- * (0: none, parts may be NULL), contents on entry irrelevant, nothing kept between calls.
+ * With few rows to a sequence, or a long prefix, the prefix is read and computed once for all sequences, its
+ * keys split over the GPU (a choice by sizes alone); the splits' results need `parts`:
+ * trx_attn_shared_bytes(...) bytes of device memory, asked for with the call's device current, 16-byte
+ * aligned (0: none, parts may be NULL), contents on entry irrelevant, nothing kept between calls. It wants
+ * the batch's rows evenly spaced (q_strides[0] == Sq * q_strides[1]); others take one pass, whatever it costs.
  * `workspace` as for trx_attn_fwd. No counterpart in the reference, whose attention takes one batch
  * (trinix/kernels/attention_kernel.py:498-664) and has the prefix repeated for every sequence.
  */
-size_t trx_attn_shared_bytes(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int64_t Hk, int64_t D);
+size_t trx_attn_shared_bytes(int64_t B, int64_t Sq, int64_t P, int64_t S, int64_t Hq, int64_t Hk,
+                             int64_t D);
 int trx_attn_fwd_shared(const void* q, const void* prefix_k, const void* prefix_v, const void* k,
                         const void* v, void* out, float* lse_or_null, const float* slopes_or_null,
                         const int32_t* lengths_or_null, int64_t B, int64_t Sq, int64_t P, int64_t S,

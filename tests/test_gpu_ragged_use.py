@@ -22,8 +22,8 @@ def run_packed(s, **how):
     return T.attention_packed(*s, causal=True, return_lse=True, **how)
 
 
-def shared_state(dev, seed, Sq=1, lens=(30, 200, 77)):
-    return (*inputs(dev, torch.bfloat16, len(lens), Sq, 900, 200, 8, 2, 128, seed=seed), lengths(lens, dev))
+def shared_state(dev, seed, Sq=1, P=6000, lens=(30, 200, 77)):
+    return (*inputs(dev, torch.bfloat16, len(lens), Sq, P, 200, 8, 2, 128, seed=seed), lengths(lens, dev))
 
 
 def run_shared(s):
@@ -36,9 +36,17 @@ KINDS = {
     "packed, many items": (lambda d, s: packed_state(d, s, [500, 30] * 20, [0, 300] * 20), run_packed),
     "packed, few rows": (lambda d, s: packed_state(d, s, (1, 1, 3, 1), (900, 5, 200, 0)),
                          lambda s: run_packed(s, max_seqlen_q=3)),
-    "shared, tokens": (shared_state, run_shared),
-    "shared, rows": (lambda d, s: shared_state(d, s, 25), run_shared),
+    "shared, in parts": (shared_state, run_shared),
+    "shared, in parts of many rows": (lambda d, s: shared_state(d, s, 28, 20_000, (30, 200, 77) * 3), run_shared),
+    "shared, one pass": (lambda d, s: shared_state(d, s, 25, 300), run_shared),
 }
+
+
+def test_kinds(cuda):
+    """That the kinds take the ways they are named after."""
+    size = T._lib.load().trx_attn_shared_bytes
+    assert size(3, 1, 6000, 200, 8, 2, 128) > 0 and size(9, 28, 20_000, 200, 8, 2, 128) > 0
+    assert size(3, 25, 300, 200, 8, 2, 128) == 0
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -32,7 +32,7 @@ def lengths(lens, dev):
 @pytest.mark.parametrize("heads,kv", [(1, 1), (4, 1), (8, 2), (6, 2), (5, 5)])
 @pytest.mark.parametrize("Sq,lens", [(1, [1, 40, 7, 0, 130]), (3, [3, 5, 129, 1, 0]), (16, [16, 100, 260, 31, 128]),
                                      (17, [17, 128, 300, 4, 0]), (150, [150, 300, 151, 20])], ids=str)
-@pytest.mark.parametrize("P", [0, 1, 127, 128, 300, 1500])
+@pytest.mark.parametrize("P", [0, 1, 127, 128, 300, 1500, 4097, 6500])
 def test_lengths(cuda, P, Sq, lens, heads, kv):
     dtype, dim = (torch.bfloat16, 128) if heads % 2 else (torch.float16, 64)
     q, pk, pv, k, v = inputs(cuda, dtype, len(lens), Sq, P, max(lens) + 5, heads, kv, dim)
@@ -43,22 +43,22 @@ def test_lengths(cuda, P, Sq, lens, heads, kv):
 
 
 @pytest.mark.parametrize("heads,kv", [(3, 1), (7, 1), (32, 8), (48, 1), (71, 1), (130, 1), (16, 16)])
-@pytest.mark.parametrize("Sq", [1, 2, 33])
-def test_groups(cuda, heads, kv, Sq):
+@pytest.mark.parametrize("Sq,P", [(1, 500), (2, 5000), (33, 500), (33, 5000)])
+def test_groups(cuda, heads, kv, Sq, P):
     lens = [33, 50, 64]
-    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 3, Sq, 500, 64, heads, kv, 64, seed=20)
+    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 3, Sq, P, 64, heads, kv, 64, seed=20)
     out, lse = T.attention_shared_prefix(q, pk, pv, k, v, lengths(lens, cuda), return_lse=True)
     check(out, lse, q, pk, pv, k, v, lens)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 80, 16])
-@pytest.mark.parametrize("Sq", [1, 4, 100])
+@pytest.mark.parametrize("Sq,P", [(1, 700), (4, 5555), (100, 700), (60, 9001)])
 @pytest.mark.parametrize("how", [dict(alibi=True), dict(scale=0.4), dict(alibi=True, scale=0.01)], ids=str)
-def test_biases(cuda, how, Sq, dim):
+def test_biases(cuda, how, Sq, P, dim):
     how = dict(how)
     slopes = slopes_of(8, cuda) if how.pop("alibi", False) else None
     lens = [100, 333, 128]
-    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 3, Sq, 700, 333, 8, 2, dim, seed=30)
+    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 3, Sq, P, 333, 8, 2, dim, seed=30)
     out, lse = T.attention_shared_prefix(q, pk, pv, k, v, lengths(lens, cuda), alibi_slopes=slopes,
                                          return_lse=True, **how)
     check(out, lse, q, pk, pv, k, v, lens, slopes=slopes, **how)
@@ -87,10 +87,10 @@ def test_many_rows(cuda, Sq, B, alibi):
     check(out, lse, q, pk, pv, k, v, [320] * B, slopes=slopes)
 
 
-@pytest.mark.parametrize("Sq", [1, 6, 40])
-def test_views(cuda, Sq):
+@pytest.mark.parametrize("Sq,P", [(1, 200), (6, 200), (40, 200), (1, 5000), (6, 5000), (40, 9000)])
+def test_views(cuda, Sq, P):
     """Caches of another layout (batch, heads, rows, head_dim), a prefix and queries that are slices."""
-    B, P, S, hq, hk, d = 3, 200, 60, 8, 2, 128
+    B, S, hq, hk, d = 3, 60, 8, 2, 128
     lens = [40, 60, 51]
     qkv = make(50, cuda, torch.bfloat16, B, Sq, hq + 2 * hk, d)
     pre = make(51, cuda, torch.bfloat16, P, 2, hk, d)

@@ -50,7 +50,7 @@ I64x3 = _lib.I64x3
 
 def shared(lib, **change):
     a = dict(q=ONE, pk=ONE, pv=ONE, k=ONE, v=ONE, out=ONE, lse=None, slopes=None, lengths=None, b=2, sq=1,
-             p=100, s=20, hq=4, hk=2, d=128, qs=I64x3(512, 512, 128), pks=I64x2(256, 128),
+             p=9000, s=20, hq=4, hk=2, d=128, qs=I64x3(512, 512, 128), pks=I64x2(256, 128),
              pvs=I64x2(256, 128), ks=I64x3(5120, 256, 128), vs=I64x3(5120, 256, 128),
              os=I64x3(512, 512, 128), scale=1.0, dtype=2, parts=ONE, pb=1 << 30, ws=ONE, wsb=256, stream=None)
     assert set(change) <= set(a)
@@ -77,14 +77,16 @@ def test_shared_entry_has_nothing_to_do(lib):
 
 
 def test_shared_bytes(lib):
-    """Space for the results of the prefix's splits: none without a prefix, none with many rows."""
+    """Space for the results of the prefix's splits: none without a prefix, none for one pass."""
     size = lib.trx_attn_shared_bytes
-    assert size(64, 1, 0, 32, 8, 128) == 0 and size(4, 17, 5000, 32, 8, 128) == 0
+    assert size(64, 1, 0, 100, 32, 8, 128) == 0  # no prefix
+    assert size(16, 320, 4096, 384, 32, 8, 128) == 0 and size(16, 8, 1024, 512, 32, 8, 128) == 0
     row = 64 * 32 * 129 * 4
-    n = size(64, 1, 8192, 32, 8, 128)
+    n = size(64, 1, 8192, 1024, 32, 8, 128)
     assert n >= row and n % row == 0
-    assert size(64, 1, 100, 32, 8, 128) == row  # a single tile of keys cannot be split
-    for bad in ((0, 1, 5, 4, 2, 64), (1, 1, -1, 4, 2, 64), (1, 1, 5, 4, 3, 64), (1 << 20, 1, 5, 4, 2, 64)):
+    assert size(4, 100, 30000, 300, 32, 8, 128) > 0  # many rows, but a long prefix
+    for bad in ((0, 1, 5, 5, 4, 2, 64), (1, 1, -1, 5, 4, 2, 64), (1, 1, 5, -1, 4, 2, 64), (1, 1, 5, 5, 4, 3, 64),
+                (1 << 20, 1, 5, 5, 4, 2, 64), (60000, 1 << 20, 5, 5, 4, 2, 64)):
         assert size(*bad) == 0
 
 

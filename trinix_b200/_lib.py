@@ -93,10 +93,11 @@ SIGNATURES = {
                                     c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
                                     c_int64, *[c_void_p] * 4, c_float, c_int, c_int64,
                                     c_int64, c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p]),
-    "trx_attn_shared_bytes": (c_size_t, [c_int64] * 6),
+    "trx_attn_shared_bytes": (c_size_t, [c_int64] * 7),
     "trx_attn_fwd_shared": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
-                                    c_int64, c_int64, c_int64, *[c_void_p] * 6, c_float, c_int, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
+                                    c_int64, c_int64, c_int64, *[c_void_p] * 6, c_float, c_int,
+                                    c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
     "trx_attn_status": (c_int, [c_void_p, c_void_p, c_void_p]),
     "trx_attn_mirror": (c_int, [c_void_p, c_void_p, c_void_p]),
     "trx_attn_fwd_static_scratch": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

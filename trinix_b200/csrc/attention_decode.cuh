@@ -539,22 +539,26 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
 // single shapes (32 / 8 heads, head dim 128, that / this / the tcgen05 kernel): 24 x 256 keys, 16 rows
 // 40.6 / 23.7 / 28.6 us; 8 x 256 keys, 16 rows 14.8 / 11.2 / 10.8 us; 2 x 4096 keys, 1 row 18.2 / 12.6
 // / 69.5 us.
-inline int decode_splits(int64_t keys, int64_t units, bool wide) {
+inline int64_t decode_cost(int64_t n, int64_t keys, int64_t units, bool wide) {
   const int64_t sms = sm_count_of_current_device(), slots = sms * DEC_CTAS_PER_SM;
   const int64_t tiles = (keys + DEC_KEYS - 1) / DEC_KEYS;
-  auto cost = [&](int64_t n) {
-    const int64_t ctas = units * n, waves = (ctas + slots - 1) / slots;
-    const int64_t chain = (tiles + n * DEC_WARPS - 1) / (n * DEC_WARPS);
-    int64_t ends = 14;
-    if (n > 1) ends += waves > 1 ? 13 : 10;
-    if (ctas > sms) ends += wide ? 10 : 5;
-    if (n >= 8 && ctas > 64) ends += n == 8 ? 4 : 6;
-    if (n == 16) ends += 1;
-    return waves * (ends + 4 * chain);
-  };
+  const int64_t ctas = units * n, waves = (ctas + slots - 1) / slots;
+  const int64_t chain = (tiles + n * DEC_WARPS - 1) / (n * DEC_WARPS);
+  int64_t ends = 14;
+  if (n > 1) ends += waves > 1 ? 13 : 10;
+  if (ctas > sms) ends += wide ? 10 : 5;
+  if (n >= 8 && ctas > 64) ends += n == 8 ? 4 : 6;
+  if (n == 16) ends += 1;
+  return waves * (ends + 4 * chain);
+}
+inline int decode_splits(int64_t keys, int64_t units, bool wide) {
+  const int64_t slots = sm_count_of_current_device() * DEC_CTAS_PER_SM;
+  const int64_t tiles = (keys + DEC_KEYS - 1) / DEC_KEYS;
   int best = 1;
   for (int n = 2; n <= DEC_MAX_SPLIT && tiles >= n * DEC_WARPS; n *= 2)
-    if ((n == 2 || units * n <= slots) && cost(n) < cost(best)) best = n;
+    if ((n == 2 || units * n <= slots) &&
+        decode_cost(n, keys, units, wide) < decode_cost(best, keys, units, wide))
+      best = n;
   return best;
 }
 

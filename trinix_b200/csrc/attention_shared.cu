@@ -1,11 +1,12 @@
-// Attention for a batch whose sequences share a prefix: launches and C entries. Two ways:
+// Attention for a batch whose sequences share a prefix: launches and C entries. Two ways, of which a cost
+// picks one (shared_plan):
 //
-//   few rows (decoding)   the rows of the whole batch are one run of query rows against the prefix, whose
-//                         keys are split over the CTAs (attention_plain.cuh, ATT_PREFIX): the prefix is read
-//                         and multiplied once for all, at 128 rows to a tile where a sequence alone would
-//                         fill a few. The decode kernel then does the sequences' own keys and merges.
-//   many rows (prompts)   one pass over the prefix's tiles and the sequence's own (ATT_SHARED): its own rows
-//                         fill the tiles, and the prefix comes from L2.
+//   in parts   the rows of the whole batch are one run of query rows against the prefix, whose keys are split
+//              over the CTAs (attention_plain.cuh, ATT_PREFIX): the prefix is read and multiplied once for
+//              all, at 128 rows to a tile where a sequence alone would fill a few. The decode kernel then
+//              does the sequences' own keys and merges. For few rows to a sequence, or a long prefix.
+//   one pass   over the prefix's tiles and the sequence's own (ATT_SHARED): its own rows fill the tiles, and
+//              the prefix comes from L2. For many rows, or a short prefix.
 #include "attention_decode.cuh"
 #include "attention_plain.cuh"
 
@@ -40,28 +41,49 @@ static int launch_form_rows(const P& p, int64_t D, dim3 grid, cudaStream_t s) {
 
 struct SharedPlan {
   RaggedParams tile;  // tile_heads, tile_tokens, head_tiles
-  bool few;
-  int splits, split_tiles;  // of the prefix, with few rows
+  bool in_parts;
+  int splits, split_tiles;  // of the prefix
   bool halves;              // one Q tile holds all rows, and the two have halves of a split's keys
   int parts;                // results of the splits, or halves
 };
-static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int64_t Hk) {
+// The cost, in us: a launch of attention_plain.cuh starts and ends in 6, an item in 4.5, a KV tile takes 1.95
+// with both Q tiles at work on it, 1.5 with one, 0.95 with every second one each; the decode kernel by its
+// own cost (decode_cost), more with two row tiles to a warp, 0.15 for each part that it merges. Over 54
+// shapes (1 to 32 sequences of 4 to 160 rows behind 500 to 30000 keys, 16 / 16 heads x 64, 32 / 4 and 32 / 8
+// x 128) the way that it picks is 1 % slower than the better one in the mean, 15 % at worst. In parts / one
+// pass, 32 / 8 heads x 128: 32 x 4 rows behind 8192 keys 38 / 202 us, 32 x 48 351 / 268, 4 x 48 53 / 113, 16 x
+// 8 behind 1024 37 / 26, 1 x 8 behind 500 16.7 / 14.8. One pass for more than 16 rows and only then: up to 4
+// times as long (4 x 24 behind 8192 42 / 104).
+static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t S, int64_t Hq, int64_t Hk) {
   SharedPlan s{};
   s.tile.Hq = static_cast<int>(Hq);
   s.tile.group = static_cast<int>(Hq / Hk);
   choose_tile(s.tile);
-  const int64_t row_tiles = (s.tile.group * Sq + 15) / 16;
-  s.few = Sq <= 16 && Hk * row_tiles <= 65535;
-  if (!s.few || P == 0) return s;
-  const int64_t step = ATT_NQ * s.tile.tile_tokens;
-  const int64_t items = Hq / s.tile.tile_heads * ((B * Sq + step - 1) / step);
-  const int64_t tiles = (P + ATT_BN - 1) / ATT_BN;
-  int64_t parts = sm_count_of_current_device() / items;
-  parts = parts < 1 ? 1 : parts > tiles ? tiles : parts;
-  s.split_tiles = static_cast<int>((tiles + parts - 1) / parts);
-  s.splits = static_cast<int>((tiles + s.split_tiles - 1) / s.split_tiles);
-  s.halves = B * Sq <= s.tile.tile_tokens && s.split_tiles > 1;
+  const int64_t sms = sm_count_of_current_device(), tokens = s.tile.tile_tokens, step = ATT_NQ * tokens;
+  const bool wide = s.tile.group * Sq > 16;
+  const int64_t row_tiles = (s.tile.group * Sq + (wide ? 31 : 15)) / (wide ? 32 : 16);
+  auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+  if (Hk * row_tiles > 65535) return s;
+  if (P == 0) {  // the sequences' own keys alone
+    s.in_parts = Sq <= 16;
+    return s;
+  }
+  const int64_t rows = B * Sq, tiles = up(P, ATT_BN), items = s.tile.head_tiles * up(rows, step);
+  int64_t splits = sms / items;
+  splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
+  s.split_tiles = static_cast<int>(up(tiles, splits));
+  s.splits = static_cast<int>(up(tiles, s.split_tiles));
+  s.halves = rows <= tokens && s.split_tiles > 1;
   s.parts = s.halves ? 2 * s.splits : s.splits;
+  const double visit = s.halves ? 0.95 : rows <= tokens ? 1.5 : 1.95;
+  const int64_t units = Hk * row_tiles * B;
+  const double in_parts = 6.0 + up(items * s.splits, sms) * (4.5 + visit * s.split_tiles) +
+                          (wide ? 0.286 : 0.22) * decode_cost(decode_splits(S, units, wide), S, units, wide) +
+                          0.15 * s.parts + 2.0;
+  const double one_pass = 6.0 + up(s.tile.head_tiles * up(Sq, step) * B, sms) *
+                                    (4.5 + (Sq <= tokens ? 1.5 : 1.95) * (tiles + up(S, ATT_BN)));
+  s.in_parts = in_parts < one_pass;
+  if (!s.in_parts) s.parts = 0;
   return s;
 }
 
@@ -73,11 +95,12 @@ static size_t shared_bytes(const SharedPlan& s, int64_t B, int64_t Sq, int64_t H
   return static_cast<size_t>(s.parts) * B * Sq * Hq * (D + 1) * sizeof(float);
 }
 
-extern "C" size_t trx_attn_shared_bytes(int64_t B, int64_t Sq, int64_t P, int64_t Hq, int64_t Hk, int64_t D) {
-  if (B <= 0 || Sq <= 0 || P < 0 || Hq <= 0 || Hk <= 0 || D <= 0 || Hq % Hk || B > 65535 ||
-      Sq >= (1ll << 30) || P >= (1ll << 30) || Hq > 65535)
+extern "C" size_t trx_attn_shared_bytes(int64_t B, int64_t Sq, int64_t P, int64_t S, int64_t Hq, int64_t Hk,
+                                        int64_t D) {
+  if (B <= 0 || Sq <= 0 || P < 0 || S < 0 || Hq <= 0 || Hk <= 0 || D <= 0 || Hq % Hk || B > 65535 ||
+      Sq >= (1ll << 30) || B * Sq >= (1ll << 30) || P >= (1ll << 29) || S >= (1ll << 29) || Hq > 65535)
     return 0;
-  return shared_bytes(shared_plan(B, Sq, P, Hq, Hk), B, Sq, Hq, D);
+  return shared_bytes(shared_plan(B, Sq, P, S, Hq, Hk), B, Sq, Hq, D);
 }
 
 extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const void* prefix_v, const void* k,
@@ -110,17 +133,20 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
         (i < 2 && (pk_strides[i] < 0 || pv_strides[i] < 0)))
       return TRX_ERR_STRIDE;
 
-  SharedPlan plan = shared_plan(B, Sq, P, Hq, Hk);
+  SharedPlan plan = shared_plan(B, Sq, P, S, Hq, Hk);
   // the rows of the batch as one run: what the prefix's launch wants
   const int64_t row_stride = Sq == 1 ? q_strides[0] : q_strides[1];
-  if (plan.few && B > 1 && Sq > 1 && q_strides[0] != Sq * q_strides[1]) plan.few = false;
-  if (plan.few && plan.parts > 0 &&
+  if (plan.parts > 0 && B > 1 && Sq > 1 && q_strides[0] != Sq * q_strides[1]) {
+    plan.in_parts = false;
+    plan.parts = 0;
+  }
+  if (plan.parts > 0 &&
       (!parts || !aligned_to(parts, 16) || parts_bytes < shared_bytes(plan, B, Sq, Hq, D)))
     return TRX_ERR_WORKSPACE;
 
   SharedParams p{};
   const int is_bf16 = dtype == TRX_BF16, tokens = plan.tile.tile_tokens, heads = plan.tile.tile_heads;
-  const int box = plan.few ? DEC_KEYS : ATT_BN;
+  const int box = plan.in_parts ? DEC_KEYS : ATT_BN;
   // without keys nothing is loaded: any legal map
   int rc = make_map(&p.tm_k, S > 0 ? k : q, is_bf16, D, S > 0 ? S : 1, Hk, B, k_strides[0], k_strides[1],
                     k_strides[2], box);
@@ -155,13 +181,13 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   p.is_bf16 = is_bf16;
   p.reverse_kv = slopes_or_null ? 1 : 0;  // ALiBi: backwards, see attention_plain.cuh
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t step = ATT_NQ * tokens, rows = plan.few ? B * Sq : Sq;
+  const int64_t step = ATT_NQ * tokens, rows = plan.parts > 0 ? B * Sq : Sq;
   const int64_t blocks = (rows + step - 1) / step;
-  if (blocks > 65535) return TRX_ERR_SHAPE;
+  if (blocks > 65535 && !(plan.in_parts && plan.parts == 0)) return TRX_ERR_SHAPE;
   dim3 grid(static_cast<unsigned>(Hq / heads), static_cast<unsigned>(blocks), static_cast<unsigned>(B));
 
   bool beside = false;
-  if (plan.few && plan.parts > 0) {
+  if (plan.parts > 0) {
     PrefixParams f{};
     static_cast<RaggedParams&>(f) = p;
     rc = make_ragged_q_map(&f.tm_q, q, is_bf16, D, B * Sq, Hq, 1, 0, row_stride, q_strides[2], heads, tokens);
@@ -197,7 +223,7 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   p.lse = lse_or_null;
   p.lse_stride_b = Hq * Sq;
   p.lse_stride_h = Sq;
-  if (plan.few) {
+  if (plan.in_parts) {
     p.q = q;
     p.q_stride_b = q_strides[0];
     p.q_stride_s = q_strides[1];

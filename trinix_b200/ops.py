@@ -808,8 +808,8 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     concatenation and sees the keys up to there; alibi_slopes (Hq,) add -slope * distance. A query
     without a key is 0. With return_lse also the fp32 (B, Hq, Sq) log-sum-exp.
 
-    Up to 16 tokens (decoding): the prefix is read once for the whole batch and multiplied with all its
-    rows together. More: one pass over both, the prefix from L2.
+    With few tokens to a sequence (decoding), or a long prefix, the prefix is read once for the whole
+    batch and multiplied with all its rows together; otherwise one pass over both, the prefix from L2.
     """
     dev = _need_cuda(q, prefix_k, prefix_v, k, v, lengths, alibi_slopes)
     dtype, own = q.dtype, k.shape
@@ -842,16 +842,16 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     dp = _padded_dim(d)
     q, prefix_k, prefix_v = _packed_view(q, dp), _packed_view(prefix_k, dp), _packed_view(prefix_v, dp)
     k, v = _packed_view(k, dp), _packed_view(v, dp)
-    if B > 1 and 1 < Sq <= 16 and q.stride(0) != Sq * q.stride(1):
-        q = q.contiguous()  # the rows of the batch as one run
     out = _empty(q, (B, Sq, Hq, dp))
     lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
     if dev.index == torch.cuda.current_device():
-        size = _lib.load().trx_attn_shared_bytes(B, Sq, P, Hq, Hk, dp)
+        size = _lib.load().trx_attn_shared_bytes(B, Sq, P, S, Hq, Hk, dp)
     else:  # the number of parts goes by the SMs of the current device
         with torch.cuda.device(dev):
-            size = _lib.load().trx_attn_shared_bytes(B, Sq, P, Hq, Hk, dp)
+            size = _lib.load().trx_attn_shared_bytes(B, Sq, P, S, Hq, Hk, dp)
     parts = _empty(q, size, dtype=torch.uint8)
+    if size and B > 1 and Sq > 1 and q.stride(0) != Sq * q.stride(1):
+        q = q.contiguous()  # the rows of the batch as one run
     ws = _workspace(dev)
     _raise_if_failed("trx_attn_fwd_shared", dev)  # of an earlier launch, before more work is queued
     strides = _I64x16(*q.stride()[:3], *prefix_k.stride()[:2], *prefix_v.stride()[:2], *k.stride()[:3],
@@ -860,8 +860,8 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     _launch("trx_attn_fwd_shared", dev, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k.data_ptr(),
             v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(slopes), _ptr(lengths), B, Sq, P, S, Hq, Hk, dp,
             at, at + 24, at + 40, at + 56, at + 80, at + 104, scale, _DTYPE_CODE[dtype], parts.data_ptr(),
-            parts.numel(), ws.data_ptr(), ws.numel())
-    if parts.numel():
+            size, ws.data_ptr(), ws.numel())
+    if size:
         _count()  # the prefix is a launch of its own
     out = out if dp == d else out[..., :d].contiguous()
     return (out, lse) if return_lse else out
