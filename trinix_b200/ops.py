@@ -681,6 +681,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     return (out, lse) if return_lse else out
 
 
+def _same_device(q: torch.Tensor, *ts: Optional[torch.Tensor]) -> torch.device:
+    """_need_cuda by device numbers: device objects of seven tensors cost the host 2 us."""
+    index = q.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            index = -1
+    return q.device if index >= 0 else _need_cuda(q, *ts)
+
+
 def _packed_view(t: torch.Tensor, d: int) -> torch.Tensor:
     """A view with head dim d (zero columns are appended to fewer) whose last dim is dense, whose base
     is 16-byte aligned and whose other strides are multiples of 8 elements and at least a row apart, as
@@ -745,7 +754,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     output; in `out`, if given (it then is the result), they stay what they were. With return_lse
     also the fp32 (Hq, Tq) log-sum-exp, -inf for rows without a key and rows behind the last.
     """
-    dev = _need_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, alibi_slopes, out)
+    dev = _same_device(q, k, v, cu_seqlens_q, cu_seqlens_k, alibi_slopes, out)
     dtype, shape = q.dtype, k.shape
     if not (dtype == k.dtype == v.dtype) or dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("attention needs q, k, v of one dtype, bfloat16 or float16")
@@ -774,7 +783,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError("out must have the shape and dtype of q")
     q, k, v = _packed_view(q, dp), _packed_view(k, dp), _packed_view(v, dp)
     if out is None:
-        o = _empty(q, (Tq, Hq, dp))
+        o = _new(q)
     else:
         o = _packed_view(out, dp)  # a copy where the kernel cannot write into it
     lse = _empty(q, (Hq, Tq), dtype=torch.float32) if return_lse else None
@@ -811,7 +820,7 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     With few tokens to a sequence (decoding), or a long prefix, the prefix is read once for the whole
     batch and multiplied with all its rows together; otherwise one pass over both, the prefix from L2.
     """
-    dev = _need_cuda(q, prefix_k, prefix_v, k, v, lengths, alibi_slopes)
+    dev = _same_device(q, prefix_k, prefix_v, k, v, lengths, alibi_slopes)
     dtype, own = q.dtype, k.shape
     if (not (dtype == prefix_k.dtype == prefix_v.dtype == k.dtype == v.dtype)
             or dtype not in (torch.bfloat16, torch.float16)):
@@ -842,7 +851,7 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     dp = _padded_dim(d)
     q, prefix_k, prefix_v = _packed_view(q, dp), _packed_view(prefix_k, dp), _packed_view(prefix_v, dp)
     k, v = _packed_view(k, dp), _packed_view(v, dp)
-    out = _empty(q, (B, Sq, Hq, dp))
+    out = _new(q)
     lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
     if dev.index == torch.cuda.current_device():
         size = _lib.load().trx_attn_shared_bytes(B, Sq, P, S, Hq, Hk, dp)
