@@ -91,6 +91,42 @@ def test_masks_and_biases(cuda, how, dim):
     check(out, lse, q, k, v, len_q, len_k, slopes=slopes, **how)
 
 
+# rows of up to 16, promised: the kernel for decoding
+@pytest.mark.parametrize("heads,kv,dim", [(1, 1, 128), (8, 2, 128), (32, 8, 64), (3, 1, 128), (71, 1, 64), (5, 5, 80)])
+@pytest.mark.parametrize("how", [
+    dict(causal=True), dict(), dict(window=(300, 0)), dict(window=(0, 0)), dict(causal=True, alibi=True),
+    dict(alibi=True), dict(window=(40, 20), alibi=True), dict(causal=True, scale=-0.2),
+], ids=str)
+def test_few_rows(cuda, how, heads, kv, dim):
+    how = dict(how)
+    slopes = slopes_of(heads, cuda) if how.pop("alibi", False) else None
+    len_q = [1, 16, 0, 3, 1, 7, 1, 2, 5, 1] * 2
+    len_k = [1, 16, 9, 700, 3000, 2, 0, 129, 5, 64] * 2
+    dtype = torch.float16 if heads % 2 else torch.bfloat16
+    q = make(50, cuda, dtype, sum(len_q) + 21, heads, dim)
+    k, v = (make(i, cuda, dtype, sum(len_k) + 30, kv, dim) for i in (51, 52))
+    k[sum(len_k):], v[sum(len_k):] = float("nan"), float("inf")
+    out, lse = T.attention_packed(q, k, v, starts(len_q, cuda), starts(len_k, cuda), return_lse=True,
+                                  alibi_slopes=slopes, max_seqlen_q=16, **how)
+    check(out, lse, q, k, v, len_q, len_k, slopes=slopes, **how)
+    held = q.clone()
+    T.attention_packed(q, k, v, starts(len_q, cuda), starts(len_k, cuda), alibi_slopes=slopes,
+                       max_seqlen_q=16, out=held, **how)
+    n = sum(len_q)
+    assert torch.equal(held[:n], out[:n]) and torch.equal(held[n:], q[n:])
+
+
+def test_scales_next_to_nothing(cuda):
+    """A ramp divided by the scale would not be finite."""
+    lens = [40, 300]
+    q = make(53, cuda, torch.bfloat16, 340, 4, 64)
+    k, v = make(54, cuda, torch.bfloat16, 340, 4, 64), make(55, cuda, torch.bfloat16, 340, 4, 64)
+    for scale in (1e-37, 1e-31, 1e-20):
+        out, lse = T.attention_packed(q, k, v, starts(lens, cuda), causal=True, scale=scale, return_lse=True,
+                                      alibi_slopes=slopes_of(4, cuda))
+        check(out, lse, q, k, v, lens, lens, causal=True, scale=scale, slopes=slopes_of(4, cuda))
+
+
 @pytest.mark.parametrize("alibi", [False, True])
 def test_several_items_per_cta(cuda, alibi):
     """More work items than SMs: the items that a CTA takes behind its first one, skipped slots."""
@@ -182,8 +218,10 @@ def test_neighbours_and_rest_never_matter(cuda, max_q):
             lo, hi = int(cu_k[s]), int(cu_k[s + 1])
             for t in (kk, vv):
                 t[:lo], t[hi:] = bad, bad
-            got = T.attention_packed(q, kk, vv, cu_q, cu_k, causal=True, max_seqlen_q=max_q)
             a, b = int(cu_q[s]), int(cu_q[s + 1])
+            qq = torch.full_like(q, bad)
+            qq[a:b] = q[a:b]
+            got = T.attention_packed(qq, kk, vv, cu_q, cu_k, causal=True, max_seqlen_q=max_q)
             assert torch.equal(got[a:b], want[a:b])
 
 

@@ -60,7 +60,7 @@ def shared(lib, **change):
 
 @pytest.mark.parametrize("change,code", [
     (dict(dtype=0), -2), (dict(hk=3), -3), (dict(b=-1), -3), (dict(p=-1), -3), (dict(s=-1), -3),
-    (dict(d=96), -6), (dict(scale=0.0), -6), (dict(scale=float("nan")), -6), (dict(q=None), -1),
+    (dict(d=96), -6), (dict(scale=0.0), -6), (dict(scale=1e-31), -6), (dict(scale=float("nan")), -6), (dict(q=None), -1),
     (dict(pk=None), -1), (dict(pv=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(out=None), -1),
     (dict(ws=None), -9), (dict(parts=None), -9), (dict(parts=ctypes.c_void_p(4104)), -9), (dict(pb=16), -9),
     (dict(b=1 << 17), -3), (dict(p=1 << 29), -3), (dict(s=1 << 29), -3), (dict(sq=1 << 30), -3),

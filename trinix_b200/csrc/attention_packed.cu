@@ -18,7 +18,8 @@ static int launch_packed(const P& p, dim3 grid, cudaStream_t stream) {
 
 template <int D, bool BF16, bool SINGLE, class P>
 static int launch_packed_bias(const P& p, dim3 grid, cudaStream_t stream) {
-  if (!(p.scale_log2 > 0.0f)) return launch_packed<D, BF16, AP_GENERAL, SINGLE>(p, grid, stream);
+  // a score carries the ramp divided by the scale: not of one that is negative, or next to nothing
+  if (!(p.scale_log2 > 1e-30f)) return launch_packed<D, BF16, AP_GENERAL, SINGLE>(p, grid, stream);
   if (!p.slopes) return launch_packed<D, BF16, AP_NONE, SINGLE>(p, grid, stream);
   // under a causal mask, or a window that ends at the query, every visible key is at or before it
   return p.causal || p.win_right == 0 ? launch_packed<D, BF16, AP_RAMP, SINGLE>(p, grid, stream)

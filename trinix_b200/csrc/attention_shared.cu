@@ -115,7 +115,7 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   if (dtype != TRX_BF16 && dtype != TRX_F16) return TRX_ERR_DTYPE;
   if (B < 0 || Sq < 0 || P < 0 || S < 0 || Hq <= 0 || Hk <= 0 || D <= 0 || Hq % Hk != 0) return TRX_ERR_SHAPE;
   if (D != 64 && D != 128) return TRX_ERR_UNSUPPORTED;
-  if (!(scale > 0.0f)) return TRX_ERR_UNSUPPORTED;
+  if (!(scale >= 1e-30f)) return TRX_ERR_UNSUPPORTED;  // scores carry ALiBi's ramp divided by it
   if (B == 0 || Sq == 0) return TRX_OK;
   if (!q || !out || !q_strides || !pk_strides || !pv_strides || !k_strides || !v_strides || !o_strides)
     return TRX_ERR_NULL_POINTER;

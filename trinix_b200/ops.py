@@ -753,6 +753,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     decoding, which leaves rows beyond it unwritten. Rows behind cu_seqlens_q[-1] are 0 in a new
     output; in `out`, if given (it then is the result), they stay what they were. With return_lse
     also the fp32 (Hq, Tq) log-sum-exp, -inf for rows without a key and rows behind the last.
+    Forward only, as `attention`: PackedAttentionKernel.apply has a later .backward() say so.
     """
     dev = _same_device(q, k, v, cu_seqlens_q, cu_seqlens_k, alibi_slopes, out)
     dtype, shape = q.dtype, k.shape
@@ -819,6 +820,7 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
 
     With few tokens to a sequence (decoding), or a long prefix, the prefix is read once for the whole
     batch and multiplied with all its rows together; otherwise one pass over both, the prefix from L2.
+    Forward only, as `attention`: SharedPrefixAttentionKernel.apply has a later .backward() say so.
     """
     dev = _same_device(q, prefix_k, prefix_v, k, v, lengths, alibi_slopes)
     dtype, own = q.dtype, k.shape
@@ -845,8 +847,8 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
             raise ValueError(f"lengths must be an int32 tensor of {B} entries")
         lengths = lengths.contiguous()
     scale = d ** -0.5 if scale is None else float(scale)
-    if not scale > 0.0:
-        raise ValueError(f"scale must be positive, got {scale}")
+    if not scale >= 1e-30:
+        raise ValueError(f"scale must be positive, at least 1e-30, got {scale}")
     slopes = _slopes(alibi_slopes, Hq)
     dp = _padded_dim(d)
     q, prefix_k, prefix_v = _packed_view(q, dp), _packed_view(prefix_k, dp), _packed_view(prefix_v, dp)
