@@ -1,5 +1,7 @@
 // Attention forward without a dense mask or dropout: softmax(scale * Q K^T - ALiBi) V, online softmax
-// (but few query rows: attention_decode.cuh, and a single KV tile in one wave of CTAs: attention.cu).
+// (but few query rows: attention_decode.cuh, and a single KV tile in one wave of CTAs: attention.cu). One
+// batch (attention_plain.cu), packed sequences (attention_packed.cu) or a shared prefix (attention_shared.cu):
+// P::FORM, and attention_ragged.cuh for the rows and keys of the latter two.
 //
 // A work item is two 128-row Q tiles: the same 128 query rows of two query heads that share a kv head
 // (GQA / MQA: both tiles then see exactly the same keys), or 256 consecutive rows of one head
@@ -916,7 +918,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           row += r;
           live = row < p.Sq;
         } else {
-          const int tok = r / p.tile_heads;
+          const int tok = ragged_token(p, r);
           if (ALT && w.alt) row = w.m0;
           row += tok;
           hq += r - tok * p.tile_heads;
@@ -995,10 +997,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         row1 = min(p.Sq, row0 + ATT_BM) - 1;
         hi_i = p.Sk - 1;
       } else {
-        const int tok = min(rl / p.tile_heads, t_rows - 1);
+        const int tile_row = ragged_token(p, rl), tok = min(tile_row, t_rows - 1);
         if (alt) row0 = w.m0;
         if (BIAS != AP_NONE && valid && p.slopes)
-          slope2 = p.slopes[w.h + (TWO_HEADS && alt ? t * p.tile_heads : 0) + rl % p.tile_heads] *
+          slope2 = p.slopes[w.h + (TWO_HEADS && alt ? t * p.tile_heads : 0) + rl - tile_row * p.tile_heads] *
                    1.4426950408889634f;
         row1 = min(w.sq, row0 + t_rows) - 1;
         row = row0 + tok;

@@ -40,6 +40,7 @@ struct RaggedParams : AttnParams {
   int n_seq;                 // and one more, without keys, if rows behind the last are to be zeroed
   int rows, keys;            // of the whole packed q and k / v; shared: keys a sequence's cache holds
   int tile_heads, tile_tokens;
+  int per_head;              // 2^16 / tile_heads, rounded up: r / tile_heads of a row r < 128 of a tile
   int head_tiles;            // query heads / tile_heads
   int slots_first;           // packed without a table: the grid's x counts slots (and not heads)
   int seq;                   // shared: queries per sequence
@@ -64,6 +65,9 @@ __device__ __forceinline__ int ragged_tokens(const RaggedParams& p) { return p.t
 __device__ __forceinline__ uint32_t ragged_q_bytes(const RaggedParams& p) {  // of 64 columns of a Q tile
   return 128u * p.tile_heads * p.tile_tokens;
 }
+// The token of row r of a Q tile. r * per_head is off r * 2^16 / tile_heads by less than 128: r / tile_heads
+// is never nearer to the next whole number than 1 / 128.
+__device__ __forceinline__ int ragged_token(const RaggedParams& p, int r) { return (r * p.per_head) >> 16; }
 __device__ __forceinline__ int ragged_tokens(const AttnParams&) { return 0; }
 __device__ __forceinline__ uint32_t ragged_q_bytes(const AttnParams&) { return 0; }
 
@@ -387,6 +391,7 @@ inline void choose_tile(RaggedParams& p) {  // from its Hq and group
   for (int h = 2; h <= p.group && h <= ATT_BM; ++h)
     if (p.group % h == 0 && ATT_BM / h * h * 10 >= ATT_BM * 9) p.tile_heads = h;
   p.tile_tokens = ATT_BM / p.tile_heads;
+  p.per_head = (65536 + p.tile_heads - 1) / p.tile_heads;
   p.head_tiles = p.Hq / p.tile_heads;
 }
 

@@ -162,6 +162,7 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   if (rc != TRX_OK) return rc;
   p.tile_heads = heads;
   p.tile_tokens = tokens;
+  p.per_head = plan.tile.per_head;
   p.head_tiles = plan.tile.head_tiles;
   p.group = plan.tile.group;
   p.k_hdiv = p.v_hdiv = p.group;
