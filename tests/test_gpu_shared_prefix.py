@@ -77,6 +77,22 @@ def test_one_tile_of_rows(cuda, P, heads, kv, alibi):
     check(out, lse, q, pk, pv, k, v, lens, slopes=slopes)
 
 
+@pytest.mark.parametrize("alibi", [False, True])
+@pytest.mark.parametrize("B,Sq,P,heads,kv", [(5, 2, 3000, 160, 160), (1300, 1, 1500, 32, 8)])
+def test_more_prefix_items_than_sms(cuda, B, Sq, P, heads, kv, alibi):
+    """Many heads, all rows in one tile; many rows. The prefix's launch is of several items per CTA."""
+    assert T._lib.load().trx_attn_shared_bytes(B, Sq, P, 40, heads, kv, 64) > 0
+    slopes = slopes_of(heads, cuda) if alibi else None
+    lens = [2 + (7 * b) % 39 for b in range(B)]
+    q, pk, pv, k, v = inputs(cuda, torch.float16, B, Sq, P, 40, heads, kv, 64, seed=47)
+    out, lse = T.attention_shared_prefix(q, pk, pv, k, v, lengths(lens, cuda), return_lse=True,
+                                         alibi_slopes=slopes)
+    some = torch.arange(0, B, max(1, B // 25), device=cuda)
+    check(out[some], lse[some], q[some], pk, pv, k[some], v[some], [lens[b] for b in some.tolist()],
+          slopes=slopes)
+    assert bool(torch.isfinite(out).all())
+
+
 @pytest.mark.parametrize("Sq,B", [(1, 100), (5, 60), (300, 12)])
 @pytest.mark.parametrize("alibi", [False, True])
 def test_many_rows(cuda, Sq, B, alibi):
