@@ -7,6 +7,7 @@ raise otherwise — there is no CPU path and no fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from typing import Optional, Tuple
 
@@ -723,9 +724,9 @@ def _padded_dim(d: int) -> int:
     return 64 if d <= 64 else 128
 
 
-# Element strides of an entry's tensors in one block, its parts passed by address: an array object for
-# each tensor costs the host 0.6 us.
-_I64x8, _I64x16 = ctypes.c_int64 * 8, ctypes.c_int64 * 16
+# All strides of an entry's tensors in one block (the last dim's 1 among them), its parts passed by
+# address: an array object for each tensor costs the host 0.6 us.
+_PackedStrides, _SharedStrides = ctypes.c_int64 * (4 * 3), ctypes.c_int64 * (4 * 4 + 2 * 3)
 
 
 def _cu_seqlens(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -792,17 +793,24 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         lse.fill_(float("-inf"))  # rows behind the last sequence are not touched
     ws = _workspace(dev)
     _raise_if_failed("trx_attn_fwd_packed", dev)  # of an earlier launch, before more work is queued
-    strides = _I64x8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *o.stride()[:2])
+    strides = _PackedStrides(*q.stride(), *k.stride(), *v.stride(), *o.stride())
     at = ctypes.addressof(strides)
     _launch("trx_attn_fwd_packed", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse),
             _ptr(slopes), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, Tq, Tk, Hq, Hk, dp, at,
-            at + 16, at + 32, at + 48, scale, 1 if causal else 0, wl, wr, int(max_seqlen_q or 0),
+            at + 24, at + 48, at + 72, scale, 1 if causal else 0, wl, wr, int(max_seqlen_q or 0),
             1 if out is None else 0, _DTYPE_CODE[dtype], ws.data_ptr(), ws.numel())
     if out is None:
         o = o if dp == d else o[..., :d].contiguous()
     elif o is not out:
         o = out.copy_(o[..., :d])
     return (o, lse) if return_lse else o
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_bytes(index: int, *sizes: int) -> int:
+    """trx_attn_shared_bytes on a device (the number of parts goes by its SMs)."""
+    with torch.cuda.device(index):
+        return _lib.load().trx_attn_shared_bytes(*sizes)
 
 
 def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
@@ -855,23 +863,19 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     k, v = _packed_view(k, dp), _packed_view(v, dp)
     out = _new(q)
     lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
-    if dev.index == torch.cuda.current_device():
-        size = _lib.load().trx_attn_shared_bytes(B, Sq, P, S, Hq, Hk, dp)
-    else:  # the number of parts goes by the SMs of the current device
-        with torch.cuda.device(dev):
-            size = _lib.load().trx_attn_shared_bytes(B, Sq, P, S, Hq, Hk, dp)
-    parts = _empty(q, size, dtype=torch.uint8)
+    size = _shared_bytes(dev.index, B, Sq, P, S, Hq, Hk, dp)
+    parts = _empty(q, size, dtype=torch.uint8) if size else None
     if size and B > 1 and Sq > 1 and q.stride(0) != Sq * q.stride(1):
         q = q.contiguous()  # the rows of the batch as one run
     ws = _workspace(dev)
     _raise_if_failed("trx_attn_fwd_shared", dev)  # of an earlier launch, before more work is queued
-    strides = _I64x16(*q.stride()[:3], *prefix_k.stride()[:2], *prefix_v.stride()[:2], *k.stride()[:3],
-                      *v.stride()[:3], *out.stride()[:3])
+    strides = _SharedStrides(*q.stride(), *prefix_k.stride(), *prefix_v.stride(), *k.stride(), *v.stride(),
+                             *out.stride())
     at = ctypes.addressof(strides)
     _launch("trx_attn_fwd_shared", dev, q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), k.data_ptr(),
             v.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(slopes), _ptr(lengths), B, Sq, P, S, Hq, Hk, dp,
-            at, at + 24, at + 40, at + 56, at + 80, at + 104, scale, _DTYPE_CODE[dtype], parts.data_ptr(),
-            size, ws.data_ptr(), ws.numel())
+            at, at + 32, at + 56, at + 80, at + 112, at + 144, scale, _DTYPE_CODE[dtype], _ptr(parts), size,
+            ws.data_ptr(), ws.numel())
     if size:
         _count()  # the prefix is a launch of its own
     out = out if dp == d else out[..., :d].contiguous()
