@@ -246,3 +246,37 @@ def test_no_sequences_and_no_rows(cuda):
     assert T.attention_packed(q[:0], k, v, cu_q * 0, cu_k).shape == (0, 8, 128)
     out = T.attention_packed(q, k[:0], v[:0], cu_q, cu_k * 0)
     assert not out.any()
+
+
+@pytest.mark.parametrize("B,Sq,P,hq,hk,d", [(3, 1, 6000, 8, 2, 128), (9, 28, 20_000, 8, 2, 64), (70, 2, 5000, 6, 2, 128),
+                                            (5, 1, 3000, 160, 160, 64)])
+def test_nothing_beside_the_outputs_is_written(cuda, B, Sq, P, hq, hk, d):
+    """The space for the parts, the output and the sums, each in the middle of a larger buffer."""
+    from trinix_b200 import ops
+    lib = T._lib.load()
+    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, B, Sq, P, 64, hq, hk, d, seed=110)
+    n = lengths([1 + (11 * b) % 64 for b in range(B)], cuda)
+    want, want_lse = T.attention_shared_prefix(q, pk, pv, k, v, n, return_lse=True)
+    size = lib.trx_attn_shared_bytes(B, Sq, P, 64, hq, hk, d)
+    assert size > 0
+
+    def guarded(numel, dtype):
+        t = torch.full((numel + 512,), 7, dtype=dtype, device=cuda)
+        return t, t[256:256 + numel]
+
+    parts_all, parts = guarded(size, torch.uint8)
+    out_all, out = guarded(q.numel(), torch.bfloat16)
+    lse_all, lse = guarded(B * hq * Sq, torch.float32)
+    strides = [T._lib.I64x3(*t.stride()[:3]) for t in (q, k, v)]
+    rows = [T._lib.I64x3(*t.stride()[:2], 0) for t in (pk, pv)]
+    ws = ops._workspace(cuda)
+    rc = lib.trx_attn_fwd_shared(
+        q.data_ptr(), pk.data_ptr(), pv.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+        None, n.data_ptr(), B, Sq, P, 64, hq, hk, d, strides[0], rows[0], rows[1], strides[1], strides[2],
+        T._lib.I64x3(*q.stride()[:3]), d ** -0.5, T._lib.TRX_BF16, parts.data_ptr(), size, ws.data_ptr(),
+        ws.numel(), torch.cuda.current_stream(cuda).cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize(cuda)
+    for t in (parts_all, out_all, lse_all):
+        assert bool((t[:256] == 7).all()) and bool((t[-256:] == 7).all())
+    assert torch.equal(out.view(want.shape), want) and torch.equal(lse.view(want_lse.shape), want_lse)
