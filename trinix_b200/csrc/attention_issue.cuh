@@ -1,7 +1,7 @@
-// Order of work of an issuing warp of attention_plain.cuh, without any CUDA, so that a model on the host
-// can run it too.
+// Order of work of an issuing warp of attention_plain.cuh, and how its producer comes by the next work item,
+// without any CUDA, so that models on the host can run them too.
 //
-// The work is the sequence of one Q tile's visits over all items of the CTA. The Q K^T run one visit
+// An issuing warp's work is the sequence of one Q tile's visits over all items of the CTA. The Q K^T run one visit
 // ahead of the P V, into the next item too:  .. P V(v), Q K(v + 1), P V(v + 1) ..  The K and V tiles of
 // visits without this Q tile are only released. Nothing ahead of a pending P V is waited for: the ring may
 // be held up by a V tile that this P V frees.
@@ -166,6 +166,25 @@ TRX_ISSUE bool plain_issue(Steps& s) {
     if (pc.item != qc.item || pc.v < qc.v) step_pv(pc);
   }
   return ok;
+}
+
+// The CTA's next work item: blocks of the grid that have not started are asked for until one holds rows, or
+// none is left. Which block an answer names is the hardware's choice: one without rows says nothing of those
+// that are answered after it. So every answer is looked at, and a refusal alone is the end (behind it nothing
+// may be asked for). `ask` requests a block, `there` waits for the answer (false: the CTA gives up), `look`
+// reads it and makes the block the next item if it holds rows. `more`: there is a next item.
+enum class Block { NONE_LEFT, NO_ROWS, ITEM };
+template <class Ask, class There, class Look>
+TRX_ISSUE void next_item(Ask&& ask, There&& there, Look&& look, bool& ok, bool& more) {
+  Block block;
+#pragma unroll 1
+  do {
+    ask();
+    ok = there();
+    if (!ok) break;
+    block = look();
+    more = block == Block::ITEM;
+  } while (block == Block::NO_ROWS);
 }
 
 }  // namespace trx

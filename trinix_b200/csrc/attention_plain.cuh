@@ -656,6 +656,34 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           request_block(sbase + L::NEXT_OFF, bar(B_NEXT));
           asked = true;
         };
+        auto there = [&] { return wait(B_NEXT, asks & 1); };
+        auto look = [&]() -> Block {
+          int x, y, z;
+          asked = false;
+          ++asks;
+          const bool more = requested_block(sbase + L::NEXT_OFF, x, y, z);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before it is written again
+          if (!more) {
+            w.valid = 0;
+            return Block::NONE_LEFT;
+          }
+          if constexpr (FORM == ATT_BATCH) {
+            w = plain_item(p, x, y, z);
+          } else {
+            if constexpr (FORM == ATT_PACKED) {
+              if (use_table) {
+                if (x >= table->first[p.n_seq]) return Block::NO_ROWS;
+                cursor.template look_up<ALT>(p, *table, x);
+              } else {
+                cursor.seek_alone(p, ragged_slot(p, x, y));
+                cursor.head = ragged_head(p, x, y);
+              }
+            }
+            w = ragged_item(p, cursor, x, y, z);
+          }
+          kv_heads(w, kh, vh);
+          return FORM != ATT_PACKED || ragged_has_rows(w) ? Block::ITEM : Block::NO_ROWS;
+        };
         auto fill_one = [&](int fill) {
           const int g = base + fill;
           if (g >= STAGES) ok = wait(B_KVEMPTY + g % STAGES, ((g / STAGES) & 1) ^ 1);
@@ -672,56 +700,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if constexpr (SINGLE) break;  // no other item, and no answer to wait for
           // The next item is asked for when this one's last tiles have been: some visits before its
           // end, enough to hide the answer; earlier would take items from CTAs that are done sooner.
-          bool more = false, rest = false;
-#pragma unroll 1
-          do {  // a slot between two packed sequences may hold no rows: the next one then
-            ask();
-            ok = wait(B_NEXT, asks & 1);
-            if (!ok) break;
-            asked = false;
-            ++asks;
-            int x, y, z;
-            more = requested_block(sbase + L::NEXT_OFF, x, y, z);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            if (more) {
-              if constexpr (FORM == ATT_BATCH) {
-                w = plain_item(p, x, y, z);
-              } else {
-                if constexpr (FORM == ATT_PACKED) {
-                  rest = use_table && x >= table->first[p.n_seq];  // as is every block behind it
-                  if (use_table) {
-                    cursor.template look_up<ALT>(p, *table, x);
-                  } else {
-                    cursor.seek_alone(p, ragged_slot(p, x, y));
-                    cursor.head = ragged_head(p, x, y);
-                  }
-                }
-                w = ragged_item(p, cursor, x, y, z);
-              }
-              kv_heads(w, kh, vh);
-            } else {
-              w.valid = 0;
-            }
-          } while (FORM == ATT_PACKED && more && !rest && !ragged_has_rows(w));
+          bool more = false;
+          next_item(ask, there, look, ok, more);
           if (!ok) break;
-          if (rest) {
-            more = false;
-            w.valid = 0;
-          }
           ++q;
           if (q >= 2) ok = wait(B_ITEMFREE + (q & 1), ((q >> 1) & 1) ^ 1);
           if (!ok) break;
           publish(w, q);
-          if (rest) {  // the blocks from here on have no rows: taken from the grid while the others finish
-            int x, y, z;
-            do {
-              ask();
-              ok = wait(B_NEXT, asks & 1);
-              if (!ok) break;
-              asked = false;
-              ++asks;
-            } while (requested_block(sbase + L::NEXT_OFF, x, y, z));
-          }
           if (!more) break;
           if (w.n > 0) {  // its first K tile need not wait for the Q tiles to be free
             fill_one(0);
