@@ -390,8 +390,8 @@ int trx_attn_fwd_dropout(const void* q, const void* k, const void* v, void* out,
  * (Sq == Sk), a piece of one behind cached keys and a single token (Sq == 1) need nothing else. A row
  * without a visible key returns 0 (LSE -inf).
  *   lse_or_null: fp32 (Hq, Tq);
- *   max_sq: no sequence has more rows (0: unknown). Up to 16 selects the kernel for few rows, which leaves
- *     rows beyond it unwritten;
+ *   max_sq: no sequence has more rows (0: unknown). Up to 16 selects the kernel for few rows, which does the
+ *     first max_sq rows of a longer sequence, as rows of the whole of it, and leaves the others unwritten;
  *   zero_rest: rows behind cu_q[n_seq] are written as rows without a visible key; otherwise not touched.
  * Keys outside a sequence are never used, whatever their values (NaN among them).
  * `workspace` as for trx_attn_fwd. No counterpart in the reference, whose attention takes one batch of

@@ -116,6 +116,31 @@ def test_few_rows(cuda, how, heads, kv, dim):
     assert torch.equal(held[:n], out[:n]) and torch.equal(held[n:], q[n:])
 
 
+@pytest.mark.parametrize("how", [dict(causal=True), dict(), dict(window=(20, 0)), dict(causal=True, alibi=True)],
+                         ids=str)
+@pytest.mark.parametrize("most,heads", [(1, 8), (3, 8), (16, 2)])
+def test_rows_beyond_the_announced_ones(cuda, how, most, heads):
+    """A sequence of more rows than max_seqlen_q: its first rows are those of the whole sequence, the others
+    stay as they were."""
+    how = dict(how)
+    slopes = slopes_of(heads, cuda) if how.pop("alibi", False) else None
+    len_q, len_k = [most + 1, 1, most, 40, most + 5], [60, 9, 300, 40, 3]
+    q = make(56, cuda, torch.bfloat16, sum(len_q), heads, 64)
+    k, v = (make(i, cuda, torch.bfloat16, sum(len_k), 2, 64) for i in (57, 58))
+    held = make(59, cuda, torch.bfloat16, *q.shape)
+    out, lse = T.attention_packed(q, k, v, starts(len_q, cuda), starts(len_k, cuda), max_seqlen_q=most,
+                                  alibi_slopes=slopes, return_lse=True, out=held.clone(), **how)
+    row = key = 0
+    for n, m in zip(len_q, len_k):
+        want, want_lse, allowed, allowed_lse = attend64(q[row:row + n], k[key:key + m], v[key:key + m],
+                                                        slopes=slopes, **how)
+        done = min(n, most)
+        assert_within(out[row:row + done], want[:done], allowed[:done], f"{n} rows")
+        assert_within(lse[:, row:row + done], want_lse[:, :done], allowed_lse[:, :done], f"lse of {n} rows")
+        assert torch.equal(out[row + done:row + n], held[row + done:row + n])
+        row, key = row + n, key + m
+
+
 def test_scales_next_to_nothing(cuda):
     """A ramp divided by the scale would not be finite."""
     lens = [40, 300]

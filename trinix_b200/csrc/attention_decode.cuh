@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
     }
     b = by_keys(p, b);
     q0 = ragged_row(p, b);
-    sq = min(max(0, ragged_row(p, b + 1) - q0), p.Sq);
+    sq = max(0, ragged_row(p, b + 1) - q0);
     k0 = ragged_key(p, b);
     sk = max(0, ragged_key(p, b + 1) - k0);
   }
@@ -158,8 +158,11 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
     sk = ragged_length(p, b);
   }
   if constexpr (FORM != ATT_BATCH) {
-    if (r0 >= group * sq) return;  // the whole cluster: a shorter sequence than the longest
+    // positions go by all rows of the sequence, where they are more than the caller announced too: of those
+    // the first p.Sq are done
     shift = sk - sq;
+    sq = min(sq, p.Sq);
+    if (r0 >= group * sq) return;  // the whole cluster: a shorter sequence than the longest
   }
   const int rows = group * sq;
 

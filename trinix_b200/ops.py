@@ -751,9 +751,10 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     call. A row that sees nothing is 0.
 
     max_seqlen_q, if given, promises that no sequence has more rows; up to 16 selects the kernel for
-    decoding, which leaves rows beyond it unwritten. Rows behind cu_seqlens_q[-1] are 0 in a new
-    output; in `out`, if given (it then is the result), they stay what they were. With return_lse
-    also the fp32 (Hq, Tq) log-sum-exp, -inf for rows without a key and rows behind the last.
+    decoding, which of a longer sequence does the first max_seqlen_q rows only: the others are left
+    unwritten, in a new output uninitialised. Rows behind cu_seqlens_q[-1] are 0 in a new output; in
+    `out`, if given (it then is the result), they stay what they were. With return_lse also the fp32
+    (Hq, Tq) log-sum-exp, -inf for rows without a key and rows behind the last.
     Forward only, as `attention`: PackedAttentionKernel.apply has a later .backward() say so.
     """
     dev = _same_device(q, k, v, cu_seqlens_q, cu_seqlens_k, alibi_slopes, out)
