@@ -71,6 +71,23 @@ def test_shared_entry_refuses(lib, change, code):
     assert shared(lib, **change) == code
 
 
+# in parts; the sequences' own keys alone, by the kernel for few rows, which makes no tensor map of q; one pass
+@pytest.mark.parametrize("way", [dict(), dict(p=0), dict(p=0, sq=16), dict(p=0, sq=17), dict(p=9, sq=200)], ids=str)
+@pytest.mark.parametrize("change,code", [
+    (dict(qs=I64x3(1 << 20, 512, 132)), -4), (dict(qs=I64x3((1 << 20) + 4, 512, 128)), -4),
+    (dict(qs=I64x3(1 << 20, 512, 129)), -4), (dict(q=ctypes.c_void_p(4098)), -4), (dict(q=ctypes.c_void_p(4104)), -4),
+    (dict(qs=I64x3(1 << 20, 512, 64)), -5), (dict(qs=I64x3(64, 512, 128)), -5), (dict(qs=I64x3(0, 512, 128)), -5),
+], ids=str)
+def test_shared_entry_refuses_queries_it_cannot_read(lib, way, change, code):
+    assert shared(lib, **way, **change) == code
+
+
+@pytest.mark.parametrize("way", [dict(p=0, sq=16), dict(p=0, sq=17), dict(p=9, sq=200)], ids=str)
+def test_shared_entry_refuses_rows_of_queries_it_cannot_read(lib, way):
+    assert shared(lib, qs=I64x3(1 << 20, 516, 128), **way) == -4
+    assert shared(lib, qs=I64x3(1 << 20, 120, 128), **way) == -5
+
+
 def test_shared_entry_has_nothing_to_do(lib):
     assert shared(lib, b=0) == 0
     assert shared(lib, sq=0) == 0

@@ -357,12 +357,10 @@ __device__ __forceinline__ RaggedTile ragged_tile(const RaggedParamsOf<FORM, ALT
 // ------------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------------
-// (B, rows, H, D) queries for tiles of `heads` heads x `tokens` rows: dims D, head in tile, row, tile of
-// heads, B.
-inline int make_ragged_q_map(CUtensorMap* tm, const void* base, int is_bf16, int64_t D, int64_t rows, int64_t H,
-                             int64_t B, int64_t sb, int64_t ss, int64_t sh, int heads, int tokens) {
-  EncodeTiledFn enc = get_encode_fn();
-  if (!enc) return TRX_ERR_CUDA;
+// What base and element strides of (B, rows, H, D) queries have to be, for their tensor map and for the decode
+// kernel's 4-byte loads. Dims of size 1 may carry any stride: they are given a legal one.
+inline int check_ragged_q(const void* base, int64_t D, int64_t rows, int64_t H, int64_t B, int64_t& sb, int64_t& ss,
+                          int64_t& sh) {
   if (!aligned_to(base, 16)) return TRX_ERR_ALIGNMENT;
   if (rows == 1) ss = D;
   if (H == 1) sh = D;
@@ -370,6 +368,16 @@ inline int make_ragged_q_map(CUtensorMap* tm, const void* base, int is_bf16, int
   if (ss < D || sh < D || sb < D) return TRX_ERR_STRIDE;
   if (ss % 8 || sh % 8 || sb % 8) return TRX_ERR_ALIGNMENT;
   if (ss >= (1ll << 38) || sh >= (1ll << 30) || sb >= (1ll << 38)) return TRX_ERR_STRIDE;
+  return TRX_OK;
+}
+
+// Queries for tiles of `heads` heads x `tokens` rows: dims D, head in tile, row, tile of heads, B.
+inline int make_ragged_q_map(CUtensorMap* tm, const void* base, int is_bf16, int64_t D, int64_t rows, int64_t H,
+                             int64_t B, int64_t sb, int64_t ss, int64_t sh, int heads, int tokens) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return TRX_ERR_CUDA;
+  const int rc = check_ragged_q(base, D, rows, H, B, sb, ss, sh);
+  if (rc != TRX_OK) return rc;
   const cuuint64_t dims[5] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads),
                               static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(H / heads),
                               static_cast<cuuint64_t>(B)};

@@ -132,6 +132,9 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
     if (q_strides[i] < 0 || k_strides[i] < 0 || v_strides[i] < 0 || o_strides[i] < 0 ||
         (i < 2 && (pk_strides[i] < 0 || pv_strides[i] < 0)))
       return TRX_ERR_STRIDE;
+  int64_t qb = q_strides[0], qs = q_strides[1], qh = q_strides[2];
+  int rc = check_ragged_q(q, D, Sq, Hq, B, qb, qs, qh);  // whichever way is taken: one of them makes no map of q
+  if (rc != TRX_OK) return rc;
 
   SharedPlan plan = shared_plan(B, Sq, P, S, Hq, Hk);
   // the rows of the batch as one run: what the prefix's launch wants
@@ -148,7 +151,7 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   const int is_bf16 = dtype == TRX_BF16, tokens = plan.tile.tile_tokens, heads = plan.tile.tile_heads;
   const int box = plan.in_parts ? DEC_KEYS : ATT_BN;
   // without keys nothing is loaded: any legal map
-  int rc = make_map(&p.tm_k, S > 0 ? k : q, is_bf16, D, S > 0 ? S : 1, Hk, B, k_strides[0], k_strides[1],
+  rc = make_map(&p.tm_k, S > 0 ? k : q, is_bf16, D, S > 0 ? S : 1, Hk, B, k_strides[0], k_strides[1],
                     k_strides[2], box);
   if (rc != TRX_OK) return rc;
   rc = make_map(&p.tm_v, S > 0 ? v : q, is_bf16, D, S > 0 ? S : 1, Hk, B, v_strides[0], v_strides[1],
