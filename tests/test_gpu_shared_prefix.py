@@ -191,3 +191,13 @@ def test_prompts_then_tokens(cuda):
         tok = make(90 + step, cuda, torch.bfloat16, B, 1, hq, d)
         out, lse = T.attention_shared_prefix(tok, pk, pv, k, v, lengths(lens, cuda), return_lse=True)
         check(out, lse, tok, pk, pv, k, v, lens)
+
+
+def test_more_rows_than_a_grid_holds(cuda):
+    """Rows of the batch in more blocks than the prefix's launch has room for: one pass, whatever a cost says."""
+    B, Sq, P, hq = 50_000, 3, 6000, 128
+    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 1, Sq, P, 8, hq, 1, 64, seed=70)
+    many = [t.expand(B, -1, -1, -1).contiguous() for t in (q, k, v)]  # 2.5 GB of queries
+    out = T.attention_shared_prefix(many[0], pk, pv, *many[1:])
+    check(out[:1], None, q, pk, pv, k, v, [8])
+    assert bool((out == out[:1]).all())

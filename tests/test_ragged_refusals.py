@@ -107,6 +107,17 @@ def test_shared_bytes(lib):
         assert size(*bad) == 0
 
 
+@pytest.mark.parametrize("b,sq,hq,rows", [(50_000, 3, 128, 2), (65_535, 5, 64, 4), (50_000, 12, 32, 8),
+                                          (65_535, 20, 16, 16)])
+def test_shared_bytes_of_more_rows_than_a_grid_holds(lib, b, sq, hq, rows):
+    """`rows` of the batch are a block of the prefix's launch, which has room for 65535 of them: beyond that the
+    call takes one pass, whatever a cost says."""
+    size = lib.trx_attn_shared_bytes
+    assert b * sq > 65535 * rows
+    assert size(b, sq, 6000, 20, hq, 1, 128) == 0
+    assert size(65535 * rows // sq, sq, 6000, 20, hq, 1, 128) > 0
+
+
 def test_cpu_tensors_are_refused_behind_a_prefix():
     q, pk = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16), torch.zeros(5, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):

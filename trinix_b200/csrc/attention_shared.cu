@@ -69,6 +69,7 @@ static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t S, int64
     return s;
   }
   const int64_t rows = B * Sq, tiles = up(P, ATT_BN), items = s.tile.head_tiles * up(rows, step);
+  if (up(rows, step) > 65535) return s;  // more blocks of rows than the prefix's grid holds
   int64_t splits = sms / items;
   splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
   s.split_tiles = static_cast<int>(up(tiles, splits));
