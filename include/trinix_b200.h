@@ -412,7 +412,8 @@ int trx_attn_fwd_packed(const void* q, const void* k, const void* v, void* out, 
  * values (NaN among them). q, out (B, Sq, Hq, D): the last Sq tokens of each sequence. Over the P + lengths[b]
  * keys of the concatenation this is causal attention of trx_attn_fwd_packed: query i stands at
  * P + lengths[b] - Sq + i and sees the keys up to there; slopes_or_null (ALiBi) counts from there.
- * scale >= 1e-30. lse_or_null: fp32 (B, Hq, Sq).
+ * scale >= 1e-30. lse_or_null: fp32 (B, Hq, Sq). TRX_ERR_SHAPE beyond B, Hq = 65535, B * Sq = 2^30,
+ * P, S = 2^29, Sq = 65535 * 256.
  * With few rows to a sequence, or a long prefix, the prefix is read and computed once for all sequences, its
  * keys split over the GPU (a choice by sizes alone); the splits' results need `parts`:
  * trx_attn_shared_bytes(...) bytes of device memory, asked for with the call's device current, 16-byte

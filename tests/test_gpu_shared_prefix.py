@@ -201,3 +201,13 @@ def test_more_rows_than_a_grid_holds(cuda):
     out = T.attention_shared_prefix(many[0], pk, pv, *many[1:])
     check(out[:1], None, q, pk, pv, k, v, [8])
     assert bool((out == out[:1]).all())
+
+
+def test_more_rows_of_a_sequence_than_a_grid_holds(cuda):
+    """One sequence whose rows, at 128 heads to a tile, are more blocks than one pass has room for."""
+    Sq, P, n, hq = 131_075, 100, 150, 128
+    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 1, Sq, P, 200, hq, 1, 64, seed=80)  # 2.1 GB of queries
+    out, lse = T.attention_shared_prefix(q, pk, pv, k, v, lengths([n], cuda), return_lse=True)
+    last = 300  # of which the first 50 stand in front of every key, as do all rows before them
+    check(out[:, -last:], lse[:, :, -last:], q[:, -last:], pk, pv, k, v, [n])
+    assert not out[:, :-last].any() and bool((lse[:, :, :-last] == float("-inf")).all())

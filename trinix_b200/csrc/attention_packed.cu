@@ -78,7 +78,7 @@ extern "C" int trx_attn_fwd_packed(const void* q, const void* k, const void* v, 
   const int is_bf16 = dtype == TRX_BF16;
   p.Hq = static_cast<int>(Hq);
   p.group = static_cast<int>(Hq / Hk);
-  choose_tile(p);
+  choose_tile(p, 0);  // blocks of rows may run along the grid's other dimension
   int rc = make_ragged_q_map(&p.tm_q, q, is_bf16, D, Tq, Hq, 1, 0, q_strides[0], q_strides[1], p.tile_heads,
                              p.tile_tokens);
   if (rc != TRX_OK) return rc;

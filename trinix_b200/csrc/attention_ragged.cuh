@@ -393,11 +393,13 @@ inline int make_ragged_q_map(CUtensorMap* tm, const void* base, int is_bf16, int
 }
 
 // Query heads of one tile, and tokens: as many heads of the group as leave at most a tenth of a tile's 128
-// rows unused. (A group of 71 heads is none but 1 and 71, and 71 would leave 57 rows.)
-inline void choose_tile(RaggedParams& p) {  // from its Hq and group
+// rows unused, and a run of `rows` no more blocks than a grid's dimension holds. (A group of 71 heads is none
+// but 1 and 71, and 71 would leave 57 rows.)
+inline void choose_tile(RaggedParams& p, int64_t rows) {  // from its Hq and group
   p.tile_heads = 1;
   for (int h = 2; h <= p.group && h <= ATT_BM; ++h)
-    if (p.group % h == 0 && ATT_BM / h * h * 10 >= ATT_BM * 9) p.tile_heads = h;
+    if (p.group % h == 0 && ATT_BM / h * h * 10 >= ATT_BM * 9 && rows <= 65535ll * ATT_NQ * (ATT_BM / h))
+      p.tile_heads = h;
   p.tile_tokens = ATT_BM / p.tile_heads;
   p.per_head = (65536 + p.tile_heads - 1) / p.tile_heads;
   p.head_tiles = p.Hq / p.tile_heads;

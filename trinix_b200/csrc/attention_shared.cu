@@ -58,7 +58,7 @@ static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t S, int64
   SharedPlan s{};
   s.tile.Hq = static_cast<int>(Hq);
   s.tile.group = static_cast<int>(Hq / Hk);
-  choose_tile(s.tile);
+  choose_tile(s.tile, Sq);
   const int64_t sms = sm_count_of_current_device(), tokens = s.tile.tile_tokens, step = ATT_NQ * tokens;
   const bool wide = s.tile.group * Sq > 16;
   const int64_t row_tiles = (s.tile.group * Sq + (wide ? 31 : 15)) / (wide ? 32 : 16);
