@@ -1,4 +1,6 @@
 """How programs use the packed and the shared-prefix attention: streams, graphs, failures, autograd."""
+import ctypes
+
 import pytest
 import torch
 
@@ -151,6 +153,58 @@ def test_recorded_failure(cuda, kind):
     again = run(s)
     assert torch.equal(again[0], good[0]) and torch.equal(again[1], good[1])
     assert T.attention_status(cuda) == 0
+
+
+def call_packed(lib, s, out, lse, ws, max_rows=0):
+    """The C entry, which zeroes rows behind the last sequence."""
+    q, k, v, cu_q, cu_k = s
+    strides = [(ctypes.c_int64 * 2)(*t.stride()[:2]) for t in (q, k, v, out)]
+    return lib.trx_attn_fwd_packed(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), None, cu_q.data_ptr(),
+        cu_k.data_ptr(), cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], *strides,
+        q.shape[2] ** -0.5, 1, -1, -1, max_rows, 1, T._lib.TRX_BF16, ws.data_ptr(), ws.numel(),
+        torch.cuda.current_stream(q.device).cuda_stream)
+
+
+def call_shared(lib, s, out, lse, ws):
+    q, pk, pv, k, v, n = s
+    B, Sq, hq, d = q.shape
+    sizes = B, Sq, pk.shape[0], k.shape[1], hq, k.shape[2], d
+    size = lib.trx_attn_shared_bytes(*sizes)
+    parts = torch.empty(max(size, 1), dtype=torch.uint8, device=q.device)
+    st = [T._lib.I64x3(*t.stride()[:3]) for t in (q, k, v, out)]
+    rows = [T._lib.I64x3(*t.stride()[:2], 0) for t in (pk, pv)]
+    return lib.trx_attn_fwd_shared(
+        q.data_ptr(), pk.data_ptr(), pv.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+        None, n.data_ptr(), *sizes, st[0], *rows, st[1], st[2], st[3], d ** -0.5, T._lib.TRX_BF16,
+        parts.data_ptr(), size, ws.data_ptr(), ws.numel(), torch.cuda.current_stream(q.device).cuda_stream)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_nothing_is_written_behind_a_recorded_failure(cuda, kind):
+    """Output and sums of a launch that finds one, rows behind the last sequence among them. Set from the host,
+    in a workspace of its own."""
+    lib = T._lib.load()
+    s = KINDS[kind][0](cuda, 120)
+    if kind.startswith("packed"):
+        spare = torch.cat((s[0], s[0][:3]))  # three rows of no sequence
+        s = (spare, *s[1:])
+        shape, most = (s[0].shape[1], s[0].shape[0]), 3 if "few" in kind else 0
+        call = lambda *a: call_packed(*a, max_rows=most)  # noqa: E731
+    else:
+        shape, call = (s[0].shape[0], s[0].shape[2], s[0].shape[1]), call_shared
+    out, lse = torch.full_like(s[0], 7.0), torch.full(shape, 7.0, device=cuda)
+    ws = torch.zeros(256, dtype=torch.uint8, device=cuda)
+    ws[:4].view(torch.int32).fill_(4)
+    assert call(lib, s, out, lse, ws) == 0
+    torch.cuda.synchronize(cuda)
+    assert bool((out == 7.0).all()) and bool((lse == 7.0).all())
+    ws.zero_()
+    assert call(lib, s, out, lse, ws) == 0
+    if kind.startswith("packed"):
+        check_packed(out, lse, *s[:3], s[3].diff().tolist(), s[4].diff().tolist(), causal=True)
+    else:
+        check_shared(out, lse, *s[:5], s[5].tolist())
 
 
 def test_kernel_classes(cuda):

@@ -102,9 +102,14 @@ __device__ __forceinline__ int by_keys(const P& p, int z) {
   return found;
 }
 
-// Rows behind the last packed sequence: 0, LSE -inf.
+// Rows behind the last packed sequence: 0, LSE -inf. Not in a launch that follows a recorded failure, which
+// writes nothing; the CTA decides as one, and a row of a head is one CTA's.
 template <int D>
 __device__ __forceinline__ void zero_rest(const RaggedParams& p) {
+  if (__syncthreads_or(*reinterpret_cast<volatile unsigned int*>(p.status) != 0u)) {
+    if (threadIdx.x == 0) report_status(p.status);
+    return;
+  }
   const int row0 = ragged_row(p, p.n_cu);
   const long long n = static_cast<long long>(p.rows - row0) * p.Hq * (D / 8);
   const long long step = static_cast<long long>(gridDim.x) * gridDim.y * DEC_THREADS;
