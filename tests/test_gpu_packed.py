@@ -300,3 +300,17 @@ def test_more_blocks_than_a_grid_dimension_holds(cuda, few):
         want = (torch.softmax(s, -1)[..., None] * torch.stack((v[two, 0], v[two + 1, 0]), 1).double()).sum(1)
         # one rounding of each of two probabilities and one of the result, weights far closer
         assert float((out[two + 1].double() - want).abs().max()) <= 2.01 * 2 ** -8 * float(v.abs().max())
+
+
+@pytest.mark.parametrize("most", [None, 1])
+def test_strides_of_one_row(cuda, most):
+    """An output of one row, whatever the stride of its rows."""
+    q, k, v = (make(60 + i, cuda, torch.bfloat16, n, h, 64) for i, (n, h) in enumerate([(1, 8), (50, 2), (50, 2)]))
+    buf = make(64, cuda, torch.bfloat16, 3, 8 * 64 + 4)
+    held = buf.clone()
+    out = buf[:, :512].unflatten(1, (8, 64))[:1]
+    assert out.stride(0) % 8
+    got = T.attention_packed(q, k, v, starts([1], cuda), starts([50], cuda), causal=True, max_seqlen_q=most, out=out)
+    assert got is out
+    check(out, None, q, k, v, [1], [50], causal=True)
+    assert torch.equal(buf[1:], held[1:]) and torch.equal(buf[0, 512:], held[0, 512:])

@@ -70,7 +70,8 @@ extern "C" int trx_attn_fwd_packed(const void* q, const void* k, const void* v, 
     return TRX_ERR_WORKSPACE;
   if (Tq >= (1ll << 30) || Tk >= (1ll << 30) || n_seq >= (1ll << 24) || Hq > 65535) return TRX_ERR_SHAPE;
   if (!aligned_to(cu_q, 4) || !aligned_to(cu_k, 4)) return TRX_ERR_ALIGNMENT;
-  if (!aligned_to(out, 16) || o_strides[0] % 8 || o_strides[1] % 8) return TRX_ERR_ALIGNMENT;
+  // (a dim of size 1 may carry any stride)
+  if (!aligned_to(out, 16) || (Tq > 1 && o_strides[0] % 8) || (Hq > 1 && o_strides[1] % 8)) return TRX_ERR_ALIGNMENT;
   for (int i = 0; i < 2; ++i)
     if (q_strides[i] < 0 || k_strides[i] < 0 || v_strides[i] < 0 || o_strides[i] < 0) return TRX_ERR_STRIDE;
 
