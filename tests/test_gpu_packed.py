@@ -314,3 +314,13 @@ def test_strides_of_one_row(cuda, most):
     assert got is out
     check(out, None, q, k, v, [1], [50], causal=True)
     assert torch.equal(buf[1:], held[1:]) and torch.equal(buf[0, 512:], held[0, 512:])
+
+
+@pytest.mark.parametrize("most", [None, 1])
+def test_strides_of_tensors_without_keys(cuda, most):
+    """Keys and values without a row, whatever their strides are."""
+    q, k = make(60, cuda, torch.bfloat16, 1, 8, 64), make(61, cuda, torch.bfloat16, 5, 2, 64)
+    for empty in (make(65, cuda, torch.bfloat16, 7, 2, 68)[:0, :, :64], k[:0, :1].expand(-1, 4, -1)):
+        got, lse = T.attention_packed(q, empty, empty, starts([1], cuda), starts([0], cuda), max_seqlen_q=most,
+                                      return_lse=True)
+        assert not got.any() and bool((lse == float("-inf")).all())

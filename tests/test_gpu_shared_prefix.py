@@ -211,3 +211,15 @@ def test_more_rows_of_a_sequence_than_a_grid_holds(cuda):
     last = 300  # of which the first 50 stand in front of every key, as do all rows before them
     check(out[:, -last:], lse[:, :, -last:], q[:, -last:], pk, pv, k, v, [n])
     assert not out[:, :-last].any() and bool((lse[:, :, :-last] == float("-inf")).all())
+
+
+@pytest.mark.parametrize("Sq,P", [(1, 40), (1, 5000), (30, 200)])
+def test_strides_of_tensors_without_keys(cuda, Sq, P):
+    """A prefix, or caches, without keys: whatever their strides are."""
+    q, pk, pv, k, v = inputs(cuda, torch.bfloat16, 3, Sq, P, 50, 8, 2, 64, seed=90)
+    nothing = make(95, cuda, torch.bfloat16, 7, 2, 68)[:0, :, :64]
+    out, lse = T.attention_shared_prefix(q, nothing, nothing, k, v, return_lse=True)
+    check(out, lse, q, pk[:0], pv[:0], k, v, [50] * 3)
+    for empty in (make(96, cuda, torch.bfloat16, 3, 7, 2, 68)[:, :0, :, :64], k[:, :0, :1].expand(-1, -1, 2, -1)):
+        out, lse = T.attention_shared_prefix(q, pk, pv, empty, empty, return_lse=True)
+        check(out, lse, q, pk, pv, empty, empty, [0] * 3)

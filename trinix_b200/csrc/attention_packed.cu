@@ -87,11 +87,9 @@ extern "C" int trx_attn_fwd_packed(const void* q, const void* k, const void* v, 
   const int64_t row_tiles = (p.group * max_sq + 15) / 16;
   const bool decode = max_sq > 0 && max_sq <= 16 && n_seq > 0 && n_seq < 65535 && Hk * row_tiles <= 65535;
   const int box = decode ? DEC_KEYS : ATT_BN;
-  // without keys nothing is loaded: any legal map
-  const void *kk = Tk > 0 ? k : q, *vv = Tk > 0 ? v : q;
-  rc = make_map(&p.tm_k, kk, is_bf16, D, Tk > 0 ? Tk : 1, Hk, 1, 0, k_strides[0], k_strides[1], box);
+  rc = make_ragged_kv_map(&p.tm_k, k, q, is_bf16, D, Tk, Hk, 1, 0, k_strides[0], k_strides[1], box);
   if (rc != TRX_OK) return rc;
-  rc = make_map(&p.tm_v, vv, is_bf16, D, Tk > 0 ? Tk : 1, Hk, 1, 0, v_strides[0], v_strides[1], box);
+  rc = make_ragged_kv_map(&p.tm_v, v, q, is_bf16, D, Tk, Hk, 1, 0, v_strides[0], v_strides[1], box);
   if (rc != TRX_OK) return rc;
   p.out = out;
   p.lse = lse_or_null;

@@ -371,6 +371,14 @@ inline int check_ragged_q(const void* base, int64_t D, int64_t rows, int64_t H, 
   return TRX_OK;
 }
 
+// Keys or values (B, rows, H, D). Without rows nothing is loaded: any legal map, whatever strides a tensor
+// without elements carries; `other` is memory for it.
+inline int make_ragged_kv_map(CUtensorMap* tm, const void* base, const void* other, int is_bf16, int64_t D,
+                              int64_t rows, int64_t H, int64_t B, int64_t sb, int64_t ss, int64_t sh, int box_rows) {
+  if (rows == 0) return make_map(tm, other, is_bf16, D, 1, 1, 1, D, D, D, box_rows);
+  return make_map(tm, base, is_bf16, D, rows, H, B, sb, ss, sh, box_rows);
+}
+
 // Queries for tiles of `heads` heads x `tokens` rows: dims D, head in tile, row, tile of heads, B.
 inline int make_ragged_q_map(CUtensorMap* tm, const void* base, int is_bf16, int64_t D, int64_t rows, int64_t H,
                              int64_t B, int64_t sb, int64_t ss, int64_t sh, int heads, int tokens) {

@@ -151,18 +151,13 @@ extern "C" int trx_attn_fwd_shared(const void* q, const void* prefix_k, const vo
   SharedParams p{};
   const int is_bf16 = dtype == TRX_BF16, tokens = plan.tile.tile_tokens, heads = plan.tile.tile_heads;
   const int box = plan.in_parts ? DEC_KEYS : ATT_BN;
-  // without keys nothing is loaded: any legal map
-  rc = make_map(&p.tm_k, S > 0 ? k : q, is_bf16, D, S > 0 ? S : 1, Hk, B, k_strides[0], k_strides[1],
-                    k_strides[2], box);
+  rc = make_ragged_kv_map(&p.tm_k, k, q, is_bf16, D, S, Hk, B, k_strides[0], k_strides[1], k_strides[2], box);
   if (rc != TRX_OK) return rc;
-  rc = make_map(&p.tm_v, S > 0 ? v : q, is_bf16, D, S > 0 ? S : 1, Hk, B, v_strides[0], v_strides[1],
-                v_strides[2], box);
+  rc = make_ragged_kv_map(&p.tm_v, v, q, is_bf16, D, S, Hk, B, v_strides[0], v_strides[1], v_strides[2], box);
   if (rc != TRX_OK) return rc;
-  rc = make_map(&p.tm_pk, P > 0 ? prefix_k : q, is_bf16, D, P > 0 ? P : 1, Hk, 1, 0, pk_strides[0],
-                pk_strides[1], ATT_BN);
+  rc = make_ragged_kv_map(&p.tm_pk, prefix_k, q, is_bf16, D, P, Hk, 1, 0, pk_strides[0], pk_strides[1], ATT_BN);
   if (rc != TRX_OK) return rc;
-  rc = make_map(&p.tm_pv, P > 0 ? prefix_v : q, is_bf16, D, P > 0 ? P : 1, Hk, 1, 0, pv_strides[0],
-                pv_strides[1], ATT_BN);
+  rc = make_ragged_kv_map(&p.tm_pv, prefix_v, q, is_bf16, D, P, Hk, 1, 0, pv_strides[0], pv_strides[1], ATT_BN);
   if (rc != TRX_OK) return rc;
   p.tile_heads = heads;
   p.tile_tokens = tokens;
