@@ -324,3 +324,27 @@ def test_strides_of_tensors_without_keys(cuda, most):
         got, lse = T.attention_packed(q, empty, empty, starts([1], cuda), starts([0], cuda), max_seqlen_q=most,
                                       return_lse=True)
         assert not got.any() and bool((lse == float("-inf")).all())
+
+
+# the table of a launch of several items per CTA: its order within every 128 sequences, its sum over all threads,
+# its last entry (1024 sequences, or 1023 and the rows behind them; one more takes the search)
+@pytest.mark.parametrize("count", [127, 128, 129, 300, 1023, 1024, 1025])
+@pytest.mark.parametrize("short", [True, False])  # items of two tiles of heads, or of one
+@pytest.mark.parametrize("spare", [0, 5])
+def test_table_of_items(cuda, count, short, spare):
+    g = torch.Generator().manual_seed(count)
+    most = 16 if short else 70  # 8 heads of a group: 16 tokens to a tile
+    len_q = torch.randint(0, most + 1, (count,), generator=g).tolist()
+    len_q[0], len_q[-1], len_q[count // 2] = 0, most, 3 * most
+    len_k = [n + m for n, m in zip(len_q, torch.randint(0, 150, (count,), generator=g).tolist())]
+    rows = sum(len_q)
+    assert (16 * count >= rows) == short
+    q = make(66, cuda, torch.bfloat16, rows + spare, 16, 64)
+    k, v = (make(i, cuda, torch.bfloat16, sum(len_k), 2, 64) for i in (67, 68))
+    cu = starts(len_q, cuda), starts(len_k, cuda)
+    out, lse = T.attention_packed(q, k, v, *cu, causal=True, return_lse=True)
+    check(out, lse, q, k, v, len_q, len_k, causal=True)
+    held = make(69, cuda, torch.bfloat16, *q.shape)
+    again, lse2 = T.attention_packed(q, k, v, *cu, causal=True, return_lse=True, out=held.clone())
+    assert torch.equal(again[:rows], out[:rows]) and torch.equal(again[rows:], held[rows:])
+    assert torch.equal(lse2, lse)
