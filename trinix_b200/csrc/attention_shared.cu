@@ -48,12 +48,14 @@ struct SharedPlan {
 };
 // The cost, in us: a launch of attention_plain.cuh starts and ends in 6, an item in 4.5, a KV tile takes 1.95
 // with both Q tiles at work on it, 1.5 with one, 0.95 with every second one each; the decode kernel by its
-// own cost (decode_cost), more with two row tiles to a warp, 0.15 for each part that it merges. Over 54
-// shapes (1 to 32 sequences of 4 to 160 rows behind 500 to 30000 keys, 16 / 16 heads x 64, 32 / 4 and 32 / 8
-// x 128) the way that it picks is 1 % slower than the better one in the mean, 15 % at worst. In parts / one
-// pass, 32 / 8 heads x 128: 32 x 4 rows behind 8192 keys 38 / 202 us, 32 x 48 351 / 268, 4 x 48 53 / 113, 16 x
-// 8 behind 1024 37 / 26, 1 x 8 behind 500 16.7 / 14.8. One pass for more than 16 rows and only then: up to 4
-// times as long (4 x 24 behind 8192 42 / 104).
+// own cost (decode_cost), more with two row tiles to a warp, 0.15 for each part that it merges. Fitted to
+// 1 to 32 sequences of 4 to 160 rows behind 500 to 30000 keys with 16 / 16 heads x 64, 32 / 4 and 32 / 8 x 128.
+// Over 84 shapes of six head configurations, 1 to 300 own keys, with and without ALiBi, the way that it picks is
+// slower than the better one by 1 % in the mean and 27 % at worst behind 1024 and more keys (4 x 48 rows, 32 / 8
+// heads x 128, behind 1024: 33.6 / 26.4 us in parts / one pass); by 21 % in the mean and 72 % at worst behind 300 and
+// 500, where it takes one pass too often (8 x 1 behind 300, 16 / 16 heads x 64: 10.1 / 17.4). In parts / one pass,
+// 32 / 8 heads x 128: 32 x 4 rows behind 8192 keys 38 / 202 us, 32 x 48 351 / 268, 4 x 48 53 / 113, 16 x 8 behind 1024
+// 37 / 26. One pass for more than 16 rows and only then: up to 4 times as long (4 x 24 behind 8192 42 / 104).
 static SharedPlan shared_plan(int64_t B, int64_t Sq, int64_t P, int64_t S, int64_t Hq, int64_t Hk) {
   SharedPlan s{};
   s.tile.Hq = static_cast<int>(Hq);
