@@ -348,3 +348,33 @@ def test_table_of_items(cuda, count, short, spare):
     again, lse2 = T.attention_packed(q, k, v, *cu, causal=True, return_lse=True, out=held.clone())
     assert torch.equal(again[:rows], out[:rows]) and torch.equal(again[rows:], held[rows:])
     assert torch.equal(lse2, lse)
+
+
+def test_hundreds_of_thousands_of_empty_sequences(cuda):
+    """Blocks without rows by the million, between two that hold some: longer than any wait may last."""
+    n, heads = 500_000, 64
+    at = 1000
+    cu = torch.zeros(n + 1, dtype=torch.int32, device=cuda)
+    cu[at:] = 150
+    cu[-1] = 350
+    q, k, v = (make(70 + i, cuda, torch.bfloat16, 353, heads, 64) for i in range(3))
+    out, lse = T.attention_packed(q, k[:350], v[:350], cu, causal=True, return_lse=True)
+    check(out, lse, q, k[:350], v[:350], [150, 200], [150, 200], causal=True)
+    assert T.attention_status(cuda) == 0
+
+
+def test_hundreds_of_thousands_of_rows_without_keys(cuda):
+    """Items that load nothing, for longer than any wait may last, behind one that does."""
+    n, heads = 400_000, 64
+    q = make(74, cuda, torch.bfloat16, n + 150, heads, 64)  # 3.3 GB
+    k, v = (make(i, cuda, torch.bfloat16, 300, heads, 64) for i in (75, 76))
+    cu_q = torch.arange(150, n + 151, dtype=torch.int32, device=cuda)
+    cu_q[0] = 0
+    cu_k = torch.full((n + 1,), 150, dtype=torch.int32, device=cuda)
+    cu_k[0], cu_k[-1] = 0, 300
+    out, lse = T.attention_packed(q, k, v, cu_q, cu_k, causal=True, return_lse=True)
+    first, last = slice(0, 151), slice(n + 149, n + 150)
+    check(out[first], lse[:, first], q[first], k[:150], v[:150], [151], [150], causal=True)
+    check(out[last], lse[:, last], q[last], k[150:], v[150:], [1], [150], causal=True)
+    assert not out[151:-1].any() and bool((lse[:, 151:-1] == float("-inf")).all())
+    assert T.attention_status(cuda) == 0

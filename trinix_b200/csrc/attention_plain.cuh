@@ -667,12 +667,15 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             w.valid = 0;
             return Block::NONE_LEFT;
           }
+          // Every 4096th answer (some 40 ms) is an item whether or not it holds rows: no role waits for the next
+          // one longer than that, however many blocks hold none.
+          const bool pass = FORM == ATT_PACKED && (asks & 4095) != 0;
           if constexpr (FORM == ATT_BATCH) {
             w = plain_item(p, x, y, z);
           } else {
             if constexpr (FORM == ATT_PACKED) {
               if (use_table) {
-                if (x >= table->first[p.n_seq]) return Block::NO_ROWS;
+                if (pass && x >= table->first[p.n_seq]) return Block::NO_ROWS;
                 cursor.template look_up<ALT>(p, *table, x);
               } else {
                 cursor.seek_alone(p, ragged_slot(p, x, y));
@@ -682,7 +685,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             w = ragged_item(p, cursor, x, y, z);
           }
           kv_heads(w, kh, vh);
-          return FORM != ATT_PACKED || ragged_has_rows(w) ? Block::ITEM : Block::NO_ROWS;
+          if (pass && !ragged_has_rows(w)) return Block::NO_ROWS;
+          // an item without keys is progress too: warp 15 sees nothing else of it (even: draining goes by the parity)
+          if (FORM == ATT_PACKED && w.n == 0) fills_issued[0] += 2;
+          return Block::ITEM;
         };
         auto fill_one = [&](int fill) {
           const int g = base + fill;
