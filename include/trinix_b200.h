@@ -52,6 +52,12 @@ typedef enum trx_row_act {
   TRX_ACT_SQUARED_RELU = 2  /* max(n, 0)^2 */
 } trx_row_act;
 
+/* Norm of a query's or key's row (trx_qk_norm_rope_fwd). */
+typedef enum trx_norm {
+  TRX_NORM_RMS = 0,  /* x rsqrt(mean x^2 + eps) */
+  TRX_NORM_LAYER = 1 /* (x - mean) rsqrt(mean (x - mean)^2 + eps) */
+} trx_norm;
+
 /* ABI version of the loaded library (TRX_ABI_VERSION at build time). */
 int trx_version(void);
 
@@ -191,6 +197,42 @@ int trx_rope_fwd(const void* q, const void* k, const void* cos_table, const void
                  const int64_t qo_strides[3], const int64_t ko_strides[3],
                  int64_t table_row_stride, int table_dtype, int x_dtype, int inverse,
                  void* stream);
+
+/*
+ * Norm of every query's and key's row of D values, with weight w and (TRX_NORM_LAYER only, NULL: none) bias b,
+ * and the rotation of trx_rope_fwd, q and k in one launch: y = rotate(norm(x) w + b) with norm_first != 0,
+ * else y = norm(rotate(x)) w + b. All arithmetic is fp32, rounded once. D is even and at most 512, tensors are
+ * (B, S, H, D) with D contiguous. Row r of the tables (table_rows, >= D/2) has the angles of position r;
+ * a token's position is positions[b, s] (int32, or int64 with positions_64 != 0), without positions its index
+ * s. A position outside the tables makes its rows NaN. `table_dtype` is TRX_F32 or `x_dtype`; `w_dtype`, of
+ * weights and biases, is any. `strides`: (batch, seq, head) of q, k, q_out, k_out, (batch, seq) of positions.
+ * Replaces the sequence of trinix/layers/embeddings/rope.py:83-134 and the q / k norm modules in
+ * trinix/layers/attention/grouped_query_attention.py:167-178.
+ */
+int trx_qk_norm_rope_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                         const void* q_bias_or_null, const void* k_bias_or_null, const void* cos_table,
+                         const void* sin_table, const void* positions_or_null, void* q_out, void* k_out,
+                         int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, const int64_t strides[14],
+                         int64_t table_rows, int64_t table_row_stride, float eps, int norm, int norm_first,
+                         int positions_64, int table_dtype, int w_dtype, int x_dtype, void* stream);
+
+/*
+ * Gradients of trx_qk_norm_rope_fwd: dq_out / dk_out are those of its outputs, dq / dk (contiguous in D) the
+ * inputs'. Those of the weights and biases, in `w_dtype`, are summed in fp32 in an order fixed by the sizes and
+ * the device; NULL: not asked for. `strides`: (batch, seq, head) of dq_out, dk_out, q, k, dq, dk,
+ * (batch, seq) of positions. The workspace is 16-byte aligned and holds nothing between calls.
+ */
+int trx_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k,
+                         const void* q_weight, const void* k_weight, const void* cos_table,
+                         const void* sin_table, const void* positions_or_null, void* dq, void* dk,
+                         void* dq_weight_or_null, void* dk_weight_or_null, void* dq_bias_or_null,
+                         void* dk_bias_or_null, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D,
+                         const int64_t strides[20], int64_t table_rows, int64_t table_row_stride, float eps,
+                         int norm, int norm_first, int positions_64, int table_dtype, int w_dtype,
+                         int x_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of that workspace on the current device; 0 for a head_dim that is refused. */
+size_t trx_qk_norm_rope_bwd_workspace_bytes(int64_t D);
 
 /*
  * Gated linear unit forward: y[r, c] = up[r, c] * act(gate[r, c]) for R rows of H columns.

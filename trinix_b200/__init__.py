@@ -10,6 +10,7 @@ from .fusion import FastFusedRMSNormInt8, RowwiseInt8Quant, fuse, register_fusio
 from .install import install, uninstall
 from .kernels import (
     PackedAttentionKernel,
+    QKNormRoPEKernel,
     RowwiseInt8Kernel,
     SharedPrefixAttentionKernel,
     TritonAttentionKernel,
@@ -49,6 +50,8 @@ from .ops import (
     glu_pair,
     layernorm,
     layernorm_backward,
+    qk_norm_rope,
+    qk_norm_rope_backward,
     quantize_rowwise,
     residual_layernorm,
     residual_rmsnorm,

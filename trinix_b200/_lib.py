@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libtrinix_b
 
 TRX_F32, TRX_F16, TRX_BF16 = 0, 1, 2
 GLU_SWIGLU, GLU_GEGLU_TANH, GLU_REGLU = 0, 1, 2
+NORM_RMS, NORM_LAYER = 0, 1
 TRX_ERR_DEVICE_STATUS = -8
 
 I64x3 = c_int64 * 3
@@ -47,6 +48,11 @@ SIGNATURES = {
     "trx_rope_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                              c_int64, c_int64, c_int64, c_int64, I64x3, I64x3, I64x3, I64x3,
                              c_int64, c_int, c_int, c_int, c_void_p]),
+    "trx_qk_norm_rope_fwd": (c_int, [*[c_void_p] * 11, *[c_int64] * 5, c_void_p, c_int64, c_int64,
+                                     c_float, *[c_int] * 6, c_void_p]),
+    "trx_qk_norm_rope_bwd": (c_int, [*[c_void_p] * 15, *[c_int64] * 5, c_void_p, c_int64, c_int64,
+                                     c_float, *[c_int] * 6, c_void_p, c_size_t, c_void_p]),
+    "trx_qk_norm_rope_bwd_workspace_bytes": (c_size_t, [c_int64]),
     "trx_glu_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                             c_int64, c_int, c_int, c_void_p]),
     "trx_glu_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,

@@ -1,0 +1,554 @@
+// Norms of queries and keys, a row of head_dim values at a time, with the rotation by position in the same
+// pass, and their gradients.
+//
+//   n(x) = x rsqrt(mean x^2 + eps)                    RMSNorm
+//   n(x) = (x - mean x) rsqrt(mean (x - mean x)^2 + eps)   LayerNorm
+//   a(x) = w n(x) (+ b);  R: the two halves of a row turned by the angles of its position
+//   forward   y = R a(x)  or  y = a(R x)
+//   backward  with g = R^T dy or dy, and n, rstd of x or of R x:
+//             dw = sum g n,  db = sum g,  d = g w,  dz = rstd (d - n mean(d n) [- mean d])
+//             dx = dz or R^T dz
+// All in fp32, one rounding at the end; row statistics are recomputed in the backward pass, where the row is in
+// registers anyway. Memory bounds both: a row is read once and stays with its few lanes (head_rows.cuh), no
+// shared memory and no barrier in the loop.
+#include "head_rows.cuh"
+
+namespace trx {
+
+struct QkSide {
+  const void* x;
+  const void* dy;   // backward
+  void* y;          // forward: y; backward: dx
+  const void* w;
+  const void* b;    // LayerNorm's bias, or null
+  int64_t xs[3], dys[3], ys[3];  // (batch, seq, head) strides in elements
+  int H;
+};
+struct QkParams {
+  QkSide side[2];  // queries, keys
+  const void* cos_t;
+  const void* sin_t;
+  const void* positions;  // null: a token's own index in its sequence
+  int64_t pos_strides[2];
+  int64_t table_rows, table_stride;
+  int64_t tokens, S;
+  int D, pos64;
+  int table_dtype, w_dtype;
+  int layer, first;   // LayerNorm; the norm comes before the rotation
+  float eps;
+  int q_chunks;       // forward: of the grid's y
+  int heads_per_cta;
+  int q_blocks;       // backward: of the grid's x
+  float* part;        // backward: [blocks][2][D] sums of g n and of g
+};
+
+constexpr int QK_THREADS = 128;
+
+// cos and sin of a token for a lane's columns. A position outside the tables has none: its rows become NaN.
+template <int VEC, int CH, int LPR>
+__device__ __forceinline__ void load_angles(const QkParams& p, int64_t b, int64_t s, int lane, int half,
+                                            float (&c)[VEC * CH], float (&sn)[VEC * CH]) {
+  int64_t pos = s;
+  if (p.positions) {
+    const int64_t at = b * p.pos_strides[0] + s * p.pos_strides[1];
+    pos = p.pos64 ? __ldg(static_cast<const long long*>(p.positions) + at)
+                  : __ldg(static_cast<const int*>(p.positions) + at);
+  }
+  const bool there = pos >= 0 && pos < p.table_rows;
+  const float fill = there ? 0.0f : __int_as_float(0x7fffffff);
+  load_columns<VEC, CH, LPR>(p.cos_t, p.table_dtype, pos * p.table_stride, lane, there ? half : 0, fill, c);
+  load_columns<VEC, CH, LPR>(p.sin_t, p.table_dtype, pos * p.table_stride, lane, there ? half : 0, fill, sn);
+}
+
+// x1, x2 become the normalised row (0 in columns behind it); the factor that a gradient is scaled by.
+template <int VEC, int CH, int LPR>
+__device__ __forceinline__ float normalise(float (&x1)[VEC * CH], float (&x2)[VEC * CH], int lane, int half,
+                                           float inv_d, float eps, int layer) {
+  constexpr int N = VEC * CH;
+  auto inside = [&](int i) { return ((i / VEC) * LPR + lane) * VEC < half; };
+  if (layer) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += x1[i] + x2[i];
+    const float mean = lanes_sum<LPR>(sum) * inv_d;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x1[i] = inside(i) ? x1[i] - mean : 0.0f;
+      x2[i] = inside(i) ? x2[i] - mean : 0.0f;
+    }
+  }
+  float sq = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) sq = fmaf(x1[i], x1[i], fmaf(x2[i], x2[i], sq));
+  const float rstd = rsqrtf(fmaf(lanes_sum<LPR>(sq), inv_d, eps));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x1[i] *= rstd;
+    x2[i] *= rstd;
+  }
+  return rstd;
+}
+
+// Grid (tokens, chunks of heads of q, then of k): a thread has its columns' weights and angles for all heads of
+// its chunk, ROWS of them in flight.
+template <typename T, int VEC, int LPR, int CH, int ROWS>
+__global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const __grid_constant__ QkParams p) {
+  constexpr int N = VEC * CH;
+  const int lane = threadIdx.x % LPR, half = p.D / 2;
+  int64_t token = static_cast<int64_t>(blockIdx.x) * (QK_THREADS / LPR) + threadIdx.x / LPR;
+  const bool live = token < p.tokens;
+  if (!live) token = p.tokens - 1;  // its lanes take part in the shuffles
+  const int64_t b = token / p.S, s = token - b * p.S;
+  const bool keys = static_cast<int>(blockIdx.y) >= p.q_chunks;
+  const QkSide& side = p.side[keys ? 1 : 0];
+  const int h_begin = (static_cast<int>(blockIdx.y) - (keys ? p.q_chunks : 0)) * p.heads_per_cta;
+  const int h_end = min(side.H, h_begin + p.heads_per_cta);
+  const T* x = static_cast<const T*>(side.x) + b * side.xs[0] + s * side.xs[1];
+  T* y = static_cast<T*>(side.y) + b * side.ys[0] + s * side.ys[1];
+
+  float c[N], sn[N], w1[N], w2[N];
+  load_angles<VEC, CH, LPR>(p, b, s, lane, half, c, sn);
+  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, 0, lane, half, 0.0f, w1);
+  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, half, lane, half, 0.0f, w2);
+  const float inv_d = __fdiv_rn(1.0f, static_cast<float>(p.D));
+
+  for (int h0 = h_begin; h0 < h_end; h0 += ROWS) {
+    HalfRow<T, VEC, CH> r1[ROWS], r2[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const T* row = x + min(h0 + u, h_end - 1) * side.xs[2];
+      r1[u].template load<LPR>(row, lane, half);
+      r2[u].template load<LPR>(row + half, lane, half);
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      float x1[N], x2[N];
+      r1[u].unpack(x1);
+      r2[u].unpack(x2);
+      if (!p.first) turn(x1, x2, c, sn);
+      normalise<VEC, CH, LPR>(x1, x2, lane, half, inv_d, p.eps, p.layer);
+      if (side.b) {
+        float b1[N], b2[N];
+        load_columns<VEC, CH, LPR>(side.b, p.w_dtype, 0, lane, half, 0.0f, b1);
+        load_columns<VEC, CH, LPR>(side.b, p.w_dtype, half, lane, half, 0.0f, b2);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          x1[i] = fmaf(x1[i], w1[i], b1[i]);
+          x2[i] = fmaf(x2[i], w2[i], b2[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          x1[i] *= w1[i];
+          x2[i] *= w2[i];
+        }
+      }
+      if (p.first) turn(x1, x2, c, sn);
+      if (live && h0 + u < h_end) {
+        T* row = y + (h0 + u) * side.ys[2];
+        store_half<T, VEC, CH, LPR>(row, lane, half, x1);
+        store_half<T, VEC, CH, LPR>(row + half, lane, half, x2);
+      }
+    }
+  }
+}
+
+// Blocks [0, q_blocks) walk over the queries, the others over the keys, ROWS heads of a token at a time; every
+// thread keeps the sums of its columns' weight gradients, which meet in shared memory at the end.
+template <typename T, int VEC, int LPR, int CH, int ROWS, bool LAYER>
+__global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_bwd_kernel(const __grid_constant__ QkParams p) {
+  constexpr int N = VEC * CH, GROUPS = QK_THREADS / LPR;
+  const int lane = threadIdx.x % LPR, half = p.D / 2;
+  const bool keys = static_cast<int>(blockIdx.x) >= p.q_blocks;
+  const QkSide& side = p.side[keys ? 1 : 0];
+  const int blocks = keys ? gridDim.x - p.q_blocks : p.q_blocks;
+  const int block = keys ? blockIdx.x - p.q_blocks : blockIdx.x;
+  const float inv_d = __fdiv_rn(1.0f, static_cast<float>(p.D));
+
+  float w1[N], w2[N], dw1[N], dw2[N], db1[LAYER ? N : 1], db2[LAYER ? N : 1];
+  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, 0, lane, half, 0.0f, w1);
+  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, half, lane, half, 0.0f, w2);
+#pragma unroll
+  for (int i = 0; i < N; ++i) dw1[i] = dw2[i] = 0.0f;
+  if constexpr (LAYER)
+#pragma unroll
+    for (int i = 0; i < N; ++i) db1[i] = db2[i] = 0.0f;
+
+  const unsigned chunks = (side.H + ROWS - 1) / ROWS;
+  const unsigned items = static_cast<unsigned>(p.tokens) * chunks;
+  // whole warps leave together: the item of a warp's first row decides
+  for (unsigned first = (block * QK_THREADS + (threadIdx.x & ~31)) / LPR; first < items;
+       first += blocks * GROUPS) {
+    const unsigned item = first + (threadIdx.x % 32) / LPR;
+    const bool live = item < items;
+    const unsigned token = (live ? item : items - 1) / chunks, h0 = ((live ? item : items - 1) - token * chunks) * ROWS;
+    const unsigned seq = static_cast<unsigned>(p.S);
+    const int64_t b = token / seq, s = token - static_cast<unsigned>(b) * seq;
+    const T* x = static_cast<const T*>(side.x) + b * side.xs[0] + s * side.xs[1];
+    const T* dy = static_cast<const T*>(side.dy) + b * side.dys[0] + s * side.dys[1];
+    T* dx = static_cast<T*>(side.y) + b * side.ys[0] + s * side.ys[1];
+    HalfRow<T, VEC, CH> r1[ROWS], r2[ROWS], g1[ROWS], g2[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const int h = min(static_cast<int>(h0) + u, side.H - 1);
+      r1[u].template load<LPR>(x + h * side.xs[2], lane, half);
+      r2[u].template load<LPR>(x + h * side.xs[2] + half, lane, half);
+      g1[u].template load<LPR>(dy + h * side.dys[2], lane, half);
+      g2[u].template load<LPR>(dy + h * side.dys[2] + half, lane, half);
+    }
+    float c[N], sn[N];
+    load_angles<VEC, CH, LPR>(p, b, s, lane, half, c, sn);
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const bool row_live = live && static_cast<int>(h0) + u < side.H;
+      float x1[N], x2[N], d1[N], d2[N];
+      r1[u].unpack(x1);
+      r2[u].unpack(x2);
+      g1[u].unpack(d1);
+      g2[u].unpack(d2);
+      if (p.first)
+        turn_back(d1, d2, c, sn);
+      else
+        turn(x1, x2, c, sn);
+      const float rstd = normalise<VEC, CH, LPR>(x1, x2, lane, half, inv_d, p.eps, LAYER);
+      float dn = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (row_live) {
+          dw1[i] = fmaf(d1[i], x1[i], dw1[i]);
+          dw2[i] = fmaf(d2[i], x2[i], dw2[i]);
+          if constexpr (LAYER) {
+            db1[i] += d1[i];
+            db2[i] += d2[i];
+          }
+        }
+        d1[i] *= w1[i];
+        d2[i] *= w2[i];
+        dn = fmaf(d1[i], x1[i], fmaf(d2[i], x2[i], dn));
+        if constexpr (LAYER) sum += d1[i] + d2[i];
+      }
+      dn = lanes_sum<LPR>(dn) * inv_d;
+      if constexpr (LAYER) sum = lanes_sum<LPR>(sum) * inv_d;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        d1[i] = rstd * (fmaf(-dn, x1[i], d1[i]) - sum);
+        d2[i] = rstd * (fmaf(-dn, x2[i], d2[i]) - sum);
+      }
+      if (!p.first) turn_back(d1, d2, c, sn);
+      if (row_live) {
+        T* row = dx + (static_cast<int>(h0) + u) * side.ys[2];
+        store_half<T, VEC, CH, LPR>(row, lane, half, d1);
+        store_half<T, VEC, CH, LPR>(row + half, lane, half, d2);
+      }
+    }
+  }
+
+  // the warp's rows, then the CTA's warps, in a fixed order
+  __shared__ float sums[QK_THREADS / 32][2 * N * LPR];
+  float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.D;
+#pragma unroll
+  for (int pass = 0; pass < (LAYER ? 2 : 1); ++pass) {
+    if (pass) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float a = dw1[i], e = dw2[i];
+      if constexpr (LAYER)
+        if (pass) {
+          a = db1[i];
+          e = db2[i];
+        }
+#pragma unroll
+      for (int o = 16; o >= LPR; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        e += __shfl_xor_sync(0xffffffffu, e, o);
+      }
+      if (threadIdx.x % 32 < LPR) {
+        const int col = ((i / VEC) * LPR + lane) * VEC + i % VEC;
+        sums[threadIdx.x / 32][col] = a;
+        sums[threadIdx.x / 32][N * LPR + col] = e;
+      }
+    }
+    __syncthreads();
+    for (int col = threadIdx.x; col < p.D; col += QK_THREADS) {
+      const int at = col < half ? col : N * LPR + col - half;
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < QK_THREADS / 32; ++i) v += sums[i][at];
+      part[pass * p.D + col] = v;
+    }
+  }
+}
+
+struct QkReduce {
+  const float* part;
+  void* out[4];      // dw of q, of k, db of q, of k; null: not asked for
+  int q_blocks, blocks, D, dtype;
+};
+// Grid (columns / 32, 4): a block's 32 rows of threads have every 32nd partial sum of 32 columns.
+__global__ void __launch_bounds__(1024) qk_norm_reduce_kernel(const QkReduce r) {
+  __shared__ float sm[32][33];
+  void* out = r.out[blockIdx.y];
+  if (!out) return;
+  const bool keys = blockIdx.y & 1;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
+  float v = 0.0f;
+  if (col < r.D)
+    for (int i = (keys ? r.q_blocks : 0) + ty; i < (keys ? r.blocks : r.q_blocks); i += 32)
+      v += r.part[(static_cast<int64_t>(i) * 2 + (blockIdx.y >> 1)) * r.D + col];
+  sm[ty][tx] = v;
+  __syncthreads();
+  const float sum = warp_reduce<false>(sm[tx][ty]);  // of column ty
+  const int c = blockIdx.x * 32 + ty;
+  if (tx == 0 && c < r.D) {
+    if (r.dtype == TRX_F32) Pack<float>::store1(static_cast<float*>(out) + c, sum);
+    else if (r.dtype == TRX_F16) Pack<__half>::store1(static_cast<__half*>(out) + c, sum);
+    else Pack<__nv_bfloat16>::store1(static_cast<__nv_bfloat16*>(out) + c, sum);
+  }
+}
+
+// Whether every row, of every tensor and table, can be read in 16-byte vectors of the activation type, at most
+// one to a lane of a warp.
+static bool qk_vector(const QkParams& p, int vec, bool backward) {
+  const int half = p.D / 2;
+  if (half % vec || half > 32 * vec) return false;
+  const int table_vec = p.table_dtype == TRX_F32 ? 4 : 8;
+  if (!aligned_to(p.cos_t, 16) || !aligned_to(p.sin_t, 16) || p.table_stride % table_vec) return false;
+  for (const QkSide& s : p.side) {
+    if (s.H == 0) continue;
+    if (!aligned_to(s.x, 16) || !aligned_to(s.y, 16) || !aligned_to(s.w, 16) || (s.b && !aligned_to(s.b, 16)) ||
+        (backward && !aligned_to(s.dy, 16)))
+      return false;
+    for (int i = 0; i < 3; ++i)
+      if (s.xs[i] % vec || s.ys[i] % vec || (backward && s.dys[i] % vec)) return false;
+  }
+  return true;
+}
+
+template <typename T, int VEC, int LPR, int CH, int ROWS>
+static int launch_qk(QkParams& p, cudaStream_t stream) {
+  constexpr int TOKENS = QK_THREADS / LPR;
+  const int64_t blocks = (p.tokens + TOKENS - 1) / TOKENS;
+  // eight heads to a CTA where the grid fills the chip, else fewer for more CTAs
+  p.heads_per_cta = 8;
+  while (p.heads_per_cta > ROWS &&
+         blocks * (p.side[0].H + p.side[1].H) < p.heads_per_cta * sm_count_of_current_device())
+    p.heads_per_cta /= 2;
+  p.q_chunks = (p.side[0].H + p.heads_per_cta - 1) / p.heads_per_cta;
+  const int chunks = p.q_chunks + (p.side[1].H + p.heads_per_cta - 1) / p.heads_per_cta;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(chunks));
+  qk_norm_rope_kernel<T, VEC, LPR, CH, ROWS><<<grid, QK_THREADS, 0, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
+}
+
+template <typename T>
+static int launch_qk_forward(QkParams& p, cudaStream_t s) {
+  constexpr int VEC = Pack<T>::VEC;
+  if (!qk_vector(p, VEC, false))
+    return p.D <= 128 ? launch_qk<T, 1, 32, 2, 2>(p, s) : launch_qk<T, 1, 32, 8, 1>(p, s);
+  switch (lanes_for(p.D / 2, VEC)) {
+    case 4: return launch_qk<T, VEC, 4, 1, 4>(p, s);
+    case 8: return launch_qk<T, VEC, 8, 1, 4>(p, s);
+    case 16: return launch_qk<T, VEC, 16, 1, 4>(p, s);
+    default: return launch_qk<T, VEC, 32, 1, 4>(p, s);
+  }
+}
+
+constexpr int QK_BWD_CTAS_PER_SM = 4;
+static int qk_bwd_blocks() { return sm_count_of_current_device() * QK_BWD_CTAS_PER_SM; }
+
+template <typename T, int VEC, int LPR, int CH, int ROWS>
+static int launch_qk_bwd(QkParams& p, QkReduce& r, cudaStream_t stream) {
+  constexpr int GROUPS = QK_THREADS / LPR;
+  auto needs = [&](const QkSide& s) {
+    return (p.tokens * ((s.H + ROWS - 1) / ROWS) + GROUPS - 1) / GROUPS;
+  };
+  const int64_t most = qk_bwd_blocks(), nq = needs(p.side[0]), nk = needs(p.side[1]);
+  int64_t q = nq, k = nk;
+  if (nq + nk > most) {  // a share each, and one block at least
+    q = most * nq / (nq + nk);
+    q = nq && q < 1 ? 1 : q;
+    q = nk && q > most - 1 ? most - 1 : q;
+    k = nk < most - q ? nk : most - q;
+  }
+  p.q_blocks = static_cast<int>(q);
+  if (q + k > 0) {
+    auto run = [&](auto kernel) { kernel<<<static_cast<unsigned>(q + k), QK_THREADS, 0, stream>>>(p); };
+    if (p.layer) run(qk_norm_rope_bwd_kernel<T, VEC, LPR, CH, ROWS, true>);
+    else run(qk_norm_rope_bwd_kernel<T, VEC, LPR, CH, ROWS, false>);
+    if (cudaGetLastError() != cudaSuccess) return TRX_ERR_CUDA;
+  }
+  bool any = false;
+  for (void* o : r.out) any = any || o;
+  if (!any) return TRX_OK;
+  r.part = p.part;
+  r.q_blocks = p.q_blocks;
+  r.blocks = static_cast<int>(q + k);
+  r.D = p.D;
+  r.dtype = p.w_dtype;
+  qk_norm_reduce_kernel<<<dim3((p.D + 31) / 32, 4), 1024, 0, stream>>>(r);
+  return cudaGetLastError() == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
+}
+
+template <typename T>
+static int launch_qk_backward(QkParams& p, QkReduce& r, cudaStream_t s) {
+  constexpr int VEC = Pack<T>::VEC;
+  if (!qk_vector(p, VEC, true))
+    return p.D <= 128 ? launch_qk_bwd<T, 1, 32, 2, 1>(p, r, s) : launch_qk_bwd<T, 1, 32, 8, 1>(p, r, s);
+  switch (lanes_for(p.D / 2, VEC)) {
+    case 4: return launch_qk_bwd<T, VEC, 4, 1, 2>(p, r, s);
+    case 8: return launch_qk_bwd<T, VEC, 8, 1, 2>(p, r, s);
+    case 16: return launch_qk_bwd<T, VEC, 16, 1, 2>(p, r, s);
+    default: return launch_qk_bwd<T, VEC, 32, 1, 2>(p, r, s);
+  }
+}
+
+// What both directions check; TRX_OK with p.tokens == 0 for nothing to do.
+static int qk_check(QkParams& p, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                    const void* q_bias, const void* k_bias, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
+                    int64_t D, int norm, int x_dtype) {
+  if (x_dtype != TRX_F32 && x_dtype != TRX_F16 && x_dtype != TRX_BF16) return TRX_ERR_DTYPE;
+  if (p.table_dtype != TRX_F32 && p.table_dtype != x_dtype) return TRX_ERR_DTYPE;
+  if (p.w_dtype != TRX_F32 && p.w_dtype != TRX_F16 && p.w_dtype != TRX_BF16) return TRX_ERR_DTYPE;
+  if (norm != TRX_NORM_RMS && norm != TRX_NORM_LAYER) return TRX_ERR_UNSUPPORTED;
+  if (B < 0 || S < 0 || Hq < 0 || Hk < 0 || D <= 0 || D % 2 || p.table_rows < 0) return TRX_ERR_SHAPE;
+  if (D > 512) return TRX_ERR_UNSUPPORTED;
+  if (Hq > 65535 || Hk > 65535) return TRX_ERR_SHAPE;
+  if (!(p.eps >= 0.0f)) return TRX_ERR_UNSUPPORTED;
+  if (B > 0 && S > ((1ll << 31) - 1) / B) return TRX_ERR_SHAPE;
+  if (B * S > 0 && (B * S) * (Hq > Hk ? Hq : Hk) >= (1ll << 31)) return TRX_ERR_SHAPE;
+  p.tokens = B * S;
+  p.S = S;
+  p.D = static_cast<int>(D);
+  p.layer = norm == TRX_NORM_LAYER;
+  const void* x[2] = {q, k};
+  const void* w[2] = {q_weight, k_weight};
+  const void* b[2] = {q_bias, k_bias};
+  const int64_t heads[2] = {Hq, Hk};
+  for (int i = 0; i < 2; ++i) {
+    p.side[i].x = x[i];
+    p.side[i].w = w[i];
+    p.side[i].b = b[i];
+    p.side[i].H = static_cast<int>(heads[i]);
+  }
+  if (p.tokens == 0 || Hq + Hk == 0) {
+    p.tokens = 0;
+    return TRX_OK;
+  }
+  if (!p.cos_t || !p.sin_t) return TRX_ERR_NULL_POINTER;
+  if (p.table_stride < D / 2) return TRX_ERR_STRIDE;
+  for (const QkSide& s : p.side)
+    if (s.H > 0) {
+      if (!s.x || !s.w || !s.y) return TRX_ERR_NULL_POINTER;
+      for (int i = 0; i < 3; ++i)
+        if (s.xs[i] < 0 || s.ys[i] < 0) return TRX_ERR_STRIDE;
+    }
+  if (!p.positions && p.table_rows < S) return TRX_ERR_SHAPE;
+  if (p.positions && (p.pos_strides[0] < 0 || p.pos_strides[1] < 0)) return TRX_ERR_STRIDE;
+  if (p.positions && !aligned_to(p.positions, p.pos64 ? 8 : 4)) return TRX_ERR_ALIGNMENT;
+  return TRX_OK;
+}
+
+static void take_strides(int64_t (&to)[3], const int64_t* from) {
+  for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+
+}  // namespace trx
+
+using namespace trx;
+
+extern "C" int trx_qk_norm_rope_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                    const void* q_bias_or_null, const void* k_bias_or_null,
+                                    const void* cos_table, const void* sin_table,
+                                    const void* positions_or_null, void* q_out, void* k_out, int64_t B,
+                                    int64_t S, int64_t Hq, int64_t Hk, int64_t D, const int64_t strides[14],
+                                    int64_t table_rows, int64_t table_row_stride, float eps, int norm,
+                                    int norm_first, int positions_64, int table_dtype, int w_dtype,
+                                    int x_dtype, void* stream) {
+  if (!strides) return TRX_ERR_NULL_POINTER;
+  QkParams p{};
+  take_strides(p.side[0].xs, strides);
+  take_strides(p.side[1].xs, strides + 3);
+  take_strides(p.side[0].ys, strides + 6);
+  take_strides(p.side[1].ys, strides + 9);
+  p.pos_strides[0] = strides[12];
+  p.pos_strides[1] = strides[13];
+  p.side[0].y = q_out;
+  p.side[1].y = k_out;
+  p.cos_t = cos_table;
+  p.sin_t = sin_table;
+  p.positions = positions_or_null;
+  p.pos64 = positions_64;
+  p.table_rows = table_rows;
+  p.table_stride = table_row_stride;
+  p.table_dtype = table_dtype;
+  p.w_dtype = w_dtype;
+  p.first = norm_first;
+  p.eps = eps;
+  const int rc = qk_check(p, q, k, q_weight, k_weight, q_bias_or_null, k_bias_or_null, B, S, Hq, Hk, D, norm,
+                          x_dtype);
+  if (rc != TRX_OK || p.tokens == 0) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (x_dtype == TRX_F32) return launch_qk_forward<float>(p, s);
+  return x_dtype == TRX_F16 ? launch_qk_forward<__half>(p, s) : launch_qk_forward<__nv_bfloat16>(p, s);
+}
+
+extern "C" size_t trx_qk_norm_rope_bwd_workspace_bytes(int64_t D) {
+  if (D <= 0 || D > 512) return 0;
+  return static_cast<size_t>(qk_bwd_blocks()) * 2 * D * sizeof(float);
+}
+
+extern "C" int trx_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k,
+                                    const void* q_weight, const void* k_weight, const void* cos_table,
+                                    const void* sin_table, const void* positions_or_null, void* dq, void* dk,
+                                    void* dq_weight_or_null, void* dk_weight_or_null, void* dq_bias_or_null,
+                                    void* dk_bias_or_null, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
+                                    int64_t D, const int64_t strides[20], int64_t table_rows,
+                                    int64_t table_row_stride, float eps, int norm, int norm_first,
+                                    int positions_64, int table_dtype, int w_dtype, int x_dtype,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  if (!strides) return TRX_ERR_NULL_POINTER;
+  QkParams p{};
+  for (int i = 0; i < 2; ++i) {
+    take_strides(p.side[i].dys, strides + 3 * i);
+    take_strides(p.side[i].xs, strides + 6 + 3 * i);
+    take_strides(p.side[i].ys, strides + 12 + 3 * i);
+  }
+  p.pos_strides[0] = strides[18];
+  p.pos_strides[1] = strides[19];
+  p.side[0].dy = dq_out;
+  p.side[1].dy = dk_out;
+  p.side[0].y = dq;
+  p.side[1].y = dk;
+  p.cos_t = cos_table;
+  p.sin_t = sin_table;
+  p.positions = positions_or_null;
+  p.pos64 = positions_64;
+  p.table_rows = table_rows;
+  p.table_stride = table_row_stride;
+  p.table_dtype = table_dtype;
+  p.w_dtype = w_dtype;
+  p.first = norm_first;
+  p.eps = eps;
+  const int rc = qk_check(p, q, k, q_weight, k_weight, nullptr, nullptr, B, S, Hq, Hk, D, norm, x_dtype);
+  if (rc != TRX_OK) return rc;
+  if (norm == TRX_NORM_RMS && (dq_bias_or_null || dk_bias_or_null)) return TRX_ERR_UNSUPPORTED;
+  if (p.tokens > 0)
+    for (const QkSide& s : p.side)
+      if (s.H > 0) {
+        if (!s.dy) return TRX_ERR_NULL_POINTER;
+        for (int i = 0; i < 3; ++i)
+          if (s.dys[i] < 0) return TRX_ERR_STRIDE;
+      }
+  if (!workspace || !aligned_to(workspace, 16) ||
+      workspace_bytes < trx_qk_norm_rope_bwd_workspace_bytes(D))
+    return TRX_ERR_WORKSPACE;
+  p.part = static_cast<float*>(workspace);
+  QkReduce r{};
+  r.out[0] = dq_weight_or_null;
+  r.out[1] = dk_weight_or_null;
+  r.out[2] = dq_bias_or_null;
+  r.out[3] = dk_bias_or_null;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (x_dtype == TRX_F32) return launch_qk_backward<float>(p, r, s);
+  return x_dtype == TRX_F16 ? launch_qk_backward<__half>(p, r, s) : launch_qk_backward<__nv_bfloat16>(p, r, s);
+}

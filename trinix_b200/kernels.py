@@ -190,6 +190,34 @@ class _RoPEFn(torch.autograd.Function):
         return dq, dk, None, None
 
 
+class _QKNormRoPEFn(torch.autograd.Function):
+    """The q / k norms and the rotation of trinix/layers/attention/grouped_query_attention.py:167-178 as
+    one function. Saves its inputs; the row statistics are recomputed."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, q_bias, k_bias, eps, norm, norm_first, positions):
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.how = {"eps": eps, "norm": norm, "norm_first": norm_first}
+        ctx.dtypes = (k_weight.dtype, *(None if b is None else b.dtype for b in (q_bias, k_bias)))
+        return ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_bias=q_bias, k_bias=k_bias,
+                                positions=positions, **ctx.how)
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = ops.qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin,
+                                          positions=positions, need_dw=need[2] or need[3],
+                                          need_db=need[6] or need[7], **ctx.how)
+        dq, dk, dqw, *rest = grads
+        # those of another dtype than q's weight were summed in its dtype
+        dkw, dqb, dkb = (None if g is None or t is None else g.to(t) for g, t in zip(rest, ctx.dtypes))
+        # the shapes of weights that are not one-dimensional
+        if dqw is not None:
+            dqw, dkw = dqw.view(q_weight.shape), dkw.view(k_weight.shape)
+        return dq, dk, dqw, dkw, None, None, dqb, dkb, None, None, None, None
+
+
 class TritonRMSNormKernel:
     """Same interface as trinix/kernels/rmsnorm_kernel.py:324-389."""
 
@@ -278,6 +306,28 @@ class TritonRoPEKernel:
         if _needs_graph(q, k):
             return _RoPEFn.apply(q, k, cos, sin)
         return ops.rope(q, k, cos, sin)
+
+
+class QKNormRoPEKernel:
+    """Norms of queries and keys and their rotary embedding in one pass (`ops.qk_norm_rope`), differentiable
+    in q, k, the weights and the biases. The reference has no such class: its attention modules rotate, then
+    call two norm modules (trinix/layers/attention/grouped_query_attention.py:167-178)."""
+
+    @staticmethod
+    def is_available() -> bool:
+        return _available()
+
+    @staticmethod
+    def apply(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+              cos: torch.Tensor, sin: torch.Tensor, q_bias: Optional[torch.Tensor] = None,
+              k_bias: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: str = "rmsnorm",
+              norm_first: bool = True, positions: Optional[torch.Tensor] = None
+              ) -> Tuple[torch.Tensor, torch.Tensor]:
+        if _needs_graph(q, k, q_weight, k_weight, q_bias, k_bias):
+            return _QKNormRoPEFn.apply(q, k, q_weight, k_weight, cos, sin, q_bias, k_bias, eps, norm,
+                                       norm_first, positions)
+        return ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_bias=q_bias, k_bias=k_bias, eps=eps,
+                                norm=norm, norm_first=norm_first, positions=positions)
 
 
 class TritonSwiGLUKernel:

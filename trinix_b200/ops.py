@@ -19,6 +19,7 @@ from ._lib import I64x3
 _DTYPE_CODE = {torch.float32: _lib.TRX_F32, torch.float16: _lib.TRX_F16,
                torch.bfloat16: _lib.TRX_BF16}
 
+HEAD_NORMS = {"rmsnorm": _lib.NORM_RMS, "layernorm": _lib.NORM_LAYER}
 GLU_ACTS = {"swiglu": _lib.GLU_SWIGLU, "geglu": _lib.GLU_GEGLU_TANH, "reglu": _lib.GLU_REGLU}
 
 # Number of kernels launched through this module (the benchmark reports it).
@@ -345,6 +346,139 @@ def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
             I64x3(*k.stride()[:3]), I64x3(*qo.stride()[:3]), I64x3(*ko.stride()[:3]),
             cos2.stride(0), _code(cos2), _code(q), int(bool(inverse)))
     return qo, ko
+
+
+_QKStrides, _QKBackwardStrides = ctypes.c_int64 * (4 * 3 + 2), ctypes.c_int64 * (6 * 3 + 2)
+
+
+def _tables(cos: torch.Tensor, sin: torch.Tensor, dtype: torch.dtype, half: int):
+    """Rotation tables as rows of at least `half` columns, in fp32 or `dtype`."""
+    if cos.dim() != 2 or not cos.is_contiguous():
+        cos = cos.reshape(-1, cos.shape[-1]).contiguous()
+    if sin.dim() != 2 or not sin.is_contiguous():
+        sin = sin.reshape(-1, sin.shape[-1]).contiguous()
+    if cos.shape != sin.shape or cos.shape[1] < half:
+        raise ValueError("cos/sin tables must be (positions, >= head_dim/2) and alike")
+    if cos.dtype != sin.dtype or cos.dtype not in (torch.float32, dtype):
+        cos, sin = cos.float(), sin.float()
+    return cos, sin
+
+
+def _positions(positions: Optional[torch.Tensor], B: int, S: int, rows: int):
+    """(tensor, its batch and token strides, whether it is int64) of positions (S,) or (B, S)."""
+    if positions is None:
+        if rows < S:
+            raise ValueError(f"the tables have {rows} positions, the sequences {S}")
+        return None, 0, 0, 0
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64")
+    if positions.shape not in ((S,), (1, S), (B, S)):
+        raise ValueError(f"positions {tuple(positions.shape)} are not ({S},) or ({B}, {S})")
+    wide = int(positions.dtype == torch.int64)
+    if positions.dim() == 2 and positions.shape[0] == B:
+        return positions, positions.stride(0), positions.stride(1), wide
+    return positions, 0, positions.stride(-1), wide
+
+
+def _head_params(D: int, *ts: Optional[torch.Tensor]):
+    """Weights and biases of a head's norm, as the kernels read them: of D elements and one dtype."""
+    dtype = ts[0].dtype
+    out = []
+    for t in ts:
+        if t is not None:
+            if t.numel() != D:
+                raise ValueError(f"weight/bias has {t.numel()} elements, a head has {D}")
+            t = _dense(t if t.dtype == dtype else t.detach().to(dtype))
+        out.append(t)
+    return out
+
+
+def _qk_inputs(q, k, q_weight, k_weight, cos, sin, norm: str, positions, *more):
+    """Checks that the forward and the backward pass of qk_norm_rope share."""
+    if norm not in HEAD_NORMS:
+        raise ValueError(f"Unsupported norm '{norm}'. Supported: {sorted(HEAD_NORMS)}")
+    dev = _same_device(q, k, q_weight, k_weight, cos, sin, positions, *more)
+    if q.dtype != k.dtype:
+        raise TypeError("q and k must share a dtype")
+    _code(q), _code(q_weight)
+    q, k = _bshd(q), _bshd(k)
+    B, S, Hq, D = q.shape
+    if k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
+        raise ValueError(f"k shape {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    if D % 2 or not 0 < D <= 512:
+        raise ValueError(f"head_dim must be even and at most 512, got {D}")
+    cos, sin = _tables(cos, sin, q.dtype, D // 2)
+    pos, pb, ps, wide = _positions(positions, B, S, cos.shape[0])
+    return dev, q, k, cos, sin, pos, (pb, ps), wide
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                 cos: torch.Tensor, sin: torch.Tensor, *, q_bias: Optional[torch.Tensor] = None,
+                 k_bias: Optional[torch.Tensor] = None, eps: float = 1e-6, norm: str = "rmsnorm",
+                 norm_first: bool = True, positions: Optional[torch.Tensor] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Norm of every head's row of q (B,S,Hq,D) and k (B,S,Hk,D) and its rotary embedding, in one launch.
+
+    norm: "rmsnorm", or "layernorm" (which may have biases); weights and biases have D elements. norm_first:
+    rotate(norm(x)); else norm(rotate(x)), the order of the attention modules. cos / sin are tables
+    (positions, >= D/2) as rope() takes them; positions, (S,) or (B,S) of int32 or int64, says which row
+    a token has (None: its index in the sequence); one that the tables lack gives rows of NaN. All
+    arithmetic is fp32, rounded once to q's dtype. D is even and at most 512.
+    """
+    if norm != "layernorm" and (q_bias is not None or k_bias is not None):
+        raise ValueError("only layernorm has biases")
+    dev, q, k, cos, sin, pos, pos_strides, wide = _qk_inputs(q, k, q_weight, k_weight, cos, sin, norm,
+                                                             positions, q_bias, k_bias)
+    B, S, Hq, D = q.shape
+    qw, kw, qb, kb = _head_params(D, q_weight, k_weight, q_bias, k_bias)
+    qo, ko = _new(q), _new(k)
+    strides = _QKStrides(*q.stride()[:3], *k.stride()[:3], *qo.stride()[:3], *ko.stride()[:3], *pos_strides)
+    _launch("trx_qk_norm_rope_fwd", dev, q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), _ptr(qb),
+            _ptr(kb), cos.data_ptr(), sin.data_ptr(), _ptr(pos), qo.data_ptr(), ko.data_ptr(), B, S, Hq,
+            k.shape[2], D, ctypes.addressof(strides), cos.shape[0], cos.stride(0), float(eps),
+            HEAD_NORMS[norm], int(bool(norm_first)), wide, _code(cos), _code(qw), _code(q))
+    return qo, ko
+
+
+def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                          sin: torch.Tensor, *, eps: float = 1e-6, norm: str = "rmsnorm",
+                          norm_first: bool = True, positions: Optional[torch.Tensor] = None,
+                          need_dw: bool = True, need_db: bool = False):
+    """(dq, dk, dq_weight, dk_weight, dq_bias, dk_bias) of qk_norm_rope given the gradients of its two
+    outputs; those of the weights are None unless need_dw, those of the biases unless need_db ("layernorm"
+    only). They have the dtype of q_weight and are summed in fp32 in a fixed order."""
+    if need_db and norm != "layernorm":
+        raise ValueError("only layernorm has biases")
+    dev, q, k, cos, sin, pos, pos_strides, wide = _qk_inputs(q, k, q_weight, k_weight, cos, sin, norm,
+                                                             positions, dq_out, dk_out)
+    for d, x in ((dq_out, q), (dk_out, k)):
+        if d.shape != x.shape or d.dtype != x.dtype:
+            raise ValueError("gradients must have the shape and dtype of the outputs")
+    B, S, Hq, D = q.shape
+    dq_out, dk_out = _bshd(dq_out), _bshd(dk_out)
+    qw, kw = _head_params(D, q_weight, k_weight)
+    dq, dk = _new(q), _new(k)
+    dw = (_empty(qw, D), _empty(qw, D)) if need_dw else (None, None)
+    db = (_empty(qw, D), _empty(qw, D)) if need_db else (None, None)
+    ws = _empty(q, _qk_workspace_bytes(dev.index, D), dtype=torch.uint8)
+    strides = _QKBackwardStrides(*dq_out.stride()[:3], *dk_out.stride()[:3], *q.stride()[:3],
+                                 *k.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *pos_strides)
+    _launch("trx_qk_norm_rope_bwd", dev, dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
+            qw.data_ptr(), kw.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(pos), dq.data_ptr(),
+            dk.data_ptr(), _ptr(dw[0]), _ptr(dw[1]), _ptr(db[0]), _ptr(db[1]), B, S, Hq, k.shape[2], D,
+            ctypes.addressof(strides), cos.shape[0], cos.stride(0), float(eps), HEAD_NORMS[norm],
+            int(bool(norm_first)), wide, _code(cos), _code(qw), _code(q), ws.data_ptr(), ws.numel())
+    if need_dw or need_db:
+        _count()  # the sums are a launch of their own
+    return dq, dk, *dw, *db
+
+
+@functools.lru_cache(maxsize=1024)
+def _qk_workspace_bytes(index: int, D: int) -> int:
+    """trx_qk_norm_rope_bwd_workspace_bytes on a device (it goes by the number of its SMs)."""
+    with torch.cuda.device(index):
+        return _lib.load().trx_qk_norm_rope_bwd_workspace_bytes(D)
 
 
 # ----------------------------------------------------------------------------- GLU
