@@ -490,6 +490,64 @@ int trx_attn_fwd_shared(const void* q, const void* prefix_k, const void* prefix_
 int trx_attn_status(const void* workspace, unsigned int* host_word, void* stream);
 
 /*
+ * A cache of keys and values in pages, and a batch's place in it. `k_pages` / `v_pages` are (pages, Hk,
+ * page_size, D) of the activation type, or, with scales, (pages, Hk, page_size, D / 2) bytes of two 4-bit codes
+ * each (column 2 j of a row low, 2 j + 1 high) with scales (pages, Hk, page_size, 2) of fp32 (step, lowest):
+ * a value is lowest + code * step; a row's lowest value has code 0, its highest 15, the others the nearest
+ * (halfway: the even one), step is (highest - lowest) * fp32(1/15). A row whose values are within 2^-76 of each
+ * other has step 0 and codes 0; one with a value that is not finite, or that spans more than 2^120, has both
+ * numbers NaN. D is 64 or 128, page_size a multiple of 16 up to 4096. Position p of sequence b is row
+ * p % page_size of page block_table[b][p / page_size] of (n_seq, width); numbers outside [0, pages) name no page:
+ * nothing is written there and rows of zeros are read. Strides: (page, head, row) of k_pages, v_pages in elements
+ * (codes: bytes, rows contiguous), (page, head) of k_scales, v_scales, the row of block_table: 11 in this order,
+ * the last in each entry's `strides`. Bases are 16-byte aligned and strides multiples of 16 bytes.
+ * No counterparts in the reference, whose cache is a concatenation for each step
+ * (trinix/layers/attention/grouped_query_attention.py:178-184).
+ */
+
+/*
+ * Append: n_seq sequences of S new tokens each (k, v (n_seq, S, Hk, D)), or with `cu` (n_seq + 1 first rows,
+ * ascending from 0) S packed rows in all. Token i of n of sequence b gets position lengths[b] - n + i: `lengths`
+ * count the new tokens. With tables (rows of at least D/2 by position, fp32 or `dtype`) keys are rotated on the
+ * way as by trx_rope_fwd with fp32 tables, and with q (.., Hq, D) queries into q_out. A token whose position is
+ * negative, behind the tables or on no page is not written and its rows of q_out are 0; so are q_out's rows behind
+ * the last sequence. Two tokens at one place leave either's values, or parts of both.
+ * strides: (sequence, token, head) of q, k, v, q_out (packed: the first is not used), then the cache's.
+ */
+int trx_paged_append(const void* q_or_null, const void* k, const void* v, void* q_out, void* k_pages,
+                     void* v_pages, float* k_scales_or_null, float* v_scales_or_null,
+                     const int32_t* block_table, const int32_t* lengths, const int32_t* cu_or_null,
+                     const void* cos_or_null, const void* sin_or_null, int64_t n_seq, int64_t S, int64_t Hq,
+                     int64_t Hk, int64_t D, int64_t pages, int64_t page_size, int64_t width,
+                     const int64_t strides[23], int64_t table_rows, int64_t table_row_stride, int table_dtype,
+                     int dtype, void* stream);
+
+/*
+ * Read back: rows cu[b] .. cu[b + 1] - 1 of k_out and v_out (rows, Hk, D), contiguous, become the first of sequence
+ * b's in the cache, as trx_attn_fwd_packed takes them. Rows behind the last sequence become 0 with `zero_rest`, else
+ * stay. strides: the cache's.
+ */
+int trx_paged_gather(const void* k_pages, const void* v_pages, const float* k_scales_or_null,
+                     const float* v_scales_or_null, const int32_t* block_table, const int32_t* cu, void* k_out,
+                     void* v_out, int64_t n_seq, int64_t rows, int64_t Hk, int64_t D, int64_t pages,
+                     int64_t page_size, int64_t width, const int64_t strides[11], int zero_rest, int dtype,
+                     void* stream);
+
+/*
+ * Causal attention of the last Sq tokens of each sequence, q (B, Sq, Hq, D), over the lengths[b] keys of it in the
+ * cache, theirs among them: query i stands at position lengths[b] - Sq + i and sees the keys up to there, with
+ * window_left >= 0 only the last window_left + 1 of these. slopes: ALiBi. A query that sees nothing is 0, its
+ * LSE -inf. For few rows (decoding, drafts): the time grows with every 32 (4 bits: 16) of Sq * Hq / Hk.
+ * strides: (batch, token, head) of q, out, then the cache's. Workspace and status as for trx_attn_fwd.
+ */
+int trx_attn_fwd_paged(const void* q, const void* k_pages, const void* v_pages, const float* k_scales_or_null,
+                       const float* v_scales_or_null, void* out, float* lse_or_null,
+                       const float* slopes_or_null, const int32_t* block_table, const int32_t* lengths,
+                       int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D, int64_t pages,
+                       int64_t page_size, int64_t width, const int64_t strides[17], float scale,
+                       int64_t window_left, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Attach a word of pinned host memory to an attention workspace (NULL detaches it; the workspace
  * must have been zeroed before). From then on every launch on that workspace that gives up on a
  * bounded wait, or that finds such a failure recorded and skips its work, also writes the status

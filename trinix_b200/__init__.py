@@ -10,6 +10,7 @@ from .fusion import FastFusedRMSNormInt8, RowwiseInt8Quant, fuse, register_fusio
 from .install import install, uninstall
 from .kernels import (
     PackedAttentionKernel,
+    PagedAttentionKernel,
     QKNormRoPEKernel,
     RowwiseInt8Kernel,
     SharedPrefixAttentionKernel,
@@ -40,11 +41,14 @@ from .layers import (
     FastSwiGLU,
 )
 from .ops import (
+    append_paged,
     attention,
     attention_packed,
+    attention_paged,
     attention_shared_prefix,
     attention_status,
     dequantize_rowwise,
+    gather_paged,
     glu,
     glu_backward,
     glu_pair,

@@ -28,6 +28,7 @@
 #pragma once
 
 #include "attention_common.cuh"
+#include "paged_cache.cuh"
 
 namespace trx {
 
@@ -54,6 +55,11 @@ template <int F, bool A = false>
 struct RaggedParamsOf : RaggedParams {
   static constexpr int FORM = F;
   static constexpr bool ALT = A;
+};
+
+struct PagedAttnParams : RaggedParams {
+  static constexpr int FORM = ATT_PAGED;
+  PagedCache c;
 };
 
 struct RaggedItem : PlainItem {

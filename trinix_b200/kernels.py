@@ -446,6 +446,40 @@ class SharedPrefixAttentionKernel:
             q, prefix_k, prefix_v, k, v)
 
 
+class PagedAttentionKernel:
+    """Attention over a paged cache of 16 or 4 bits, and what fills the cache (`ops.attention_paged`,
+    `ops.append_paged`). No counterpart in the reference, whose cache is a concatenation for each step
+    (trinix/layers/attention/grouped_query_attention.py:178-184). Forward only, as attention is."""
+
+    @staticmethod
+    def is_available() -> bool:
+        return _available()
+
+    @staticmethod
+    def append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+               block_table: torch.Tensor, lengths: torch.Tensor, k_scales: Optional[torch.Tensor] = None,
+               v_scales: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+               sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+               cu_seqlens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        return _run(
+            lambda a, b, c: ops.append_paged(a, b, k_pages, v_pages, block_table, lengths,
+                                             k_scales=k_scales, v_scales=v_scales, cos=cos, sin=sin, q=c,
+                                             cu_seqlens=cu_seqlens),
+            k, v, q)
+
+    @staticmethod
+    def apply(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+              lengths: torch.Tensor, k_scales: Optional[torch.Tensor] = None,
+              v_scales: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+              window_size: Optional[tuple] = None,
+              alibi_slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return _run(
+            lambda a: ops.attention_paged(a, k_pages, v_pages, block_table, lengths, k_scales=k_scales,
+                                          v_scales=v_scales, scale=scale, window=window_size,
+                                          alibi_slopes=alibi_slopes),
+            q)
+
+
 class RowwiseInt8Kernel:
     """Per-row symmetric int8 ops. The reference has no such class; the naming follows its
     kernel-class convention so the ops are reachable the same way."""

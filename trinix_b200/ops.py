@@ -1015,3 +1015,211 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
         _count()  # the prefix is a launch of its own
     out = out if dp == d else out[..., :d].contiguous()
     return (out, lse) if return_lse else out
+
+
+# ----------------------------------------------------------------------------- paged cache
+_AppendStrides, _CacheStrides = ctypes.c_int64 * (4 * 3 + 11), ctypes.c_int64 * 11
+_PagedStrides = ctypes.c_int64 * (2 * 3 + 11)
+_NO_SCALES = (0, 0, 0, 0)
+
+
+def _cache(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: Optional[torch.Tensor],
+           v_scales: Optional[torch.Tensor], block_table: torch.Tensor, sequences: int, dtype: torch.dtype):
+    """((kv heads, head_dim, pages, page size, width of the table), the cache's strides) of a paged cache, whose
+    tensors are taken as they are: nothing of them can be a copy."""
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("the paged cache serves bfloat16 and float16")
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be alike, "
+                         f"(pages, kv heads, page size, head_dim) or, of 4 bits, head_dim / 2")
+    pages, heads, size, d = k_pages.shape
+    if (k_scales is None) != (v_scales is None):
+        raise ValueError("k_scales and v_scales come together")
+    if k_scales is None:
+        if k_pages.dtype != dtype or v_pages.dtype != dtype:
+            raise TypeError(f"the cache holds {k_pages.dtype} and {v_pages.dtype}, the call's tensors are {dtype}")
+        scale_strides = _NO_SCALES
+    else:
+        d *= 2
+        if k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8:
+            raise TypeError("a cache with scales holds codes of 4 bits, two to a uint8")
+        shape = (pages, heads, size, 2)
+        for t in (k_scales, v_scales):
+            if t.dtype != torch.float32 or t.shape != shape:
+                raise ValueError(f"scales must be float32 of {shape}")
+            if t.stride()[2:] != (2, 1) and t.numel():
+                raise ValueError("a head's scales on a page must be contiguous")
+        scale_strides = (*k_scales.stride()[:2], *v_scales.stride()[:2])
+    for t in (k_pages, v_pages):
+        if t.stride(3) != 1 and t.numel():
+            raise ValueError("head_dim must be the contiguous dimension of the pages")
+    if size % 16 or not 0 < size <= 4096:
+        raise ValueError(f"page size must be a multiple of 16 up to 4096, got {size}")
+    if d not in (64, 128):
+        raise ValueError(f"the paged cache serves head_dim 64 and 128, got {d}")
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != sequences
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        raise ValueError(f"block_table must be int32 of ({sequences}, pages of a sequence), its rows contiguous")
+    strides = (*k_pages.stride()[:3], *v_pages.stride()[:3], *scale_strides, block_table.stride(0))
+    return (heads, d, pages, size, block_table.shape[1]), strides
+
+
+def _vector_view(t: torch.Tensor) -> torch.Tensor:
+    """A view whose rows can be read in 16-byte pieces, whatever the other strides are; else a copy."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    if t.numel() == 0 or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+                          and all(n == 1 or step % 8 == 0 for n, step in zip(t.shape[:-1], t.stride()))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides3(t: torch.Tensor):
+    """(sequence, token, head) strides of (sequences, tokens, heads, d) or of packed (tokens, heads, d); a dim of
+    size 1 may carry any stride, here 0."""
+    steps = [0 if n == 1 else step for n, step in zip(t.shape[:-1], t.stride())]
+    return steps if len(steps) == 3 else (0, *steps)
+
+
+def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 block_table: torch.Tensor, lengths: torch.Tensor, *,
+                 k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None,
+                 cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                 q: Optional[torch.Tensor] = None,
+                 cu_seqlens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write new tokens' keys and values into a paged cache, rotating the keys on the way.
+
+    k / v (B, S, Hk, D): S new tokens of each sequence; or, with cu_seqlens (int32 on the device, first rows
+    and the end, ascending from 0), packed (T, Hk, D). lengths (B,) int32: keys of each sequence with the new
+    ones, so that token i of n stands at position lengths[b] - n + i. k_pages / v_pages (pages, Hk, page size, D),
+    block_table (B, pages of a sequence) int32: position p is row p % page size of page
+    block_table[b, p // page size]; page size is a multiple of 16, D 64 or 128. With k_scales / v_scales
+    (pages, Hk, page size, 2) float32 the cache is of 4 bits: pages are uint8 (.., D / 2), two codes to a byte,
+    and a row of D values is held as lowest + code * step (scales: step, lowest), each within half a step.
+
+    cos / sin: tables by position, as rope() takes them; keys (and q, alike in shape but for its heads) are
+    rotated in fp32 and rounded once. Returns the rotated queries, None without q. A token whose position is
+    negative (a padded sequence of length 0), behind the tables or on no page (a number outside the cache,
+    such as -1) is not written, its queries are 0; so are those behind the last packed sequence. No two tokens
+    may have the same place. Not differentiable: what is written is no part of an autograd graph.
+    """
+    dev = _same_device(k, v, k_pages, v_pages, block_table, lengths, k_scales, v_scales, cos, sin, q, cu_seqlens)
+    packed, dtype = cu_seqlens is not None, k.dtype
+    if k.dim() != (3 if packed else 4) or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be alike, "
+                         + ("(rows, heads, head_dim)" if packed else "(batch, tokens, heads, head_dim)"))
+    if v.dtype != dtype or (q is not None and q.dtype != dtype):
+        raise TypeError("q, k and v must share a dtype")
+    cu = _cu_seqlens(cu_seqlens, "cu_seqlens") if packed else None
+    n_seq, tokens = (cu.numel() - 1, k.shape[0]) if packed else k.shape[:2]
+    if lengths.dtype != torch.int32 or lengths.shape != (n_seq,):
+        raise ValueError(f"lengths must be an int32 tensor of {n_seq} entries")
+    (Hk, D, pages, size, width), cache = _cache(k_pages, v_pages, k_scales, v_scales, block_table, n_seq, dtype)
+    if k.shape[-2:] != (Hk, D):
+        raise ValueError(f"k {tuple(k.shape)} does not match the cache's {Hk} heads of {D}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    rows, step, table_code = 0, 0, 0
+    if cos is not None:
+        cos, sin = _tables(cos, sin, dtype, D // 2)
+        if cos.shape[1] * cos.element_size() % 16 or cos.data_ptr() % 16 or sin.data_ptr() % 16:
+            cos, sin = (t[:, : D // 2].clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+        rows, step, table_code = cos.shape[0], cos.shape[1], _code(cos)
+    out, Hq = None, 0
+    if q is not None:
+        if cos is None:
+            raise ValueError("q is rotated: it needs cos and sin")
+        if q.dim() != k.dim() or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != D:
+            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
+        q, Hq = _vector_view(q), q.shape[-2]
+        out = _new(q)
+        if packed and n_seq == 0:
+            return out.zero_()
+    k, v, lengths = _vector_view(k), _vector_view(v), lengths.contiguous()
+    strides = _AppendStrides(*(_strides3(q) if q is not None else (0, 0, 0)), *_strides3(k), *_strides3(v),
+                             *(_strides3(out) if q is not None else (0, 0, 0)), *cache)
+    if k.numel() or Hq:
+        _launch("trx_paged_append", dev, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(out), k_pages.data_ptr(),
+                v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), block_table.data_ptr(), lengths.data_ptr(),
+                _ptr(cu), _ptr(cos), _ptr(sin), n_seq, tokens, Hq, Hk, D, pages, size, width,
+                ctypes.addressof(strides), rows, step, table_code, _DTYPE_CODE[dtype])
+    return out
+
+
+def gather_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                 cu_seqlens: torch.Tensor, *, rows: int, k_scales: Optional[torch.Tensor] = None,
+                 v_scales: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The sequences of a paged cache (append_paged) as packed keys and values, what attention_packed reads.
+
+    cu_seqlens (B + 1,) int32 on the device: sequence b's first cu_seqlens[b + 1] - cu_seqlens[b] keys become
+    rows cu_seqlens[b] .. of two new (rows, Hk, D) tensors; `rows`, known to the host, is at least the last
+    entry, and rows behind that are 0. So are rows on no page. A cache of 4 bits gives `dtype` (bfloat16 unless
+    given), each value rounded once.
+    """
+    dev = _same_device(k_pages, v_pages, block_table, cu_seqlens, k_scales, v_scales)
+    if dtype is None:
+        dtype = torch.bfloat16 if k_scales is not None else k_pages.dtype
+    cu = _cu_seqlens(cu_seqlens, "cu_seqlens")
+    (Hk, D, pages, size, width), cache = _cache(k_pages, v_pages, k_scales, v_scales, block_table,
+                                                cu.numel() - 1, dtype)
+    if rows < 0:
+        raise ValueError("rows must be >= 0")
+    k, v = (torch.empty((rows, Hk, D), dtype=dtype, device=dev) for _ in range(2))
+    strides = _CacheStrides(*cache)
+    if k.numel():
+        _launch("trx_paged_gather", dev, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+                block_table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), cu.numel() - 1, rows, Hk, D,
+                pages, size, width, ctypes.addressof(strides), 1, _DTYPE_CODE[dtype])
+    return k, v
+
+
+def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    lengths: torch.Tensor, *, k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    window: Optional[Tuple[int, int]] = None, alibi_slopes: Optional[torch.Tensor] = None,
+                    return_lse: bool = False):
+    """Causal attention of each sequence's last tokens over its keys in a paged cache (append_paged).
+
+    q (B, Sq, Hq, D): the last Sq tokens of each sequence, whose keys are among its lengths[b] (int32 on the
+    device) in the cache; Hq % Hk == 0. Query i stands at position lengths[b] - Sq + i and sees the keys up to
+    there, with window = (left, right) no more than left of them before its own; alibi_slopes (Hq,) add -slope *
+    distance. A query without a key (a padded sequence of length 0) is 0. Pages as in append_paged, of 16 bits
+    or, with scales, of 4; a page number outside the cache reads as zeros (pages that the window has left behind
+    may be given away). With return_lse also the fp32 (B, Hq, Sq) log-sum-exp.
+
+    For few rows, tokens and drafts: keys are read once for every 32 (4 bits: 16) of Sq * Hq / Hk rows. Longer
+    pieces of prompts go through gather_paged and attention_packed.
+    Forward only, as `attention`: PagedAttentionKernel.apply has a later .backward() say so.
+    """
+    dev = _same_device(q, k_pages, v_pages, block_table, lengths, k_scales, v_scales, alibi_slopes)
+    if q.dim() != 4:
+        raise ValueError(f"expected q (batch, rows, heads, head_dim), got {tuple(q.shape)}")
+    B, Sq, Hq, d = q.shape
+    (Hk, D, pages, size, width), cache = _cache(k_pages, v_pages, k_scales, v_scales, block_table, B, q.dtype)
+    if d != D:
+        raise ValueError(f"q {tuple(q.shape)} does not match the cache's head_dim {D}")
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError(f"query heads ({Hq}) must be a multiple of kv heads ({Hk})")
+    if pages == 0:
+        raise ValueError("the cache has no pages")
+    if lengths.dtype != torch.int32 or lengths.shape != (B,):
+        raise ValueError(f"lengths must be an int32 tensor of {B} entries")
+    left = -1
+    if window is not None:
+        left = int(window[0])
+        if left < 0 or int(window[1]) < 0:
+            raise ValueError("window sizes must be >= 0")
+    slopes = _slopes(alibi_slopes, Hq)
+    scale = D ** -0.5 if scale is None else float(scale)
+    q, lengths = _vector_view(q), lengths.contiguous()
+    out = _new(q)
+    lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
+    ws = _workspace(dev)
+    _raise_if_failed("trx_attn_fwd_paged", dev)  # of an earlier launch, before more work is queued
+    strides = _PagedStrides(*_strides3(q), *_strides3(out), *cache)
+    _launch("trx_attn_fwd_paged", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
+            _ptr(v_scales), out.data_ptr(), _ptr(lse), _ptr(slopes), block_table.data_ptr(), lengths.data_ptr(),
+            B, Sq, Hq, Hk, D, pages, size, width, ctypes.addressof(strides), scale, left, _DTYPE_CODE[q.dtype],
+            ws.data_ptr(), ws.numel())
+    return (out, lse) if return_lse else out
