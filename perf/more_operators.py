@@ -392,10 +392,11 @@ def _append_own(c, s):
     import trinix_b200 as T
 
     scales = {"k_scales": s.get("k_scales"), "v_scales": s.get("v_scales")}
+    # without a rotation there is nothing to be done with queries
     q = T.append_paged(s["k"], s["v"], s["k_pages"], s["v_pages"], s["block_table"], s["lengths"],
-                       cos=s.get("cos"), sin=s.get("sin"), q=s.get("q"), cu_seqlens=s.get("starts"),
-                       **scales)
-    out = {"q": q} if c["queries"] else {}
+                       cos=s.get("cos"), sin=s.get("sin"), q=s.get("q") if c["rotate"] else None,
+                       cu_seqlens=s.get("starts"), **scales)
+    out = {"q": q if c["rotate"] else s["q"]} if c["queries"] else {}
     if c["bits"] == 16:
         return out | {"k_pages": s["k_pages"], "v_pages": s["v_pages"]}
     out["k"], out["v"] = T.gather_paged(s["k_pages"], s["v_pages"], s["block_table"], s["starts_k"],
