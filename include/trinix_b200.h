@@ -537,15 +537,21 @@ int trx_paged_gather(const void* k_pages, const void* v_pages, const float* k_sc
  * Causal attention of the last Sq tokens of each sequence, q (B, Sq, Hq, D), over the lengths[b] keys of it in the
  * cache, theirs among them: query i stands at position lengths[b] - Sq + i and sees the keys up to there, with
  * window_left >= 0 only the last window_left + 1 of these. slopes: ALiBi. A query that sees nothing is 0, its
- * LSE -inf. For few rows (decoding, drafts): the time grows with every 32 (4 bits: 16) of Sq * Hq / Hk.
- * strides: (batch, token, head) of q, out, then the cache's. Workspace and status as for trx_attn_fwd.
+ * LSE -inf. For few rows (decoding, drafts): the time grows with every 16 of Sq * Hq / Hk.
+ * strides: (batch, token, head) of q, out, then the cache's. `parts` is trx_attn_paged_bytes() of device memory,
+ * 16-byte aligned, for this call alone; it holds nothing between calls. Workspace and status as for trx_attn_fwd.
  */
 int trx_attn_fwd_paged(const void* q, const void* k_pages, const void* v_pages, const float* k_scales_or_null,
                        const float* v_scales_or_null, void* out, float* lse_or_null,
                        const float* slopes_or_null, const int32_t* block_table, const int32_t* lengths,
                        int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D, int64_t pages,
                        int64_t page_size, int64_t width, const int64_t strides[17], float scale,
-                       int64_t window_left, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+                       int64_t window_left, int dtype, void* parts_or_null, size_t parts_bytes,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of `parts` on the current device, 0 for none; keys: width * page_size. */
+size_t trx_attn_paged_bytes(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D, int64_t keys,
+                            int64_t window_left, int four_bits);
 
 /*
  * Attach a word of pinned host memory to an attention workspace (NULL detaches it; the workspace

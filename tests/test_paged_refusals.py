@@ -97,8 +97,8 @@ def attend(lib, bits=16, **change):
     scales = ONE if bits == 4 else None
     a = dict(q=ONE, kp=ONE, vp=ONE, ks=scales, vs=scales, out=ONE, lse=None, slopes=None, table=ONE, lengths=ONE, n=2, sq=1,
              hq=4, hk=2, d=128, pages=20, size=16, width=10,
-             strides=block(512, 512, 128, 512, 512, 128, *cache_strides(bits)), scale=1.0, left=-1, dtype=2, ws=ONE, wsb=256,
-             stream=None)
+             strides=block(512, 512, 128, 512, 512, 128, *cache_strides(bits)), scale=1.0, left=-1, dtype=2, parts=ONE, pb=ALL,
+             ws=ONE, wsb=256, stream=None)
     assert set(change) <= set(a)
     a.update(change)
     return lib.trx_attn_fwd_paged(*a.values())
@@ -119,6 +119,17 @@ def test_attention_refuses(lib, bits, change, code):
     if bits == 4 and "strides" in change and change["strides"] is not None:
         change = {"strides": block(*list(change["strides"])[:6], *cache_strides(4))}
     assert attend(lib, bits, **change) == code
+
+
+def test_attention_refuses_too_little_room(lib):
+    size = lambda width, left=-1, bits=16: lib.trx_attn_paged_bytes(2, 1, 4, 2, 128, 16 * width, left, int(bits == 4))  # noqa: E731
+    for bits in (16, 4):
+        assert size(10, bits=bits) == 0 and size(1000, 100, bits=bits) == 0  # a CTA to a sequence and head
+        assert size(1000, bits=bits) > 0
+        for change in (dict(parts=None), dict(pb=size(1000, bits=bits) - 1), dict(parts=ODD)):
+            assert attend(lib, bits, width=1000, **change) == -9
+    for bad in ((0, 1, 4, 2, 128), (2, 0, 4, 2, 128), (2, 1, 4, 3, 128), (2, 1, 4, 2, 96), (1 << 17, 1, 4, 2, 64)):
+        assert lib.trx_attn_paged_bytes(*bad, 1 << 20, -1, 0) == 0
 
 
 def test_attention_has_nothing_to_do(lib):

@@ -108,7 +108,8 @@ SIGNATURES = {
                                  c_int, c_void_p]),
     "trx_paged_gather": (c_int, [*[c_void_p] * 8, *[c_int64] * 7, c_void_p, c_int, c_int, c_void_p]),
     "trx_attn_fwd_paged": (c_int, [*[c_void_p] * 10, *[c_int64] * 8, c_void_p, c_float, c_int64, c_int,
-                                   c_void_p, c_size_t, c_void_p]),
+                                   c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
+    "trx_attn_paged_bytes": (c_size_t, [*[c_int64] * 7, c_int]),
     "trx_attn_status": (c_int, [c_void_p, c_void_p, c_void_p]),
     "trx_attn_mirror": (c_int, [c_void_p, c_void_p, c_void_p]),
     "trx_attn_fwd_static_scratch": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -26,7 +26,7 @@ enum AttnStatus : unsigned {
 };
 
 // How the rows and keys of a launch are laid out (attention_plain.cuh).
-enum AttnForm { ATT_BATCH = 0, ATT_PACKED = 1, ATT_SHARED = 2, ATT_PREFIX = 3, ATT_PAGED = 4 };
+enum AttnForm { ATT_BATCH = 0, ATT_PACKED = 1, ATT_SHARED = 2, ATT_PREFIX = 3 };
 
 struct AttnParams {
   static constexpr int FORM = ATT_BATCH;

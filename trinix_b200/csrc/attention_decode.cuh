@@ -1,6 +1,5 @@
 // Attention forward for few query rows against many keys (decoding against a KV cache): of one batch, of
-// packed sequences, of a batch whose shared prefix has been done, or of one whose keys are in pages
-// (attention_ragged.cuh).
+// packed sequences, or of a batch whose shared prefix has been done (attention_ragged.cuh).
 //
 // The work is reading K and V once: per key and kv head 4 * D bytes and, with `group` query heads
 // of Sq rows on that kv head, only group * Sq rows of arithmetic. The tcgen05 kernel gives such a
@@ -159,7 +158,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
     k0 = ragged_key(p, b);
     sk = max(0, ragged_key(p, b + 1) - k0);
   }
-  if constexpr (FORM == ATT_SHARED || FORM == ATT_PAGED) {
+  if constexpr (FORM == ATT_SHARED) {
     if (p.lengths) b = by_keys(p, b);
     sk = ragged_length(p, b);
   }
@@ -197,23 +196,9 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
   const uint32_t bars = sbase + L::BAR_OFF + warp * DEC_STAGES * 8;
   int* no_result = reinterpret_cast<int*>(smem + L::FLAG_OFF);  // [DEC_WARPS], then the CTA's
   volatile int* abort_flag = no_result + warp;
-  const int kh = h0 / p.k_hdiv, vh = h0 / p.v_hdiv;
-  // Pages: a tile of 16 keys lies in one. A lane has the page of one of this warp's 32 next tiles.
-  auto load_pages = [&](int it) {
-    int page = -1;
-    if constexpr (FORM == ATT_PAGED)
-      if (it + lane < n_it) page = page_of(p.c, b, (first + (it + lane) * DEC_WARPS) * DEC_KEYS);
-    return page;
-  };
-  int pages_to_fill = load_pages(0);
-  auto issue_fill = [&](int it, int page) {  // one lane: K and V of the it-th tile of this warp
-    const int s = it % DEC_STAGES;
-    int key0 = k0 + (first + it * DEC_WARPS) * DEC_KEYS;
-    int kb = b * p.k_bmul, vb = b * p.v_bmul;
-    if constexpr (FORM == ATT_PAGED) {
-      key0 %= p.c.page_size;
-      kb = vb = page < 0 ? p.c.pages : page;  // none: behind the tensor, which reads zeros
-    }
+  const int kh = h0 / p.k_hdiv, vh = h0 / p.v_hdiv, kb = b * p.k_bmul, vb = b * p.v_bmul;
+  auto issue_fill = [&](int it) {  // one lane: K and V of the it-th tile of this warp
+    const int s = it % DEC_STAGES, key0 = k0 + (first + it * DEC_WARPS) * DEC_KEYS;
     mbar_expect_tx(bars + 8 * s, 2 * L::TILE_BYTES);
 #pragma unroll
     for (int c = 0; c < L::CHUNKS; ++c)
@@ -229,10 +214,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  for (int it = 0; it < min(n_it, DEC_STAGES); ++it) {
-    const int page = FORM == ATT_PAGED ? __shfl_sync(0xffffffffu, pages_to_fill, it) : 0;
-    if (lane == 0) issue_fill(it, page);
+    for (int it = 0; it < min(n_it, DEC_STAGES); ++it) issue_fill(it);
   }
   __syncwarp();
   // A launch that follows a recorded failure writes nothing; the copies above are waited for. The
@@ -384,12 +366,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DEC_CTAS_PER_SM)
       }
     }
     __syncwarp();  // every lane has read the tile
-    int page = 0;
-    if constexpr (FORM == ATT_PAGED) {
-      if ((it + DEC_STAGES) % 32 == 0) pages_to_fill = load_pages(it + DEC_STAGES);
-      page = __shfl_sync(0xffffffffu, pages_to_fill, (it + DEC_STAGES) % 32);
-    }
-    if (lane == 0 && !skip && it + DEC_STAGES < n_it) issue_fill(it + DEC_STAGES, page);
+    if (lane == 0 && !skip && it + DEC_STAGES < n_it) issue_fill(it + DEC_STAGES);
   }
   if (!ok) {  // gave up on tile `it`: wait (bounded) for the copies still in flight
     for (int f = it; f < min(n_it, it + DEC_STAGES); ++f) {

@@ -1,0 +1,829 @@
+// Attention forward for few query rows against the keys in the pages of a cache (paged_cache.cuh), of 16 bits or
+// of 4.
+//
+// Reading the keys is the work, and sequences of one batch may have a hundred times the keys of others. So the
+// tiles of keys of the whole batch, (sequence, kv head, tile of rows) one after the other, are one line that is
+// cut into as many equal pieces as there are CTAs: a CTA works on the end of one such unit, some whole ones and
+// the beginning of another. What it has of a unit that is not whole goes to memory, unnormalised, and a second
+// launch, which starts beside the first one's end, adds the parts up. The cuts follow from the lengths, which only
+// the device knows: every CTA adds them up when it starts. The sums' order is fixed by the lengths and the SM
+// count. A cache of so few keys to a sequence that there is nothing to cut has a CTA to a unit, and one launch.
+//
+//   * Both products are transposed: S^T = K Q^T and O^T = V^T P^T, so that a tile's 16 is keys, or columns of V,
+//     and its 8 is query rows: a group of four heads fills half of the tile where it would be a quarter. The
+//     scores' fragment becomes the operand of the second product by one movmatrix per 8 keys.
+//   * Each warp has a ring of tiles of its own, and its own running maximum, sum and O; the next unit's first tiles
+//     are on their way while the CTA's warps' results meet in shared memory.
+//   * The reference maximum of a row follows only when it is far behind (by ATT_LAZY_RESCALE), and until a lane
+//     sees that, the rows' maxima, three shuffles each, are not asked for.
+//
+// 4 bits. A key costs D + 16 bytes (codes, step and lowest of K and of V) where 16 bits cost 4 D, so of the same
+// bandwidth four times the keys come by, and what is done to each has to be that much cheaper:
+//   * The codes enter the matrix instructions as they are: a code c in the low bits of a 16-bit half is the
+//     subnormal fp16 number c * 2^-24, one in the next four bits 16 times that, and mma.sync takes subnormal
+//     operands. A word of eight codes becomes four operand registers by one shift and four ANDs; nothing is
+//     converted, and nothing is multiplied, since with one step and lowest to a row
+//         score = step_k (q . c_k) + lowest_k sum(q),    O = sum(p step_v c_v) + sum(p lowest_v).
+//     The powers of two are put into Q and taken out of the results, exactly.
+//   * Which column of the row a fragment's element is does not matter as long as both sides agree: a lane reads 16
+//     (K) and 8 (V) bytes of a row in one piece. Of 8 keys the fragment's rows are in the order 0, 4, 1, 5, ...:
+//     then the four V rows that a load reads are neighbours.
+//   * fp16 operands serve both activation types: Q's rows are scaled by a power of two to below 2^14 (what is
+//     2^-28 of the row's largest value or more stays exact). Probabilities are weighed with step_v before
+//     they are rounded to 11 bits, and the running maximum is that of the weighed ones, so that the largest
+//     weight of a row is of the order of 1 whatever the steps are.
+// Scores, sums and O are fp32.
+#pragma once
+
+#include "attention_decode.cuh"
+#include "paged_cache.cuh"
+
+namespace trx {
+
+constexpr int PG_WARPS = 4;
+constexpr int PG_THREADS = PG_WARPS * 32;
+constexpr int PG_RUN = 16;  // keys that lie in one page
+// The steps of V that are 0, of rows of one value, are weighed as this; the others are larger (paged_cache.cuh). A
+// weight over this and the keys of a sequence times 2^20 stay within fp32.
+constexpr float PG_LEAST_STEP = 0x1p-80f;
+
+// What a CTA of the first launch leaves for the second one: the unit that it found begun, if there is one.
+struct PagedPiece {
+  long long lo;          // the CTA's first place on the line
+  long long unit, end;   // where the unit begins, and its last tile ends; unit < 0: none
+  int b, m;              // its sequence, and kv head * row tiles + row tile
+};
+
+struct PagedParams {
+  CUtensorMap tm_k, tm_v;  // 16 bits
+  PagedCache c;
+  const void* q;
+  void* out;
+  float* lse;
+  const float* slopes;
+  const int* lengths;
+  unsigned int* status;
+  long long q_stride_b, q_stride_s, q_stride_h;
+  long long o_stride_b, o_stride_s, o_stride_h;
+  int B, Sq, Hq, group, row_tiles;
+  int units;               // of a sequence: kv heads * row tiles
+  int capacity;            // keys that a row of the block table holds
+  int win_left;            // < 0: no window
+  int whole;               // a CTA to a unit
+  float scale_log2;
+  PagedPiece* pieces;      // [CTAs]
+  float* part;             // [CTAs][2]: of the unit found begun, of the one left unfinished: O, m, l
+};
+
+template <int D, bool FOUR, int NT>
+struct PgShape {
+  static constexpr int KEYS = FOUR ? 32 : 16;  // of a tile
+  static constexpr int RUNS = KEYS / PG_RUN;
+  static constexpr int STAGES = FOUR ? 4 : 3;
+  static constexpr int CTAS_PER_SM = FOUR && (NT == 1 || D == 64) ? 3 : 2;
+  static constexpr int CODES = PG_RUN * D / 2, SCALES = PG_RUN * 8;  // bytes of 16 keys
+  static constexpr int RUN_BYTES = 2 * (CODES + SCALES);             // K codes, V codes, K scales, V scales
+  static constexpr int CHUNKS = D / 64, CHUNK_BYTES = 16 * 128, HALF_BYTES = CHUNKS * CHUNK_BYTES;  // 16 bits
+  static constexpr int STAGE_BYTES = FOUR ? RUNS * RUN_BYTES : 2 * HALF_BYTES;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int ROWS = 8 * NT;
+  // a warp's partial O takes the place of this many stages, the next unit's tiles the others
+  static constexpr int O_STAGES = FOUR ? NT : 1;
+  static constexpr int O_BYTES = 8 * D * 4;  // of 8 rows
+  static_assert(FOUR ? O_BYTES <= STAGE_BYTES && O_STAGES < STAGES : NT * O_BYTES <= STAGE_BYTES, "partial O");
+  static constexpr int BAR_OFF = PG_WARPS * RING_BYTES;
+  static constexpr int ML_OFF = BAR_OFF + PG_WARPS * STAGES * 8;      // max, sum per warp and row
+  static constexpr int AT_OFF = ML_OFF + 2 * PG_WARPS * ROWS * 4;     // where each warp's O is
+  static constexpr int FLAG_OFF = AT_OFF + PG_WARPS * NT * 4;         // a flag per warp: it has no result
+  static constexpr int TOTAL = FLAG_OFF + (PG_WARPS + 1) * 4;
+  static constexpr int ALIGN = FOUR ? 128 : 1024;
+  static constexpr int DYN_BYTES = TOTAL + ALIGN;
+  static constexpr int PART_FLOATS = ROWS * (D + 2);  // of one part in memory
+  // What a unit costs beside its tiles, in tiles, and what a piece of the line has at least.
+  static constexpr int UNIT_COST = FOUR ? 4 : 4;
+  static constexpr int LEAST_PIECE = FOUR ? 16 : 24;
+  static_assert(RING_BYTES >= PG_THREADS * 8, "the sums of the lengths");
+};
+
+// What is read where no page is.
+__device__ uint4 pg_zeros[PG_RUN * 128 / 2 / 16];
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+template <int WORDS>
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[WORDS]) {
+  static_assert(WORDS == 1 || WORDS == 2 || WORDS == 4, "one load");
+  if constexpr (WORDS == 4)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr)
+                 : "memory");
+  else if constexpr (WORDS == 2)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float2 lds_float2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// The keys that some query of sequence b sees, in tiles.
+struct PagedKeys {
+  int sk, first, tiles;
+};
+template <int KEYS>
+__device__ __forceinline__ PagedKeys paged_keys(const PagedParams& p, int b) {
+  PagedKeys k;
+  k.sk = min(max(__ldg(p.lengths + b), 0), p.capacity);
+  int lo = 0;
+  if (p.win_left >= 0) lo = max(0, k.sk - p.Sq - p.win_left);
+  k.first = lo / KEYS;
+  k.tiles = k.sk > 0 ? (k.sk - 1) / KEYS + 1 - k.first : 0;
+  return k;
+}
+
+// Where partial result `which` of CTA `cta` is: O [ROWS][D], then the rows' maxima, then their sums.
+template <int D, bool FOUR, int NT>
+__device__ __forceinline__ float* paged_part(const PagedParams& p, int cta, int which) {
+  return p.part + (2ll * cta + which) * PgShape<D, FOUR, NT>::PART_FLOATS;
+}
+
+// Four columns of a row of the result, and the row's LSE: acc / l. A row without keys has l == 0.
+template <int D, bool BF16>
+__device__ __forceinline__ void paged_emit(const PagedParams& p, int b, int m, int r0, int r, int c4, float4 acc,
+                                           float mx, float l) {
+  const int s = (r0 + r) / p.group, h = m / p.row_tiles * p.group + (r0 + r) % p.group;
+  const float inv = l > 0.0f ? __fdividef(1.0f, l) : l == l ? 0.0f : l;
+  uint2 v;
+  v.x = pack16<BF16>(acc.x * inv, acc.y * inv);
+  v.y = pack16<BF16>(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + b * p.o_stride_b + s * p.o_stride_s +
+                            h * p.o_stride_h + 4 * c4) = v;
+  if (p.lse && c4 == 0)
+    p.lse[(static_cast<long long>(b) * p.Hq + h) * p.Sq + s] =
+        l == 0.0f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int D, bool BF16, bool FOUR, int NT>
+__global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
+    attn_paged_kernel(const __grid_constant__ PagedParams p) {
+  using L = PgShape<D, FOUR, NT>;
+  constexpr int KEYS = L::KEYS, RUNS = L::RUNS, STAGES = L::STAGES;
+  constexpr int KW = D / 32;       // 4 bits: words of a K row to a thread
+  constexpr int VW = D / 64;       // of a V row
+  constexpr int MTILES = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + L::ALIGN - 1) &
+                                             ~static_cast<uintptr_t>(L::ALIGN - 1));
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t4 = lane & 3, g8 = lane >> 2;
+  const uint32_t ring = sbase + warp * L::RING_BYTES;
+  const uint32_t bars = sbase + L::BAR_OFF + warp * STAGES * 8;
+  float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);  // [2][PG_WARPS][ROWS]
+  int* o_at = reinterpret_cast<int*>(smem + L::AT_OFF);    // [PG_WARPS][NT]
+  volatile int* no_result = reinterpret_cast<int*>(smem + L::FLAG_OFF);
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(bars + 8 * s, 1);
+    no_result[warp] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (threadIdx.x == 0) no_result[PG_WARPS] = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
+
+  // ---- this CTA's piece [at, stop) of the line, and the sequence that it begins in --------------
+  long long at = 0, stop = 0, seq_at = 0;  // seq_at: where that sequence's units begin
+  int b = 0;
+  PagedKeys keys{};
+  if (p.whole) {
+    b = blockIdx.x / p.units;
+    keys = paged_keys<KEYS>(p, b);
+    at = static_cast<long long>(blockIdx.x - b * p.units) * (keys.tiles + L::UNIT_COST);
+    stop = at + keys.tiles + L::UNIT_COST;
+    __syncthreads();
+  } else {
+    long long* sums = reinterpret_cast<long long*>(smem);  // [PG_THREADS]
+    auto cost = [&](int i) -> long long { return i < p.B ? paged_keys<KEYS>(p, i).tiles + L::UNIT_COST : 0; };
+    const long long first_cost = cost(threadIdx.x);
+    long long mine = first_cost;
+    for (int i = threadIdx.x + PG_THREADS; i < p.B; i += PG_THREADS) mine += cost(i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    long long all = 0;
+#pragma unroll
+    for (int w = 0; w < PG_WARPS; ++w) all += sums[w];
+    all *= p.units;
+    const long long most = all / L::LEAST_PIECE;
+    const long long ctas = most < 1 ? 1 : most < gridDim.x ? most : gridDim.x;
+    at = static_cast<long long>(blockIdx.x) < ctas ? blockIdx.x * all / ctas : all;
+    stop = static_cast<long long>(blockIdx.x) < ctas ? (blockIdx.x + 1) * all / ctas : all;
+    if (threadIdx.x == 0) {
+      PagedPiece piece{at, -1, -1, 0, 0};
+      p.pieces[blockIdx.x] = piece;  // until it is known better
+    }
+    if (at >= stop) return;
+    // the sequence of `at`: sums over 128 of them at a time
+    for (int i0 = 0; i0 < p.B; i0 += PG_THREADS) {
+      long long v = i0 == 0 ? first_cost : cost(i0 + threadIdx.x);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
+      }
+      __syncthreads();
+      sums[threadIdx.x] = v;  // within the warp
+      __syncthreads();
+      long long before = seq_at;
+      int found = -1;
+      for (int w = 0; w < PG_WARPS && found < 0; ++w) {
+        const long long in_warp = sums[32 * w + 31] * p.units;
+        if (at < before + in_warp) {
+          const unsigned behind = __ballot_sync(0xffffffffu, before + sums[32 * w + lane] * p.units > at);
+          const int i = __ffs(behind) - 1;
+          found = i0 + 32 * w + i;
+          seq_at = before + (i > 0 ? sums[32 * w + i - 1] * p.units : 0);
+        }
+        before += in_warp;
+      }
+      if (found >= 0) {
+        b = found;
+        break;
+      }
+      seq_at = before;
+    }
+    keys = paged_keys<KEYS>(p, b);
+    __syncthreads();  // the sums have been read: the ring is there
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (no_result[PG_WARPS]) {  // a launch that follows a recorded failure writes nothing
+    if (threadIdx.x == 0) report_status(p.status);
+    return;
+  }
+
+  // every CTA runs: the second launch may take its place beside this one
+  if (!p.whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- units ---------------------------------------------------------------------------------
+  struct Unit {
+    int valid, b, m, r0, h0;
+    int sk, t0, t1;      // its tiles that this CTA has
+    int which;           // 0, 1: the part of it that this CTA leaves, -1: all of it
+    int hi, hi_min, lo_max;
+  };
+  auto next_unit = [&](Unit& u) {
+    u.valid = 0;
+    while (at < stop) {
+      while (at >= seq_at + static_cast<long long>(p.units) * (keys.tiles + L::UNIT_COST)) {
+        seq_at += static_cast<long long>(p.units) * (keys.tiles + L::UNIT_COST);
+        if (b + 1 >= p.B) {  // lengths that another stream has changed meanwhile
+          at = stop;
+          return;
+        }
+        keys = paged_keys<KEYS>(p, ++b);
+      }
+      const int cost = keys.tiles + L::UNIT_COST;
+      const int m = static_cast<int>((at - seq_at) / cost);
+      const long long unit = seq_at + static_cast<long long>(m) * cost;
+      const int t0 = static_cast<int>(at - unit);
+      const int t1 = static_cast<int>(stop - unit < keys.tiles ? stop - unit : keys.tiles);
+      at = unit + cost < stop ? unit + cost : stop;
+      if (t0 < t1 || (keys.tiles == 0 && t0 == 0)) {
+        const int rows = p.group * p.Sq, shift = keys.sk - p.Sq;
+        u.valid = 1;
+        u.b = b;
+        u.m = m;
+        u.h0 = m / p.row_tiles * p.group;
+        u.r0 = (m % p.row_tiles) * L::ROWS;
+        u.sk = keys.sk;
+        u.t0 = keys.first + t0;
+        u.t1 = keys.first + t1;
+        u.which = t0 > 0 ? 0 : t1 < keys.tiles ? 1 : -1;
+        const int s_min = u.r0 / p.group, s_max = min(rows - 1, u.r0 + L::ROWS - 1) / p.group;
+        u.hi = s_max + shift;
+        u.hi_min = s_min + shift;
+        u.lo_max = p.win_left >= 0 ? s_max + shift - p.win_left : 0;
+        if (t0 > 0 && threadIdx.x == 0) {
+          PagedPiece piece{unit + t0, unit, unit + keys.tiles, b, m};
+          p.pieces[blockIdx.x] = piece;
+        }
+        return;
+      }
+    }
+  };
+
+  // ---- the warp's ring: fills and reads count on over all units -----------------------------------
+  int filled = 0, read = 0;  // tiles since the start
+  int run_page = -1, run_row = 0;  // of one of the 16 keys' runs of the unit's next tiles, a lane's each
+  constexpr int AHEAD = 32 / RUNS;
+  // A lane's copy: run lane % RUNS, of K codes, V codes, K scales, V scales.
+  const int copy_run = lane % RUNS, copy_of = lane / RUNS;
+  const bool of_codes = copy_of < 2, of_k = (copy_of & 1) == 0;
+  const int64_t copy_page = of_codes ? (of_k ? p.c.kp : p.c.vp)[0] : 4 * (of_k ? p.c.ksp : p.c.vsp)[0];
+  const int64_t copy_head = of_codes ? (of_k ? p.c.kp : p.c.vp)[1] : 4 * (of_k ? p.c.ksp : p.c.vsp)[1];
+  const uint8_t* copy_base = of_codes ? static_cast<const uint8_t*>(of_k ? p.c.k : p.c.v)
+                                      : reinterpret_cast<const uint8_t*>(of_k ? p.c.k_scales : p.c.v_scales);
+  const uint32_t copy_dst =
+      copy_run * L::RUN_BYTES + (of_codes ? (of_k ? 0 : L::CODES) : 2 * L::CODES + (of_k ? 0 : L::SCALES));
+  auto fill = [&](const Unit& u, int i, int n) {  // the i-th of the warp's n tiles of a unit; the whole warp
+    if (i % AHEAD == 0) {
+      const int j = i + lane / RUNS, key = (u.t0 + warp + j * PG_WARPS) * KEYS + (lane % RUNS) * PG_RUN;
+      run_page = -1;
+      run_row = 0;
+      if (j < n && key < u.sk) {  // a run behind the last key is on a page of nobody's, perhaps
+        run_page = page_of(p.c, u.b, key);
+        run_row = key % p.c.page_size;
+      }
+    }
+    const int from = (i % AHEAD) * RUNS + (FOUR ? copy_run : 0);
+    const int page = __shfl_sync(0xffffffffu, run_page, from), row = __shfl_sync(0xffffffffu, run_row, from);
+    const int s = filled % STAGES;
+    const uint32_t bar = bars + 8 * s, to = ring + s * L::STAGE_BYTES;
+    ++filled;
+    if (lane == 0) mbar_expect_tx(bar, L::STAGE_BYTES);
+    if constexpr (FOUR) {
+      __syncwarp();
+      if (lane < 4 * RUNS) {
+        const uint8_t* src =
+            copy_base + page * copy_page + (u.m / p.row_tiles) * copy_head + row * (of_codes ? D / 2 : 8);
+        bulk_load(to + copy_dst, page < 0 ? reinterpret_cast<const uint8_t*>(pg_zeros) : src,
+                  of_codes ? L::CODES : L::SCALES, bar);
+      }
+    } else if (lane == 0) {
+      const int head = u.m / p.row_tiles, from_page = page < 0 ? p.c.pages : page;  // none: zeros, behind the tensor
+#pragma unroll
+      for (int c = 0; c < L::CHUNKS; ++c) {
+        tma_load_4d(to + c * L::CHUNK_BYTES, &p.tm_k, bar, c * 64, row, head, from_page);
+        tma_load_4d(to + L::HALF_BYTES + c * L::CHUNK_BYTES, &p.tm_v, bar, c * 64, row, head, from_page);
+      }
+    }
+  };
+  auto tiles_of = [&](const Unit& u) { return u.valid ? max(0, (u.t1 - u.t0 - warp + PG_WARPS - 1) / PG_WARPS) : 0; };
+
+  const float sl2 = p.scale_log2;
+  const bool has_alibi = p.slopes != nullptr;
+  const int key_of_row = FOUR ? (g8 >> 1) + ((g8 & 1) << 2) : g8;  // 4 bits: 0, 4, 1, 5, 2, 6, 3, 7
+  const int rows = p.group * p.Sq;
+  Unit u;
+  next_unit(u);
+  int n_it = tiles_of(u);
+  for (int i = 0; i < min(n_it, STAGES); ++i) fill(u, i, n_it);
+  bool ok = true;
+
+#pragma unroll 1
+  while (u.valid) {
+    // Q: row 8 n + g8 of the tile is the operand's column g8. 4 bits: word w of a thread has the row's columns
+    // t4 * D / 4 + 8 w .. + 7, which the ANDs below take as (0, 4), (1, 5), (2, 6), (3, 7), the second and the
+    // fourth pair 16 times too large.
+    uint32_t qf[NT][MTILES][2];
+    float factor[NT][2], q_sum[NT][2], slope2[NT][2];  // of rows 8 n + 2 t4, + 1, the scores' columns
+    int row_at[NT][2];                                 // their positions
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = u.r0 + 8 * n + g8;
+      const bool live = r < rows;
+      const int rr = live ? r : rows - 1;
+      const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + u.b * p.q_stride_b +
+                             (rr / p.group) * p.q_stride_s + (u.h0 + rr % p.group) * p.q_stride_h;
+      float down = sl2, sum = 0.0f;
+      if constexpr (FOUR) {
+        float x[8 * KW], top = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const uint4 v = live ? __ldg(reinterpret_cast<const uint4*>(qrow + t4 * (D / 4)) + w)
+                               : make_uint4(0u, 0u, 0u, 0u);
+          float f[8];
+          if constexpr (BF16) Pack<__nv_bfloat16>::unpack(v, f);
+          else Pack<__half>::unpack(v, f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[8 * w + i] = f[i];
+            top = fmaxf(top, fabsf(f[i]));
+            sum += f[i];
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        // the power of two that brings the row's largest value to 2^13 .. 2^14, and what takes it out again
+        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 240);
+        const float up = __uint_as_float(static_cast<unsigned>(267 - e) << 23);
+        down = __uint_as_float(static_cast<unsigned>(e - 13) << 23) * 0x1p24f * sl2;
+#pragma unroll
+        for (int w = 0; w < KW; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float f = i & 1 ? up * 0.0625f : up;
+            qf[n][2 * w + i / 2][i & 1] = Pack<__half>::pack2(x[8 * w + i] * f, x[8 * w + i + 4] * f);
+          }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < MTILES; ++ks)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            qf[n][ks][c] = live ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 * c + 2 * t4)) : 0u;
+      }
+      const float slope = has_alibi ? p.slopes[u.h0 + rr % p.group] * 1.4426950408889634f : 0.0f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int from = 4 * (2 * t4 + c);
+        factor[n][c] = FOUR ? __shfl_sync(0xffffffffu, down, from) : sl2;
+        q_sum[n][c] = FOUR ? __shfl_sync(0xffffffffu, sum, from) * sl2 : 0.0f;
+        slope2[n][c] = __shfl_sync(0xffffffffu, slope, from);
+        row_at[n][c] = min(rows - 1, u.r0 + 8 * n + 2 * t4 + c) / p.group + u.sk - p.Sq;
+      }
+    }
+
+    float o[MTILES][NT][4];
+    float m_run[NT][2], l_run[NT][2], low_run[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m_run[n][c] = -INFINITY;
+        l_run[n][c] = low_run[n][c] = 0.0f;
+      }
+#pragma unroll
+      for (int m = 0; m < MTILES; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[m][n][i] = 0.0f;
+    }
+
+    int next_fill = min(n_it, STAGES);
+#pragma unroll 1
+    for (int it = 0; it < n_it; ++it) {
+      const int st = read % STAGES;
+      ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, (read / STAGES) & 1, no_result + warp, p.status,
+                                             ATT_ST_SOFTMAX));
+      if (!ok) break;
+      ++read;
+      const uint32_t tile = ring + st * L::STAGE_BYTES;
+      const int c0 = (u.t0 + warp + it * PG_WARPS) * KEYS;
+      const bool need_mask = c0 + KEYS - 1 > u.hi_min || c0 < u.lo_max;
+
+      // scores of keys key_of_row (+ 8) of each run; 4 bits: weighed with V's step, x + log2 step_v
+      float x[RUNS][NT][4];
+      float v_low[RUNS][2], v_inv[RUNS][2];
+#pragma unroll
+      for (int k = 0; k < RUNS; ++k) {
+        const uint32_t sub = tile + k * L::RUN_BYTES;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+        if constexpr (FOUR) {
+          uint32_t ka[KW], kb[KW];
+          lds_words<KW>(sub + key_of_row * (D / 2) + t4 * (D / 8), ka);
+          lds_words<KW>(sub + (key_of_row + 8) * (D / 2) + t4 * (D / 8), kb);
+#pragma unroll
+          for (int w = 0; w < KW; ++w) {
+            const uint32_t a[2] = {ka[w], ka[w] >> 8}, c[2] = {kb[w], kb[w] >> 8};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t f[4] = {a[i] & 0x000F000Fu, c[i] & 0x000F000Fu, a[i] & 0x00F000F0u, c[i] & 0x00F000F0u};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_16816<false>(s[n], f, qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
+            }
+          }
+        } else {
+          const int key = lane & 15, half = lane >> 4;  // ldmatrix rows: keys 0-15 by column halves
+#pragma unroll
+          for (int ks = 0; ks < MTILES; ++ks) {
+            uint32_t f[4];
+            const int col = (ks % 4) * 2 + half;
+            ldsm_x4(tile + (ks / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<BF16>(s[n], f, qf[n][ks][0], qf[n][ks][1]);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = key_of_row + 8 * e, j = c0 + PG_RUN * k + key;
+          float2 ks = make_float2(1.0f, 0.0f);
+          float log_step = 0.0f;
+          v_low[k][e] = 0.0f;
+          v_inv[k][e] = 1.0f;
+          if constexpr (FOUR) {
+            ks = lds_float2(sub + 2 * L::CODES + 8 * key);
+            const float2 vs = lds_float2(sub + 2 * L::CODES + L::SCALES + 8 * key);
+            // fmaxf would turn a step that is not a number into the least one
+            const float step = vs.x < PG_LEAST_STEP ? PG_LEAST_STEP : vs.x;
+            asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log_step) : "f"(step));
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inv[k][e]) : "f"(step));
+            v_low[k][e] = vs.y;
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float v = s[n][2 * e + c] * factor[n][c];
+              if constexpr (FOUR) v = fmaf(v, ks.x, fmaf(q_sum[n][c], ks.y, log_step));
+              if (has_alibi) v = fmaf(-slope2[n][c], static_cast<float>(row_at[n][c] - j), v);
+              if (need_mask && (j > row_at[n][c] || (p.win_left >= 0 && j < row_at[n][c] - p.win_left))) v = -INFINITY;
+              x[k][n][2 * e + c] = v;
+            }
+        }
+      }
+      bool behind = false;
+      float mx[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          mx[n][c] = fmaxf(x[0][n][c], x[0][n][2 + c]);
+#pragma unroll
+          for (int k = 1; k < RUNS; ++k) mx[n][c] = max3(mx[n][c], x[k][n][c], x[k][n][2 + c]);
+          // (-inf + anything is -inf: a first value is larger)
+          behind = behind || mx[n][c] > m_run[n][c] + ATT_LAZY_RESCALE;
+        }
+      if (__any_sync(0xffffffffu, behind)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = mx[n][c];
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+            if (m > m_run[n][c] + ATT_LAZY_RESCALE) {
+              const float f = fast_exp2(m_run[n][c] - m);  // 0 when m_run == -inf
+              m_run[n][c] = m;
+              l_run[n][c] *= f;
+              low_run[n][c] *= f;
+#pragma unroll
+              for (int i = 0; i < MTILES; ++i) {
+                o[i][n][c] *= f;
+                o[i][n][2 + c] *= f;
+              }
+            }
+          }
+      }
+      uint32_t pf[RUNS][NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float ref[2] = {m_run[n][0] == -INFINITY ? 0.0f : m_run[n][0],
+                              m_run[n][1] == -INFINITY ? 0.0f : m_run[n][1]};
+#pragma unroll
+        for (int k = 0; k < RUNS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float w[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              w[c] = fast_exp2(x[k][n][2 * e + c] - ref[c]);
+              if constexpr (FOUR) {
+                float prob = w[c] * v_inv[k][e], low = prob * v_low[k][e];
+                // a key that the row does not see may be anything: behind the last one there is what was there
+                if (need_mask && x[k][n][2 * e + c] == -INFINITY) prob = low = 0.0f;
+                l_run[n][c] += prob;
+                low_run[n][c] += low;
+              } else {
+                l_run[n][c] += w[c];
+              }
+            }
+            pf[k][n][e] = transpose_8x8(pack16<BF16 && !FOUR>(w[0], w[1]));
+          }
+      }
+      if constexpr (FOUR) {
+#pragma unroll
+        for (int k = 0; k < RUNS; ++k) {
+          const uint32_t sub = tile + k * L::RUN_BYTES + L::CODES + t4 * (D / 2) + g8 * (D / 16);
+          uint32_t v0[VW], v1[VW], v2[VW], v3[VW];  // keys t4, + 4, + 8, + 12
+          lds_words<VW>(sub, v0);
+          lds_words<VW>(sub + 4 * (D / 2), v1);
+          lds_words<VW>(sub + 8 * (D / 2), v2);
+          lds_words<VW>(sub + 12 * (D / 2), v3);
+#pragma unroll
+          for (int w = 0; w < VW; ++w)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const unsigned pick = half ? 0x7632u : 0x5410u;
+              uint32_t a = __byte_perm(v0[w], v1[w], pick), c = __byte_perm(v2[w], v3[w], pick);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t f[4] = {a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_16816<false>(o[4 * w + 2 * half + i][n], f, pf[k][n][0], pf[k][n][1]);
+                a >>= 8;
+                c >>= 8;
+              }
+            }
+        }
+      } else {
+        // V behind the sequence's last key may be anything: keys 2 t4, 2 t4 + 1 of either half, if they are its
+        uint32_t keep[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int left = u.sk - c0 - 8 * e - 2 * t4;
+          keep[e] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+        }
+        const int key = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int m = 0; m < MTILES; ++m) {
+          uint32_t f[4];
+          const int col = (m % 4) * 2 + half;
+          ldsm_x4_trans(tile + L::HALF_BYTES + (m / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
+          if (need_mask)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] &= keep[i >> 1];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816<BF16>(o[m][n], f, pf[0][n][0], pf[0][n][1]);
+        }
+      }
+      __syncwarp();  // every lane has read the tile
+      if (next_fill < n_it) fill(u, next_fill++, n_it);
+    }
+
+    // ---- the next unit's first tiles, then this warp's partial result where the ring has room --------------
+    Unit next;
+    next.valid = 0;
+    int next_n = 0;
+    if (ok) {
+      next_unit(next);
+      next_n = tiles_of(next);
+      for (int i = 0; i < min(next_n, STAGES - L::O_STAGES); ++i) fill(next, i, next_n);
+    } else if (lane == 0) {
+      no_result[warp] = 1;
+      report_status(p.status);
+    }
+    // (a warp that gave up may still have copies on the way into its ring: it leaves no result)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int off = warp * L::RING_BYTES +
+                      (FOUR ? ((filled + n) % STAGES) * L::STAGE_BYTES : (filled % STAGES) * L::STAGE_BYTES + n * L::O_BYTES);
+      float* ow = reinterpret_cast<float*>(smem + off);
+      if (lane == 0) o_at[warp * NT + n] = off;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = 2 * t4 + c, swap = t4 << 3;  // a row's columns are 8 t4 apart from where they would be
+        float l = l_run[n][c], low = low_run[n][c];
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+          l += __shfl_xor_sync(0xffffffffu, l, w);
+          if constexpr (FOUR) low += __shfl_xor_sync(0xffffffffu, low, w);
+        }
+        if (g8 == 0) {
+          ml[warp * L::ROWS + 8 * n + r] = m_run[n][c];
+          ml[(PG_WARPS + warp) * L::ROWS + 8 * n + r] = l;
+        }
+        if (ok)
+#pragma unroll
+          for (int m = 0; m < MTILES; ++m) {
+            if constexpr (FOUR) {  // columns 2 m, 2 m + 1 of this lane's D / 8
+              *reinterpret_cast<float2*>(ow + r * D + ((g8 * (D / 8) + 2 * m) ^ swap)) =
+                  make_float2(fmaf(o[m][n][c], 0x1p24f, low), fmaf(o[m][n][2 + c], 0x1p20f, low));
+            } else {
+              ow[r * D + ((16 * m + g8) ^ swap)] = o[m][n][c];
+              ow[r * D + ((16 * m + 8 + g8) ^ swap)] = o[m][n][2 + c];
+            }
+          }
+      }
+    }
+    __syncthreads();
+    bool complete = true;  // every warp has a result; else nothing is written
+#pragma unroll
+    for (int w = 0; w < PG_WARPS; ++w) complete = complete && no_result[w] == 0;
+    if (!complete) break;
+
+    // the sum of the warps' results: weights 2^(m_i - max m), 0 for an empty part
+    const int live_rows = min(L::ROWS, rows - u.r0);
+    float* part = u.which < 0 ? nullptr : paged_part<D, FOUR, NT>(p, blockIdx.x, u.which);
+    for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += PG_THREADS) {
+      const int r = idx / (D / 4), c4 = idx % (D / 4);
+      float top = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < PG_WARPS; ++w) top = fmaxf(top, ml[w * L::ROWS + r]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < PG_WARPS; ++w) {
+        const float f = fast_exp2(ml[w * L::ROWS + r] - ref);
+        const float4 v = *reinterpret_cast<const float4*>(
+            reinterpret_cast<const float*>(smem + o_at[w * NT + (r >> 3)]) + (r & 7) * D +
+            ((4 * c4) ^ (((r & 7) >> 1) << 3)));
+        l = fmaf(f, ml[(PG_WARPS + w) * L::ROWS + r], l);
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+      }
+      if (part) {
+        *reinterpret_cast<float4*>(part + r * D + 4 * c4) = acc;
+        if (c4 == 0) {
+          part[L::ROWS * D + r] = top;
+          part[L::ROWS * (D + 1) + r] = l;
+        }
+      } else {
+        paged_emit<D, BF16>(p, u.b, u.m, u.r0, r, c4, acc, top, l);
+      }
+    }
+    __syncthreads();  // all of it has been read: the ring has its room back
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    u = next;
+    n_it = next_n;
+    for (int i = min(n_it, STAGES - L::O_STAGES); i < min(n_it, STAGES); ++i) fill(u, i, n_it);
+  }
+  // Copies on their way, where a warp of this CTA gave up: wait for them (bounded) before the CTA ends.
+  for (; read < filled; ++read) {
+    const uint64_t t0 = global_ns();
+    bool done = false;
+    while (!done && global_ns() - t0 < ATT_WAIT_NS) done = mbar_try_wait(bars + 8 * (read % STAGES), (read / STAGES) & 1);
+    if (!done) atomicOr(p.status, ATT_ST_DRAIN);
+  }
+}
+
+// The units that CTAs of the first launch share: block c has the one that CTA c found begun, if c - 1 began it.
+template <int D, bool BF16, bool FOUR, int NT>
+__global__ void __launch_bounds__(PG_THREADS) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
+  using L = PgShape<D, FOUR, NT>;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x + 1, ctas = gridDim.x + 1;
+  const PagedPiece piece = p.pieces[c];
+  if (piece.unit < 0 || piece.unit < p.pieces[c - 1].lo) return;
+  if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
+  int last = c;  // the last CTA that has tiles of the unit
+  while (last + 1 < ctas && p.pieces[last + 1].lo < piece.end) ++last;
+  const int rows = p.group * p.Sq, r0 = (piece.m % p.row_tiles) * L::ROWS, live_rows = min(L::ROWS, rows - r0);
+  for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += PG_THREADS) {
+    const int r = idx / (D / 4), c4 = idx % (D / 4);
+    float top = -INFINITY, l = 0.0f;
+    for (int k = c - 1; k <= last; ++k) top = fmaxf(top, paged_part<D, FOUR, NT>(p, k, k < c ? 1 : 0)[L::ROWS * D + r]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = c - 1; k <= last; ++k) {
+      const float* part = paged_part<D, FOUR, NT>(p, k, k < c ? 1 : 0);
+      const float f = fast_exp2(part[L::ROWS * D + r] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(part + r * D + 4 * c4);
+      l = fmaf(f, part[L::ROWS * (D + 1) + r], l);
+      acc.x = fmaf(f, v.x, acc.x);
+      acc.y = fmaf(f, v.y, acc.y);
+      acc.z = fmaf(f, v.z, acc.z);
+      acc.w = fmaf(f, v.w, acc.w);
+    }
+    paged_emit<D, BF16>(p, piece.b, piece.m, r0, r, c4, acc, top, l);
+  }
+}
+
+// How a call is cut: CTAs of the first launch, and bytes of the workspace.
+struct PagedPlan {
+  int64_t ctas;
+  bool whole;
+  size_t pieces_bytes, bytes;
+};
+template <int D, bool FOUR, int NT>
+static PagedPlan paged_plan(int64_t units, int64_t keys) {
+  using L = PgShape<D, FOUR, NT>;
+  PagedPlan plan{};
+  const int64_t tiles = (keys + L::KEYS - 1) / L::KEYS;
+  plan.whole = tiles <= 2 * L::LEAST_PIECE;
+  plan.ctas = plan.whole ? units : static_cast<int64_t>(sm_count_of_current_device()) * L::CTAS_PER_SM;
+  if (!plan.whole) {
+    plan.pieces_bytes = (plan.ctas * sizeof(PagedPiece) + 15) / 16 * 16;
+    plan.bytes = plan.pieces_bytes + plan.ctas * 2 * L::PART_FLOATS * sizeof(float);
+  }
+  return plan;
+}
+
+template <int D, bool BF16, bool FOUR, int NT>
+static int launch_paged(PagedParams& p, const PagedPlan& plan, cudaStream_t stream) {
+  using L = PgShape<D, FOUR, NT>;
+  auto kernel = attn_paged_kernel<D, BF16, FOUR, NT>;
+  static std::atomic<bool> configured[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return TRX_ERR_CUDA;
+  const bool cacheable = dev >= 0 && dev < 64;
+  if (!cacheable || !configured[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::DYN_BYTES) != cudaSuccess)
+      return TRX_ERR_CUDA;
+    if (cacheable) configured[dev].store(true, std::memory_order_release);
+  }
+  kernel<<<static_cast<unsigned>(plan.ctas), PG_THREADS, L::DYN_BYTES, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return TRX_ERR_CUDA;
+  if (plan.whole || plan.ctas < 2) return TRX_OK;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.ctas - 1));
+  cfg.blockDim = dim3(PG_THREADS);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_paged_merge_kernel<D, BF16, FOUR, NT>, p) == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
+}
+
+}  // namespace trx

@@ -28,7 +28,6 @@
 #pragma once
 
 #include "attention_common.cuh"
-#include "paged_cache.cuh"
 
 namespace trx {
 
@@ -55,11 +54,6 @@ template <int F, bool A = false>
 struct RaggedParamsOf : RaggedParams {
   static constexpr int FORM = F;
   static constexpr bool ALT = A;
-};
-
-struct PagedAttnParams : RaggedParams {
-  static constexpr int FORM = ATT_PAGED;
-  PagedCache c;
 };
 
 struct RaggedItem : PlainItem {

@@ -1188,8 +1188,8 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     or, with scales, of 4; a page number outside the cache reads as zeros (pages that the window has left behind
     may be given away). With return_lse also the fp32 (B, Hq, Sq) log-sum-exp.
 
-    For few rows, tokens and drafts: keys are read once for every 32 (4 bits: 16) of Sq * Hq / Hk rows. Longer
-    pieces of prompts go through gather_paged and attention_packed.
+    For few rows, tokens and drafts: keys are read once for every 16 of Sq * Hq / Hk rows. Longer pieces
+    of prompts go through gather_paged and attention_packed.
     Forward only, as `attention`: PagedAttentionKernel.apply has a later .backward() say so.
     """
     dev = _same_device(q, k_pages, v_pages, block_table, lengths, k_scales, v_scales, alibi_slopes)
@@ -1217,9 +1217,21 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lse = _empty(q, (B, Hq, Sq), dtype=torch.float32) if return_lse else None
     ws = _workspace(dev)
     _raise_if_failed("trx_attn_fwd_paged", dev)  # of an earlier launch, before more work is queued
+    four = k_scales is not None
+    parts = _paged_bytes(dev.index, B, Sq, Hq, Hk, D, width * size, left, four)
+    room = _empty(q, parts, dtype=torch.uint8) if parts else None
     strides = _PagedStrides(*_strides3(q), *_strides3(out), *cache)
     _launch("trx_attn_fwd_paged", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
             _ptr(v_scales), out.data_ptr(), _ptr(lse), _ptr(slopes), block_table.data_ptr(), lengths.data_ptr(),
             B, Sq, Hq, Hk, D, pages, size, width, ctypes.addressof(strides), scale, left, _DTYPE_CODE[q.dtype],
-            ws.data_ptr(), ws.numel())
+            _ptr(room), parts, ws.data_ptr(), ws.numel())
+    if parts:
+        _count()  # the sequences' parts are added up by a launch of their own
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_bytes(index: int, *sizes) -> int:
+    """trx_attn_paged_bytes on a device (the number of parts goes by its SMs)."""
+    with torch.cuda.device(index):
+        return _lib.load().trx_attn_paged_bytes(*sizes)
