@@ -43,9 +43,12 @@ namespace trx {
 constexpr int PG_WARPS = 4;
 constexpr int PG_THREADS = PG_WARPS * 32;
 constexpr int PG_RUN = 16;  // keys that lie in one page
+constexpr int PG_MOST_CTAS = 1024;  // of a launch that cuts units
 // The steps of V that are 0, of rows of one value, are weighed as this; the others are larger (paged_cache.cuh). A
 // weight over this and the keys of a sequence times 2^20 stay within fp32.
 constexpr float PG_LEAST_STEP = 0x1p-80f;
+// The reference maximum of a row that has seen nothing: finite, so that no difference of it is not a number.
+constexpr float PG_NOTHING = -1e30f;
 
 // What a CTA of the first launch leaves for the second one: the unit that it found begun, if there is one.
 struct PagedPiece {
@@ -82,9 +85,10 @@ struct PgShape {
   static constexpr int STAGES = FOUR ? 4 : 3;
   static constexpr int CTAS_PER_SM = FOUR && (NT == 1 || D == 64) ? 3 : 2;
   static constexpr int CODES = PG_RUN * D / 2, SCALES = PG_RUN * 8;  // bytes of 16 keys
-  static constexpr int RUN_BYTES = 2 * (CODES + SCALES);             // K codes, V codes, K scales, V scales
+  // a tile's K codes, V codes, K scales, V scales
+  static constexpr int V_OFF = RUNS * CODES, KS_OFF = 2 * V_OFF, VS_OFF = KS_OFF + RUNS * SCALES;
   static constexpr int CHUNKS = D / 64, CHUNK_BYTES = 16 * 128, HALF_BYTES = CHUNKS * CHUNK_BYTES;  // 16 bits
-  static constexpr int STAGE_BYTES = FOUR ? RUNS * RUN_BYTES : 2 * HALF_BYTES;
+  static constexpr int STAGE_BYTES = FOUR ? VS_OFF + RUNS * SCALES : 2 * HALF_BYTES;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int ROWS = 8 * NT;
   // a warp's partial O takes the place of this many stages, the next unit's tiles the others
@@ -100,13 +104,17 @@ struct PgShape {
   static constexpr int DYN_BYTES = TOTAL + ALIGN;
   static constexpr int PART_FLOATS = ROWS * (D + 2);  // of one part in memory
   // What a unit costs beside its tiles, in tiles, and what a piece of the line has at least.
-  static constexpr int UNIT_COST = FOUR ? 4 : 4;
-  static constexpr int LEAST_PIECE = FOUR ? 16 : 24;
+#ifndef XUC
+#define XUC 12
+#define XLP 16
+#endif
+  static constexpr int UNIT_COST = XUC;
+  static constexpr int LEAST_PIECE = XLP;
   static_assert(RING_BYTES >= PG_THREADS * 8, "the sums of the lengths");
 };
 
 // What is read where no page is.
-__device__ uint4 pg_zeros[PG_RUN * 128 / 2 / 16];
+__device__ uint4 pg_zeros[2 * PG_RUN * 128 / 2 / 16];
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -328,24 +336,35 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   int filled = 0, read = 0;  // tiles since the start
   int run_page = -1, run_row = 0;  // of one of the 16 keys' runs of the unit's next tiles, a lane's each
   constexpr int AHEAD = 32 / RUNS;
-  // A lane's copy: run lane % RUNS, of K codes, V codes, K scales, V scales.
-  const int copy_run = lane % RUNS, copy_of = lane / RUNS;
+  // A lane's copy: of K codes, V codes, K scales or V scales, run lane % RUNS, or, where pages hold whole tiles, both.
+  const bool whole_tiles = p.c.page_size % KEYS == 0;
+  const int copy_run = whole_tiles ? 0 : lane % RUNS, copy_of = whole_tiles ? lane : lane / RUNS;
   const bool of_codes = copy_of < 2, of_k = (copy_of & 1) == 0;
   const int64_t copy_page = of_codes ? (of_k ? p.c.kp : p.c.vp)[0] : 4 * (of_k ? p.c.ksp : p.c.vsp)[0];
   const int64_t copy_head = of_codes ? (of_k ? p.c.kp : p.c.vp)[1] : 4 * (of_k ? p.c.ksp : p.c.vsp)[1];
   const uint8_t* copy_base = of_codes ? static_cast<const uint8_t*>(of_k ? p.c.k : p.c.v)
                                       : reinterpret_cast<const uint8_t*>(of_k ? p.c.k_scales : p.c.v_scales);
-  const uint32_t copy_dst =
-      copy_run * L::RUN_BYTES + (of_codes ? (of_k ? 0 : L::CODES) : 2 * L::CODES + (of_k ? 0 : L::SCALES));
+  const int copy_unit = of_codes ? L::CODES : L::SCALES, copy_bytes = whole_tiles ? RUNS * copy_unit : copy_unit;
+  const uint32_t copy_dst = copy_run * copy_unit + (of_codes ? (of_k ? 0 : L::V_OFF) : of_k ? L::KS_OFF : L::VS_OFF);
+  // The runs' pages are looked up a batch of AHEAD tiles before they are needed: `soon` is this unit's next batch,
+  // or, in its last one, the next unit's first.
+  Unit u, next;
+  int n_it, next_n = 0;  // the warp's tiles of the two
+  int soon_page = -1, soon_row = 0;
+  auto look_up = [&](const Unit& u, int i, int n) {
+    const int j = i + lane / RUNS, key = (u.t0 + warp + j * PG_WARPS) * KEYS + (lane % RUNS) * PG_RUN;
+    soon_page = -1;
+    if (j < n && key < u.sk) {  // a run behind the last key is on a page of nobody's, perhaps
+      soon_page = page_of(p.c, u.b, key);
+      soon_row = key % p.c.page_size;
+    }
+  };
   auto fill = [&](const Unit& u, int i, int n) {  // the i-th of the warp's n tiles of a unit; the whole warp
     if (i % AHEAD == 0) {
-      const int j = i + lane / RUNS, key = (u.t0 + warp + j * PG_WARPS) * KEYS + (lane % RUNS) * PG_RUN;
-      run_page = -1;
-      run_row = 0;
-      if (j < n && key < u.sk) {  // a run behind the last key is on a page of nobody's, perhaps
-        run_page = page_of(p.c, u.b, key);
-        run_row = key % p.c.page_size;
-      }
+      run_page = soon_page;
+      run_row = soon_row;
+      if (i + AHEAD < n) look_up(u, i + AHEAD, n);
+      else if (i > 0) look_up(next, 0, next_n);
     }
     const int from = (i % AHEAD) * RUNS + (FOUR ? copy_run : 0);
     const int page = __shfl_sync(0xffffffffu, run_page, from), row = __shfl_sync(0xffffffffu, run_row, from);
@@ -355,11 +374,11 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     if (lane == 0) mbar_expect_tx(bar, L::STAGE_BYTES);
     if constexpr (FOUR) {
       __syncwarp();
-      if (lane < 4 * RUNS) {
+      if (lane < (whole_tiles ? 4 : 4 * RUNS)) {
         const uint8_t* src =
             copy_base + page * copy_page + (u.m / p.row_tiles) * copy_head + row * (of_codes ? D / 2 : 8);
         bulk_load(to + copy_dst, page < 0 ? reinterpret_cast<const uint8_t*>(pg_zeros) : src,
-                  of_codes ? L::CODES : L::SCALES, bar);
+                  copy_bytes, bar);
       }
     } else if (lane == 0) {
       const int head = u.m / p.row_tiles, from_page = page < 0 ? p.c.pages : page;  // none: zeros, behind the tensor
@@ -376,14 +395,24 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   const bool has_alibi = p.slopes != nullptr;
   const int key_of_row = FOUR ? (g8 >> 1) + ((g8 & 1) << 2) : g8;  // 4 bits: 0, 4, 1, 5, 2, 6, 3, 7
   const int rows = p.group * p.Sq;
-  Unit u;
   next_unit(u);
-  int n_it = tiles_of(u);
+  n_it = tiles_of(u);
+  look_up(u, 0, n_it);
   for (int i = 0; i < min(n_it, STAGES); ++i) fill(u, i, n_it);
   bool ok = true;
 
 #pragma unroll 1
   while (u.valid) {
+    next_unit(next);
+    next_n = tiles_of(next);
+    if (n_it <= AHEAD) look_up(next, 0, next_n);
+    if (next.valid) {  // its queries, a 32nd of a row to a lane
+      const int r = next.r0 + lane / 4;
+      if (r < rows)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint16_t*>(p.q) + next.b * p.q_stride_b +
+                                                      (r / p.group) * p.q_stride_s +
+                                                      (next.h0 + r % p.group) * p.q_stride_h + t4 * (D / 4)));
+    }
     // Q: row 8 n + g8 of the tile is the operand's column g8. 4 bits: word w of a thread has the row's columns
     // t4 * D / 4 + 8 w .. + 7, which the ANDs below take as (0, 4), (1, 5), (2, 6), (3, 7), the second and the
     // fourth pair 16 times too large.
@@ -441,8 +470,10 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int from = 4 * (2 * t4 + c);
-        factor[n][c] = FOUR ? __shfl_sync(0xffffffffu, down, from) : sl2;
-        q_sum[n][c] = FOUR ? __shfl_sync(0xffffffffu, sum, from) * sl2 : 0.0f;
+        if constexpr (FOUR) {
+          factor[n][c] = __shfl_sync(0xffffffffu, down, from);
+          q_sum[n][c] = __shfl_sync(0xffffffffu, sum, from) * sl2;
+        }
         slope2[n][c] = __shfl_sync(0xffffffffu, slope, from);
         row_at[n][c] = min(rows - 1, u.r0 + 8 * n + 2 * t4 + c) / p.group + u.sk - p.Sq;
       }
@@ -454,7 +485,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        m_run[n][c] = -INFINITY;
+        m_run[n][c] = PG_NOTHING;
         l_run[n][c] = low_run[n][c] = 0.0f;
       }
 #pragma unroll
@@ -477,10 +508,9 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 
       // scores of keys key_of_row (+ 8) of each run; 4 bits: weighed with V's step, x + log2 step_v
       float x[RUNS][NT][4];
-      float v_low[RUNS][2], v_inv[RUNS][2];
+      float v_low[RUNS][2], v_inv[RUNS][2];  // 4 bits
 #pragma unroll
       for (int k = 0; k < RUNS; ++k) {
-        const uint32_t sub = tile + k * L::RUN_BYTES;
         float s[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -488,8 +518,9 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
           for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
         if constexpr (FOUR) {
           uint32_t ka[KW], kb[KW];
-          lds_words<KW>(sub + key_of_row * (D / 2) + t4 * (D / 8), ka);
-          lds_words<KW>(sub + (key_of_row + 8) * (D / 2) + t4 * (D / 8), kb);
+          const uint32_t sub = tile + k * L::CODES + key_of_row * (D / 2) + t4 * (D / 8);
+          lds_words<KW>(sub, ka);
+          lds_words<KW>(sub + 8 * (D / 2), kb);
 #pragma unroll
           for (int w = 0; w < KW; ++w) {
             const uint32_t a[2] = {ka[w], ka[w] >> 8}, c[2] = {kb[w], kb[w] >> 8};
@@ -513,31 +544,51 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int key = key_of_row + 8 * e, j = c0 + PG_RUN * k + key;
-          float2 ks = make_float2(1.0f, 0.0f);
-          float log_step = 0.0f;
-          v_low[k][e] = 0.0f;
-          v_inv[k][e] = 1.0f;
+          const int key = key_of_row + 8 * e;
           if constexpr (FOUR) {
-            ks = lds_float2(sub + 2 * L::CODES + 8 * key);
-            const float2 vs = lds_float2(sub + 2 * L::CODES + L::SCALES + 8 * key);
+            const float2 ks = lds_float2(tile + L::KS_OFF + k * L::SCALES + 8 * key);
+            const float2 vs = lds_float2(tile + L::VS_OFF + k * L::SCALES + 8 * key);
             // fmaxf would turn a step that is not a number into the least one
             const float step = vs.x < PG_LEAST_STEP ? PG_LEAST_STEP : vs.x;
+            float log_step;
             asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log_step) : "f"(step));
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inv[k][e]) : "f"(step));
             v_low[k][e] = vs.y;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                x[k][n][2 * e + c] =
+                    fmaf(s[n][2 * e + c] * factor[n][c], ks.x, fmaf(q_sum[n][c], ks.y, log_step));
+          } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) x[k][n][2 * e + c] = s[n][2 * e + c] * sl2;
           }
+        }
+      }
+      if (has_alibi) {
+#pragma unroll
+        for (int k = 0; k < RUNS; ++k)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float v = s[n][2 * e + c] * factor[n][c];
-              if constexpr (FOUR) v = fmaf(v, ks.x, fmaf(q_sum[n][c], ks.y, log_step));
-              if (has_alibi) v = fmaf(-slope2[n][c], static_cast<float>(row_at[n][c] - j), v);
-              if (need_mask && (j > row_at[n][c] || (p.win_left >= 0 && j < row_at[n][c] - p.win_left))) v = -INFINITY;
-              x[k][n][2 * e + c] = v;
+            for (int i = 0; i < 4; ++i) {
+              const int j = c0 + PG_RUN * k + key_of_row + 8 * (i >> 1);
+              x[k][n][i] = fmaf(-slope2[n][i & 1], static_cast<float>(row_at[n][i & 1] - j), x[k][n][i]);
             }
-        }
+      }
+      if (need_mask) {
+#pragma unroll
+        for (int k = 0; k < RUNS; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int away = row_at[n][i & 1] - (c0 + PG_RUN * k + key_of_row + 8 * (i >> 1));
+              if (away < 0 || (p.win_left >= 0 && away > p.win_left)) x[k][n][i] = -INFINITY;
+            }
       }
       bool behind = false;
       float mx[NT][2];
@@ -548,7 +599,6 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
           mx[n][c] = fmaxf(x[0][n][c], x[0][n][2 + c]);
 #pragma unroll
           for (int k = 1; k < RUNS; ++k) mx[n][c] = max3(mx[n][c], x[k][n][c], x[k][n][2 + c]);
-          // (-inf + anything is -inf: a first value is larger)
           behind = behind || mx[n][c] > m_run[n][c] + ATT_LAZY_RESCALE;
         }
       if (__any_sync(0xffffffffu, behind)) {
@@ -560,7 +610,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
             if (m > m_run[n][c] + ATT_LAZY_RESCALE) {
-              const float f = fast_exp2(m_run[n][c] - m);  // 0 when m_run == -inf
+              const float f = fast_exp2(m_run[n][c] - m);  // 0 where nothing was seen
               m_run[n][c] = m;
               l_run[n][c] *= f;
               low_run[n][c] *= f;
@@ -573,35 +623,37 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
           }
       }
       uint32_t pf[RUNS][NT][2];
+      // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there
+      auto weigh = [&](auto masked) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float ref[2] = {m_run[n][0] == -INFINITY ? 0.0f : m_run[n][0],
-                              m_run[n][1] == -INFINITY ? 0.0f : m_run[n][1]};
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int k = 0; k < RUNS; ++k)
+          for (int k = 0; k < RUNS; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float w[2];
+            for (int e = 0; e < 2; ++e) {
+              float w[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              w[c] = fast_exp2(x[k][n][2 * e + c] - ref[c]);
-              if constexpr (FOUR) {
-                float prob = w[c] * v_inv[k][e], low = prob * v_low[k][e];
-                // a key that the row does not see may be anything: behind the last one there is what was there
-                if (need_mask && x[k][n][2 * e + c] == -INFINITY) prob = low = 0.0f;
-                l_run[n][c] += prob;
-                low_run[n][c] += low;
-              } else {
-                l_run[n][c] += w[c];
+              for (int c = 0; c < 2; ++c) {
+                w[c] = fast_exp2(x[k][n][2 * e + c] - m_run[n][c]);
+                if constexpr (FOUR) {
+                  float prob = w[c] * v_inv[k][e], low = v_low[k][e];
+                  if constexpr (decltype(masked)::value)
+                    if (x[k][n][2 * e + c] == -INFINITY) prob = low = 0.0f;
+                  l_run[n][c] += prob;
+                  low_run[n][c] = fmaf(prob, low, low_run[n][c]);
+                } else {
+                  l_run[n][c] += w[c];
+                }
               }
+              pf[k][n][e] = transpose_8x8(pack16<BF16 && !FOUR>(w[0], w[1]));
             }
-            pf[k][n][e] = transpose_8x8(pack16<BF16 && !FOUR>(w[0], w[1]));
-          }
-      }
+      };
+      if (FOUR && need_mask) weigh(std::true_type{});
+      else weigh(std::false_type{});
       if constexpr (FOUR) {
 #pragma unroll
         for (int k = 0; k < RUNS; ++k) {
-          const uint32_t sub = tile + k * L::RUN_BYTES + L::CODES + t4 * (D / 2) + g8 * (D / 16);
+          const uint32_t sub = tile + L::V_OFF + k * L::CODES + t4 * (D / 2) + g8 * (D / 16);
           uint32_t v0[VW], v1[VW], v2[VW], v3[VW];  // keys t4, + 4, + 8, + 12
           lds_words<VW>(sub, v0);
           lds_words<VW>(sub + 4 * (D / 2), v1);
@@ -649,12 +701,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     }
 
     // ---- the next unit's first tiles, then this warp's partial result where the ring has room --------------
-    Unit next;
-    next.valid = 0;
-    int next_n = 0;
     if (ok) {
-      next_unit(next);
-      next_n = tiles_of(next);
       for (int i = 0; i < min(next_n, STAGES - L::O_STAGES); ++i) fill(next, i, next_n);
     } else if (lane == 0) {
       no_result[warp] = 1;
@@ -704,14 +751,13 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     float* part = u.which < 0 ? nullptr : paged_part<D, FOUR, NT>(p, blockIdx.x, u.which);
     for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += PG_THREADS) {
       const int r = idx / (D / 4), c4 = idx % (D / 4);
-      float top = -INFINITY, l = 0.0f;
+      float top = PG_NOTHING, l = 0.0f;
 #pragma unroll
       for (int w = 0; w < PG_WARPS; ++w) top = fmaxf(top, ml[w * L::ROWS + r]);
-      const float ref = top == -INFINITY ? 0.0f : top;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < PG_WARPS; ++w) {
-        const float f = fast_exp2(ml[w * L::ROWS + r] - ref);
+        const float f = fast_exp2(ml[w * L::ROWS + r] - top);
         const float4 v = *reinterpret_cast<const float4*>(
             reinterpret_cast<const float*>(smem + o_at[w * NT + (r >> 3)]) + (r & 7) * D +
             ((4 * c4) ^ (((r & 7) >> 1) << 3)));
@@ -746,35 +792,88 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   }
 }
 
-// The units that CTAs of the first launch share: block c has the one that CTA c found begun, if c - 1 began it.
+// The units that CTAs of the first launch share: block (c, y) has two rows of the one that CTA c + 1 found begun, if
+// CTA c began it. A unit may have as many parts as there are CTAs: the rows' weights are made first, by as many
+// threads as there are parts, then groups of threads add up every PG_GROUPS-th part, eight loads in flight (one
+// after the other, 2 x 131072 keys, 56 parts to a unit, took 27 us).
+constexpr int PG_MERGE_ROWS = 2, PG_MERGE_THREADS = 256;
 template <int D, bool BF16, bool FOUR, int NT>
-__global__ void __launch_bounds__(PG_THREADS) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(PG_MERGE_THREADS) attn_paged_merge_kernel(const __grid_constant__ PagedParams p) {
   using L = PgShape<D, FOUR, NT>;
+  constexpr int ITEMS = PG_MERGE_ROWS * D / 4, GROUPS = PG_MERGE_THREADS / ITEMS;  // float4 of the rows
+  __shared__ float weight[PG_MOST_CTAS][PG_MERGE_ROWS], sum[PG_MOST_CTAS][PG_MERGE_ROWS];
+  __shared__ float red[2][PG_MERGE_THREADS / 32][PG_MERGE_ROWS];
+  __shared__ float4 sums[GROUPS][ITEMS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x + 1, ctas = gridDim.x + 1;
   const PagedPiece piece = p.pieces[c];
   if (piece.unit < 0 || piece.unit < p.pieces[c - 1].lo) return;
-  if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
-  int last = c;  // the last CTA that has tiles of the unit
-  while (last + 1 < ctas && p.pieces[last + 1].lo < piece.end) ++last;
-  const int rows = p.group * p.Sq, r0 = (piece.m % p.row_tiles) * L::ROWS, live_rows = min(L::ROWS, rows - r0);
-  for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += PG_THREADS) {
-    const int r = idx / (D / 4), c4 = idx % (D / 4);
-    float top = -INFINITY, l = 0.0f;
-    for (int k = c - 1; k <= last; ++k) top = fmaxf(top, paged_part<D, FOUR, NT>(p, k, k < c ? 1 : 0)[L::ROWS * D + r]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = c - 1; k <= last; ++k) {
-      const float* part = paged_part<D, FOUR, NT>(p, k, k < c ? 1 : 0);
-      const float f = fast_exp2(part[L::ROWS * D + r] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(part + r * D + 4 * c4);
-      l = fmaf(f, part[L::ROWS * (D + 1) + r], l);
-      acc.x = fmaf(f, v.x, acc.x);
-      acc.y = fmaf(f, v.y, acc.y);
-      acc.z = fmaf(f, v.z, acc.z);
-      acc.w = fmaf(f, v.w, acc.w);
+  const int rows = p.group * p.Sq, r0 = (piece.m % p.row_tiles) * L::ROWS, row0 = PG_MERGE_ROWS * blockIdx.y;
+  if (r0 + row0 >= rows || *reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
+  // the CTAs that have tiles of the unit: c - 1 .. c - 2 + parts
+  int parts = 1;
+  for (int k = c;; k += PG_MERGE_THREADS) {  // `lo` ascends
+    const int i = k + static_cast<int>(threadIdx.x);
+    const int n = __syncthreads_count(i < ctas && p.pieces[min(i, ctas - 1)].lo < piece.end);
+    parts += n;
+    if (n < PG_MERGE_THREADS) break;
+  }
+  auto part = [&](int k) { return paged_part<D, FOUR, NT>(p, c - 1 + k, k > 0 ? 0 : 1); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float top[PG_MERGE_ROWS], l[PG_MERGE_ROWS];
+#pragma unroll
+  for (int r = 0; r < PG_MERGE_ROWS; ++r) {
+    top[r] = PG_NOTHING;
+    for (int k = threadIdx.x; k < parts; k += PG_MERGE_THREADS) {
+      const float m = part(k)[L::ROWS * D + row0 + r];
+      weight[k][r] = m;
+      sum[k][r] = part(k)[L::ROWS * (D + 1) + row0 + r];
+      top[r] = fmaxf(top[r], m);
     }
-    paged_emit<D, BF16>(p, piece.b, piece.m, r0, r, c4, acc, top, l);
+    top[r] = warp_reduce<true>(top[r]);
+    if (lane == 0) red[0][warp][r] = top[r];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < PG_MERGE_ROWS; ++r) {
+#pragma unroll
+    for (int w = 0; w < PG_MERGE_THREADS / 32; ++w) top[r] = fmaxf(top[r], red[0][w][r]);
+    l[r] = 0.0f;
+    for (int k = threadIdx.x; k < parts; k += PG_MERGE_THREADS) {
+      const float f = fast_exp2(weight[k][r] - top[r]);
+      weight[k][r] = f;
+      l[r] = fmaf(f, sum[k][r], l[r]);
+    }
+    l[r] = warp_reduce<false>(l[r]);
+    if (lane == 0) red[1][warp][r] = l[r];
+  }
+  __syncthreads();
+  const int group = threadIdx.x / ITEMS, item = threadIdx.x % ITEMS, r = item / (D / 4), c4 = item % (D / 4);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+  for (int k = group; k < parts; k += GROUPS) {
+    const float f = weight[k][r];
+    const float4 v = *reinterpret_cast<const float4*>(part(k) + (row0 + r) * D + 4 * c4);
+    acc.x = fmaf(f, v.x, acc.x);
+    acc.y = fmaf(f, v.y, acc.y);
+    acc.z = fmaf(f, v.z, acc.z);
+    acc.w = fmaf(f, v.w, acc.w);
+  }
+  sums[group][item] = acc;
+  __syncthreads();
+  if (group == 0 && r0 + row0 + r < rows) {
+    float total = 0.0f, most = PG_NOTHING;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) {
+      const float4 v = sums[g][item];
+      acc = make_float4(acc.x + v.x, acc.y + v.y, acc.z + v.z, acc.w + v.w);
+    }
+#pragma unroll
+    for (int w = 0; w < PG_MERGE_THREADS / 32; ++w) {
+      total += red[1][w][r];
+      most = fmaxf(most, red[0][w][r]);
+    }
+    paged_emit<D, BF16>(p, piece.b, piece.m, r0, row0 + r, c4, acc, most, total);
   }
 }
 
@@ -790,7 +889,8 @@ static PagedPlan paged_plan(int64_t units, int64_t keys) {
   PagedPlan plan{};
   const int64_t tiles = (keys + L::KEYS - 1) / L::KEYS;
   plan.whole = tiles <= 2 * L::LEAST_PIECE;
-  plan.ctas = plan.whole ? units : static_cast<int64_t>(sm_count_of_current_device()) * L::CTAS_PER_SM;
+  const int64_t slots = static_cast<int64_t>(sm_count_of_current_device()) * L::CTAS_PER_SM;
+  plan.ctas = plan.whole ? units : slots < PG_MOST_CTAS ? slots : PG_MOST_CTAS;
   if (!plan.whole) {
     plan.pieces_bytes = (plan.ctas * sizeof(PagedPiece) + 15) / 16 * 16;
     plan.bytes = plan.pieces_bytes + plan.ctas * 2 * L::PART_FLOATS * sizeof(float);
@@ -818,8 +918,8 @@ static int launch_paged(PagedParams& p, const PagedPlan& plan, cudaStream_t stre
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(plan.ctas - 1));
-  cfg.blockDim = dim3(PG_THREADS);
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.ctas - 1), L::ROWS / PG_MERGE_ROWS);
+  cfg.blockDim = dim3(PG_MERGE_THREADS);
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
