@@ -65,7 +65,7 @@ extern "C" int trx_attn_fwd_paged(const void* q, const void* k_pages, const void
   p.group = static_cast<int>(Hq / Hk);
   const int64_t rows = Sq * p.group, tile = rows > 8 ? 16 : 8;
   p.row_tiles = static_cast<int>((rows + tile - 1) / tile);
-  if (Hk * p.row_tiles > 65535 || B * Hk * p.row_tiles >= (1ll << 31)) return TRX_ERR_SHAPE;
+  if (Hk * p.row_tiles > 65535 || B * Hk * p.row_tiles >= (1ll << 31) / PG_MOST_SPLITS) return TRX_ERR_SHAPE;
   if (!aligned_to(q, 16) || !aligned_to(out, 16) || !aligned_to(lengths, 4)) return TRX_ERR_ALIGNMENT;
   for (int i = 0; i < 6; ++i) {
     if (strides[i] < 0) return TRX_ERR_STRIDE;
@@ -77,7 +77,7 @@ extern "C" int trx_attn_fwd_paged(const void* q, const void* k_pages, const void
   const PagedPlan plan = plan_of(B, Sq, Hq, Hk, D, p.capacity, p.win_left, four);
   if (plan.bytes > 0 && (!parts_or_null || !aligned_to(parts_or_null, 16) || parts_bytes < plan.bytes))
     return TRX_ERR_WORKSPACE;
-  p.whole = plan.whole;
+  p.splits = plan.splits;
   p.pieces = static_cast<PagedPiece*>(parts_or_null);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(parts_or_null) + plan.pieces_bytes);
   p.q = q;
@@ -95,7 +95,11 @@ extern "C" int trx_attn_fwd_paged(const void* q, const void* k_pages, const void
   p.B = static_cast<int>(B);
   p.Sq = static_cast<int>(Sq);
   p.Hq = static_cast<int>(Hq);
-  p.units = static_cast<int>(Hk) * p.row_tiles;
+  p.heads = static_cast<int>(Hk);
+  p.units = p.heads * p.row_tiles;
+  // r * magic / 2^32 is off r / group by less than r * group / 2^32 / group
+  if (p.group > 1 && rows * p.group < (1ll << 32))
+    p.group_magic = static_cast<unsigned>(((1ull << 32) + p.group - 1) / p.group);
   p.scale_log2 = scale * 1.4426950408889634f;
   if (!four) {
     const PagedCache& c = p.c;

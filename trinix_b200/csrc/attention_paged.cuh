@@ -5,9 +5,12 @@
 // tiles of keys of the whole batch, (sequence, kv head, tile of rows) one after the other, are one line that is
 // cut into as many equal pieces as there are CTAs: a CTA works on the end of one such unit, some whole ones and
 // the beginning of another. What it has of a unit that is not whole goes to memory, unnormalised, and a second
-// launch, which starts beside the first one's end, adds the parts up. The cuts follow from the lengths, which only
-// the device knows: every CTA adds them up when it starts. The sums' order is fixed by the lengths and the SM
-// count. A cache of so few keys to a sequence that there is nothing to cut has a CTA to a unit, and one launch.
+// launch, prepared beside the first one's end, adds the parts up. The cuts follow from the lengths, which only the
+// device knows: every CTA adds them up when it starts. The sums' order is fixed by the lengths and the SM count.
+// All that costs a call 5 to 7 us. (Parts added up by the CTA that finds them all there, told by flags, so that
+// there is one launch: 2 x 131072 keys of 4 bits 48 us, so 44; 48 sequences of up to 8192 of 16 bits 73, so 71.)
+// Where the cache holds few keys to a sequence a unit has a CTA, or, where there are
+// few units, a cluster, whose CTAs share its keys alike and add up over distributed shared memory.
 //
 //   * Both products are transposed: S^T = K Q^T and O^T = V^T P^T, so that a tile's 16 is keys, or columns of V,
 //     and its 8 is query rows: a group of four heads fills half of the tile where it would be a quarter. The
@@ -43,6 +46,7 @@ namespace trx {
 constexpr int PG_WARPS = 4;
 constexpr int PG_THREADS = PG_WARPS * 32;
 constexpr int PG_RUN = 16;  // keys that lie in one page
+constexpr int PG_MOST_SPLITS = 8;
 constexpr int PG_MOST_CTAS = 1024;  // of a launch that cuts units
 // The steps of V that are 0, of rows of one value, are weighed as this; the others are larger (paged_cache.cuh). A
 // weight over this and the keys of a sequence times 2^20 stay within fp32.
@@ -54,7 +58,7 @@ constexpr float PG_NOTHING = -1e30f;
 struct PagedPiece {
   long long lo;          // the CTA's first place on the line
   long long unit, end;   // where the unit begins, and its last tile ends; unit < 0: none
-  int b, m;              // its sequence, and kv head * row tiles + row tile
+  int b, head, r0, pad;
 };
 
 struct PagedParams {
@@ -69,10 +73,11 @@ struct PagedParams {
   long long q_stride_b, q_stride_s, q_stride_h;
   long long o_stride_b, o_stride_s, o_stride_h;
   int B, Sq, Hq, group, row_tiles;
-  int units;               // of a sequence: kv heads * row tiles
+  int heads, units;        // kv heads; units of a sequence: these * row tiles
+  unsigned group_magic;    // 2^32 / group, rounded up, where that divides every row; or 0
   int capacity;            // keys that a row of the block table holds
   int win_left;            // < 0: no window
-  int whole;               // a CTA to a unit
+  int splits;              // CTAs of a unit's cluster; 0: the batch is one line
   float scale_log2;
   PagedPiece* pieces;      // [CTAs]
   float* part;             // [CTAs][2]: of the unit found begun, of the one left unfinished: O, m, l
@@ -80,10 +85,11 @@ struct PagedParams {
 
 template <int D, bool FOUR, int NT>
 struct PgShape {
-  static constexpr int KEYS = FOUR ? 32 : 16;  // of a tile
+  static constexpr int KEYS = FOUR ? 64 : 16;  // of a tile
   static constexpr int RUNS = KEYS / PG_RUN;
-  static constexpr int STAGES = FOUR ? 4 : 3;
-  static constexpr int CTAS_PER_SM = FOUR && (NT == 1 || D == 64) ? 3 : 2;
+  static constexpr int STEP = FOUR ? 32 : 16;  // keys that a warp works on at a time
+  static constexpr int STAGES = FOUR ? 2 : 3;
+    static constexpr int CTAS_PER_SM = FOUR && (NT == 1 || D == 64) ? 3 : 2;
   static constexpr int CODES = PG_RUN * D / 2, SCALES = PG_RUN * 8;  // bytes of 16 keys
   // a tile's K codes, V codes, K scales, V scales
   static constexpr int V_OFF = RUNS * CODES, KS_OFF = 2 * V_OFF, VS_OFF = KS_OFF + RUNS * SCALES;
@@ -92,29 +98,26 @@ struct PgShape {
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int ROWS = 8 * NT;
   // a warp's partial O takes the place of this many stages, the next unit's tiles the others
-  static constexpr int O_STAGES = FOUR ? NT : 1;
   static constexpr int O_BYTES = 8 * D * 4;  // of 8 rows
-  static_assert(FOUR ? O_BYTES <= STAGE_BYTES && O_STAGES < STAGES : NT * O_BYTES <= STAGE_BYTES, "partial O");
+  static constexpr int O_STAGES = NT * O_BYTES <= STAGE_BYTES ? 1 : NT;
+  static_assert(O_BYTES <= STAGE_BYTES && O_STAGES < STAGES, "partial O");
   static constexpr int BAR_OFF = PG_WARPS * RING_BYTES;
   static constexpr int ML_OFF = BAR_OFF + PG_WARPS * STAGES * 8;      // max, sum per warp and row
-  static constexpr int AT_OFF = ML_OFF + 2 * PG_WARPS * ROWS * 4;     // where each warp's O is
+  static constexpr int CTA_ML_OFF = ML_OFF + 2 * PG_WARPS * ROWS * 4;
+  static constexpr int AT_OFF = CTA_ML_OFF + 2 * ROWS * 4;            // where each warp's O is
   static constexpr int FLAG_OFF = AT_OFF + PG_WARPS * NT * 4;         // a flag per warp: it has no result
   static constexpr int TOTAL = FLAG_OFF + (PG_WARPS + 1) * 4;
   static constexpr int ALIGN = FOUR ? 128 : 1024;
   static constexpr int DYN_BYTES = TOTAL + ALIGN;
   static constexpr int PART_FLOATS = ROWS * (D + 2);  // of one part in memory
   // What a unit costs beside its tiles, in tiles, and what a piece of the line has at least.
-#ifndef XUC
-#define XUC 12
-#define XLP 16
-#endif
-  static constexpr int UNIT_COST = XUC;
-  static constexpr int LEAST_PIECE = XLP;
+  static constexpr int UNIT_COST = FOUR ? 6 : 12;
+  static constexpr int LEAST_PIECE = FOUR ? 8 : 16;
   static_assert(RING_BYTES >= PG_THREADS * 8, "the sums of the lengths");
 };
 
 // What is read where no page is.
-__device__ uint4 pg_zeros[2 * PG_RUN * 128 / 2 / 16];
+__device__ uint4 pg_zeros[64 * 128 / 2 / 16];
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -167,11 +170,16 @@ __device__ __forceinline__ float* paged_part(const PagedParams& p, int cta, int 
   return p.part + (2ll * cta + which) * PgShape<D, FOUR, NT>::PART_FLOATS;
 }
 
+// r / group of a row r of a sequence.
+__device__ __forceinline__ int paged_token(const PagedParams& p, int r) {
+  return p.group == 1 ? r : p.group_magic ? static_cast<int>(__umulhi(r, p.group_magic)) : r / p.group;
+}
+
 // Four columns of a row of the result, and the row's LSE: acc / l. A row without keys has l == 0.
 template <int D, bool BF16>
-__device__ __forceinline__ void paged_emit(const PagedParams& p, int b, int m, int r0, int r, int c4, float4 acc,
-                                           float mx, float l) {
-  const int s = (r0 + r) / p.group, h = m / p.row_tiles * p.group + (r0 + r) % p.group;
+__device__ __forceinline__ void paged_emit(const PagedParams& p, int b, int head, int row, int c4, float4 acc, float mx,
+                                           float l) {
+  const int s = paged_token(p, row), h = head * p.group + row - s * p.group;
   const float inv = l > 0.0f ? __fdividef(1.0f, l) : l == l ? 0.0f : l;
   uint2 v;
   v.x = pack16<BF16>(acc.x * inv, acc.y * inv);
@@ -199,7 +207,8 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   const int t4 = lane & 3, g8 = lane >> 2;
   const uint32_t ring = sbase + warp * L::RING_BYTES;
   const uint32_t bars = sbase + L::BAR_OFF + warp * STAGES * 8;
-  float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);  // [2][PG_WARPS][ROWS]
+  float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);          // [2][PG_WARPS][ROWS]
+  float* cta_ml = reinterpret_cast<float*>(smem + L::CTA_ML_OFF);  // [2][ROWS]
   int* o_at = reinterpret_cast<int*>(smem + L::AT_OFF);    // [PG_WARPS][NT]
   volatile int* no_result = reinterpret_cast<int*>(smem + L::FLAG_OFF);
   if (lane == 0) {
@@ -214,10 +223,13 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   long long at = 0, stop = 0, seq_at = 0;  // seq_at: where that sequence's units begin
   int b = 0;
   PagedKeys keys{};
-  if (p.whole) {
-    b = blockIdx.x / p.units;
+  int split = 0;
+  if (p.splits) {
+    const int i = blockIdx.x / p.splits;
+    split = blockIdx.x - i * p.splits;
+    b = i / p.units;
     keys = paged_keys<KEYS>(p, b);
-    at = static_cast<long long>(blockIdx.x - b * p.units) * (keys.tiles + L::UNIT_COST);
+    at = static_cast<long long>(i - b * p.units) * (keys.tiles + L::UNIT_COST);
     stop = at + keys.tiles + L::UNIT_COST;
     __syncthreads();
   } else {
@@ -239,7 +251,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     at = static_cast<long long>(blockIdx.x) < ctas ? blockIdx.x * all / ctas : all;
     stop = static_cast<long long>(blockIdx.x) < ctas ? (blockIdx.x + 1) * all / ctas : all;
     if (threadIdx.x == 0) {
-      PagedPiece piece{at, -1, -1, 0, 0};
+      PagedPiece piece{at, -1, -1, 0, 0, 0, 0};
       p.pieces[blockIdx.x] = piece;  // until it is known better
     }
     if (at >= stop) return;
@@ -276,58 +288,72 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     __syncthreads();  // the sums have been read: the ring is there
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (no_result[PG_WARPS]) {  // a launch that follows a recorded failure writes nothing
+  // A launch that follows a recorded failure writes nothing. The word may turn non-zero at any time, so that CTAs of
+  // a cluster may see it differently: they all stay to the end.
+  const bool skip = no_result[PG_WARPS] != 0;
+  if (skip) {
     if (threadIdx.x == 0) report_status(p.status);
-    return;
+    if (p.splits < 2) return;
   }
 
   // every CTA runs: the second launch may take its place beside this one
-  if (!p.whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!p.splits) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- units ---------------------------------------------------------------------------------
   struct Unit {
-    int valid, b, m, r0, h0;
+    int valid, b, head, r0;
     int sk, t0, t1;      // its tiles that this CTA has
     int which;           // 0, 1: the part of it that this CTA leaves, -1: all of it
+    int tiles;           // of the whole unit
     int hi, hi_min, lo_max;
   };
+  const int rows = p.group * p.Sq;
+  // where the next one begins, which it is
+  int unit_head, unit_tile;
+  long long unit_at;
+  {
+    const int cost = keys.tiles + L::UNIT_COST, m = static_cast<int>((at - seq_at) / cost);
+    unit_at = seq_at + static_cast<long long>(m) * cost;
+    unit_head = m / p.row_tiles;
+    unit_tile = m - unit_head * p.row_tiles;
+  }
   auto next_unit = [&](Unit& u) {
     u.valid = 0;
-    while (at < stop) {
-      while (at >= seq_at + static_cast<long long>(p.units) * (keys.tiles + L::UNIT_COST)) {
-        seq_at += static_cast<long long>(p.units) * (keys.tiles + L::UNIT_COST);
-        if (b + 1 >= p.B) {  // lengths that another stream has changed meanwhile
-          at = stop;
-          return;
-        }
-        keys = paged_keys<KEYS>(p, ++b);
-      }
-      const int cost = keys.tiles + L::UNIT_COST;
-      const int m = static_cast<int>((at - seq_at) / cost);
-      const long long unit = seq_at + static_cast<long long>(m) * cost;
-      const int t0 = static_cast<int>(at - unit);
-      const int t1 = static_cast<int>(stop - unit < keys.tiles ? stop - unit : keys.tiles);
-      at = unit + cost < stop ? unit + cost : stop;
+    while (at < stop && !u.valid) {
+      const long long end = unit_at + keys.tiles + L::UNIT_COST;
+      const int t0 = static_cast<int>(at - unit_at);
+      const int t1 = static_cast<int>(stop - unit_at < keys.tiles ? stop - unit_at : keys.tiles);
       if (t0 < t1 || (keys.tiles == 0 && t0 == 0)) {
-        const int rows = p.group * p.Sq, shift = keys.sk - p.Sq;
+        const int shift = keys.sk - p.Sq;
         u.valid = 1;
         u.b = b;
-        u.m = m;
-        u.h0 = m / p.row_tiles * p.group;
-        u.r0 = (m % p.row_tiles) * L::ROWS;
+        u.head = unit_head;
+        u.r0 = unit_tile * L::ROWS;
         u.sk = keys.sk;
         u.t0 = keys.first + t0;
         u.t1 = keys.first + t1;
         u.which = t0 > 0 ? 0 : t1 < keys.tiles ? 1 : -1;
-        const int s_min = u.r0 / p.group, s_max = min(rows - 1, u.r0 + L::ROWS - 1) / p.group;
+        u.tiles = keys.tiles;
+        const int s_min = paged_token(p, u.r0), s_max = paged_token(p, min(rows - 1, u.r0 + L::ROWS - 1));
         u.hi = s_max + shift;
         u.hi_min = s_min + shift;
         u.lo_max = p.win_left >= 0 ? s_max + shift - p.win_left : 0;
         if (t0 > 0 && threadIdx.x == 0) {
-          PagedPiece piece{unit + t0, unit, unit + keys.tiles, b, m};
+          PagedPiece piece{at, unit_at, unit_at + keys.tiles, b, unit_head, u.r0, 0};
           p.pieces[blockIdx.x] = piece;
         }
-        return;
+      }
+      at = end < stop ? end : stop;
+      if (at < stop) {
+        unit_at = end;
+        if (++unit_tile == p.row_tiles) {
+          unit_tile = 0;
+          if (++unit_head == p.heads) {
+            unit_head = 0;
+            if (++b < p.B) keys = paged_keys<KEYS>(p, b);
+            else stop = at;  // lengths that another stream has changed meanwhile
+          }
+        }
       }
     }
   };
@@ -376,12 +402,12 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
       __syncwarp();
       if (lane < (whole_tiles ? 4 : 4 * RUNS)) {
         const uint8_t* src =
-            copy_base + page * copy_page + (u.m / p.row_tiles) * copy_head + row * (of_codes ? D / 2 : 8);
+            copy_base + page * copy_page + u.head * copy_head + row * (of_codes ? D / 2 : 8);
         bulk_load(to + copy_dst, page < 0 ? reinterpret_cast<const uint8_t*>(pg_zeros) : src,
                   copy_bytes, bar);
       }
     } else if (lane == 0) {
-      const int head = u.m / p.row_tiles, from_page = page < 0 ? p.c.pages : page;  // none: zeros, behind the tensor
+      const int head = u.head, from_page = page < 0 ? p.c.pages : page;  // none: zeros, behind the tensor
 #pragma unroll
       for (int c = 0; c < L::CHUNKS; ++c) {
         tma_load_4d(to + c * L::CHUNK_BYTES, &p.tm_k, bar, c * 64, row, head, from_page);
@@ -394,9 +420,13 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   const float sl2 = p.scale_log2;
   const bool has_alibi = p.slopes != nullptr;
   const int key_of_row = FOUR ? (g8 >> 1) + ((g8 & 1) << 2) : g8;  // 4 bits: 0, 4, 1, 5, 2, 6, 3, 7
-  const int rows = p.group * p.Sq;
   next_unit(u);
-  n_it = tiles_of(u);
+  if (p.splits > 1) {  // the unit's tiles alike
+    const int share = (u.tiles + p.splits - 1) / p.splits, first = u.t0;
+    u.t1 = first + min(u.tiles, (split + 1) * share);
+    u.t0 = first + min(u.tiles, split * share);
+  }
+  n_it = skip ? 0 : tiles_of(u);
   look_up(u, 0, n_it);
   for (int i = 0; i < min(n_it, STAGES); ++i) fill(u, i, n_it);
   bool ok = true;
@@ -407,12 +437,15 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     next_n = tiles_of(next);
     if (n_it <= AHEAD) look_up(next, 0, next_n);
     if (next.valid) {  // its queries, a 32nd of a row to a lane
-      const int r = next.r0 + lane / 4;
+      const int r = next.r0 + lane / 4, token = paged_token(p, r);
       if (r < rows)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint16_t*>(p.q) + next.b * p.q_stride_b +
-                                                      (r / p.group) * p.q_stride_s +
-                                                      (next.h0 + r % p.group) * p.q_stride_h + t4 * (D / 4)));
+                                                      token * p.q_stride_s +
+                                                      ((next.head - token) * p.group + r) * p.q_stride_h +
+                                                      t4 * (D / 4)));
     }
+    float o[MTILES][NT][4];
+    float m_run[NT][2], l_run[NT][2], low_run[NT][2];
     // Q: row 8 n + g8 of the tile is the operand's column g8. 4 bits: word w of a thread has the row's columns
     // t4 * D / 4 + 8 w .. + 7, which the ANDs below take as (0, 4), (1, 5), (2, 6), (3, 7), the second and the
     // fourth pair 16 times too large.
@@ -423,42 +456,37 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     for (int n = 0; n < NT; ++n) {
       const int r = u.r0 + 8 * n + g8;
       const bool live = r < rows;
-      const int rr = live ? r : rows - 1;
-      const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + u.b * p.q_stride_b +
-                             (rr / p.group) * p.q_stride_s + (u.h0 + rr % p.group) * p.q_stride_h;
-      float down = sl2, sum = 0.0f;
+      const int rr = live ? r : rows - 1, token = paged_token(p, rr);
+      const int h = u.head * p.group + rr - token * p.group;
+      const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + u.b * p.q_stride_b + token * p.q_stride_s +
+                             h * p.q_stride_h;
+      float down = sl2;
       if constexpr (FOUR) {
-        float x[8 * KW], top = 0.0f;
+        using P = std::conditional_t<BF16, Pack<__nv_bfloat16>, Pack<__half>>;
+        uint4 v[KW];
+        auto top2 = P::absacc_init();
 #pragma unroll
         for (int w = 0; w < KW; ++w) {
-          const uint4 v = live ? __ldg(reinterpret_cast<const uint4*>(qrow + t4 * (D / 4)) + w)
-                               : make_uint4(0u, 0u, 0u, 0u);
-          float f[8];
-          if constexpr (BF16) Pack<__nv_bfloat16>::unpack(v, f);
-          else Pack<__half>::unpack(v, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[8 * w + i] = f[i];
-            top = fmaxf(top, fabsf(f[i]));
-            sum += f[i];
-          }
+          v[w] = live ? __ldg(reinterpret_cast<const uint4*>(qrow + t4 * (D / 4)) + w) : make_uint4(0u, 0u, 0u, 0u);
+          P::absacc(v[w], top2);
         }
+        float top = P::absacc_final(top2);
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
+        for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         // the power of two that brings the row's largest value to 2^13 .. 2^14, and what takes it out again
         const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 240);
         const float up = __uint_as_float(static_cast<unsigned>(267 - e) << 23);
         down = __uint_as_float(static_cast<unsigned>(e - 13) << 23) * 0x1p24f * sl2;
 #pragma unroll
-        for (int w = 0; w < KW; ++w)
+        for (int w = 0; w < KW; ++w) {
+          float x[8];
+          P::unpack(v[w], x);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float f = i & 1 ? up * 0.0625f : up;
-            qf[n][2 * w + i / 2][i & 1] = Pack<__half>::pack2(x[8 * w + i] * f, x[8 * w + i + 4] * f);
+            qf[n][2 * w + i / 2][i & 1] = Pack<__half>::pack2(x[i] * f, x[i + 4] * f);
           }
+        }
       } else {
 #pragma unroll
         for (int ks = 0; ks < MTILES; ++ks)
@@ -466,21 +494,27 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
           for (int c = 0; c < 2; ++c)
             qf[n][ks][c] = live ? __ldg(reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 * c + 2 * t4)) : 0u;
       }
-      const float slope = has_alibi ? p.slopes[u.h0 + rr % p.group] * 1.4426950408889634f : 0.0f;
+      const float slope = has_alibi ? p.slopes[h] * 1.4426950408889634f : 0.0f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int from = 4 * (2 * t4 + c);
         if constexpr (FOUR) {
           factor[n][c] = __shfl_sync(0xffffffffu, down, from);
-          q_sum[n][c] = __shfl_sync(0xffffffffu, sum, from) * sl2;
         }
         slope2[n][c] = __shfl_sync(0xffffffffu, slope, from);
-        row_at[n][c] = min(rows - 1, u.r0 + 8 * n + 2 * t4 + c) / p.group + u.sk - p.Sq;
+        row_at[n][c] = __shfl_sync(0xffffffffu, token, from) + u.sk - p.Sq;
+      }
+      if constexpr (FOUR) {
+        // sum(q): the product with ones, and 16 where Q has a 16th
+        const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x4C004C00u, 0x4C004C00u};
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ks = 0; ks < MTILES; ++ks) mma_16816<false>(sum, ones, qf[n][ks][0], qf[n][ks][1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) q_sum[n][c] = sum[c] * factor[n][c] * 0x1p-24f;
       }
     }
 
-    float o[MTILES][NT][4];
-    float m_run[NT][2], l_run[NT][2], low_run[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -502,198 +536,213 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
                                              ATT_ST_SOFTMAX));
       if (!ok) break;
       ++read;
-      const uint32_t tile = ring + st * L::STAGE_BYTES;
-      const int c0 = (u.t0 + warp + it * PG_WARPS) * KEYS;
-      const bool need_mask = c0 + KEYS - 1 > u.hi_min || c0 < u.lo_max;
+      constexpr int SUBS = L::STEP / PG_RUN;
+#pragma unroll 1
+      for (int step = 0; step < KEYS / L::STEP; ++step) {
+        const uint32_t tile = ring + st * L::STAGE_BYTES + step * SUBS * L::CODES;
+        const uint32_t scales = tile + L::KS_OFF + step * SUBS * (L::SCALES - L::CODES);
+        const int c0 = (u.t0 + warp + it * PG_WARPS) * KEYS + step * L::STEP;
+        if (c0 > u.hi) break;
+        const bool need_mask = c0 + L::STEP - 1 > u.hi_min || c0 < u.lo_max;
 
-      // scores of keys key_of_row (+ 8) of each run; 4 bits: weighed with V's step, x + log2 step_v
-      float x[RUNS][NT][4];
-      float v_low[RUNS][2], v_inv[RUNS][2];  // 4 bits
+        // scores of keys key_of_row (+ 8) of each run; 4 bits: weighed with V's step, x + log2 step_v
+        float x[SUBS][NT][4];
+        float v_low[SUBS][2], v_inv[SUBS][2];  // 4 bits
 #pragma unroll
-      for (int k = 0; k < RUNS; ++k) {
-        float s[NT][4];
+        for (int k = 0; k < SUBS; ++k) {
+          // the products of a run's columns in two sums: one alone would wait for itself
+          constexpr int CHAINS = NT == 1 ? 2 : 1;
+          float s[NT][4], s2[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
-        if constexpr (FOUR) {
-          uint32_t ka[KW], kb[KW];
-          const uint32_t sub = tile + k * L::CODES + key_of_row * (D / 2) + t4 * (D / 8);
-          lds_words<KW>(sub, ka);
-          lds_words<KW>(sub + 8 * (D / 2), kb);
-#pragma unroll
-          for (int w = 0; w < KW; ++w) {
-            const uint32_t a[2] = {ka[w], ka[w] >> 8}, c[2] = {kb[w], kb[w] >> 8};
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t f[4] = {a[i] & 0x000F000Fu, c[i] & 0x000F000Fu, a[i] & 0x00F000F0u, c[i] & 0x00F000F0u};
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma_16816<false>(s[n], f, qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
-            }
-          }
-        } else {
-          const int key = lane & 15, half = lane >> 4;  // ldmatrix rows: keys 0-15 by column halves
-#pragma unroll
-          for (int ks = 0; ks < MTILES; ++ks) {
-            uint32_t f[4];
-            const int col = (ks % 4) * 2 + half;
-            ldsm_x4(tile + (ks / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816<BF16>(s[n], f, qf[n][ks][0], qf[n][ks][1]);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = key_of_row + 8 * e;
+            for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.0f;
           if constexpr (FOUR) {
-            const float2 ks = lds_float2(tile + L::KS_OFF + k * L::SCALES + 8 * key);
-            const float2 vs = lds_float2(tile + L::VS_OFF + k * L::SCALES + 8 * key);
-            // fmaxf would turn a step that is not a number into the least one
-            const float step = vs.x < PG_LEAST_STEP ? PG_LEAST_STEP : vs.x;
-            float log_step;
-            asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log_step) : "f"(step));
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inv[k][e]) : "f"(step));
-            v_low[k][e] = vs.y;
+            uint32_t ka[KW], kb[KW];
+            const uint32_t sub = tile + k * L::CODES + key_of_row * (D / 2) + t4 * (D / 8);
+            lds_words<KW>(sub, ka);
+            lds_words<KW>(sub + 8 * (D / 2), kb);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int w = 0; w < KW; ++w) {
+              const uint32_t a[2] = {ka[w], ka[w] >> 8}, c[2] = {kb[w], kb[w] >> 8};
 #pragma unroll
-              for (int c = 0; c < 2; ++c)
-                x[k][n][2 * e + c] =
-                    fmaf(s[n][2 * e + c] * factor[n][c], ks.x, fmaf(q_sum[n][c], ks.y, log_step));
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t f[4] = {a[i] & 0x000F000Fu, c[i] & 0x000F000Fu, a[i] & 0x00F000F0u, c[i] & 0x00F000F0u};
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma_16816<false>(i < CHAINS - 1 ? s2[n] : s[n], f, qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
+              }
+            }
           } else {
+            const int key = lane & 15, half = lane >> 4;  // ldmatrix rows: keys 0-15 by column halves
+#pragma unroll
+            for (int ks = 0; ks < MTILES; ++ks) {
+              uint32_t f[4];
+              const int col = (ks % 4) * 2 + half;
+              ldsm_x4(tile + (ks / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                mma_16816<BF16>(ks % 2 < CHAINS - 1 ? s2[n] : s[n], f, qf[n][ks][0], qf[n][ks][1]);
+            }
+          }
+          if constexpr (CHAINS == 2)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int c = 0; c < 2; ++c) x[k][n][2 * e + c] = s[n][2 * e + c] * sl2;
+              for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = key_of_row + 8 * e;
+            if constexpr (FOUR) {
+              const float2 ks = lds_float2(scales + k * L::SCALES + 8 * key);
+              const float2 vs = lds_float2(scales + L::VS_OFF - L::KS_OFF + k * L::SCALES + 8 * key);
+              // (of a row that is not a number `lowest` says so)
+              const float v_step = fmaxf(vs.x, PG_LEAST_STEP);
+              float log_step;
+              asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log_step) : "f"(v_step));
+              asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inv[k][e]) : "f"(v_step));
+              v_low[k][e] = vs.y;
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                  x[k][n][2 * e + c] =
+                      fmaf(s[n][2 * e + c] * factor[n][c], ks.x, fmaf(q_sum[n][c], ks.y, log_step));
+            } else {
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) x[k][n][2 * e + c] = s[n][2 * e + c] * sl2;
+            }
           }
         }
-      }
-      if (has_alibi) {
+        if (has_alibi) {
 #pragma unroll
-        for (int k = 0; k < RUNS; ++k)
+          for (int k = 0; k < SUBS; ++k)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int j = c0 + PG_RUN * k + key_of_row + 8 * (i >> 1);
-              x[k][n][i] = fmaf(-slope2[n][i & 1], static_cast<float>(row_at[n][i & 1] - j), x[k][n][i]);
-            }
-      }
-      if (need_mask) {
-#pragma unroll
-        for (int k = 0; k < RUNS; ++k)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int away = row_at[n][i & 1] - (c0 + PG_RUN * k + key_of_row + 8 * (i >> 1));
-              if (away < 0 || (p.win_left >= 0 && away > p.win_left)) x[k][n][i] = -INFINITY;
-            }
-      }
-      bool behind = false;
-      float mx[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          mx[n][c] = fmaxf(x[0][n][c], x[0][n][2 + c]);
-#pragma unroll
-          for (int k = 1; k < RUNS; ++k) mx[n][c] = max3(mx[n][c], x[k][n][c], x[k][n][2 + c]);
-          behind = behind || mx[n][c] > m_run[n][c] + ATT_LAZY_RESCALE;
+              for (int i = 0; i < 4; ++i) {
+                const int j = c0 + PG_RUN * k + key_of_row + 8 * (i >> 1);
+                x[k][n][i] = fmaf(-slope2[n][i & 1], static_cast<float>(row_at[n][i & 1] - j), x[k][n][i]);
+              }
         }
-      if (__any_sync(0xffffffffu, behind)) {
+        if (need_mask) {
+#pragma unroll
+          for (int k = 0; k < SUBS; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int away = row_at[n][i & 1] - (c0 + PG_RUN * k + key_of_row + 8 * (i >> 1));
+                if (away < 0 || (p.win_left >= 0 && away > p.win_left)) x[k][n][i] = -INFINITY;
+              }
+        }
+        bool behind = false;
+        float mx[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float m = mx[n][c];
+            mx[n][c] = fmaxf(x[0][n][c], x[0][n][2 + c]);
 #pragma unroll
-            for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-            if (m > m_run[n][c] + ATT_LAZY_RESCALE) {
-              const float f = fast_exp2(m_run[n][c] - m);  // 0 where nothing was seen
-              m_run[n][c] = m;
-              l_run[n][c] *= f;
-              low_run[n][c] *= f;
-#pragma unroll
-              for (int i = 0; i < MTILES; ++i) {
-                o[i][n][c] *= f;
-                o[i][n][2 + c] *= f;
-              }
-            }
+            for (int k = 1; k < SUBS; ++k) mx[n][c] = max3(mx[n][c], x[k][n][c], x[k][n][2 + c]);
+            behind = behind || mx[n][c] > m_run[n][c] + ATT_LAZY_RESCALE;
           }
-      }
-      uint32_t pf[RUNS][NT][2];
-      // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there
-      auto weigh = [&](auto masked) {
+        if (__any_sync(0xffffffffu, behind)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int k = 0; k < RUNS; ++k)
+            for (int c = 0; c < 2; ++c) {
+              float m = mx[n][c];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float w[2];
+              for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+              if (m > m_run[n][c] + ATT_LAZY_RESCALE) {
+                const float f = fast_exp2(m_run[n][c] - m);  // 0 where nothing was seen
+                m_run[n][c] = m;
+                l_run[n][c] *= f;
+                low_run[n][c] *= f;
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                w[c] = fast_exp2(x[k][n][2 * e + c] - m_run[n][c]);
-                if constexpr (FOUR) {
-                  float prob = w[c] * v_inv[k][e], low = v_low[k][e];
-                  if constexpr (decltype(masked)::value)
-                    if (x[k][n][2 * e + c] == -INFINITY) prob = low = 0.0f;
-                  l_run[n][c] += prob;
-                  low_run[n][c] = fmaf(prob, low, low_run[n][c]);
-                } else {
-                  l_run[n][c] += w[c];
+                for (int i = 0; i < MTILES; ++i) {
+                  o[i][n][c] *= f;
+                  o[i][n][2 + c] *= f;
                 }
               }
-              pf[k][n][e] = transpose_8x8(pack16<BF16 && !FOUR>(w[0], w[1]));
             }
-      };
-      if (FOUR && need_mask) weigh(std::true_type{});
-      else weigh(std::false_type{});
-      if constexpr (FOUR) {
+        }
+        uint32_t pf[SUBS][NT][2];
+        // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there
+        auto weigh = [&](auto masked) {
 #pragma unroll
-        for (int k = 0; k < RUNS; ++k) {
-          const uint32_t sub = tile + L::V_OFF + k * L::CODES + t4 * (D / 2) + g8 * (D / 16);
-          uint32_t v0[VW], v1[VW], v2[VW], v3[VW];  // keys t4, + 4, + 8, + 12
-          lds_words<VW>(sub, v0);
-          lds_words<VW>(sub + 4 * (D / 2), v1);
-          lds_words<VW>(sub + 8 * (D / 2), v2);
-          lds_words<VW>(sub + 12 * (D / 2), v3);
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int w = 0; w < VW; ++w)
+            for (int k = 0; k < SUBS; ++k)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const unsigned pick = half ? 0x7632u : 0x5410u;
-              uint32_t a = __byte_perm(v0[w], v1[w], pick), c = __byte_perm(v2[w], v3[w], pick);
+              for (int e = 0; e < 2; ++e) {
+                float w[2];
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t f[4] = {a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u};
-#pragma unroll
-                for (int n = 0; n < NT; ++n) mma_16816<false>(o[4 * w + 2 * half + i][n], f, pf[k][n][0], pf[k][n][1]);
-                a >>= 8;
-                c >>= 8;
+                for (int c = 0; c < 2; ++c) {
+                  w[c] = fast_exp2(x[k][n][2 * e + c] - m_run[n][c]);
+                  if constexpr (FOUR) {
+                    float prob = w[c] * v_inv[k][e], low = v_low[k][e];
+                    if constexpr (decltype(masked)::value)
+                      if (x[k][n][2 * e + c] == -INFINITY) prob = low = 0.0f;
+                    l_run[n][c] += prob;
+                    low_run[n][c] = fmaf(prob, low, low_run[n][c]);
+                  } else {
+                    l_run[n][c] += w[c];
+                  }
+                }
+                pf[k][n][e] = transpose_8x8(pack16<BF16 && !FOUR>(w[0], w[1]));
               }
-            }
-        }
-      } else {
-        // V behind the sequence's last key may be anything: keys 2 t4, 2 t4 + 1 of either half, if they are its
-        uint32_t keep[2];
+        };
+        if (FOUR && need_mask) weigh(std::true_type{});
+        else weigh(std::false_type{});
+        if constexpr (FOUR) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int left = u.sk - c0 - 8 * e - 2 * t4;
-          keep[e] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
-        }
-        const int key = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+          for (int k = 0; k < SUBS; ++k) {
+            const uint32_t sub = tile + L::V_OFF + k * L::CODES + t4 * (D / 2) + g8 * (D / 16);
+            uint32_t v0[VW], v1[VW], v2[VW], v3[VW];  // keys t4, + 4, + 8, + 12
+            lds_words<VW>(sub, v0);
+            lds_words<VW>(sub + 4 * (D / 2), v1);
+            lds_words<VW>(sub + 8 * (D / 2), v2);
+            lds_words<VW>(sub + 12 * (D / 2), v3);
 #pragma unroll
-        for (int m = 0; m < MTILES; ++m) {
-          uint32_t f[4];
-          const int col = (m % 4) * 2 + half;
-          ldsm_x4_trans(tile + L::HALF_BYTES + (m / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
-          if (need_mask)
+            for (int w = 0; w < VW; ++w)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] &= keep[i >> 1];
+              for (int half = 0; half < 2; ++half) {
+                const unsigned pick = half ? 0x7632u : 0x5410u;
+                uint32_t a = __byte_perm(v0[w], v1[w], pick), c = __byte_perm(v2[w], v3[w], pick);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16816<BF16>(o[m][n], f, pf[0][n][0], pf[0][n][1]);
+                for (int i = 0; i < 2; ++i) {
+                  const uint32_t f[4] = {a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u};
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) mma_16816<false>(o[4 * w + 2 * half + i][n], f, pf[k][n][0], pf[k][n][1]);
+                  a >>= 8;
+                  c >>= 8;
+                }
+              }
+          }
+        } else {
+          // V behind the sequence's last key may be anything: keys 2 t4, 2 t4 + 1 of either half, if they are its
+          uint32_t keep[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int left = u.sk - c0 - 8 * e - 2 * t4;
+            keep[e] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+          }
+          const int key = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+          for (int m = 0; m < MTILES; ++m) {
+            uint32_t f[4];
+            const int col = (m % 4) * 2 + half;
+            ldsm_x4_trans(tile + L::HALF_BYTES + (m / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
+            if (need_mask)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) f[i] &= keep[i >> 1];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<BF16>(o[m][n], f, pf[0][n][0], pf[0][n][1]);
+          }
         }
       }
       __syncwarp();  // every lane has read the tile
@@ -711,7 +760,8 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int off = warp * L::RING_BYTES +
-                      (FOUR ? ((filled + n) % STAGES) * L::STAGE_BYTES : (filled % STAGES) * L::STAGE_BYTES + n * L::O_BYTES);
+                      (L::O_STAGES > 1 ? ((filled + n) % STAGES) * L::STAGE_BYTES
+                                       : (filled % STAGES) * L::STAGE_BYTES + n * L::O_BYTES);
       float* ow = reinterpret_cast<float*>(smem + off);
       if (lane == 0) o_at[warp * NT + n] = off;
 #pragma unroll
@@ -744,11 +794,12 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     bool complete = true;  // every warp has a result; else nothing is written
 #pragma unroll
     for (int w = 0; w < PG_WARPS; ++w) complete = complete && no_result[w] == 0;
-    if (!complete) break;
+    complete = complete && !skip;
+    if (!complete && p.splits < 2) break;
 
     // the sum of the warps' results: weights 2^(m_i - max m), 0 for an empty part
     const int live_rows = min(L::ROWS, rows - u.r0);
-    float* part = u.which < 0 ? nullptr : paged_part<D, FOUR, NT>(p, blockIdx.x, u.which);
+    float* part = u.which < 0 || p.splits ? nullptr : paged_part<D, FOUR, NT>(p, blockIdx.x, u.which);
     for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += PG_THREADS) {
       const int r = idx / (D / 4), c4 = idx % (D / 4);
       float top = PG_NOTHING, l = 0.0f;
@@ -767,15 +818,54 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
         acc.z = fmaf(f, v.z, acc.z);
         acc.w = fmaf(f, v.w, acc.w);
       }
-      if (part) {
+      if (p.splits > 1) {  // this thread's own elements
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(smem + o_at[r >> 3]) + (r & 7) * D +
+                                   ((4 * c4) ^ (((r & 7) >> 1) << 3))) = acc;
+        if (c4 == 0) {
+          cta_ml[r] = top;
+          cta_ml[L::ROWS + r] = l;
+        }
+      } else if (part) {
         *reinterpret_cast<float4*>(part + r * D + 4 * c4) = acc;
         if (c4 == 0) {
           part[L::ROWS * D + r] = top;
           part[L::ROWS * (D + 1) + r] = l;
         }
       } else {
-        paged_emit<D, BF16>(p, u.b, u.m, u.r0, r, c4, acc, top, l);
+        paged_emit<D, BF16>(p, u.b, u.head, u.r0 + r, c4, acc, top, l);
       }
+    }
+    if (p.splits > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cluster = cg::this_cluster();
+      if (threadIdx.x == 0) no_result[PG_WARPS] = complete ? 0 : 1;
+      cluster.sync();
+      int* flags = reinterpret_cast<int*>(smem + L::FLAG_OFF);
+      static_assert(PG_MOST_SPLITS <= 32, "one lane per CTA");
+      complete = __all_sync(0xffffffffu, lane >= p.splits || cluster.map_shared_rank(flags, lane)[PG_WARPS] == 0);
+      for (int idx = split * PG_THREADS + threadIdx.x; complete && idx < live_rows * (D / 4);
+           idx += p.splits * PG_THREADS) {
+        const int r = idx / (D / 4), c4 = idx % (D / 4);
+        float top = PG_NOTHING, l = 0.0f;
+        for (int k = 0; k < p.splits; ++k) top = fmaxf(top, cluster.map_shared_rank(cta_ml, k)[r]);
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < p.splits; ++k) {
+          const float* kml = cluster.map_shared_rank(cta_ml, k);
+          const float f = fast_exp2(kml[r] - top);
+          const int off = cluster.map_shared_rank(o_at, k)[r >> 3];
+          const float4 v = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(cluster.map_shared_rank(smem, k) + off) + (r & 7) * D +
+              ((4 * c4) ^ (((r & 7) >> 1) << 3)));
+          l = fmaf(f, kml[L::ROWS + r], l);
+          acc.x = fmaf(f, v.x, acc.x);
+          acc.y = fmaf(f, v.y, acc.y);
+          acc.z = fmaf(f, v.z, acc.z);
+          acc.w = fmaf(f, v.w, acc.w);
+        }
+        paged_emit<D, BF16>(p, u.b, u.head, u.r0 + r, c4, acc, top, l);
+      }
+      cluster.sync();  // no CTA leaves while another one reads its shared memory
+      break;
     }
     __syncthreads();  // all of it has been read: the ring has its room back
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -807,19 +897,33 @@ __global__ void __launch_bounds__(PG_MERGE_THREADS) attn_paged_merge_kernel(cons
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x + 1, ctas = gridDim.x + 1;
   const PagedPiece piece = p.pieces[c];
-  if (piece.unit < 0 || piece.unit < p.pieces[c - 1].lo) return;
-  const int rows = p.group * p.Sq, r0 = (piece.m % p.row_tiles) * L::ROWS, row0 = PG_MERGE_ROWS * blockIdx.y;
-  if (r0 + row0 >= rows || *reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
-  // the CTAs that have tiles of the unit: c - 1 .. c - 2 + parts
-  int parts = 1;
-  for (int k = c;; k += PG_MERGE_THREADS) {  // `lo` ascends
-    const int i = k + static_cast<int>(threadIdx.x);
-    const int n = __syncthreads_count(i < ctas && p.pieces[min(i, ctas - 1)].lo < piece.end);
+  const long long began = p.pieces[c - 1].lo;
+  const bool failed = *reinterpret_cast<volatile unsigned int*>(p.status) != 0u;
+  // the first of the CTAs that may have tiles of the unit: `lo` ascends
+  long long lo = p.pieces[min(c + static_cast<int>(threadIdx.x), ctas - 1)].lo;
+  if (piece.unit < 0 || piece.unit < began) return;
+  const int rows = p.group * p.Sq, r0 = piece.r0, row0 = PG_MERGE_ROWS * blockIdx.y;
+  if (r0 + row0 >= rows || failed) return;
+  int parts = 1;  // CTAs c - 1 .. c - 2 + parts
+  for (int k = c;;) {
+    const int n = __syncthreads_count(k + static_cast<int>(threadIdx.x) < ctas && lo < piece.end);
     parts += n;
     if (n < PG_MERGE_THREADS) break;
+    k += PG_MERGE_THREADS;
+    lo = p.pieces[min(k + static_cast<int>(threadIdx.x), ctas - 1)].lo;
   }
   auto part = [&](int k) { return paged_part<D, FOUR, NT>(p, c - 1 + k, k > 0 ? 0 : 1); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = threadIdx.x / ITEMS, item = threadIdx.x % ITEMS, r = item / (D / 4), c4 = item % (D / 4);
+  // a thread's first parts of O, on their way with the rows' maxima and sums
+  constexpr int EARLY = 8;
+  float4 o[EARLY];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) {
+    const int k = group + i * GROUPS;
+    o[i] = k < parts ? *reinterpret_cast<const float4*>(part(k) + (row0 + r) * D + 4 * c4)
+                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
   float top[PG_MERGE_ROWS], l[PG_MERGE_ROWS];
 #pragma unroll
   for (int r = 0; r < PG_MERGE_ROWS; ++r) {
@@ -830,6 +934,9 @@ __global__ void __launch_bounds__(PG_MERGE_THREADS) attn_paged_merge_kernel(cons
       sum[k][r] = part(k)[L::ROWS * (D + 1) + row0 + r];
       top[r] = fmaxf(top[r], m);
     }
+  }
+#pragma unroll
+  for (int r = 0; r < PG_MERGE_ROWS; ++r) {
     top[r] = warp_reduce<true>(top[r]);
     if (lane == 0) red[0][warp][r] = top[r];
   }
@@ -848,17 +955,20 @@ __global__ void __launch_bounds__(PG_MERGE_THREADS) attn_paged_merge_kernel(cons
     if (lane == 0) red[1][warp][r] = l[r];
   }
   __syncthreads();
-  const int group = threadIdx.x / ITEMS, item = threadIdx.x % ITEMS, r = item / (D / 4), c4 = item % (D / 4);
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-  for (int k = group; k < parts; k += GROUPS) {
+  auto add = [&](int k, const float4& v) {
     const float f = weight[k][r];
-    const float4 v = *reinterpret_cast<const float4*>(part(k) + (row0 + r) * D + 4 * c4);
     acc.x = fmaf(f, v.x, acc.x);
     acc.y = fmaf(f, v.y, acc.y);
     acc.z = fmaf(f, v.z, acc.z);
     acc.w = fmaf(f, v.w, acc.w);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i)
+    if (group + i * GROUPS < parts) add(group + i * GROUPS, o[i]);
+#pragma unroll 8
+  for (int k = group + EARLY * GROUPS; k < parts; k += GROUPS)
+    add(k, *reinterpret_cast<const float4*>(part(k) + (row0 + r) * D + 4 * c4));
   sums[group][item] = acc;
   __syncthreads();
   if (group == 0 && r0 + row0 + r < rows) {
@@ -873,14 +983,14 @@ __global__ void __launch_bounds__(PG_MERGE_THREADS) attn_paged_merge_kernel(cons
       total += red[1][w][r];
       most = fmaxf(most, red[0][w][r]);
     }
-    paged_emit<D, BF16>(p, piece.b, piece.m, r0, row0 + r, c4, acc, most, total);
+    paged_emit<D, BF16>(p, piece.b, piece.head, r0 + row0 + r, c4, acc, most, total);
   }
 }
 
-// How a call is cut: CTAs of the first launch, and bytes of the workspace.
+// How a call is cut: CTAs, and bytes of the parts.
 struct PagedPlan {
   int64_t ctas;
-  bool whole;
+  int splits;  // 0: one line
   size_t pieces_bytes, bytes;
 };
 template <int D, bool FOUR, int NT>
@@ -888,11 +998,17 @@ static PagedPlan paged_plan(int64_t units, int64_t keys) {
   using L = PgShape<D, FOUR, NT>;
   PagedPlan plan{};
   const int64_t tiles = (keys + L::KEYS - 1) / L::KEYS;
-  plan.whole = tiles <= 2 * L::LEAST_PIECE;
   const int64_t slots = static_cast<int64_t>(sm_count_of_current_device()) * L::CTAS_PER_SM;
-  plan.ctas = plan.whole ? units : slots < PG_MOST_CTAS ? slots : PG_MOST_CTAS;
-  if (!plan.whole) {
-    plan.pieces_bytes = (plan.ctas * sizeof(PagedPiece) + 15) / 16 * 16;
+  // clusters of as many CTAs as leave a warp two tiles (4 bits: one), within one wave
+  int n = 1;
+  while (n < PG_MOST_SPLITS && units * 2 * n <= slots && tiles >= 2 * n * PG_WARPS * (FOUR ? 1 : 2)) n *= 2;
+  const int64_t chain = (tiles + n * PG_WARPS - 1) / (n * PG_WARPS);
+  // more than a few tiles to a warp, or units that do not all run at once: the line
+  const bool line = chain > (units * n <= slots ? (FOUR ? 5 : 16) : (FOUR ? 2 : 3));
+  plan.splits = line ? 0 : n;
+  plan.ctas = !line ? units * n : slots < PG_MOST_CTAS ? slots : PG_MOST_CTAS;
+  if (line) {
+    plan.pieces_bytes = plan.ctas * sizeof(PagedPiece);
     plan.bytes = plan.pieces_bytes + plan.ctas * 2 * L::PART_FLOATS * sizeof(float);
   }
   return plan;
@@ -911,18 +1027,24 @@ static int launch_paged(PagedParams& p, const PagedPlan& plan, cudaStream_t stre
       return TRX_ERR_CUDA;
     if (cacheable) configured[dev].store(true, std::memory_order_release);
   }
-  kernel<<<static_cast<unsigned>(plan.ctas), PG_THREADS, L::DYN_BYTES, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return TRX_ERR_CUDA;
-  if (plan.whole || plan.ctas < 2) return TRX_OK;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = plan.splits > 1 ? plan.splits : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.ctas));
+  cfg.blockDim = dim3(PG_THREADS);
+  cfg.dynamicSmemBytes = L::DYN_BYTES;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return TRX_ERR_CUDA;
+  if (plan.splits || plan.ctas < 2) return TRX_OK;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(plan.ctas - 1), L::ROWS / PG_MERGE_ROWS);
   cfg.blockDim = dim3(PG_MERGE_THREADS);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, attn_paged_merge_kernel<D, BF16, FOUR, NT>, p) == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
 }
 
