@@ -46,6 +46,32 @@ struct HalfRow {
   }
 };
 
+// The same in pairs of columns, for packed arithmetic.
+template <int N>
+struct HalfPairs {
+  float2 v[N / 2];
+  static_assert(N % 2 == 0, "pairs");
+};
+template <typename T, int VEC, int CH>
+__device__ __forceinline__ HalfPairs<VEC * CH> pairs_of(const HalfRow<T, VEC, CH>& h) {
+  HalfPairs<VEC * CH> r;
+  if constexpr (VEC > 1) {
+    Pack<T>::unpack2(h.raw, r.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) r.v[i] = make_float2(h.one[2 * i], h.one[2 * i + 1]);
+  }
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void unpair(const HalfPairs<N>& p, float (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    f[2 * i] = p.v[i].x;
+    f[2 * i + 1] = p.v[i].y;
+  }
+}
+
 template <typename T, int VEC, int CH, int LPR>
 __device__ __forceinline__ void store_half(T* p, int lane, int half, const float (&f)[VEC * CH]) {
   if constexpr (VEC > 1) {
@@ -86,17 +112,6 @@ __device__ __forceinline__ void turn(float (&x1)[N], float (&x2)[N], const float
     x1[i] = a;
   }
 }
-template <int N>
-__device__ __forceinline__ void turn_back(float (&x1)[N], float (&x2)[N], const float (&c)[N],
-                                          const float (&s)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float a = __fadd_rn(__fmul_rn(x1[i], c[i]), __fmul_rn(x2[i], s[i]));
-    x2[i] = __fsub_rn(__fmul_rn(x2[i], c[i]), __fmul_rn(x1[i], s[i]));
-    x1[i] = a;
-  }
-}
-
 // The smallest power of two of lanes, 4 to 32, that hold `half` columns at `vec` to a lane.
 inline int lanes_for(int half, int vec) {
   int lanes = 4;

@@ -43,11 +43,36 @@ struct QkParams {
 };
 
 constexpr int QK_THREADS = 128;
+#ifndef XB
+#define XB 3
+#define XR 2
+#endif
+constexpr int QK_BWD_CTAS_PER_SM = XB;
 
-// cos and sin of a token for a lane's columns. A position outside the tables has none: its rows become NaN.
+// A row's two halves, and what they are turned by: cos, sin, -sin.
+template <int N>
+struct QkRow {
+  HalfPairs<N> a, b;
+};
+template <int N>
+struct QkAngles {
+  HalfPairs<N> c, s, ns;
+};
+
 template <int VEC, int CH, int LPR>
-__device__ __forceinline__ void load_angles(const QkParams& p, int64_t b, int64_t s, int lane, int half,
-                                            float (&c)[VEC * CH], float (&sn)[VEC * CH]) {
+__device__ __forceinline__ HalfPairs<VEC * CH> load_pairs(const void* base, int dtype, int64_t first, int lane, int n,
+                                                          float fill) {
+  float f[VEC * CH];
+  load_columns<VEC, CH, LPR>(base, dtype, first, lane, n, fill, f);
+  HalfPairs<VEC * CH> r;
+#pragma unroll
+  for (int i = 0; i < VEC * CH / 2; ++i) r.v[i] = make_float2(f[2 * i], f[2 * i + 1]);
+  return r;
+}
+
+// The angles of a token for a lane's columns. A position outside the tables has none: its rows become NaN.
+template <int VEC, int CH, int LPR>
+__device__ __forceinline__ QkAngles<VEC * CH> load_angles(const QkParams& p, int64_t b, int64_t s, int lane, int half) {
   int64_t pos = s;
   if (p.positions) {
     const int64_t at = b * p.pos_strides[0] + s * p.pos_strides[1];
@@ -56,37 +81,59 @@ __device__ __forceinline__ void load_angles(const QkParams& p, int64_t b, int64_
   }
   const bool there = pos >= 0 && pos < p.table_rows;
   const float fill = there ? 0.0f : __int_as_float(0x7fffffff);
-  load_columns<VEC, CH, LPR>(p.cos_t, p.table_dtype, pos * p.table_stride, lane, there ? half : 0, fill, c);
-  load_columns<VEC, CH, LPR>(p.sin_t, p.table_dtype, pos * p.table_stride, lane, there ? half : 0, fill, sn);
+  QkAngles<VEC * CH> r;
+  r.c = load_pairs<VEC, CH, LPR>(p.cos_t, p.table_dtype, pos * p.table_stride, lane, there ? half : 0, fill);
+  r.s = load_pairs<VEC, CH, LPR>(p.sin_t, p.table_dtype, pos * p.table_stride, lane, there ? half : 0, fill);
+#pragma unroll
+  for (int i = 0; i < VEC * CH / 2; ++i) r.ns.v[i] = make_float2(-r.s.v[i].x, -r.s.v[i].y);
+  return r;
 }
 
-// x1, x2 become the normalised row (0 in columns behind it); the factor that a gradient is scaled by.
+// (x1, x2) turned by the angles, and back: (x1 c - x2 s, x2 c + x1 s), (x1 c + x2 s, x2 c - x1 s).
+template <int N>
+__device__ __forceinline__ void turn_pairs(QkRow<N>& x, const HalfPairs<N>& c, const HalfPairs<N>& s,
+                                           const HalfPairs<N>& ns) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 a = fma2(x.b.v[i], ns.v[i], mul2(x.a.v[i], c.v[i]));
+    x.b.v[i] = fma2(x.a.v[i], s.v[i], mul2(x.b.v[i], c.v[i]));
+    x.a.v[i] = a;
+  }
+}
+
+// Sum over the row of x y.
+template <int LPR, int N>
+__device__ __forceinline__ float row_dot(const QkRow<N>& x, const QkRow<N>& y) {
+  float2 sum = mul2(x.a.v[0], y.a.v[0]);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    if (i > 0) sum = fma2(x.a.v[i], y.a.v[i], sum);
+    sum = fma2(x.b.v[i], y.b.v[i], sum);
+  }
+  return lanes_sum<LPR>(sum.x + sum.y);
+}
+template <int LPR, int N>
+__device__ __forceinline__ float row_sum(const QkRow<N>& x) {
+  float2 sum = x.a.v[0];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    if (i > 0) sum = add2(sum, x.a.v[i]);
+    sum = add2(sum, x.b.v[i]);
+  }
+  return lanes_sum<LPR>(sum.x + sum.y);
+}
+
+// A LayerNorm's row minus its mean (0 in columns behind the row).
 template <int VEC, int CH, int LPR>
-__device__ __forceinline__ float normalise(float (&x1)[VEC * CH], float (&x2)[VEC * CH], int lane, int half,
-                                           float inv_d, float eps, int layer) {
-  constexpr int N = VEC * CH;
+__device__ __forceinline__ void centre(QkRow<VEC * CH>& x, int lane, int half, float inv_d) {
+  const float mean = row_sum<LPR>(x) * inv_d;
   auto inside = [&](int i) { return ((i / VEC) * LPR + lane) * VEC < half; };
-  if (layer) {
-    float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += x1[i] + x2[i];
-    const float mean = lanes_sum<LPR>(sum) * inv_d;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x1[i] = inside(i) ? x1[i] - mean : 0.0f;
-      x2[i] = inside(i) ? x2[i] - mean : 0.0f;
-    }
+  for (int i = 0; i < VEC * CH / 2; ++i) {
+    const float2 m = make_float2(inside(2 * i) ? -mean : 0.0f, inside(2 * i + 1) ? -mean : 0.0f);
+    x.a.v[i] = add2(x.a.v[i], m);
+    x.b.v[i] = add2(x.b.v[i], m);
   }
-  float sq = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) sq = fmaf(x1[i], x1[i], fmaf(x2[i], x2[i], sq));
-  const float rstd = rsqrtf(fmaf(lanes_sum<LPR>(sq), inv_d, eps));
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    x1[i] *= rstd;
-    x2[i] *= rstd;
-  }
-  return rstd;
 }
 
 // Grid (tokens, chunks of heads of q, then of k): a thread has its columns' weights and angles for all heads of
@@ -106,10 +153,9 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const __grid_c
   const T* x = static_cast<const T*>(side.x) + b * side.xs[0] + s * side.xs[1];
   T* y = static_cast<T*>(side.y) + b * side.ys[0] + s * side.ys[1];
 
-  float c[N], sn[N], w1[N], w2[N];
-  load_angles<VEC, CH, LPR>(p, b, s, lane, half, c, sn);
-  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, 0, lane, half, 0.0f, w1);
-  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, half, lane, half, 0.0f, w2);
+  const QkAngles<N> t = load_angles<VEC, CH, LPR>(p, b, s, lane, half);
+  const HalfPairs<N> w1 = load_pairs<VEC, CH, LPR>(side.w, p.w_dtype, 0, lane, half, 0.0f);
+  const HalfPairs<N> w2 = load_pairs<VEC, CH, LPR>(side.w, p.w_dtype, half, lane, half, 0.0f);
   const float inv_d = __fdiv_rn(1.0f, static_cast<float>(p.D));
 
   for (int h0 = h_begin; h0 < h_end; h0 += ROWS) {
@@ -122,41 +168,45 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const __grid_c
     }
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) {
-      float x1[N], x2[N];
-      r1[u].unpack(x1);
-      r2[u].unpack(x2);
-      if (!p.first) turn(x1, x2, c, sn);
-      normalise<VEC, CH, LPR>(x1, x2, lane, half, inv_d, p.eps, p.layer);
+      QkRow<N> z{pairs_of(r1[u]), pairs_of(r2[u])};
+      if (!p.first) turn_pairs(z, t.c, t.s, t.ns);
+      if (p.layer) centre<VEC, CH, LPR>(z, lane, half, inv_d);
+      const float rstd = rsqrtf(fmaf(row_dot<LPR>(z, z), inv_d, p.eps));
+      const float2 rstd2 = make_float2(rstd, rstd);
       if (side.b) {
-        float b1[N], b2[N];
-        load_columns<VEC, CH, LPR>(side.b, p.w_dtype, 0, lane, half, 0.0f, b1);
-        load_columns<VEC, CH, LPR>(side.b, p.w_dtype, half, lane, half, 0.0f, b2);
+        const HalfPairs<N> b1 = load_pairs<VEC, CH, LPR>(side.b, p.w_dtype, 0, lane, half, 0.0f);
+        const HalfPairs<N> b2 = load_pairs<VEC, CH, LPR>(side.b, p.w_dtype, half, lane, half, 0.0f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          x1[i] = fmaf(x1[i], w1[i], b1[i]);
-          x2[i] = fmaf(x2[i], w2[i], b2[i]);
+        for (int i = 0; i < N / 2; ++i) {
+          z.a.v[i] = fma2(mul2(z.a.v[i], rstd2), w1.v[i], b1.v[i]);
+          z.b.v[i] = fma2(mul2(z.b.v[i], rstd2), w2.v[i], b2.v[i]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          x1[i] *= w1[i];
-          x2[i] *= w2[i];
+        for (int i = 0; i < N / 2; ++i) {
+          z.a.v[i] = mul2(mul2(z.a.v[i], rstd2), w1.v[i]);
+          z.b.v[i] = mul2(mul2(z.b.v[i], rstd2), w2.v[i]);
         }
       }
-      if (p.first) turn(x1, x2, c, sn);
+      if (p.first) turn_pairs(z, t.c, t.s, t.ns);
       if (live && h0 + u < h_end) {
         T* row = y + (h0 + u) * side.ys[2];
-        store_half<T, VEC, CH, LPR>(row, lane, half, x1);
-        store_half<T, VEC, CH, LPR>(row + half, lane, half, x2);
+        float f[N];
+        unpair(z.a, f);
+        store_half<T, VEC, CH, LPR>(row, lane, half, f);
+        unpair(z.b, f);
+        store_half<T, VEC, CH, LPR>(row + half, lane, half, f);
       }
     }
   }
 }
 
 // Blocks [0, q_blocks) walk over the queries, the others over the keys, ROWS heads of a token at a time; every
-// thread keeps the sums of its columns' weight gradients, which meet in shared memory at the end.
+// thread keeps the sums of its columns' weight gradients, which meet in shared memory at the end. With z the row
+// that is normalised (a LayerNorm's centred) and e = rstd g w: dx = e - z rstd^2 mean(e z) [- mean e].
 template <typename T, int VEC, int LPR, int CH, int ROWS, bool LAYER>
-__global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_bwd_kernel(const __grid_constant__ QkParams p) {
+__global__ void __launch_bounds__(QK_THREADS, QK_BWD_CTAS_PER_SM)
+    qk_norm_rope_bwd_kernel(const __grid_constant__ QkParams p) {
   constexpr int N = VEC * CH, GROUPS = QK_THREADS / LPR;
   const int lane = threadIdx.x % LPR, half = p.D / 2;
   const bool keys = static_cast<int>(blockIdx.x) >= p.q_blocks;
@@ -165,23 +215,20 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_bwd_kernel(const __gr
   const int block = keys ? blockIdx.x - p.q_blocks : blockIdx.x;
   const float inv_d = __fdiv_rn(1.0f, static_cast<float>(p.D));
 
-  float w1[N], w2[N], dw1[N], dw2[N], db1[LAYER ? N : 1], db2[LAYER ? N : 1];
-  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, 0, lane, half, 0.0f, w1);
-  load_columns<VEC, CH, LPR>(side.w, p.w_dtype, half, lane, half, 0.0f, w2);
+  const HalfPairs<N> w1 = load_pairs<VEC, CH, LPR>(side.w, p.w_dtype, 0, lane, half, 0.0f);
+  const HalfPairs<N> w2 = load_pairs<VEC, CH, LPR>(side.w, p.w_dtype, half, lane, half, 0.0f);
+  QkRow<N> dw, db;
 #pragma unroll
-  for (int i = 0; i < N; ++i) dw1[i] = dw2[i] = 0.0f;
-  if constexpr (LAYER)
-#pragma unroll
-    for (int i = 0; i < N; ++i) db1[i] = db2[i] = 0.0f;
+  for (int i = 0; i < N / 2; ++i) dw.a.v[i] = dw.b.v[i] = db.a.v[i] = db.b.v[i] = make_float2(0.0f, 0.0f);
 
   const unsigned chunks = (side.H + ROWS - 1) / ROWS;
   const unsigned items = static_cast<unsigned>(p.tokens) * chunks;
   // whole warps leave together: the item of a warp's first row decides
   for (unsigned first = (block * QK_THREADS + (threadIdx.x & ~31)) / LPR; first < items;
        first += blocks * GROUPS) {
-    const unsigned item = first + (threadIdx.x % 32) / LPR;
-    const bool live = item < items;
-    const unsigned token = (live ? item : items - 1) / chunks, h0 = ((live ? item : items - 1) - token * chunks) * ROWS;
+    const unsigned item = min(first + (threadIdx.x % 32) / LPR, items - 1);
+    const bool live = first + (threadIdx.x % 32) / LPR < items;
+    const unsigned token = item / chunks, h0 = (item - token * chunks) * ROWS;
     const unsigned seq = static_cast<unsigned>(p.S);
     const int64_t b = token / seq, s = token - static_cast<unsigned>(b) * seq;
     const T* x = static_cast<const T*>(side.x) + b * side.xs[0] + s * side.xs[1];
@@ -191,54 +238,56 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_bwd_kernel(const __gr
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) {
       const int h = min(static_cast<int>(h0) + u, side.H - 1);
+      const int there = live && static_cast<int>(h0) + u < side.H ? half : 0;  // rows twice have no gradient
       r1[u].template load<LPR>(x + h * side.xs[2], lane, half);
       r2[u].template load<LPR>(x + h * side.xs[2] + half, lane, half);
-      g1[u].template load<LPR>(dy + h * side.dys[2], lane, half);
-      g2[u].template load<LPR>(dy + h * side.dys[2] + half, lane, half);
+      g1[u].template load<LPR>(dy + h * side.dys[2], lane, there);
+      g2[u].template load<LPR>(dy + h * side.dys[2] + half, lane, there);
     }
-    float c[N], sn[N];
-    load_angles<VEC, CH, LPR>(p, b, s, lane, half, c, sn);
+    const QkAngles<N> t = load_angles<VEC, CH, LPR>(p, b, s, lane, half);
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) {
-      const bool row_live = live && static_cast<int>(h0) + u < side.H;
-      float x1[N], x2[N], d1[N], d2[N];
-      r1[u].unpack(x1);
-      r2[u].unpack(x2);
-      g1[u].unpack(d1);
-      g2[u].unpack(d2);
-      if (p.first)
-        turn_back(d1, d2, c, sn);
-      else
-        turn(x1, x2, c, sn);
-      const float rstd = normalise<VEC, CH, LPR>(x1, x2, lane, half, inv_d, p.eps, LAYER);
-      float dn = 0.0f, sum = 0.0f;
+      QkRow<N> z{pairs_of(r1[u]), pairs_of(r2[u])}, g{pairs_of(g1[u]), pairs_of(g2[u])};
+      if (p.first) turn_pairs(g, t.c, t.ns, t.s);
+      else turn_pairs(z, t.c, t.s, t.ns);
+      if constexpr (LAYER) centre<VEC, CH, LPR>(z, lane, half, inv_d);
+      const float rstd = rsqrtf(fmaf(row_dot<LPR>(z, z), inv_d, p.eps));
+      const float2 rstd2 = make_float2(rstd, rstd);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (row_live) {
-          dw1[i] = fmaf(d1[i], x1[i], dw1[i]);
-          dw2[i] = fmaf(d2[i], x2[i], dw2[i]);
-          if constexpr (LAYER) {
-            db1[i] += d1[i];
-            db2[i] += d2[i];
-          }
+      for (int i = 0; i < N / 2; ++i) {
+        if constexpr (LAYER) {
+          db.a.v[i] = add2(db.a.v[i], g.a.v[i]);
+          db.b.v[i] = add2(db.b.v[i], g.b.v[i]);
         }
-        d1[i] *= w1[i];
-        d2[i] *= w2[i];
-        dn = fmaf(d1[i], x1[i], fmaf(d2[i], x2[i], dn));
-        if constexpr (LAYER) sum += d1[i] + d2[i];
+        g.a.v[i] = mul2(g.a.v[i], rstd2);
+        g.b.v[i] = mul2(g.b.v[i], rstd2);
+        dw.a.v[i] = fma2(g.a.v[i], z.a.v[i], dw.a.v[i]);
+        dw.b.v[i] = fma2(g.b.v[i], z.b.v[i], dw.b.v[i]);
+        g.a.v[i] = mul2(g.a.v[i], w1.v[i]);
+        g.b.v[i] = mul2(g.b.v[i], w2.v[i]);
       }
-      dn = lanes_sum<LPR>(dn) * inv_d;
-      if constexpr (LAYER) sum = lanes_sum<LPR>(sum) * inv_d;
+      const float k = -row_dot<LPR>(g, z) * inv_d * rstd * rstd;
+      const float2 k2 = make_float2(k, k);
+      float mean = 0.0f;
+      if constexpr (LAYER) mean = -row_sum<LPR>(g) * inv_d;
+      const float2 mean2 = make_float2(mean, mean);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        d1[i] = rstd * (fmaf(-dn, x1[i], d1[i]) - sum);
-        d2[i] = rstd * (fmaf(-dn, x2[i], d2[i]) - sum);
+      for (int i = 0; i < N / 2; ++i) {
+        g.a.v[i] = fma2(z.a.v[i], k2, g.a.v[i]);
+        g.b.v[i] = fma2(z.b.v[i], k2, g.b.v[i]);
+        if constexpr (LAYER) {
+          g.a.v[i] = add2(g.a.v[i], mean2);
+          g.b.v[i] = add2(g.b.v[i], mean2);
+        }
       }
-      if (!p.first) turn_back(d1, d2, c, sn);
-      if (row_live) {
+      if (!p.first) turn_pairs(g, t.c, t.ns, t.s);
+      if (live && static_cast<int>(h0) + u < side.H) {
         T* row = dx + (static_cast<int>(h0) + u) * side.ys[2];
-        store_half<T, VEC, CH, LPR>(row, lane, half, d1);
-        store_half<T, VEC, CH, LPR>(row + half, lane, half, d2);
+        float f[N];
+        unpair(g.a, f);
+        store_half<T, VEC, CH, LPR>(row, lane, half, f);
+        unpair(g.b, f);
+        store_half<T, VEC, CH, LPR>(row + half, lane, half, f);
       }
     }
   }
@@ -249,25 +298,19 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_bwd_kernel(const __gr
 #pragma unroll
   for (int pass = 0; pass < (LAYER ? 2 : 1); ++pass) {
     if (pass) __syncthreads();
+    float f[2][N];
+    unpair(pass ? db.a : dw.a, f[0]);
+    unpair(pass ? db.b : dw.b, f[1]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float a = dw1[i], e = dw2[i];
-      if constexpr (LAYER)
-        if (pass) {
-          a = db1[i];
-          e = db2[i];
-        }
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int o = 16; o >= LPR; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        e += __shfl_xor_sync(0xffffffffu, e, o);
+      for (int e = 0; e < 2; ++e) {
+        float a = f[e][i];
+#pragma unroll
+        for (int o = 16; o >= LPR; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (threadIdx.x % 32 < LPR)
+          sums[threadIdx.x / 32][e * N * LPR + ((i / VEC) * LPR + lane) * VEC + i % VEC] = a;
       }
-      if (threadIdx.x % 32 < LPR) {
-        const int col = ((i / VEC) * LPR + lane) * VEC + i % VEC;
-        sums[threadIdx.x / 32][col] = a;
-        sums[threadIdx.x / 32][N * LPR + col] = e;
-      }
-    }
     __syncthreads();
     for (int col = threadIdx.x; col < p.D; col += QK_THREADS) {
       const int at = col < half ? col : N * LPR + col - half;
@@ -292,9 +335,18 @@ __global__ void __launch_bounds__(1024) qk_norm_reduce_kernel(const QkReduce r) 
   const bool keys = blockIdx.y & 1;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, col = blockIdx.x * 32 + tx;
   float v = 0.0f;
-  if (col < r.D)
-    for (int i = (keys ? r.q_blocks : 0) + ty; i < (keys ? r.blocks : r.q_blocks); i += 32)
-      v += r.part[(static_cast<int64_t>(i) * 2 + (blockIdx.y >> 1)) * r.D + col];
+  constexpr int N = 8;  // loads in flight
+  const int end = keys ? r.blocks : r.q_blocks;
+  for (int i0 = (keys ? r.q_blocks : 0) + ty; i0 < end; i0 += 32 * N) {
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      f[i] = col < r.D && i0 + 32 * i < end
+                 ? r.part[(static_cast<int64_t>(i0 + 32 * i) * 2 + (blockIdx.y >> 1)) * r.D + col]
+                 : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v += f[i];
+  }
   sm[ty][tx] = v;
   __syncthreads();
   const float sum = warp_reduce<false>(sm[tx][ty]);  // of column ty
@@ -353,7 +405,6 @@ static int launch_qk_forward(QkParams& p, cudaStream_t s) {
   }
 }
 
-constexpr int QK_BWD_CTAS_PER_SM = 4;
 static int qk_bwd_blocks() { return sm_count_of_current_device() * QK_BWD_CTAS_PER_SM; }
 
 template <typename T, int VEC, int LPR, int CH, int ROWS>
@@ -395,10 +446,10 @@ static int launch_qk_backward(QkParams& p, QkReduce& r, cudaStream_t s) {
   if (!qk_vector(p, VEC, true))
     return p.D <= 128 ? launch_qk_bwd<T, 1, 32, 2, 1>(p, r, s) : launch_qk_bwd<T, 1, 32, 8, 1>(p, r, s);
   switch (lanes_for(p.D / 2, VEC)) {
-    case 4: return launch_qk_bwd<T, VEC, 4, 1, 2>(p, r, s);
-    case 8: return launch_qk_bwd<T, VEC, 8, 1, 2>(p, r, s);
-    case 16: return launch_qk_bwd<T, VEC, 16, 1, 2>(p, r, s);
-    default: return launch_qk_bwd<T, VEC, 32, 1, 2>(p, r, s);
+    case 4: return launch_qk_bwd<T, VEC, 4, 1, XR>(p, r, s);
+    case 8: return launch_qk_bwd<T, VEC, 8, 1, XR>(p, r, s);
+    case 16: return launch_qk_bwd<T, VEC, 16, 1, XR>(p, r, s);
+    default: return launch_qk_bwd<T, VEC, 32, 1, XR>(p, r, s);
   }
 }
 
