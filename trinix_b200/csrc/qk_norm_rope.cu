@@ -37,7 +37,7 @@ struct QkParams {
   int layer, first;   // LayerNorm; the norm comes before the rotation
   float eps;
   int q_chunks;       // forward: of the grid's y
-  int heads_per_cta;
+  int heads_per_cta;  // backward: of an item
   int q_blocks;       // backward: of the grid's x
   float* part;        // backward: [blocks][2][D] sums of g n and of g
 };
@@ -46,6 +46,9 @@ constexpr int QK_THREADS = 128;
 #ifndef XB
 #define XB 3
 #define XR 2
+#endif
+#ifndef XH
+#define XH 8
 #endif
 constexpr int QK_BWD_CTAS_PER_SM = XB;
 
@@ -214,6 +217,7 @@ __global__ void __launch_bounds__(QK_THREADS, QK_BWD_CTAS_PER_SM)
   const int blocks = keys ? gridDim.x - p.q_blocks : p.q_blocks;
   const int block = keys ? blockIdx.x - p.q_blocks : blockIdx.x;
   const float inv_d = __fdiv_rn(1.0f, static_cast<float>(p.D));
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const HalfPairs<N> w1 = load_pairs<VEC, CH, LPR>(side.w, p.w_dtype, 0, lane, half, 0.0f);
   const HalfPairs<N> w2 = load_pairs<VEC, CH, LPR>(side.w, p.w_dtype, half, lane, half, 0.0f);
@@ -221,73 +225,75 @@ __global__ void __launch_bounds__(QK_THREADS, QK_BWD_CTAS_PER_SM)
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) dw.a.v[i] = dw.b.v[i] = db.a.v[i] = db.b.v[i] = make_float2(0.0f, 0.0f);
 
-  const unsigned chunks = (side.H + ROWS - 1) / ROWS;
+  const unsigned chunks = (side.H + p.heads_per_cta - 1) / p.heads_per_cta;
   const unsigned items = static_cast<unsigned>(p.tokens) * chunks;
   // whole warps leave together: the item of a warp's first row decides
   for (unsigned first = (block * QK_THREADS + (threadIdx.x & ~31)) / LPR; first < items;
        first += blocks * GROUPS) {
     const unsigned item = min(first + (threadIdx.x % 32) / LPR, items - 1);
     const bool live = first + (threadIdx.x % 32) / LPR < items;
-    const unsigned token = item / chunks, h0 = (item - token * chunks) * ROWS;
-    const unsigned seq = static_cast<unsigned>(p.S);
+    const unsigned token = item / chunks, seq = static_cast<unsigned>(p.S);
+    const int h_begin = (item - token * chunks) * p.heads_per_cta;
     const int64_t b = token / seq, s = token - static_cast<unsigned>(b) * seq;
-    const T* x = static_cast<const T*>(side.x) + b * side.xs[0] + s * side.xs[1];
-    const T* dy = static_cast<const T*>(side.dy) + b * side.dys[0] + s * side.dys[1];
-    T* dx = static_cast<T*>(side.y) + b * side.ys[0] + s * side.ys[1];
-    HalfRow<T, VEC, CH> r1[ROWS], r2[ROWS], g1[ROWS], g2[ROWS];
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      const int h = min(static_cast<int>(h0) + u, side.H - 1);
-      const int there = live && static_cast<int>(h0) + u < side.H ? half : 0;  // rows twice have no gradient
-      r1[u].template load<LPR>(x + h * side.xs[2], lane, half);
-      r2[u].template load<LPR>(x + h * side.xs[2] + half, lane, half);
-      g1[u].template load<LPR>(dy + h * side.dys[2], lane, there);
-      g2[u].template load<LPR>(dy + h * side.dys[2] + half, lane, there);
-    }
+    const T* x = static_cast<const T*>(side.x) + b * side.xs[0] + s * side.xs[1] + h_begin * side.xs[2];
+    const T* dy = static_cast<const T*>(side.dy) + b * side.dys[0] + s * side.dys[1] + h_begin * side.dys[2];
+    T* dx = static_cast<T*>(side.y) + b * side.ys[0] + s * side.ys[1] + h_begin * side.ys[2];
     const QkAngles<N> t = load_angles<VEC, CH, LPR>(p, b, s, lane, half);
+    const int heads = side.H - h_begin;  // at least one; rows behind them are the last one again, without a gradient
+    for (int h0 = 0; h0 < p.heads_per_cta; h0 += ROWS) {
+      HalfRow<T, VEC, CH> r1[ROWS], r2[ROWS], g1[ROWS], g2[ROWS];
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      QkRow<N> z{pairs_of(r1[u]), pairs_of(r2[u])}, g{pairs_of(g1[u]), pairs_of(g2[u])};
-      if (p.first) turn_pairs(g, t.c, t.ns, t.s);
-      else turn_pairs(z, t.c, t.s, t.ns);
-      if constexpr (LAYER) centre<VEC, CH, LPR>(z, lane, half, inv_d);
-      const float rstd = rsqrtf(fmaf(row_dot<LPR>(z, z), inv_d, p.eps));
-      const float2 rstd2 = make_float2(rstd, rstd);
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        if constexpr (LAYER) {
-          db.a.v[i] = add2(db.a.v[i], g.a.v[i]);
-          db.b.v[i] = add2(db.b.v[i], g.b.v[i]);
-        }
-        g.a.v[i] = mul2(g.a.v[i], rstd2);
-        g.b.v[i] = mul2(g.b.v[i], rstd2);
-        dw.a.v[i] = fma2(g.a.v[i], z.a.v[i], dw.a.v[i]);
-        dw.b.v[i] = fma2(g.b.v[i], z.b.v[i], dw.b.v[i]);
-        g.a.v[i] = mul2(g.a.v[i], w1.v[i]);
-        g.b.v[i] = mul2(g.b.v[i], w2.v[i]);
+      for (int u = 0; u < ROWS; ++u) {
+        const int h = min(h0 + u, heads - 1), there = live && h0 + u < heads ? half : 0;
+        r1[u].template load<LPR>(x + h * side.xs[2], lane, half);
+        r2[u].template load<LPR>(x + h * side.xs[2] + half, lane, half);
+        g1[u].template load<LPR>(dy + h * side.dys[2], lane, there);
+        g2[u].template load<LPR>(dy + h * side.dys[2] + half, lane, there);
       }
-      const float k = -row_dot<LPR>(g, z) * inv_d * rstd * rstd;
-      const float2 k2 = make_float2(k, k);
-      float mean = 0.0f;
-      if constexpr (LAYER) mean = -row_sum<LPR>(g) * inv_d;
-      const float2 mean2 = make_float2(mean, mean);
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        g.a.v[i] = fma2(z.a.v[i], k2, g.a.v[i]);
-        g.b.v[i] = fma2(z.b.v[i], k2, g.b.v[i]);
-        if constexpr (LAYER) {
-          g.a.v[i] = add2(g.a.v[i], mean2);
-          g.b.v[i] = add2(g.b.v[i], mean2);
+      for (int u = 0; u < ROWS; ++u) {
+        QkRow<N> z{pairs_of(r1[u]), pairs_of(r2[u])}, g{pairs_of(g1[u]), pairs_of(g2[u])};
+        if (p.first) turn_pairs(g, t.c, t.ns, t.s);
+        else turn_pairs(z, t.c, t.s, t.ns);
+        if constexpr (LAYER) centre<VEC, CH, LPR>(z, lane, half, inv_d);
+        const float rstd = rsqrtf(fmaf(row_dot<LPR>(z, z), inv_d, p.eps));
+        const float2 rstd2 = make_float2(rstd, rstd);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          if constexpr (LAYER) {
+            db.a.v[i] = add2(db.a.v[i], g.a.v[i]);
+            db.b.v[i] = add2(db.b.v[i], g.b.v[i]);
+          }
+          g.a.v[i] = mul2(g.a.v[i], rstd2);
+          g.b.v[i] = mul2(g.b.v[i], rstd2);
+          dw.a.v[i] = fma2(g.a.v[i], z.a.v[i], dw.a.v[i]);
+          dw.b.v[i] = fma2(g.b.v[i], z.b.v[i], dw.b.v[i]);
+          g.a.v[i] = mul2(g.a.v[i], w1.v[i]);
+          g.b.v[i] = mul2(g.b.v[i], w2.v[i]);
         }
-      }
-      if (!p.first) turn_pairs(g, t.c, t.ns, t.s);
-      if (live && static_cast<int>(h0) + u < side.H) {
-        T* row = dx + (static_cast<int>(h0) + u) * side.ys[2];
-        float f[N];
-        unpair(g.a, f);
-        store_half<T, VEC, CH, LPR>(row, lane, half, f);
-        unpair(g.b, f);
-        store_half<T, VEC, CH, LPR>(row + half, lane, half, f);
+        const float k = -row_dot<LPR>(g, z) * inv_d * rstd * rstd;
+        const float2 k2 = make_float2(k, k);
+        float mean = 0.0f;
+        if constexpr (LAYER) mean = -row_sum<LPR>(g) * inv_d;
+        const float2 mean2 = make_float2(mean, mean);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          g.a.v[i] = fma2(z.a.v[i], k2, g.a.v[i]);
+          g.b.v[i] = fma2(z.b.v[i], k2, g.b.v[i]);
+          if constexpr (LAYER) {
+            g.a.v[i] = add2(g.a.v[i], mean2);
+            g.b.v[i] = add2(g.b.v[i], mean2);
+          }
+        }
+        if (!p.first) turn_pairs(g, t.c, t.ns, t.s);
+        if (live && h0 + u < heads) {
+          T* row = dx + (h0 + u) * side.ys[2];
+          float f[N];
+          unpair(g.a, f);
+          store_half<T, VEC, CH, LPR>(row, lane, half, f);
+          unpair(g.b, f);
+          store_half<T, VEC, CH, LPR>(row + half, lane, half, f);
+        }
       }
     }
   }
@@ -330,6 +336,7 @@ struct QkReduce {
 // Grid (columns / 32, 4): a block's 32 rows of threads have every 32nd partial sum of 32 columns.
 __global__ void __launch_bounds__(1024) qk_norm_reduce_kernel(const QkReduce r) {
   __shared__ float sm[32][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   void* out = r.out[blockIdx.y];
   if (!out) return;
   const bool keys = blockIdx.y & 1;
@@ -410,8 +417,12 @@ static int qk_bwd_blocks() { return sm_count_of_current_device() * QK_BWD_CTAS_P
 template <typename T, int VEC, int LPR, int CH, int ROWS>
 static int launch_qk_bwd(QkParams& p, QkReduce& r, cudaStream_t stream) {
   constexpr int GROUPS = QK_THREADS / LPR;
+  // eight heads of a token to an item, fewer where that leaves threads without one
+  const int64_t heads = p.side[0].H + p.side[1].H;
+  p.heads_per_cta = XH;
+  while (p.heads_per_cta > ROWS && p.tokens * heads < p.heads_per_cta * qk_bwd_blocks() * GROUPS) p.heads_per_cta /= 2;
   auto needs = [&](const QkSide& s) {
-    return (p.tokens * ((s.H + ROWS - 1) / ROWS) + GROUPS - 1) / GROUPS;
+    return (p.tokens * ((s.H + p.heads_per_cta - 1) / p.heads_per_cta) + GROUPS - 1) / GROUPS;
   };
   const int64_t most = qk_bwd_blocks(), nq = needs(p.side[0]), nk = needs(p.side[1]);
   int64_t q = nq, k = nk;
@@ -436,8 +447,16 @@ static int launch_qk_bwd(QkParams& p, QkReduce& r, cudaStream_t stream) {
   r.blocks = static_cast<int>(q + k);
   r.D = p.D;
   r.dtype = p.w_dtype;
-  qk_norm_reduce_kernel<<<dim3((p.D + 31) / 32, 4), 1024, 0, stream>>>(r);
-  return cudaGetLastError() == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};  // prepared beside the end of the launch in front, which it waits for
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((p.D + 31) / 32, 4);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = q + k > 0 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, qk_norm_reduce_kernel, r) == cudaSuccess ? TRX_OK : TRX_ERR_CUDA;
 }
 
 template <typename T>
