@@ -197,24 +197,27 @@ class _QKNormRoPEFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, q_bias, k_bias, eps, norm, norm_first, positions):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.how = {"eps": eps, "norm": norm, "norm_first": norm_first}
-        ctx.dtypes = (k_weight.dtype, *(None if b is None else b.dtype for b in (q_bias, k_bias)))
-        return ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_bias=q_bias, k_bias=k_bias,
-                                positions=positions, **ctx.how)
+        ctx.how = (eps, norm, norm_first)
+        ctx.dtypes = (k_weight.dtype, None if q_bias is None else q_bias.dtype,
+                      None if k_bias is None else k_bias.dtype)
+        return ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_bias=q_bias, k_bias=k_bias, eps=eps,
+                                norm=norm, norm_first=norm_first, positions=positions)
 
     @staticmethod
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        grads = ops.qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin,
-                                          positions=positions, need_dw=need[2] or need[3],
-                                          need_db=need[6] or need[7], **ctx.how)
-        dq, dk, dqw, *rest = grads
+        need, (eps, norm, norm_first) = ctx.needs_input_grad, ctx.how
+        grads = list(ops.qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, eps=eps,
+                                               norm=norm, norm_first=norm_first, positions=positions,
+                                               need_dw=need[2] or need[3], need_db=need[6] or need[7]))
         # those of another dtype than q's weight were summed in its dtype
-        dkw, dqb, dkb = (None if g is None or t is None else g.to(t) for g, t in zip(rest, ctx.dtypes))
-        # the shapes of weights that are not one-dimensional
-        if dqw is not None:
-            dqw, dkw = dqw.view(q_weight.shape), dkw.view(k_weight.shape)
+        for i, dtype in zip((3, 4, 5), ctx.dtypes):
+            if grads[i] is not None and grads[i].dtype != dtype:
+                grads[i] = None if dtype is None else grads[i].to(dtype)
+        for i, w in ((2, q_weight), (3, k_weight)):
+            if grads[i] is not None and w.dim() != 1:
+                grads[i] = grads[i].view(w.shape)
+        dq, dk, dqw, dkw, dqb, dkb = grads
         return dq, dk, dqw, dkw, None, None, dqb, dkb, None, None, None, None
 
 

@@ -6,6 +6,7 @@ raise otherwise — there is no CPU path and no fallback.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import threading
@@ -59,6 +60,10 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# The current device without a look at whether CUDA is up: there is a CUDA tensor.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _launch(name: str, dev: torch.device, *args) -> None:
     """Call one C entry point on dev's current stream (its last argument) and raise on a status.
 
@@ -70,7 +75,7 @@ def _launch(name: str, dev: torch.device, *args) -> None:
     fn = _entries.get(name)
     if fn is None:
         fn = _entries[name] = getattr(_lib.load(), name)
-    index, current = dev.index, torch.cuda.current_device()
+    index, current = dev.index, _current_device()
     if index is None or index == current:
         rc = fn(*args, _raw_stream(current))
     else:
@@ -348,7 +353,10 @@ def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     return qo, ko
 
 
-_QKStrides, _QKBackwardStrides = ctypes.c_int64 * (4 * 3 + 2), ctypes.c_int64 * (6 * 3 + 2)
+def _block(*values: int) -> array.array:
+    """int64 values for a C entry that takes many, by their address (`.buffer_info()[0]`): 0.5 us of host
+    time, where a ctypes array of them costs 1.3."""
+    return array.array("q", values)
 
 
 def _tables(cos: torch.Tensor, sin: torch.Tensor, dtype: torch.dtype, half: int):
@@ -359,57 +367,59 @@ def _tables(cos: torch.Tensor, sin: torch.Tensor, dtype: torch.dtype, half: int)
         sin = sin.reshape(-1, sin.shape[-1]).contiguous()
     if cos.shape != sin.shape or cos.shape[1] < half:
         raise ValueError("cos/sin tables must be (positions, >= head_dim/2) and alike")
-    if cos.dtype != sin.dtype or cos.dtype not in (torch.float32, dtype):
+    kind = cos.dtype
+    if kind != sin.dtype or (kind != torch.float32 and kind != dtype):
         cos, sin = cos.float(), sin.float()
     return cos, sin
 
 
-def _positions(positions: Optional[torch.Tensor], B: int, S: int, rows: int):
-    """(tensor, its batch and token strides, whether it is int64) of positions (S,) or (B, S)."""
-    if positions is None:
-        if rows < S:
-            raise ValueError(f"the tables have {rows} positions, the sequences {S}")
-        return None, 0, 0, 0
-    if positions.dtype not in (torch.int32, torch.int64):
+def _positions(positions: torch.Tensor, B: int, S: int):
+    """(batch and token strides, whether it is int64) of positions (S,) or (B, S)."""
+    wide = positions.dtype == torch.int64
+    if not wide and positions.dtype != torch.int32:
         raise TypeError("positions must be int32 or int64")
-    if positions.shape not in ((S,), (1, S), (B, S)):
-        raise ValueError(f"positions {tuple(positions.shape)} are not ({S},) or ({B}, {S})")
-    wide = int(positions.dtype == torch.int64)
-    if positions.dim() == 2 and positions.shape[0] == B:
-        return positions, positions.stride(0), positions.stride(1), wide
-    return positions, 0, positions.stride(-1), wide
+    shape = positions.shape
+    if shape == (B, S):
+        return (*positions.stride(), wide)
+    if shape != (S,) and shape != (1, S):
+        raise ValueError(f"positions {tuple(shape)} are not ({S},) or ({B}, {S})")
+    return 0, positions.stride(-1), wide
 
 
-def _head_params(D: int, *ts: Optional[torch.Tensor]):
-    """Weights and biases of a head's norm, as the kernels read them: of D elements and one dtype."""
-    dtype = ts[0].dtype
-    out = []
-    for t in ts:
-        if t is not None:
-            if t.numel() != D:
-                raise ValueError(f"weight/bias has {t.numel()} elements, a head has {D}")
-            t = _dense(t if t.dtype == dtype else t.detach().to(dtype))
-        out.append(t)
-    return out
+def _head_param(t: torch.Tensor, D: int, dtype: torch.dtype) -> torch.Tensor:
+    """A weight or bias of a head's norm as the kernels read it."""
+    if t.numel() != D:
+        raise ValueError(f"weight/bias has {t.numel()} elements, a head has {D}")
+    if t.dtype != dtype:
+        t = t.detach().to(dtype)
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
-def _qk_inputs(q, k, q_weight, k_weight, cos, sin, norm: str, positions, *more):
-    """Checks that the forward and the backward pass of qk_norm_rope share."""
-    if norm not in HEAD_NORMS:
+def _qk_inputs(dev, q, k, cos, sin, norm: str, positions):
+    """What the forward and the backward pass of qk_norm_rope check and take: q, k, the tables, the sizes, the
+    positions' address, strides and type, the norm's number, the types' of the tables and of q."""
+    how, code = HEAD_NORMS.get(norm), _DTYPE_CODE.get(q.dtype)
+    if how is None:
         raise ValueError(f"Unsupported norm '{norm}'. Supported: {sorted(HEAD_NORMS)}")
-    dev = _same_device(q, k, q_weight, k_weight, cos, sin, positions, *more)
+    if code is None:
+        _code(q)
     if q.dtype != k.dtype:
         raise TypeError("q and k must share a dtype")
-    _code(q), _code(q_weight)
     q, k = _bshd(q), _bshd(k)
     B, S, Hq, D = q.shape
-    if k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
+    Bk, Sk, Hk, Dk = k.shape
+    if Bk != B or Sk != S or Dk != D:
         raise ValueError(f"k shape {tuple(k.shape)} does not match q {tuple(q.shape)}")
     if D % 2 or not 0 < D <= 512:
         raise ValueError(f"head_dim must be even and at most 512, got {D}")
     cos, sin = _tables(cos, sin, q.dtype, D // 2)
-    pos, pb, ps, wide = _positions(positions, B, S, cos.shape[0])
-    return dev, q, k, cos, sin, pos, (pb, ps), wide
+    if positions is None:
+        if cos.shape[0] < S:
+            raise ValueError(f"the tables have {cos.shape[0]} positions, the sequences {S}")
+        where = (0, 0, 0, 0)
+    else:
+        where = (positions.data_ptr(), *_positions(positions, B, S))
+    return q, k, cos, sin, (B, S, Hq, Hk, D), where, how, _DTYPE_CODE[cos.dtype], code
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -425,18 +435,23 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     a token has (None: its index in the sequence); one that the tables lack gives rows of NaN. All
     arithmetic is fp32, rounded once to q's dtype. D is even and at most 512.
     """
-    if norm != "layernorm" and (q_bias is not None or k_bias is not None):
-        raise ValueError("only layernorm has biases")
-    dev, q, k, cos, sin, pos, pos_strides, wide = _qk_inputs(q, k, q_weight, k_weight, cos, sin, norm,
-                                                             positions, q_bias, k_bias)
-    B, S, Hq, D = q.shape
-    qw, kw, qb, kb = _head_params(D, q_weight, k_weight, q_bias, k_bias)
+    dev = _same_device(q, k, q_weight, k_weight, cos, sin, positions, q_bias, k_bias)
+    q, k, cos, sin, sizes, (pos, pb, ps, wide), how, table_code, code = _qk_inputs(dev, q, k, cos, sin, norm,
+                                                                                   positions)
+    D, kind = sizes[4], q_weight.dtype
+    qw, kw = _head_param(q_weight, D, kind), _head_param(k_weight, D, kind)
+    qb = kb = None
+    if q_bias is not None or k_bias is not None:
+        if norm != "layernorm":
+            raise ValueError("only layernorm has biases")
+        qb, kb = (None if b is None else _head_param(b, D, kind) for b in (q_bias, k_bias))
     qo, ko = _new(q), _new(k)
-    strides = _QKStrides(*q.stride()[:3], *k.stride()[:3], *qo.stride()[:3], *ko.stride()[:3], *pos_strides)
+    strides = _block(*q.stride()[:3], *k.stride()[:3], *qo.stride()[:3], *ko.stride()[:3], pb, ps)
+    rows, step = cos.shape
     _launch("trx_qk_norm_rope_fwd", dev, q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), _ptr(qb),
-            _ptr(kb), cos.data_ptr(), sin.data_ptr(), _ptr(pos), qo.data_ptr(), ko.data_ptr(), B, S, Hq,
-            k.shape[2], D, ctypes.addressof(strides), cos.shape[0], cos.stride(0), float(eps),
-            HEAD_NORMS[norm], int(bool(norm_first)), wide, _code(cos), _code(qw), _code(q))
+            _ptr(kb), cos.data_ptr(), sin.data_ptr(), pos, qo.data_ptr(), ko.data_ptr(), *sizes,
+            strides.buffer_info()[0], rows, step, eps, how, 1 if norm_first else 0, wide, table_code, _code(qw),
+            code)
     return qo, ko
 
 
@@ -450,25 +465,26 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     only). They have the dtype of q_weight and are summed in fp32 in a fixed order."""
     if need_db and norm != "layernorm":
         raise ValueError("only layernorm has biases")
-    dev, q, k, cos, sin, pos, pos_strides, wide = _qk_inputs(q, k, q_weight, k_weight, cos, sin, norm,
-                                                             positions, dq_out, dk_out)
-    for d, x in ((dq_out, q), (dk_out, k)):
-        if d.shape != x.shape or d.dtype != x.dtype:
-            raise ValueError("gradients must have the shape and dtype of the outputs")
-    B, S, Hq, D = q.shape
+    dev = _same_device(q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out)
+    q, k, cos, sin, sizes, (pos, pb, ps, wide), how, table_code, code = _qk_inputs(dev, q, k, cos, sin, norm,
+                                                                                   positions)
+    if dq_out.shape != q.shape or dk_out.shape != k.shape or dq_out.dtype != q.dtype or dk_out.dtype != q.dtype:
+        raise ValueError("gradients must have the shape and dtype of the outputs")
+    D, kind = sizes[4], q_weight.dtype
     dq_out, dk_out = _bshd(dq_out), _bshd(dk_out)
-    qw, kw = _head_params(D, q_weight, k_weight)
+    qw, kw = _head_param(q_weight, D, kind), _head_param(k_weight, D, kind)
     dq, dk = _new(q), _new(k)
-    dw = (_empty(qw, D), _empty(qw, D)) if need_dw else (None, None)
-    db = (_empty(qw, D), _empty(qw, D)) if need_db else (None, None)
-    ws = _empty(q, _qk_workspace_bytes(dev.index, D), dtype=torch.uint8)
-    strides = _QKBackwardStrides(*dq_out.stride()[:3], *dk_out.stride()[:3], *q.stride()[:3],
-                                 *k.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *pos_strides)
+    dw = _empty(qw, (2, D)).unbind(0) if need_dw else (None, None)
+    db = _empty(qw, (2, D)).unbind(0) if need_db else (None, None)
+    size = _qk_workspace_bytes(dev.index, D)
+    ws = _empty(q, size, dtype=torch.uint8)
+    strides = _block(*dq_out.stride()[:3], *dk_out.stride()[:3], *q.stride()[:3], *k.stride()[:3],
+                     *dq.stride()[:3], *dk.stride()[:3], pb, ps)
+    rows, step = cos.shape
     _launch("trx_qk_norm_rope_bwd", dev, dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
-            qw.data_ptr(), kw.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(pos), dq.data_ptr(),
-            dk.data_ptr(), _ptr(dw[0]), _ptr(dw[1]), _ptr(db[0]), _ptr(db[1]), B, S, Hq, k.shape[2], D,
-            ctypes.addressof(strides), cos.shape[0], cos.stride(0), float(eps), HEAD_NORMS[norm],
-            int(bool(norm_first)), wide, _code(cos), _code(qw), _code(q), ws.data_ptr(), ws.numel())
+            qw.data_ptr(), kw.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos, dq.data_ptr(), dk.data_ptr(),
+            _ptr(dw[0]), _ptr(dw[1]), _ptr(db[0]), _ptr(db[1]), *sizes, strides.buffer_info()[0], rows, step,
+            eps, how, 1 if norm_first else 0, wide, table_code, _code(qw), code, ws.data_ptr(), size)
     if need_dw or need_db:
         _count()  # the sums are a launch of their own
     return dq, dk, *dw, *db
@@ -1018,8 +1034,6 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
 
 
 # ----------------------------------------------------------------------------- paged cache
-_AppendStrides, _CacheStrides = ctypes.c_int64 * (4 * 3 + 11), ctypes.c_int64 * 11
-_PagedStrides = ctypes.c_int64 * (2 * 3 + 11)
 _NO_SCALES = (0, 0, 0, 0)
 
 
@@ -1027,57 +1041,61 @@ def _cache(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: Optional[torc
            v_scales: Optional[torch.Tensor], block_table: torch.Tensor, sequences: int, dtype: torch.dtype):
     """((kv heads, head_dim, pages, page size, width of the table), the cache's strides) of a paged cache, whose
     tensors are taken as they are: nothing of them can be a copy."""
-    if dtype not in (torch.bfloat16, torch.float16):
+    if dtype != torch.bfloat16 and dtype != torch.float16:
         raise TypeError("the paged cache serves bfloat16 and float16")
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
-        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be alike, "
+    shape, held = k_pages.shape, dtype if k_scales is None else torch.uint8
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError(f"k_pages {tuple(shape)} and v_pages {tuple(v_pages.shape)} must be alike, "
                          f"(pages, kv heads, page size, head_dim) or, of 4 bits, head_dim / 2")
-    pages, heads, size, d = k_pages.shape
+    pages, heads, size, d = shape
     if (k_scales is None) != (v_scales is None):
         raise ValueError("k_scales and v_scales come together")
-    if k_scales is None:
-        if k_pages.dtype != dtype or v_pages.dtype != dtype:
-            raise TypeError(f"the cache holds {k_pages.dtype} and {v_pages.dtype}, the call's tensors are {dtype}")
-        scale_strides = _NO_SCALES
-    else:
+    if k_pages.dtype != held or v_pages.dtype != held:
+        raise TypeError(f"the cache holds {k_pages.dtype} and {v_pages.dtype}, the call's tensors are {dtype}"
+                        if k_scales is None else "a cache with scales holds codes of 4 bits, two to a uint8")
+    scale_strides = _NO_SCALES
+    if k_scales is not None:
         d *= 2
-        if k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8:
-            raise TypeError("a cache with scales holds codes of 4 bits, two to a uint8")
-        shape = (pages, heads, size, 2)
+        ks, vs = k_scales.stride(), v_scales.stride()
         for t in (k_scales, v_scales):
-            if t.dtype != torch.float32 or t.shape != shape:
-                raise ValueError(f"scales must be float32 of {shape}")
-            if t.stride()[2:] != (2, 1) and t.numel():
-                raise ValueError("a head's scales on a page must be contiguous")
-        scale_strides = (*k_scales.stride()[:2], *v_scales.stride()[:2])
-    for t in (k_pages, v_pages):
-        if t.stride(3) != 1 and t.numel():
-            raise ValueError("head_dim must be the contiguous dimension of the pages")
+            if t.dtype != torch.float32 or t.shape != (pages, heads, size, 2):
+                raise ValueError(f"scales must be float32 of ({pages}, {heads}, {size}, 2)")
+        if (ks[2:] != (2, 1) or vs[2:] != (2, 1)) and k_scales.numel():
+            raise ValueError("a head's scales on a page must be contiguous")
+        scale_strides = (ks[0], ks[1], vs[0], vs[1])
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if (ks[3] != 1 or vs[3] != 1) and k_pages.numel():
+        raise ValueError("head_dim must be the contiguous dimension of the pages")
     if size % 16 or not 0 < size <= 4096:
         raise ValueError(f"page size must be a multiple of 16 up to 4096, got {size}")
-    if d not in (64, 128):
+    if d != 128 and d != 64:
         raise ValueError(f"the paged cache serves head_dim 64 and 128, got {d}")
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != sequences
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise ValueError(f"block_table must be int32 of ({sequences}, pages of a sequence), its rows contiguous")
-    strides = (*k_pages.stride()[:3], *v_pages.stride()[:3], *scale_strides, block_table.stride(0))
-    return (heads, d, pages, size, block_table.shape[1]), strides
+    rows = block_table.shape
+    if block_table.dtype != torch.int32 or len(rows) != 2 or rows[0] != sequences:
+        raise ValueError(f"block_table must be int32 of ({sequences}, pages of a sequence)")
+    step = block_table.stride()
+    if step[1] != 1 and rows[1] > 1:
+        raise ValueError("block_table's rows must be contiguous")
+    return (heads, d, pages, size, rows[1]), (*ks[:3], *vs[:3], *scale_strides, step[0])
 
 
 def _vector_view(t: torch.Tensor) -> torch.Tensor:
     """A view whose rows can be read in 16-byte pieces, whatever the other strides are; else a copy."""
-    if t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    if t.numel() == 0 or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-                          and all(n == 1 or step % 8 == 0 for n, step in zip(t.shape[:-1], t.stride()))):
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous() or (t.stride(-1) == 1 and all(
+                n == 1 or step % 8 == 0 for n, step in zip(t.shape[:-1], t.stride()))):
+            return t
+    elif t.numel() == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides3(t: torch.Tensor):
     """(sequence, token, head) strides of (sequences, tokens, heads, d) or of packed (tokens, heads, d); a dim of
-    size 1 may carry any stride, here 0."""
-    steps = [0 if n == 1 else step for n, step in zip(t.shape[:-1], t.stride())]
+    size 1 may carry any stride: one that is no multiple of 16 bytes becomes 0."""
+    steps = t.stride()[:-1]
+    if steps[0] % 8 or steps[-1] % 8 or steps[1] % 8:
+        steps = tuple(0 if n == 1 else step for n, step in zip(t.shape[:-1], steps))
     return steps if len(steps) == 3 else (0, *steps)
 
 
@@ -1104,19 +1122,19 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     may have the same place. Not differentiable: what is written is no part of an autograd graph.
     """
     dev = _same_device(k, v, k_pages, v_pages, block_table, lengths, k_scales, v_scales, cos, sin, q, cu_seqlens)
-    packed, dtype = cu_seqlens is not None, k.dtype
-    if k.dim() != (3 if packed else 4) or v.shape != k.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be alike, "
+    packed, dtype, shape = cu_seqlens is not None, k.dtype, k.shape
+    if len(shape) != (3 if packed else 4) or v.shape != shape:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} must be alike, "
                          + ("(rows, heads, head_dim)" if packed else "(batch, tokens, heads, head_dim)"))
     if v.dtype != dtype or (q is not None and q.dtype != dtype):
         raise TypeError("q, k and v must share a dtype")
     cu = _cu_seqlens(cu_seqlens, "cu_seqlens") if packed else None
-    n_seq, tokens = (cu.numel() - 1, k.shape[0]) if packed else k.shape[:2]
+    n_seq, tokens = (cu.numel() - 1, shape[0]) if packed else shape[:2]
     if lengths.dtype != torch.int32 or lengths.shape != (n_seq,):
         raise ValueError(f"lengths must be an int32 tensor of {n_seq} entries")
     (Hk, D, pages, size, width), cache = _cache(k_pages, v_pages, k_scales, v_scales, block_table, n_seq, dtype)
-    if k.shape[-2:] != (Hk, D):
-        raise ValueError(f"k {tuple(k.shape)} does not match the cache's {Hk} heads of {D}")
+    if shape[-2:] != (Hk, D):
+        raise ValueError(f"k {tuple(shape)} does not match the cache's {Hk} heads of {D}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     rows, step, table_code = 0, 0, 0
@@ -1124,8 +1142,8 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         cos, sin = _tables(cos, sin, dtype, D // 2)
         if cos.shape[1] * cos.element_size() % 16 or cos.data_ptr() % 16 or sin.data_ptr() % 16:
             cos, sin = (t[:, : D // 2].clone(memory_format=torch.contiguous_format) for t in (cos, sin))
-        rows, step, table_code = cos.shape[0], cos.shape[1], _code(cos)
-    out, Hq = None, 0
+        (rows, step), table_code = cos.shape, _DTYPE_CODE[cos.dtype]
+    out, Hq, q_strides, out_strides = None, 0, (0, 0, 0), (0, 0, 0)
     if q is not None:
         if cos is None:
             raise ValueError("q is rotated: it needs cos and sin")
@@ -1135,14 +1153,14 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         out = _new(q)
         if packed and n_seq == 0:
             return out.zero_()
+        q_strides, out_strides = _strides3(q), _strides3(out)
     k, v, lengths = _vector_view(k), _vector_view(v), lengths.contiguous()
-    strides = _AppendStrides(*(_strides3(q) if q is not None else (0, 0, 0)), *_strides3(k), *_strides3(v),
-                             *(_strides3(out) if q is not None else (0, 0, 0)), *cache)
-    if k.numel() or Hq:
+    strides = _block(*q_strides, *_strides3(k), *_strides3(v), *out_strides, *cache)
+    if n_seq and tokens and (Hk or Hq):
         _launch("trx_paged_append", dev, _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(out), k_pages.data_ptr(),
                 v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales), block_table.data_ptr(), lengths.data_ptr(),
                 _ptr(cu), _ptr(cos), _ptr(sin), n_seq, tokens, Hq, Hk, D, pages, size, width,
-                ctypes.addressof(strides), rows, step, table_code, _DTYPE_CODE[dtype])
+                strides.buffer_info()[0], rows, step, table_code, _DTYPE_CODE[dtype])
     return out
 
 
@@ -1166,11 +1184,11 @@ def gather_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torc
     if rows < 0:
         raise ValueError("rows must be >= 0")
     k, v = (torch.empty((rows, Hk, D), dtype=dtype, device=dev) for _ in range(2))
-    strides = _CacheStrides(*cache)
+    strides = _block(*cache)
     if k.numel():
         _launch("trx_paged_gather", dev, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
                 block_table.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), cu.numel() - 1, rows, Hk, D,
-                pages, size, width, ctypes.addressof(strides), 1, _DTYPE_CODE[dtype])
+                pages, size, width, strides.buffer_info()[0], 1, _DTYPE_CODE[dtype])
     return k, v
 
 
@@ -1220,10 +1238,10 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     four = k_scales is not None
     parts = _paged_bytes(dev.index, B, Sq, Hq, Hk, D, width * size, left, four)
     room = _empty(q, parts, dtype=torch.uint8) if parts else None
-    strides = _PagedStrides(*_strides3(q), *_strides3(out), *cache)
+    strides = _block(*_strides3(q), *_strides3(out), *cache)
     _launch("trx_attn_fwd_paged", dev, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales),
             _ptr(v_scales), out.data_ptr(), _ptr(lse), _ptr(slopes), block_table.data_ptr(), lengths.data_ptr(),
-            B, Sq, Hq, Hk, D, pages, size, width, ctypes.addressof(strides), scale, left, _DTYPE_CODE[q.dtype],
+            B, Sq, Hq, Hk, D, pages, size, width, strides.buffer_info()[0], scale, left, _DTYPE_CODE[q.dtype],
             _ptr(room), parts, ws.data_ptr(), ws.numel())
     if parts:
         _count()  # the sequences' parts are added up by a launch of their own
