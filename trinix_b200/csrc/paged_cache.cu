@@ -197,17 +197,26 @@ struct GatherParams {
 };
 
 // What a word of eight codes stands for, in T: code * step and the sum with lowest apart, as the elementwise formula
-// rounds them. A code goes into the low byte of 2^23, which is subtracted again (exact).
+// rounds them (a packed product and sum would become one rounding). A code goes into the low byte of 2^23;
+// (2^23 + code) * step - 2^23 * step, rounded once, is code * step, rounded once, where 2^23 * step is finite.
 template <typename T>
 __device__ __forceinline__ uint4 values_of(uint32_t word, float2 scale) {
   const uint32_t even = word & 0x0F0F0F0Fu, odd = (word >> 4) & 0x0F0F0F0Fu;
+  const float2 step = make_float2(scale.x, scale.x), low = make_float2(scale.y, scale.y);
+  const float2 minus = make_float2(-8388608.0f * scale.x, -8388608.0f * scale.x);
   float f[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t bits = __byte_perm(i & 1 ? odd : even, 0x4B000000u, 0x7650 + i / 2);
-    // (not as packed pairs, whose product and sum the compiler makes one rounding of)
-    f[i] = __fadd_rn(scale.y, __fmul_rn(__uint_as_float(bits) - 8388608.0f, scale.x));
+  for (int i = 0; i < 4; ++i) {
+    const float2 code = make_float2(__uint_as_float(__byte_perm(even, 0x4B000000u, 0x7650 + i)),
+                                    __uint_as_float(__byte_perm(odd, 0x4B000000u, 0x7650 + i)));
+    const float2 v = add2(low, fma2(code, step, minus));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
   }
+  if (scale.x >= 0x1p100f)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      f[i] = __fadd_rn(scale.y, __fmul_rn(static_cast<float>((word >> (4 * i)) & 15u), scale.x));
   return Pack<T>::pack(f);
 }
 
