@@ -201,3 +201,31 @@ def test_cpu_tensors_are_refused(bits):
         T.attention_paged(k, **c, lengths=lengths)
     with pytest.raises(ValueError, match="CUDA"):
         T.qk_norm_rope(k, k, k[0, 0, 0], k[0, 0, 0], k[0, 0], k[0, 0])
+
+
+@pytest.mark.parametrize("change,error", [(dict(bits=8), ValueError), (dict(dtype=torch.float32), TypeError),
+                                          (dict(page_size=24), ValueError), (dict(num_pages=0), ValueError),
+                                          (dict(head_dim=96), ValueError), (dict(page_size=8192), ValueError)], ids=str)
+def test_cache_refuses(change, error):
+    a = dict(num_pages=4, page_size=16, num_kv_heads=2, head_dim=64, batch_size=2, device="cpu")
+    with pytest.raises(error):
+        T.PagedKVCache(**{**a, **change})
+
+
+def test_cache_reserves_pages():
+    c = T.PagedKVCache(6, 16, 2, 64, 2, max_pages=4, device="cpu")
+    c.reserve([17, 3])
+    assert sorted(c.block_table.flatten().tolist()) == [-1] * 5 + [0, 1, 2]
+    c.reserve(16)  # less than one has, as much as the other
+    assert (c.block_table >= 0).sum(1).tolist() == [2, 1]
+    for bad in (65, [0, 80]):
+        before = c.block_table.clone()
+        with pytest.raises(RuntimeError, match="pages"):
+            c.reserve(bad)
+        assert torch.equal(c.block_table, before)
+    for bad in ([1], [-1, 0]):
+        with pytest.raises(ValueError):
+            c.reserve(bad)
+    c.release(0)
+    c.reserve([0, 64])
+    assert (c.block_table >= 0).sum(1).tolist() == [0, 4]

@@ -5,6 +5,7 @@ kernel classes with the reference's names (`kernels`), its functional attention 
 point (`functional.triton_attn_func`), mirror modules (`layers`) and `install()`, which
 patches an installed Trinix in place. CUDA tensors only; no fallback paths.
 """
+from .cache import PagedKVCache
 from .functional import flash_attn_func, triton_attn_func
 from .fusion import FastFusedRMSNormInt8, RowwiseInt8Quant, fuse, register_fusion
 from .install import install, uninstall

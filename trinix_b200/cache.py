@@ -1,0 +1,149 @@
+"""A paged cache of keys and values for a batch that is being decoded.
+
+The reference's attention modules keep past keys and values by concatenation
+(trinix/layers/attention/grouped_query_attention.py:178-184): every step copies the whole cache. Here it is a pool of
+pages of fixed size, in the activation's 16 bits or in 4 bits (`ops.append_paged`), of which each sequence of the
+batch owns some; the attention modules take one as `past_key_value`.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import ops
+
+
+class PagedKVCache:
+    """`num_pages` pages of `page_size` tokens for `num_kv_heads` heads of `head_dim`, shared by `batch_size`
+    sequences of up to `max_pages` pages each (default: all of them).
+
+    Which page is whose is kept on the host, with the lengths that the host has reserved room for; the block table
+    and the lengths that the kernels read are on the device, so that a step (`reserve` aside) may be captured in a
+    CUDA graph and replayed: reserve the steps' tokens first. bits=4 holds each row of head_dim values in
+    head_dim / 2 + 8 bytes.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, batch_size: int = 1, *,
+                 max_pages: Optional[int] = None, bits: int = 16, dtype: torch.dtype = torch.bfloat16,
+                 device: Union[str, torch.device] = "cuda"):
+        if bits not in (4, 16):
+            raise ValueError(f"a cache holds 16 or 4 bits, got {bits}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("the paged cache serves bfloat16 and float16")
+        if min(num_pages, num_kv_heads, batch_size) < 1 or page_size < 1 or page_size % 16 or page_size > 4096:
+            raise ValueError("pages, heads and sequences must be positive, page_size a multiple of 16 up to 4096")
+        if head_dim not in (64, 128):
+            raise ValueError(f"the paged cache serves head_dim 64 and 128, got {head_dim}")
+        self.page_size, self.bits, self.dtype = page_size, bits, dtype
+        shape = (num_pages, num_kv_heads, page_size, head_dim if bits == 16 else head_dim // 2)
+        held = dtype if bits == 16 else torch.uint8
+        self.k_pages, self.v_pages = (torch.zeros(shape, dtype=held, device=device) for _ in range(2))
+        self.k_scales = self.v_scales = None
+        if bits == 4:
+            self.k_scales, self.v_scales = (torch.zeros((*shape[:3], 2), dtype=torch.float32, device=device)
+                                            for _ in range(2))
+        self.max_pages = num_pages if max_pages is None else max_pages
+        self.block_table = torch.full((batch_size, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        self._free: List[int] = list(range(num_pages - 1, -1, -1))
+        self._pages: List[List[int]] = [[] for _ in range(batch_size)]
+        self._tokens = [0] * batch_size  # that there is room for
+        self._held = [0] * batch_size    # that have been appended, as far as the host has seen to it
+
+    @property
+    def batch_size(self) -> int:
+        return len(self._pages)
+
+    def __repr__(self) -> str:
+        pages, heads, size, _ = self.k_pages.shape
+        return (f"PagedKVCache(pages={pages}, free={len(self._free)}, page_size={size}, kv_heads={heads}, "
+                f"bits={self.bits}, batch_size={self.batch_size})")
+
+    # -- pages ----------------------------------------------------------------------------------
+    def reserve(self, tokens: Union[int, Sequence[int]]) -> None:
+        """Make sure that every sequence (or each by its own number) has pages for so many tokens more than it
+        holds. Raises, with nothing changed, if the pool or the table's rows have too few."""
+        more = [tokens] * self.batch_size if isinstance(tokens, int) else list(tokens)
+        if len(more) != self.batch_size or min(more) < 0:
+            raise ValueError(f"expected {self.batch_size} numbers of tokens, none negative")
+        want = [max(t, h + n) for t, h, n in zip(self._tokens, self._held, more)]
+        need = [-(-n // self.page_size) for n in want]
+        missing = sum(max(0, n - len(p)) for n, p in zip(need, self._pages))
+        if max(need) > self.max_pages or missing > len(self._free):
+            raise RuntimeError(f"{missing} pages more are needed and {max(need)} for one sequence: the cache has "
+                               f"{len(self._free)} free ones and room for {self.max_pages}")
+        self._tokens = want
+        if missing:
+            for p, n in zip(self._pages, need):
+                while len(p) < n:
+                    p.append(self._free.pop())
+            self._write_table()
+
+    def sync(self) -> None:
+        """Read from the device how many tokens the sequences hold, after replays of captured steps."""
+        self._held = self.lengths.tolist()
+        self._tokens = [max(t, h) for t, h in zip(self._tokens, self._held)]
+
+    def release(self, sequence: int) -> None:
+        """Forget a sequence: its pages are free, its place in the batch is empty."""
+        self._free.extend(reversed(self._pages[sequence]))
+        self._pages[sequence] = []
+        self._tokens[sequence] = self._held[sequence] = 0
+        self.lengths[sequence] = 0
+        self._write_table()
+
+    def _write_table(self) -> None:
+        rows = [p + [-1] * (self.max_pages - len(p)) for p in self._pages]
+        self.block_table.copy_(torch.tensor(rows, dtype=torch.int32))
+
+    # -- kernels ----------------------------------------------------------------------------------
+    def _scales(self) -> dict:
+        return {} if self.bits == 16 else {"k_scales": self.k_scales, "v_scales": self.v_scales}
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor] = None,
+               sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """`ops.append_paged` of k / v (batch, S, heads, head_dim) behind what the sequences hold; pages are
+        reserved for them if they have not been (not while a graph is captured). Returns the rotated queries."""
+        new = k.shape[1]
+        if k.dim() != 4 or k.shape[0] != self.batch_size:
+            raise ValueError(f"expected k ({self.batch_size}, tokens, heads, head_dim), got {tuple(k.shape)}")
+        held = [h + new for h in self._held]
+        if any(h > t for h, t in zip(held, self._tokens)):
+            self.reserve(new)
+        self.lengths.add_(new)
+        out = ops.append_paged(k, v, self.k_pages, self.v_pages, self.block_table, self.lengths, cos=cos, sin=sin,
+                               q=q, **self._scales())
+        self._held = held
+        return out
+
+    def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, window: Optional[Tuple[int, int]] = None,
+               alibi_slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of the last tokens q (batch, S, heads, head_dim) over the cache: `ops.attention_paged`
+        for few of them, else the cache's rows packed (`ops.gather_paged`) and `ops.attention_packed`."""
+        B, S, Hq, D = q.shape
+        if S <= self.LONG:
+            return ops.attention_paged(q, self.k_pages, self.v_pages, self.block_table, self.lengths, scale=scale,
+                                       window=window, alibi_slopes=alibi_slopes, **self._scales())
+        starts = self._starts()
+        # room for all that the sequences' pages hold, whatever the host has seen of the lengths
+        k, v = self._gather(starts, sum(len(p) for p in self._pages) * self.page_size)
+        rows = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=q.device)
+        out = ops.attention_packed(q.reshape(B * S, Hq, D), k, v, rows, starts, causal=True, scale=scale,
+                                   window=None if window is None else (window[0], 0), alibi_slopes=alibi_slopes)
+        return out.view(B, S, Hq, D)
+
+    # Tokens to a sequence from which on the cache is read back for the kernel of packed sequences.
+    LONG = 32
+
+    def gather(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The sequences' keys and values one after the other, (tokens in all, heads, head_dim). Waits for the
+        lengths."""
+        return self._gather(self._starts(), int(self.lengths.sum()))
+
+    def _starts(self) -> torch.Tensor:
+        return torch.nn.functional.pad(self.lengths.cumsum(0, dtype=torch.int32), (1, 0))
+
+    def _gather(self, starts: torch.Tensor, rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        return ops.gather_paged(self.k_pages, self.v_pages, self.block_table, starts, rows=rows, dtype=self.dtype,
+                                **self._scales())

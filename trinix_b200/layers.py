@@ -20,8 +20,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .cache import PagedKVCache
 from .functional import triton_attn_func
 from .kernels import (
+    QKNormRoPEKernel,
     TritonFusedResidualLayerNormKernel,
     TritonFusedResidualRMSNormKernel,
     TritonFusedRMSNormActivationKernel,
@@ -322,7 +324,7 @@ class FastRoPEPositionEmbedding(nn.Module):
         self.use_triton = use_triton
         inv_freq = 1.0 / base ** (torch.arange(0, dim, 2).float() / dim)
         self.register_buffer("inv_freq", inv_freq, persistent=False)
-        self._table_key, self._tables = None, None
+        self._table_key, self._tables, self._wide_tables = None, None, None
 
     def forward(self, x: torch.Tensor, seq_len: Optional[int] = None):
         """(cos, sin) of shape (seq_len, dim) in x's dtype. The angles are always built in
@@ -343,6 +345,16 @@ class FastRoPEPositionEmbedding(nn.Module):
             self._tables = (table.cos().to(x.dtype), table.sin().to(x.dtype))
             self._table_key = key
         return self._tables
+
+    def tables(self, seq_len: int, device: torch.device):
+        """(cos, sin) of forward in fp32, of at least max_position_embeddings positions: what the kernels that
+        look a token's position up take."""
+        rows = max(seq_len, self.max_position_embeddings)
+        if self._wide_tables is None or self._wide_tables[0].shape[0] < rows or self._wide_tables[0].device != device:
+            key, kept = self._table_key, self._tables
+            self._wide_tables = self.forward(torch.empty(0, device=device), rows)
+            self._table_key, self._tables = key, kept
+        return self._wide_tables
 
     @staticmethod
     def _rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -424,7 +436,8 @@ class FastBaseAttention(nn.Module):
                  rope_base: float = 10000.0, use_sliding_window: bool = False,
                  sliding_window_size: Optional[int] = None, qk_norm: bool = False,
                  qk_norm_type: str = "rmsnorm", use_triton_norm: bool = True,
-                 use_triton_embeddings: bool = True, add_zero_attn: bool = False):
+                 use_triton_embeddings: bool = True, add_zero_attn: bool = False,
+                 fused_qk: bool = False):
         super().__init__()
         assert embed_dim % num_heads == 0, (
             f"embed_dim ({embed_dim}) must be divisible by num_heads ({num_heads})")
@@ -441,6 +454,7 @@ class FastBaseAttention(nn.Module):
         self.dropout, self.causal, self.kernel_type = dropout, causal, kernel_type
         self.use_sliding_window, self.sliding_window_size = use_sliding_window, sliding_window_size
         self.qk_norm, self.qk_norm_type = qk_norm, qk_norm_type
+        self.fused_qk = fused_qk
         if qk_norm:
             norm_cls = FastRMSNorm if qk_norm_type == "rmsnorm" else FastLayerNorm
             self.q_norm = norm_cls(self.head_dim, use_triton=use_triton_norm)
@@ -462,6 +476,15 @@ class FastBaseAttention(nn.Module):
     # -- helpers ---------------------------------------------------------------------
     def _uses_kernel(self, q: torch.Tensor) -> bool:
         return self.kernel_type in ("flash", "triton") and q.is_cuda
+
+    def _norm_and_rotate(self, q, k, positions=None):
+        """Rotation, then the q / k norms, as one kernel with fp32 in between (the modules round to the activation's
+        type in between): with fused_qk, position_method="rope" and qk_norm, on the kernel path."""
+        cos, sin = self.position_embedding.tables(q.shape[1], q.device)
+        return QKNormRoPEKernel.apply(
+            q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, getattr(self.q_norm, "bias", None),
+            getattr(self.k_norm, "bias", None), self.q_norm.eps,
+            "rmsnorm" if self.qk_norm_type == "rmsnorm" else "layernorm", False, positions)
 
     def _window_mask(self, seq_q: int, seq_k: int, device) -> torch.Tensor:
         d = torch.arange(seq_k, device=device)[None, :] - torch.arange(seq_q, device=device)[:, None]
@@ -522,6 +545,10 @@ class FastGroupedQueryAttention(FastBaseAttention):
     reference does, :140-145/:189-190) K and V are first copied out to all query heads;
     `tile_kv=False` hands the Hkv-head tensors to the kernel, which maps query head h to
     kv head h // groups itself — same result, no copy.
+
+    With fused_qk=True, rotation and q / k norm (position_method="rope", qk_norm=True) are one kernel. A
+    `past_key_value` that is a PagedKVCache takes the new keys and values and is attended over; it is then what
+    is returned beside the output.
     """
 
     def __init__(self, embed_dim: int, num_heads: int, num_kv_heads: int, dropout: float = 0.0,
@@ -531,13 +558,13 @@ class FastGroupedQueryAttention(FastBaseAttention):
                  use_sliding_window: bool = False, sliding_window_size: Optional[int] = None,
                  qk_norm: bool = False, qk_norm_type: str = "rmsnorm",
                  use_triton_norm: bool = True, use_triton_embeddings: bool = True,
-                 tile_kv: bool = True):
+                 tile_kv: bool = True, fused_qk: bool = False):
         assert num_heads % num_kv_heads == 0, (
             f"num_heads ({num_heads}) must be divisible by num_kv_heads ({num_kv_heads})")
         inner = num_heads * head_dim if head_dim is not None else embed_dim
         super().__init__(inner, num_heads, dropout, bias, kernel_type, causal, position_method,
                          max_seq_len, rope_base, use_sliding_window, sliding_window_size, qk_norm,
-                         qk_norm_type, use_triton_norm, use_triton_embeddings, False)
+                         qk_norm_type, use_triton_norm, use_triton_embeddings, False, fused_qk)
         self.num_kv_heads = num_kv_heads
         self.num_key_value_groups = num_heads // num_kv_heads
         self.tile_kv = tile_kv
@@ -558,11 +585,19 @@ class FastGroupedQueryAttention(FastBaseAttention):
         q = self.q_proj(hidden_states).view(B, S, self.num_heads, self.head_dim)
         k = self.k_proj(hidden_states).view(B, S, self.num_kv_heads, self.head_dim)
         v = self.v_proj(hidden_states).view(B, S, self.num_kv_heads, self.head_dim)
-        if self.position_method == "rope":
-            cos, sin = self.position_embedding(q, S)
-            q, k = self.position_embedding.apply_rotary_pos_emb(q, k, cos, sin, position_ids)
-        if self.qk_norm:
-            q, k = self.q_norm(q), self.k_norm(k)
+        if isinstance(past_key_value, PagedKVCache):
+            if attention_mask is not None:
+                raise ValueError("attention over a paged cache is causal and takes no mask")
+            out = self._attend_paged(q, k, v, past_key_value, position_ids)
+            return self.o_proj(out.reshape(B, S, -1)), past_key_value
+        if self.fused_qk and self.qk_norm and self.position_method == "rope" and self._uses_kernel(q):
+            q, k = self._norm_and_rotate(q, k, position_ids)
+        else:
+            if self.position_method == "rope":
+                cos, sin = self.position_embedding(q, S)
+                q, k = self.position_embedding.apply_rotary_pos_emb(q, k, cos, sin, position_ids)
+            if self.qk_norm:
+                q, k = self.q_norm(q), self.k_norm(k)
         present = None
         if past_key_value is not None:
             k = torch.cat([past_key_value[0].transpose(1, 2), k], dim=1)
@@ -574,6 +609,29 @@ class FastGroupedQueryAttention(FastBaseAttention):
             v = v.repeat_interleave(self.num_key_value_groups, dim=2)
         out = self.forward_attention(q, k, v, attention_mask)
         return self.o_proj(out.reshape(B, S, -1)), present
+
+
+    def _attend_paged(self, q, k, v, cache: PagedKVCache, position_ids=None):
+        """Append to the cache, attend over it. A token's position is its place in its sequence."""
+        if not (self.causal and self._uses_kernel(q)):
+            raise ValueError("a paged cache needs causal=True and the kernel path")
+        if position_ids is not None:
+            raise ValueError("behind a paged cache a token's position is its place in its sequence")
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            raise RuntimeError("attention over a paged cache is forward only: run it under torch.no_grad()")
+        if self.position_method != "rope":
+            if self.qk_norm:
+                q, k = self.q_norm(q), self.k_norm(k)
+            cache.append(k, v)
+        elif self.qk_norm:
+            at = cache.lengths[:, None] + torch.arange(q.shape[1], dtype=torch.int32, device=q.device)
+            q, k = self._norm_and_rotate(q, k, at)
+            cache.append(k, v)
+        else:
+            q = cache.append(k, v, *self.position_embedding.tables(q.shape[1], q.device), q=q)
+        window = (self.sliding_window_size, 0) if self.use_sliding_window else None
+        slopes = self.position_embedding.slopes if self.position_method == "alibi" else None
+        return cache.attend(q, scale=self.scale, window=window, alibi_slopes=slopes)
 
 
 class FastMultiQueryAttention(FastGroupedQueryAttention):
