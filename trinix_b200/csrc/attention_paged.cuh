@@ -550,13 +550,11 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
         float v_low[SUBS][2], v_inv[SUBS][2];  // 4 bits
 #pragma unroll
         for (int k = 0; k < SUBS; ++k) {
-          // the products of a run's columns in two sums: one alone would wait for itself
-          constexpr int CHAINS = NT == 1 ? 2 : 1;
-          float s[NT][4], s2[NT][4];
+          float s[NT][4];
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.0f;
+            for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
           if constexpr (FOUR) {
             uint32_t ka[KW], kb[KW];
             const uint32_t sub = tile + k * L::CODES + key_of_row * (D / 2) + t4 * (D / 8);
@@ -569,8 +567,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
               for (int i = 0; i < 2; ++i) {
                 const uint32_t f[4] = {a[i] & 0x000F000Fu, c[i] & 0x000F000Fu, a[i] & 0x00F000F0u, c[i] & 0x00F000F0u};
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                  mma_16816<false>(i < CHAINS - 1 ? s2[n] : s[n], f, qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
+                for (int n = 0; n < NT; ++n) mma_16816<false>(s[n], f, qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
               }
             }
           } else {
@@ -581,15 +578,9 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
               const int col = (ks % 4) * 2 + half;
               ldsm_x4(tile + (ks / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
-                mma_16816<BF16>(ks % 2 < CHAINS - 1 ? s2[n] : s[n], f, qf[n][ks][0], qf[n][ks][1]);
+              for (int n = 0; n < NT; ++n) mma_16816<BF16>(s[n], f, qf[n][ks][0], qf[n][ks][1]);
             }
           }
-          if constexpr (CHAINS == 2)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int key = key_of_row + 8 * e;
