@@ -547,6 +547,71 @@ def test_streams_and_threads(cuda, bits):
         assert all(torch.equal(w, x) for x in g)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_long_caches_captured_and_on_two_streams(cuda, bits):
+    """Calls whose keys are cut into pieces for the whole chip: captured, replayed with other lengths (short ones, none
+    at all), and two at once on streams of their own."""
+    lengths = [9000, 40, 20000, 333, 1]
+    c = make_cache(lengths, 2, 64, 128, bits, torch.bfloat16, cuda)
+    q = torch.randn(5, 1, 8, 128, device=cuda).bfloat16()
+    n = i32(lengths, cuda)
+    T.attention_paged(q, **c, lengths=n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = T.attention_paged(q, **c, lengths=n, return_lse=True)
+    for now in (lengths, [0] * 5, [5, 40, 1, 0, 1], [9000, 0, 1, 333, 0], [64, 40, 20000, 333, 1]):
+        n.copy_(i32(now, cuda))
+        graph.replay()
+        want, want_lse = T.attention_paged(q, **c, lengths=n, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        for b, m in enumerate(now):
+            assert bool(out[b].any()) == (m > 0) and bool(torch.isneginf(lse[b]).all()) == (m == 0)
+    n.copy_(i32(lengths, cuda))
+    other = torch.randn_like(q)
+    want = T.attention_paged(q, **c, lengths=n), T.attention_paged(other, **c, lengths=n)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(T.attention_paged((q, other)[i], **c, lengths=n))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
+    assert T.attention_status(cuda) == 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("Sq,heads,kv", [(1, 8, 2), (3, 12, 2), (16, 4, 4), (40, 6, 1)])
+def test_many_sequences_of_all_lengths(cuda, bits, Sq, heads, kv):
+    """More sequences than threads look at at once, most of them short, in a cache that some fill far: whole units,
+    units cut once and many times, and row tiles."""
+    g = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 200, (300,), generator=g).tolist()
+    lengths[7], lengths[150], lengths[299] = 3000, 1501, 2500
+    c = make_cache(lengths, kv, 16, 64, bits, torch.float16, cuda)
+    q = torch.randn(300, Sq, heads, 64, device=cuda).half()
+    out, lse = T.attention_paged(q, **c, lengths=i32(lengths, cuda), return_lse=True)
+    # one sequence at a time, which is a call of its own kind
+    for b in (0, 1, 7, 8, 127, 128, 129, 150, 200, 256, 298, 299):
+        one = {**c, "block_table": c["block_table"][b:b + 1, : max(1, -(-lengths[b] // 16))].contiguous()}
+        k, v = T.gather_paged(**one, cu_seqlens=i32([0, lengths[b]], cuda), rows=lengths[b], dtype=torch.float16)
+        if bits == 16:
+            want, want_lse, allowed, allowed_lse = attend64(q[b], k, v, causal=True)
+        else:
+            pages = one["block_table"][0, : -(-lengths[b] // 16)].long()
+
+            def held(x):
+                s = c[x + "_scales"][pages].transpose(1, 2).flatten(0, 1)[:lengths[b]].double()
+                code = codes_of(c[x + "_pages"][pages].transpose(1, 2).flatten(0, 1)[:lengths[b]]).double()
+                return s[..., 1:] + code * s[..., :1], s[..., :1], s[..., 1:]
+            want, want_lse, allowed, allowed_lse = attend_codes(q[b], held("k"), held("v"))
+        assert_within(out[b], want, allowed, f"sequence {b} of {lengths[b]}")
+        assert_within(lse[b], want_lse, allowed_lse, f"lse of sequence {b} of {lengths[b]}")
+
+
 def test_a_later_backward_says_so(cuda):
     c = make_cache([5], 2, 16, 64, 16, torch.float16, cuda)
     q = torch.randn(1, 1, 4, 64, device=cuda).half().requires_grad_()

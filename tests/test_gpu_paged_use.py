@@ -88,6 +88,18 @@ def test_module_over_a_paged_cache(cuda, how, bits):
     assert T.attention_status(cuda) == 0
 
 
+@pytest.mark.parametrize("how", [dict(), dict(qk_norm=True)], ids=str)
+def test_sequences_longer_than_the_module_was_told(cuda, how):
+    """Positions go as far as the cache does."""
+    a, b = (params_to_bf16(module(cuda, max_seq_len=n, **how)) for n in (256, 16))
+    b.load_state_dict(a.state_dict())
+    x = torch.randn(1, 40, E, device=cuda).bfloat16()
+    with torch.no_grad():
+        out = [[m(x[:, i:i + 8], past_key_value=c)[0] for i in range(0, 40, 8)]
+               for m, c in ((a, T.PagedKVCache(4, 16, HK, D)), (b, T.PagedKVCache(4, 16, HK, D)))]
+    assert all(torch.equal(y, z) for y, z in zip(*out)) and all(y.isfinite().all() for y in out[0])
+
+
 def test_steps_as_a_graph(cuda):
     """Steps captured and replayed do what they do one by one."""
     m = params_to_bf16(module(cuda, qk_norm=True, fused_qk=True))

@@ -477,10 +477,11 @@ class FastBaseAttention(nn.Module):
     def _uses_kernel(self, q: torch.Tensor) -> bool:
         return self.kernel_type in ("flash", "triton") and q.is_cuda
 
-    def _norm_and_rotate(self, q, k, positions=None):
+    def _norm_and_rotate(self, q, k, positions=None, most: int = 0):
         """Rotation, then the q / k norms, as one kernel with fp32 in between (the modules round to the activation's
-        type in between): with fused_qk, position_method="rope" and qk_norm, on the kernel path."""
-        cos, sin = self.position_embedding.tables(q.shape[1], q.device)
+        type in between): with fused_qk, position_method="rope" and qk_norm, on the kernel path. positions are
+        below max_seq_len, or `most`."""
+        cos, sin = self.position_embedding.tables(max(most, q.shape[1]), q.device)
         return QKNormRoPEKernel.apply(
             q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, getattr(self.q_norm, "bias", None),
             getattr(self.k_norm, "bias", None), self.q_norm.eps,
@@ -624,11 +625,13 @@ class FastGroupedQueryAttention(FastBaseAttention):
                 q, k = self.q_norm(q), self.k_norm(k)
             cache.append(k, v)
         elif self.qk_norm:
+            most = cache.max_pages * cache.page_size
             at = cache.lengths[:, None] + torch.arange(q.shape[1], dtype=torch.int32, device=q.device)
-            q, k = self._norm_and_rotate(q, k, at)
+            q, k = self._norm_and_rotate(q, k, at, most)
             cache.append(k, v)
         else:
-            q = cache.append(k, v, *self.position_embedding.tables(q.shape[1], q.device), q=q)
+            most = cache.max_pages * cache.page_size
+            q = cache.append(k, v, *self.position_embedding.tables(most, q.device), q=q)
         window = (self.sliding_window_size, 0) if self.use_sliding_window else None
         slopes = self.position_embedding.slopes if self.position_method == "alibi" else None
         return cache.attend(q, scale=self.scale, window=window, alibi_slopes=slopes)
