@@ -234,43 +234,48 @@ __global__ void __launch_bounds__(PC_THREADS) paged_gather_kernel(const __grid_c
   const int at = static_cast<int>(row) - first;
   const int page = there ? page_of(p.c, b, at) : -1, slot = there ? at % p.c.page_size : 0;
   const int h0 = blockIdx.y * PC_ROWS;
+  constexpr int BYTES = FOUR ? 1 : static_cast<int>(sizeof(T));
+  // K's and V's loads all before the first store
+  uint4 y1[2][PC_ROWS], y2[2][PC_ROWS];
+  uint32_t w1[2][PC_ROWS], w2[2][PC_ROWS];
+  float2 scale[2][PC_ROWS];
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
     const int64_t* ps = kv ? p.c.vp : p.c.kp;
     const int64_t* ss = kv ? p.c.vsp : p.c.ksp;
-    constexpr int BYTES = FOUR ? 1 : static_cast<int>(sizeof(T));
     const uint8_t* src = static_cast<const uint8_t*>(kv ? p.c.v : p.c.k) + (page * ps[0] + slot * ps[2]) * BYTES +
                          (FOUR ? 4 : 16) * lane;
     const float* scales = (kv ? p.c.v_scales : p.c.k_scales) + page * ss[0] + 2 * slot;
-    T* out = static_cast<T*>(kv ? p.vo : p.ko) + row * p.Hk * (2 * HALF) + 8 * lane;
-    uint4 y1[PC_ROWS], y2[PC_ROWS];
-    uint32_t w1[PC_ROWS], w2[PC_ROWS];
-    float2 scale[PC_ROWS];
 #pragma unroll
     for (int u = 0; u < PC_ROWS; ++u) {
       const int h = min(h0 + u, p.Hk - 1);
-      y1[u] = y2[u] = make_uint4(0u, 0u, 0u, 0u);
+      y1[kv][u] = y2[kv][u] = make_uint4(0u, 0u, 0u, 0u);
+      w1[kv][u] = w2[kv][u] = 0u;
+      scale[kv][u] = make_float2(0.0f, 0.0f);
       if (page < 0) continue;
       const uint8_t* from = src + h * ps[1] * BYTES;
       if constexpr (FOUR) {
-        w1[u] = __ldg(reinterpret_cast<const uint32_t*>(from));
-        w2[u] = __ldg(reinterpret_cast<const uint32_t*>(from + HALF / 2));
-        scale[u] = __ldg(reinterpret_cast<const float2*>(scales + h * ss[1]));
+        w1[kv][u] = __ldg(reinterpret_cast<const uint32_t*>(from));
+        w2[kv][u] = __ldg(reinterpret_cast<const uint32_t*>(from + HALF / 2));
+        scale[kv][u] = __ldg(reinterpret_cast<const float2*>(scales + h * ss[1]));
       } else {
-        y1[u] = ld_stream16(from);
-        y2[u] = ld_stream16(from + 2 * HALF);
+        y1[kv][u] = ld_stream16(from);
+        y2[kv][u] = ld_stream16(from + 2 * HALF);
       }
     }
+  }
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    T* out = static_cast<T*>(kv ? p.vo : p.ko) + row * p.Hk * (2 * HALF) + 8 * lane;
 #pragma unroll
     for (int u = 0; u < PC_ROWS; ++u) {
       if (h0 + u >= p.Hk) break;
-      if constexpr (FOUR)
-        if (page >= 0) {
-          y1[u] = values_of<T>(w1[u], scale[u]);
-          y2[u] = values_of<T>(w2[u], scale[u]);
-        }
-      st_stream16(out + (h0 + u) * (2 * HALF), y1[u]);
-      st_stream16(out + (h0 + u) * (2 * HALF) + HALF, y2[u]);
+      if constexpr (FOUR) {  // (no page: codes, step and lowest of 0)
+        y1[kv][u] = values_of<T>(w1[kv][u], scale[kv][u]);
+        y2[kv][u] = values_of<T>(w2[kv][u], scale[kv][u]);
+      }
+      st_stream16(out + (h0 + u) * (2 * HALF), y1[kv][u]);
+      st_stream16(out + (h0 + u) * (2 * HALF) + HALF, y2[kv][u]);
     }
   }
 }
