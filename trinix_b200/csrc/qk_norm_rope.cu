@@ -200,6 +200,16 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const __grid_c
   }
 }
 
+// Rows of the backward pass on their way into shared memory: QK_STAGES steps of ROWS heads, 4 ROWS vectors of 16
+// bytes to a thread each, which it alone reads: nobody waits for anybody.
+constexpr int QK_STAGES = 3;
+__device__ __forceinline__ void copy16(uint4* to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+               "l"(from), "r"(there ? 16 : 0)
+               : "memory");
+}
+
 // Blocks [0, q_blocks) walk over the queries, the others over the keys, ROWS heads of a token at a time; every
 // thread keeps the sums of its columns' weight gradients, which meet in shared memory at the end. With z the row
 // that is normalised (a LayerNorm's centred) and e = rstd g w: dx = e - z rstd^2 mean(e z) [- mean e].
@@ -221,30 +231,98 @@ __global__ void __launch_bounds__(QK_THREADS, QK_BWD_CTAS_PER_SM)
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) dw.a.v[i] = dw.b.v[i] = db.a.v[i] = db.b.v[i] = make_float2(0.0f, 0.0f);
 
+  constexpr bool RING = VEC > 1;
+  constexpr int VECTORS = 4 * ROWS;  // of a step: x's two halves, dy's two halves of each row
+  __shared__ uint4 ring[(RING ? QK_STAGES : 1) * VECTORS * QK_THREADS];
+  static_assert(sizeof(ring) >= sizeof(float) * (QK_THREADS / 32) * 2 * N * LPR, "the sums at the end");
   const unsigned chunks = (side.H + p.heads_per_cta - 1) / p.heads_per_cta;
-  const unsigned items = static_cast<unsigned>(p.tokens) * chunks;
+  const unsigned items = static_cast<unsigned>(p.tokens) * chunks, seq = static_cast<unsigned>(p.S);
+  struct Item {
+    const T* x;
+    const T* dy;
+    int64_t b, s;
+    int h, heads;  // at least one head; rows behind them are the last one again, without a gradient
+    bool live;
+  };
+  auto item_at = [&](unsigned i) {
+    Item r;
+    r.live = i < items;
+    i = r.live ? i : items - 1;
+    const unsigned token = i / chunks;
+    r.h = (i - token * chunks) * p.heads_per_cta;
+    r.heads = side.H - r.h;
+    r.b = token / seq;
+    r.s = token - static_cast<unsigned>(r.b) * seq;
+    r.x = static_cast<const T*>(side.x) + r.b * side.xs[0] + r.s * side.xs[1] + r.h * side.xs[2];
+    r.dy = static_cast<const T*>(side.dy) + r.b * side.dys[0] + r.s * side.dys[1] + r.h * side.dys[2];
+    return r;
+  };
+  const unsigned stride = blocks * GROUPS, group = (threadIdx.x % 32) / LPR;
   // whole warps leave together: the item of a warp's first row decides
-  for (unsigned first = (block * QK_THREADS + (threadIdx.x & ~31)) / LPR; first < items;
-       first += blocks * GROUPS) {
-    const unsigned item = min(first + (threadIdx.x % 32) / LPR, items - 1);
-    const bool live = first + (threadIdx.x % 32) / LPR < items;
-    const unsigned token = item / chunks, seq = static_cast<unsigned>(p.S);
-    const int h_begin = (item - token * chunks) * p.heads_per_cta;
-    const int64_t b = token / seq, s = token - static_cast<unsigned>(b) * seq;
-    const T* x = static_cast<const T*>(side.x) + b * side.xs[0] + s * side.xs[1] + h_begin * side.xs[2];
-    const T* dy = static_cast<const T*>(side.dy) + b * side.dys[0] + s * side.dys[1] + h_begin * side.dys[2];
-    T* dx = static_cast<T*>(side.y) + b * side.ys[0] + s * side.ys[1] + h_begin * side.ys[2];
-    const QkAngles<N> t = load_angles<VEC, CH, LPR>(p, b, s, lane, half);
-    const int heads = side.H - h_begin;  // at least one; rows behind them are the last one again, without a gradient
+  unsigned first = (block * QK_THREADS + (threadIdx.x & ~31)) / LPR;
+  // what is copied next, and where to
+  unsigned ahead = first;
+  int ahead_h = 0, to = 0, from = 0;
+  Item coming;
+  auto copy_step = [&]() {
+    if constexpr (RING) {
+      if (ahead < items) {
+        if (ahead_h == 0) coming = item_at(ahead + group);
+        const bool inside = lane * VEC < half;
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+          const int h = min(ahead_h + u, coming.heads - 1), col = inside ? lane * VEC : 0;
+          const bool there = inside && coming.live && ahead_h + u < coming.heads;
+          uint4* slot = ring + (to * VECTORS + 4 * u) * QK_THREADS + threadIdx.x;
+          const T* x = coming.x + h * side.xs[2] + col;
+          const T* dy = coming.dy + h * side.dys[2] + col;
+          copy16(slot, x, inside);
+          copy16(slot + QK_THREADS, x + half, inside);
+          copy16(slot + 2 * QK_THREADS, dy, there);
+          copy16(slot + 3 * QK_THREADS, dy + half, there);
+        }
+        ahead_h += ROWS;
+        if (ahead_h >= p.heads_per_cta) {
+          ahead_h = 0;
+          ahead += stride;
+        }
+        to = to + 1 == QK_STAGES ? 0 : to + 1;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < QK_STAGES - 1; ++i) copy_step();
+
+  for (; first < items; first += stride) {
+    const Item item = item_at(first + group);
+    const bool live = item.live;
+    const int heads = item.heads;
+    T* dx = static_cast<T*>(side.y) + item.b * side.ys[0] + item.s * side.ys[1] + item.h * side.ys[2];
+    const QkAngles<N> t = load_angles<VEC, CH, LPR>(p, item.b, item.s, lane, half);
     for (int h0 = 0; h0 < p.heads_per_cta; h0 += ROWS) {
       HalfRow<T, VEC, CH> r1[ROWS], r2[ROWS], g1[ROWS], g2[ROWS];
+      if constexpr (RING) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(QK_STAGES - 2) : "memory");
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const int h = min(h0 + u, heads - 1), there = live && h0 + u < heads ? half : 0;
-        r1[u].template load<LPR>(x + h * side.xs[2], lane, half);
-        r2[u].template load<LPR>(x + h * side.xs[2] + half, lane, half);
-        g1[u].template load<LPR>(dy + h * side.dys[2], lane, there);
-        g2[u].template load<LPR>(dy + h * side.dys[2] + half, lane, there);
+        for (int u = 0; u < ROWS; ++u) {
+          const uint4* slot = ring + (from * VECTORS + 4 * u) * QK_THREADS + threadIdx.x;
+          r1[u].raw = slot[0];
+          r2[u].raw = slot[QK_THREADS];
+          g1[u].raw = slot[2 * QK_THREADS];
+          g2[u].raw = slot[3 * QK_THREADS];
+        }
+        from = from + 1 == QK_STAGES ? 0 : from + 1;
+        copy_step();
+      } else {
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+          const int h = min(h0 + u, heads - 1), there = live && h0 + u < heads ? half : 0;
+          r1[u].template load<LPR>(item.x + h * side.xs[2], lane, half);
+          r2[u].template load<LPR>(item.x + h * side.xs[2] + half, lane, half);
+          g1[u].template load<LPR>(item.dy + h * side.dys[2], lane, there);
+          g2[u].template load<LPR>(item.dy + h * side.dys[2] + half, lane, there);
+        }
       }
 #pragma unroll
       for (int u = 0; u < ROWS; ++u) {
@@ -295,7 +373,9 @@ __global__ void __launch_bounds__(QK_THREADS, QK_BWD_CTAS_PER_SM)
   }
 
   // the warp's rows, then the CTA's warps, in a fixed order
-  __shared__ float sums[QK_THREADS / 32][2 * N * LPR];
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();  // the ring's memory
+  auto sums = reinterpret_cast<float(*)[2 * N * LPR]>(ring);
   float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.D;
 #pragma unroll
   for (int pass = 0; pass < (LAYER ? 2 : 1); ++pass) {
