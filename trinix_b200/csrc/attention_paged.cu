@@ -2,9 +2,6 @@
 #include "attention_paged.cuh"
 
 namespace trx {
-int make_paged_cache(PagedCache* c, const void* k_pages, const void* v_pages, const float* k_scales,
-                     const float* v_scales, const int32_t* block_table, int64_t n_seq, int64_t Hk, int64_t D,
-                     int64_t pages, int64_t page_size, int64_t width, const int64_t* strides);
 
 // The shape that a call takes: f(D, 4 bits, tiles of 8 rows) as compile-time numbers.
 template <class F>
@@ -24,8 +21,8 @@ static PagedPlan plan_of(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t 
   const int64_t rows = Sq * (Hq / Hk), tile = rows > 8 ? 16 : 8;
   if (window_left >= 0 && Sq + window_left < keys) keys = Sq + window_left;
   return paged_shape(D, four, rows, [&](auto d, auto bits, auto nt) {
-    return paged_plan<decltype(d)::value, decltype(bits)::value, decltype(nt)::value>(B * Hk * ((rows + tile - 1) / tile),
-                                                                                     keys);
+    return paged_plan<decltype(d)::value, decltype(bits)::value, decltype(nt)::value>(
+        B * Hk * ((rows + tile - 1) / tile), keys);
   });
 }
 

@@ -36,6 +36,15 @@
 //     they are rounded to 11 bits, and the running maximum is that of the weighed ones, so that the largest
 //     weight of a row is of the order of 1 whatever the steps are.
 // Scores, sums and O are fp32.
+//
+// Measured (32 / 8 heads x 128, one token to a sequence): 48 sequences of 128 to 8192 keys, 16 bits, 385 MB: 70.5 us,
+// 5.5 TB/s; 64 of 4 bits, 143 MB: 43.7 us; 2 x 131072 and fewer keys of 4 bits, 155 MB: 43.2 us, 3.6 TB/s. What bounds
+// it: 16 bits, the memory (without the arithmetic 67.7 us). 4 bits, both: loads alone would take 36 us, arithmetic
+// alone 37 (500 instructions to 32 keys of a warp, 176 of them the shifts, ANDs and permutes that make operands of
+// codes; three CTAs of 166 registers issue 45 % of the time), 8 of either the call's start, the cuts and the parts.
+// Tried: 16 keys at a time as in attention_decode.cuh and clusters of fixed splits, 4 bits 100 and 109 us; tiles of
+// 32 keys 48 and 47 us; four CTAs to an SM 64 to 67 (registers); two sums for a run's products, or two steps of 32
+// keys unrolled: nothing.
 #pragma once
 
 #include "attention_decode.cuh"
@@ -110,7 +119,9 @@ struct PgShape {
   static constexpr int ALIGN = FOUR ? 128 : 1024;
   static constexpr int DYN_BYTES = TOTAL + ALIGN;
   static constexpr int PART_FLOATS = ROWS * (D + 2);  // of one part in memory
-  // What a unit costs beside its tiles, in tiles, and what a piece of the line has at least.
+  // What a unit costs beside its tiles, in tiles, and what a piece of the line has at least. Of tiles of 32 keys of 4
+  // bits 2, 4, 8, 12, 16 for a unit made 64 sequences of 128 to 8192 keys take 71, 61, 49, 48, 50 us (tiles are now 64);
+  // of 16 bits, 48 sequences 86, 83, 73, 71, 72 us.
   static constexpr int UNIT_COST = FOUR ? 6 : 12;
   static constexpr int LEAST_PIECE = FOUR ? 8 : 16;
   static_assert(RING_BYTES >= PG_THREADS * 8, "the sums of the lengths");
@@ -994,7 +1005,9 @@ static PagedPlan paged_plan(int64_t units, int64_t keys) {
   int n = 1;
   while (n < PG_MOST_SPLITS && units * 2 * n <= slots && tiles >= 2 * n * PG_WARPS * (FOUR ? 1 : 2)) n *= 2;
   const int64_t chain = (tiles + n * PG_WARPS - 1) / (n * PG_WARPS);
-  // more than a few tiles to a warp, or units that do not all run at once: the line
+  // More than a few tiles to a warp, or units that do not all run at once: the line. Line / clusters, 16 bits and 4:
+  // 4 sequences of up to 1000 keys, 16 / 2 heads 13.7 / 9.6 us, 14.4 / 10.3; 4 of up to 8000, 32 / 8 heads 23.4 / 20.4,
+  // 18.3 / 15.1; 64 of up to 500 17.3 / 19.8 and, 4 bits, 20.5 / 14.9.
   const bool line = chain > (units * n <= slots ? (FOUR ? 5 : 16) : (FOUR ? 2 : 3));
   plan.splits = line ? 0 : n;
   plan.ctas = !line ? units * n : slots < PG_MOST_CTAS ? slots : PG_MOST_CTAS;

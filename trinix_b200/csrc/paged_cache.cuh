@@ -5,12 +5,12 @@
 // outside the cache (unused entries are -1) names no memory: nothing is written there, and zeros are read.
 //
 // 4 bits: a row x of head_dim values is held as codes 0 .. 15 and two fp32 numbers,
-//   lowest = min x,  step = (max x - lowest) / 15,  code = rint(15 (x - lowest) / (max x - lowest)),
-//   value = lowest + code * step,
+//   lowest = min x,  step = (max x - lowest) fp32(1/15),  code = rint(15 (x - lowest) / (max x - lowest)),
+//   value = lowest + code * step
 // (step 0 and codes 0 where the values are within 2^-76 of each other, both numbers NaN where a value is not finite
-// or they are 2^120 apart); byte j of the codes being column 2 j in its low bits and 2 j + 1 in its high ones. A row (and not a group of
-// its columns) has one step, because then the step comes out of both of attention's products: it scales a
-// key's score and a value's probability, and the matrix instructions see the codes themselves.
+// or they are more than 2^120 apart); byte j of the codes is column 2 j in its low bits and 2 j + 1 in its high ones.
+// A row (and not a group of its columns) has one step, because then the step comes out of both of attention's
+// products: it scales a key's score and a value's probability, and the matrix instructions see the codes themselves.
 #pragma once
 
 #include "common.cuh"
@@ -28,6 +28,11 @@ struct PagedCache {
   int64_t table_stride;
   int pages, page_size, width;  // width: entries of a table's row
 };
+
+// A C entry's arguments, checked: n_seq rows of the block table; strides as in the public header.
+int make_paged_cache(PagedCache* c, const void* k_pages, const void* v_pages, const float* k_scales,
+                     const float* v_scales, const int32_t* block_table, int64_t n_seq, int64_t Hk, int64_t D,
+                     int64_t pages, int64_t page_size, int64_t width, const int64_t* strides);
 
 // The page of position `pos`, or -1.
 __device__ __forceinline__ int page_of(const PagedCache& c, int64_t b, int pos) {

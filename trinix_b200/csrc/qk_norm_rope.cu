@@ -9,8 +9,11 @@
 //             dw = sum g n,  db = sum g,  d = g w,  dz = rstd (d - n mean(d n) [- mean d])
 //             dx = dz or R^T dz
 // All in fp32, one rounding at the end; row statistics are recomputed in the backward pass, where the row is in
-// registers anyway. Memory bounds both: a row is read once and stays with its few lanes (head_rows.cuh), no
-// shared memory and no barrier in the loop.
+// registers anyway. Memory bounds both: a row is read once and stays with its few lanes (head_rows.cuh), no barrier
+// in the loop, arithmetic in packed pairs (a half as many instructions as without: 119 us instead of 92 at a training
+// step of 8192 tokens, 32 / 8 heads x 128 bf16, which now is 79.6). There: forward 168 MB in 31.5 us, 5.3 TB/s;
+// backward, with the sums of the weight gradients, 252 MB in 48, 5.2 TB/s: three CTAs to an SM, as the sums of a
+// thread's columns leave registers for, issue 38 % of what they could and wait for rows the rest.
 #include "head_rows.cuh"
 
 namespace trx {
@@ -43,8 +46,9 @@ struct QkParams {
 };
 
 constexpr int QK_THREADS = 128;
-// Backward: one wave of so many CTAs; rows in flight to a thread. 8192 tokens, 32 / 8 heads x 128 bf16, forward and
-// backward: 3 CTAs of 2 rows 89.7 us, of 4 rows 89.6, 4 CTAs of 2 rows 93.5, 2 of 4 rows (one head to an item) 98.7.
+// Backward: one wave of so many CTAs; rows of a step. 8192 tokens, 32 / 8 heads x 128 bf16, forward and backward, with
+// 2 steps in shared memory: 3 CTAs of 2 rows 79.6 us; 3 steps 80.5; 6 of one row 79.5 (LayerNorm 23.9 us so, 23.3);
+// 4 CTAs 82 to 86 (128 registers are too few). Rows loaded where they are used, none ahead: 88.
 constexpr int QK_BWD_CTAS_PER_SM = 3;
 constexpr int QK_BWD_ROWS = 2;
 
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const __grid_c
 
 // Rows of the backward pass on their way into shared memory: QK_STAGES steps of ROWS heads, 4 ROWS vectors of 16
 // bytes to a thread each, which it alone reads: nobody waits for anybody.
-constexpr int QK_STAGES = 3;
+constexpr int QK_STAGES = 2;
 __device__ __forceinline__ void copy16(uint4* to, const void* from, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                    static_cast<uint32_t>(__cvta_generic_to_shared(to))),
