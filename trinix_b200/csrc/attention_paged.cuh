@@ -32,13 +32,13 @@
 //     (K) and 8 (V) bytes of a row in one piece. Of 8 keys the fragment's rows are in the order 0, 4, 1, 5, ...:
 //     then the four V rows that a load reads are neighbours.
 //   * fp16 operands serve both activation types: Q's rows are scaled by a power of two to below 2^14 (what is
-//     2^-28 of the row's largest value or more stays exact). Probabilities are weighed with step_v before
-//     they are rounded to 11 bits, and the running maximum is that of the weighed ones, so that the largest
-//     weight of a row is of the order of 1 whatever the steps are.
+//     2^-28 of the row's largest value or more stays exact; a row with values of 2^114 and more is not a number).
+//     Probabilities are weighed with step_v before they are rounded to 11 bits, and the running maximum is that of
+//     the weighed ones, so that the largest weight of a row is of the order of 1 whatever the steps are.
 // Scores, sums and O are fp32.
 //
 // Measured (32 / 8 heads x 128, one token to a sequence): 48 sequences of 128 to 8192 keys, 16 bits, 385 MB: 70.5 us,
-// 5.5 TB/s; 64 of 4 bits, 143 MB: 43.7 us; 2 x 131072 and fewer keys of 4 bits, 155 MB: 43.2 us, 3.6 TB/s. What bounds
+// 5.5 TB/s; 64 of 4 bits, 143 MB: 44.3 us; 2 x 131072 and fewer keys of 4 bits, 155 MB: 43.9 us, 3.5 TB/s. What bounds
 // it: 16 bits, the memory (without the arithmetic 67.7 us). 4 bits, both: loads alone would take 36 us, arithmetic
 // alone 37 (500 instructions to 32 keys of a warp, 176 of them the shifts, ANDs and permutes that make operands of
 // codes; three CTAs of 166 registers issue 45 % of the time), 8 of either the call's start, the cuts and the parts.
@@ -673,7 +673,10 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
             }
         }
         uint32_t pf[SUBS][NT][2];
-        // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there
+        // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there. What the
+        // rounding takes off a weight goes in with the code 8: only codes' distances from that, their spread, meet the
+        // rounded weight. (Without, the roundings count with the codes' mean: fp16, 24 x 5 rows behind 46 to 3001 keys
+        // 3.3e-4 off the definition instead of 2.5e-4, of which the output's own type is 2.1e-4.)
         auto weigh = [&](auto masked) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -683,19 +686,24 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
               for (int e = 0; e < 2; ++e) {
                 float w[2];
 #pragma unroll
+                for (int c = 0; c < 2; ++c) w[c] = fast_exp2(x[k][n][2 * e + c] - m_run[n][c]);
+                const uint32_t rounded = pack16<BF16 && !FOUR>(w[0], w[1]);
+                pf[k][n][e] = transpose_8x8(rounded);
+                float r[2] = {0.0f, 0.0f};
+                if constexpr (FOUR) Pack<__half>::unpack2(rounded, r[0], r[1]);
+#pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                  w[c] = fast_exp2(x[k][n][2 * e + c] - m_run[n][c]);
                   if constexpr (FOUR) {
-                    float prob = w[c] * v_inv[k][e], low = v_low[k][e];
+                    const float prob = w[c] * v_inv[k][e];
+                    float low = v_low[k][e];
                     if constexpr (decltype(masked)::value)
-                      if (x[k][n][2 * e + c] == -INFINITY) prob = low = 0.0f;
+                      if (x[k][n][2 * e + c] == -INFINITY) low = 0.0f;
                     l_run[n][c] += prob;
-                    low_run[n][c] = fmaf(prob, low, low_run[n][c]);
+                    low_run[n][c] = fmaf(8.0f, w[c] - r[c], fmaf(prob, low, low_run[n][c]));
                   } else {
                     l_run[n][c] += w[c];
                   }
                 }
-                pf[k][n][e] = transpose_8x8(pack16<BF16 && !FOUR>(w[0], w[1]));
               }
         };
         if (FOUR && need_mask) weigh(std::true_type{});
