@@ -727,7 +727,9 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
                 for (int i = 0; i < 2; ++i) {
                   const uint32_t f[4] = {a & 0x000F000Fu, a & 0x00F000F0u, c & 0x000F000Fu, c & 0x00F000F0u};
 #pragma unroll
-                  for (int n = 0; n < NT; ++n) mma_16816<false>(o[4 * w + 2 * half + i][n], f, pf[k][n][0], pf[k][n][1]);
+                  for (int n = 0; n < NT; ++n) {
+                    mma_16816<false>(o[4 * w + 2 * half + i][n], f, pf[k][n][0], pf[k][n][1]);
+                  }
                   a >>= 8;
                   c >>= 8;
                 }
@@ -887,7 +889,9 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   for (; read < filled; ++read) {
     const uint64_t t0 = global_ns();
     bool done = false;
-    while (!done && global_ns() - t0 < ATT_WAIT_NS) done = mbar_try_wait(bars + 8 * (read % STAGES), (read / STAGES) & 1);
+    while (!done && global_ns() - t0 < ATT_WAIT_NS) {
+      done = mbar_try_wait(bars + 8 * (read % STAGES), (read / STAGES) & 1);
+    }
     if (!done) atomicOr(p.status, ATT_ST_DRAIN);
   }
 }
