@@ -168,3 +168,69 @@ def test_refusals(cuda):
         with pytest.raises(ValueError, match="expected k"):
             m(x.expand(2, 2, E), past_key_value=c)
     assert c.lengths.tolist() == [0]
+
+
+def test_steps_behind_replays(cuda):
+    """A capture appends nothing; behind its replays, which the host does not see, steps find pages of their own."""
+    m = params_to_bf16(module(cuda))
+    x = torch.randn(1, 40, E, device=cuda).bfloat16()
+    tok = x[:, :1].clone()
+    a, b = (T.PagedKVCache(6, 16, HK, D) for _ in range(2))
+    with torch.no_grad():
+        m(tok, past_key_value=T.PagedKVCache(6, 16, HK, D))
+        b.reserve(16)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(tok, past_key_value=b)[0]
+        assert b.lengths.tolist() == [0]
+        for i in range(16):
+            tok.copy_(x[:, i:i + 1])
+            graph.replay()
+            assert torch.equal(out, m(x[:, i:i + 1], past_key_value=a)[0])
+        for c in (a, b):
+            for i in range(16, 20):
+                y = m(x[:, i:i + 1], past_key_value=c)[0]
+            c.last = y
+    assert torch.equal(a.last, b.last) and b.lengths.tolist() == [20]
+    assert all(torch.equal(s, t) for s, t in zip(a.gather(), b.gather()))
+
+
+def test_a_captured_step_without_room_is_refused(cuda):
+    m = params_to_bf16(module(cuda))
+    tok = torch.randn(1, 1, E, device=cuda).bfloat16()
+    c = T.PagedKVCache(1, 16, HK, D)
+    with torch.no_grad():
+        m(tok, past_key_value=T.PagedKVCache(1, 16, HK, D))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="reserve"):
+                m(tok, past_key_value=c)
+        assert c.lengths.tolist() == [0]
+        m(tok, past_key_value=c)
+    assert c.lengths.tolist() == [1]
+
+
+def test_evaluated_then_trained(cuda):
+    """Tables made in inference mode serve a training step."""
+    m = params_to_bf16(module(cuda, qk_norm=True, fused_qk=True))
+    q, k = (torch.randn(1, 4, h, D, device=cuda).bfloat16() for h in (HQ, HK))
+    with torch.inference_mode():
+        want = m._norm_and_rotate(q, k)
+    a, b = m._norm_and_rotate(q.requires_grad_(), k.requires_grad_())
+    (a.float().sum() + b.float().sum()).backward()
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1]) and q.grad.isfinite().all()
+
+
+def test_generating(cuda):
+    """A prompt through the packed kernel, then a token, into 4 bits; the lines of the README."""
+    x = torch.randn(4, 501, 1024, device=cuda).bfloat16()
+    attn = T.FastGroupedQueryAttention(1024, 8, 2, kernel_type="triton", causal=True,
+                                       position_method="rope").to(cuda).bfloat16()
+    cache = T.PagedKVCache(64, 64, 2, 128, batch_size=4, bits=4)
+    with torch.no_grad():
+        y, _ = attn(x[:4, :500], past_key_value=cache)
+        z, _ = attn(x[:4, 500:501], past_key_value=cache)
+    assert y.shape == (4, 500, 1024) and z.shape == (4, 1, 1024) and bool(y.isfinite().all() and z.isfinite().all())
+    assert cache.lengths.tolist() == [501] * 4

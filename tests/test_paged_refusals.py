@@ -229,3 +229,37 @@ def test_cache_reserves_pages():
     c.release(0)
     c.reserve([0, 64])
     assert (c.block_table >= 0).sum(1).tolist() == [0, 4]
+
+
+@pytest.mark.parametrize("kv,error", [(torch.zeros(2, 1, 2, 64, dtype=torch.float16), TypeError),
+                                      (torch.zeros(2, 1, 3, 64, dtype=torch.bfloat16), ValueError),
+                                      (torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16), ValueError),  # not on CUDA
+                                      (torch.zeros(2), ValueError)], ids=lambda x: str(getattr(x, "shape", x)))
+def test_a_refused_append_leaves_the_cache_as_it_was(kv, error):
+    c = T.PagedKVCache(6, 16, 2, 64, 2, device="cpu", bits=4)
+    with pytest.raises(error):
+        c.append(kv, kv)
+    assert c.lengths.tolist() == [0, 0] and c._held == [0, 0]
+
+
+def test_cache_reads_the_lengths_once_a_step_was_captured():
+    c = T.PagedKVCache(6, 16, 2, 64, 2, device="cpu")
+    c.reserve(16)
+    c.lengths.fill_(16)  # what replays did
+    c._captured = True
+    c.reserve(1)
+    assert (c.block_table >= 0).sum(1).tolist() == [2, 2]
+
+
+def test_long_tables_are_kept():
+    """A captured graph may read tables that later ones are longer than."""
+    rope = T.FastRoPEPositionEmbedding(64, 16)
+    cpu = torch.device("cpu")
+    with torch.inference_mode():
+        short = rope.tables(5, cpu)
+    long = rope.tables(40, cpu)
+    assert short[0].shape == (16, 64) and long[0].shape == (64, 64) and not short[0].is_inference()
+    assert torch.equal(short[0], long[0][:16]) and torch.equal(short[1], long[1][:16])
+    assert rope.tables(16, cpu) is short and rope.tables(50, cpu) is long
+    cos, sin = rope(torch.zeros(1, 64), 40)
+    assert torch.equal(cos, long[0][:40]) and torch.equal(sin, long[1][:40])

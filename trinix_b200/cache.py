@@ -20,8 +20,9 @@ class PagedKVCache:
 
     Which page is whose is kept on the host, with the lengths that the host has reserved room for; the block table
     and the lengths that the kernels read are on the device, so that a step (`reserve` aside) may be captured in a
-    CUDA graph and replayed: reserve the steps' tokens first. bits=4 holds each row of head_dim values in
-    head_dim / 2 + 8 bytes.
+    CUDA graph and replayed: reserve the steps' tokens first. What replays append the host does not see: from the
+    first capture on, `reserve` and an `append` that is not captured read the lengths from the device before they
+    look for room. bits=4 holds each row of head_dim values in head_dim / 2 + 8 bytes.
     """
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, batch_size: int = 1, *,
@@ -50,6 +51,7 @@ class PagedKVCache:
         self._pages: List[List[int]] = [[] for _ in range(batch_size)]
         self._tokens = [0] * batch_size  # that there is room for
         self._held = [0] * batch_size    # that have been appended, as far as the host has seen to it
+        self._captured = False           # a graph may append too
 
     @property
     def batch_size(self) -> int:
@@ -64,6 +66,8 @@ class PagedKVCache:
     def reserve(self, tokens: Union[int, Sequence[int]]) -> None:
         """Make sure that every sequence (or each by its own number) has pages for so many tokens more than it
         holds. Raises, with nothing changed, if the pool or the table's rows have too few."""
+        if self._captured:
+            self.sync()
         more = [tokens] * self.batch_size if isinstance(tokens, int) else list(tokens)
         if len(more) != self.batch_size or min(more) < 0:
             raise ValueError(f"expected {self.batch_size} numbers of tokens, none negative")
@@ -81,7 +85,8 @@ class PagedKVCache:
             self._write_table()
 
     def sync(self) -> None:
-        """Read from the device how many tokens the sequences hold, after replays of captured steps."""
+        """Read from the device how many tokens the sequences hold (after replays of captured steps, or a change of
+        `lengths` from outside)."""
         self._held = self.lengths.tolist()
         self._tokens = [max(t, h) for t, h in zip(self._tokens, self._held)]
 
@@ -105,16 +110,29 @@ class PagedKVCache:
                sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """`ops.append_paged` of k / v (batch, S, heads, head_dim) behind what the sequences hold; pages are
         reserved for them if they have not been (not while a graph is captured). Returns the rotated queries."""
-        new = k.shape[1]
         if k.dim() != 4 or k.shape[0] != self.batch_size:
             raise ValueError(f"expected k ({self.batch_size}, tokens, heads, head_dim), got {tuple(k.shape)}")
+        if k.dtype != self.dtype:
+            raise TypeError(f"the cache is for {self.dtype}, got {k.dtype}")
+        new, capturing = k.shape[1], k.is_cuda and torch.cuda.is_current_stream_capturing()
+        if self._captured and not capturing:
+            self.sync()
         held = [h + new for h in self._held]
         if any(h > t for h, t in zip(held, self._tokens)):
+            if capturing:
+                raise RuntimeError("a captured step finds no room: reserve its replays' tokens before the capture")
             self.reserve(new)
         self.lengths.add_(new)
-        out = ops.append_paged(k, v, self.k_pages, self.v_pages, self.block_table, self.lengths, cos=cos, sin=sin,
-                               q=q, **self._scales())
-        self._held = held
+        try:
+            out = ops.append_paged(k, v, self.k_pages, self.v_pages, self.block_table, self.lengths, cos=cos,
+                                   sin=sin, q=q, **self._scales())
+        except Exception:
+            self.lengths.sub_(new)
+            raise
+        if capturing:
+            self._captured = True  # nothing has run
+        else:
+            self._held = held
         return out
 
     def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, window: Optional[Tuple[int, int]] = None,

@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 
@@ -204,6 +205,7 @@ class _QKNormRoPEFn(torch.autograd.Function):
                                 norm=norm, norm_first=norm_first, positions=positions)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         need, (eps, norm, norm_first) = ctx.needs_input_grad, ctx.how

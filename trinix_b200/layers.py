@@ -324,7 +324,7 @@ class FastRoPEPositionEmbedding(nn.Module):
         self.use_triton = use_triton
         inv_freq = 1.0 / base ** (torch.arange(0, dim, 2).float() / dim)
         self.register_buffer("inv_freq", inv_freq, persistent=False)
-        self._table_key, self._tables, self._wide_tables = None, None, None
+        self._table_key, self._tables, self._wide_tables = None, None, []
 
     def forward(self, x: torch.Tensor, seq_len: Optional[int] = None):
         """(cos, sin) of shape (seq_len, dim) in x's dtype. The angles are always built in
@@ -337,24 +337,36 @@ class FastRoPEPositionEmbedding(nn.Module):
         # a dozen small launches per forward in a decoder stack
         key = (int(seq_len), x.device, x.dtype)
         if self._table_key != key:
-            inv_freq = 1.0 / self.base ** (
-                torch.arange(0, self.dim, 2, device=x.device, dtype=torch.float32) / self.dim)
-            pos = torch.arange(seq_len, device=x.device, dtype=torch.float32)
-            angles = torch.outer(pos, inv_freq)
-            table = torch.cat((angles, angles), dim=-1)
-            self._tables = (table.cos().to(x.dtype), table.sin().to(x.dtype))
+            self._tables = self._build(*key)
             self._table_key = key
         return self._tables
 
+    def _build(self, rows: int, device: torch.device, dtype: torch.dtype):
+        inv_freq = 1.0 / self.base ** (
+            torch.arange(0, self.dim, 2, device=device, dtype=torch.float32) / self.dim)
+        pos = torch.arange(rows, device=device, dtype=torch.float32)
+        angles = torch.outer(pos, inv_freq)
+        table = torch.cat((angles, angles), dim=-1)
+        return table.cos().to(dtype), table.sin().to(dtype)
+
     def tables(self, seq_len: int, device: torch.device):
         """(cos, sin) of forward in fp32, of at least max_position_embeddings positions: what the kernels that
-        look a token's position up take."""
+        look a token's position up take. Kept as long as the module, since a captured graph may read them; longer
+        ones are of a power of two, so that they are few."""
         rows = max(seq_len, self.max_position_embeddings)
-        if self._wide_tables is None or self._wide_tables[0].shape[0] < rows or self._wide_tables[0].device != device:
-            key, kept = self._table_key, self._tables
-            self._wide_tables = self.forward(torch.empty(0, device=device), rows)
-            self._table_key, self._tables = key, kept
-        return self._wide_tables
+        for kept in self._wide_tables:
+            if kept[0].device == device and kept[0].shape[0] >= rows:
+                return kept
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            return self._build(rows, device, torch.float32)  # the graph's own: there is nothing in them yet
+        if rows > self.max_position_embeddings:
+            rows = 1 << (rows - 1).bit_length()
+        with torch.inference_mode(False), torch.no_grad():  # a training step may save them
+            made = self._build(rows, device, torch.float32)
+        if device.type == "cuda":
+            torch.cuda.current_stream(device).synchronize()  # the next call may be on another stream
+        self._wide_tables.append(made)
+        return made
 
     @staticmethod
     def _rotate_half(x: torch.Tensor) -> torch.Tensor:
