@@ -98,7 +98,7 @@ struct PgShape {
   static constexpr int RUNS = KEYS / PG_RUN;
   static constexpr int STEP = FOUR ? 32 : 16;  // keys that a warp works on at a time
   static constexpr int STAGES = FOUR ? 2 : 3;
-    static constexpr int CTAS_PER_SM = FOUR && (NT == 1 || D == 64) ? 3 : 2;
+  static constexpr int CTAS_PER_SM = FOUR && (NT == 1 || D == 64) ? 3 : 2;
   static constexpr int CODES = PG_RUN * D / 2, SCALES = PG_RUN * 8;  // bytes of 16 keys
   // a tile's K codes, V codes, K scales, V scales
   static constexpr int V_OFF = RUNS * CODES, KS_OFF = 2 * V_OFF, VS_OFF = KS_OFF + RUNS * SCALES;
