@@ -1,0 +1,79 @@
+"""Attention over a paged cache: what becomes of the weights between the two products, of keys that a query does not
+see, and of calls at the borders of their arguments."""
+import pytest
+import torch
+
+import trinix_b200 as T
+from tests.paged_ref import make_cache
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(values, dev):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def two_kinds_of_keys(cuda, scores, n, bits, dtype, dim=64, big=1.0, heads=4):
+    """A sequence to each of `scores`, of n keys: the first has score 0 for the query (1, 0, 0, ..), all others the
+    sequence's own; the first value is 0 (column 1: `big`), the others `big` (column 1: 0)."""
+    c = make_cache([n] * len(scores), 1, 16, dim, bits, dtype, cuda)
+    exact = torch.tensor(scores, dtype=torch.float64).to(dtype).double()  # as the cache holds them
+    for b, s in enumerate(exact.tolist()):
+        pages = c["block_table"][b].long()
+        place = lambda x, first, rest: (c[x].index_fill_(0, pages, rest), c[x][pages[0], :, 0].fill_(first))  # noqa: E731
+        if bits == 16:
+            place("k_pages", 0.0, s)
+            place("v_pages", 0.0, big)
+            c["v_pages"][pages, ..., 1] = 0.0
+            c["v_pages"][pages[0], :, 0, 1] = big
+        else:
+            for x in "kv":
+                c[x + "_pages"][pages] = 0
+                c[x + "_scales"][pages] = 0.0
+            c["k_scales"][pages, ..., 1] = s
+            c["k_scales"][pages[0], :, 0] = 0.0
+            c["v_scales"][pages, ..., 0] = big / 16
+            c["v_pages"][pages] = 0xFF
+            c["v_pages"][pages, ..., 0] = 0x0F       # column 1 in the high bits
+            c["v_pages"][pages[0], :, 0] = 0
+            c["v_pages"][pages[0], :, 0, 0] = 0xF0
+    q = torch.zeros(len(scores), 1, heads, dim, device=cuda, dtype=dtype)
+    q[..., 0] = 1.0
+    out = T.attention_paged(q, **c, lengths=i32([n] * len(scores), cuda), scale=1.0)
+    w = exact.to(cuda).exp()
+    high = big if bits == 16 else 15 * big / 16
+    rest, first = (high * t / (1 + (n - 1) * w) for t in ((n - 1) * w, torch.ones_like(w)))
+    want = rest[:, None].expand(len(scores), dim).clone()
+    want[:, 1] = first
+    return out[:, 0], want[:, None]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("n,dim,heads", [(40, 64, 1), (40, 128, 4), (2000, 64, 4), (40, 128, 7), (2000, 64, 16)])
+def test_weights_are_not_rounded_to_the_cache_s_type(cuda, n, dim, heads, dtype, bits):
+    """The result is the definition's, rounded, but for fp32 errors: all of the keys but one have the same weight, so that
+    a rounding of weights is an error of the result. With y the result before its rounding, |out - exact| is at most
+    |round(exact) - exact| + 2 |y - exact|. The latter, relative to weights times values: a weight as two numbers of 16
+    bits, 2^-16; the score, the maximum and their difference, up to 6 in size, and exp2, 32 2^-24; the fp32 sums, a lane's
+    n / 32 terms and the matrix unit's n / 64 steps of two products, which may cut instead of round, and 32 more for
+    the sums of lanes, warps and parts; the same again for the normaliser."""
+    out, want = two_kinds_of_keys(cuda, [-i / 16 for i in range(64)], n, bits, dtype, dim, heads=heads)
+    y = 2.0 ** -16 + 2 * (64 + n / 32 + 4 * n / 64) * 2.0 ** -24
+    allowed = (want.to(dtype).double() - want).abs() + 2 * y * want.abs()
+    off = (out.double() - want).abs()
+    assert not (off > allowed).any(), float((off / allowed).max())
+    assert T.attention_status(cuda) == 0
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_many_small_weights_count(cuda, dtype, bits):
+    """4096 keys of weights around 2^-26 beside one of 1. fp16 operands lose what is below 2^-32 of a key, half of the
+    smallest step of them below the scale of 2^7: 4096 2^-32 of the values. Errors as above, scores up to 20 in size."""
+    n = 4097
+    out, want = two_kinds_of_keys(cuda, [-17.0, -18.0, -18.5, -19.0], n, bits, dtype, big=1024.0)
+    y = 2.0 ** -16 + 2 * (256 + n / 32 + 4 * n / 64) * 2.0 ** -24
+    allowed = (want.to(dtype).double() - want).abs() + 2 * y * want.abs() + n * 2.0 ** -32 * 1024.0
+    off = (out.double() - want).abs()
+    assert not (off > allowed).any(), float((off / allowed).max())

@@ -109,6 +109,14 @@ extern "C" int trx_attn_fwd_paged(const void* q, const void* k_pages, const void
   return paged_shape(D, four, rows, [&](auto d, auto bits, auto nt) {
     constexpr int DIM = decltype(d)::value, NT = decltype(nt)::value;
     constexpr bool FOUR = decltype(bits)::value;
-    return bf16 ? launch_paged<DIM, true, FOUR, NT>(p, plan, s) : launch_paged<DIM, false, FOUR, NT>(p, plan, s);
+    auto launch = [&](auto twice) {
+      constexpr bool TWICE = decltype(twice)::value;
+      return bf16 ? launch_paged<DIM, true, FOUR, NT, TWICE>(p, plan, s)
+                  : launch_paged<DIM, false, FOUR, NT, TWICE>(p, plan, s);
+    };
+    if constexpr (NT == 1) {
+      if (rows <= 4) return launch(std::true_type{});
+    }
+    return launch(std::false_type{});
   });
 }

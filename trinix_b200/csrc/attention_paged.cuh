@@ -33,8 +33,9 @@
 //     then the four V rows that a load reads are neighbours.
 //   * fp16 operands serve both activation types: Q's rows are scaled by a power of two to below 2^14 (what is
 //     2^-28 of the row's largest value or more stays exact; a row with values of 2^114 and more is not a number).
-//     Probabilities are weighed with step_v before they are rounded to 11 bits, and the running maximum is that of
-//     the weighed ones, so that the largest weight of a row is of the order of 1 whatever the steps are.
+//     Probabilities are weighed with step_v before they become fp16, two numbers each, and the running
+//     maximum is that of the weighed ones, so that the largest weight of a row is of the order of 1 whatever the steps
+//     are.
 // Scores, sums and O are fp32.
 //
 // Measured (32 / 8 heads x 128, one token to a sequence): 48 sequences of 128 to 8192 keys, 16 bits, 385 MB: 70.5 us,
@@ -62,6 +63,9 @@ constexpr int PG_MOST_CTAS = 1024;  // of a launch that cuts units
 constexpr float PG_LEAST_STEP = 0x1p-80f;
 // The reference maximum of a row that has seen nothing: finite, so that no difference of it is not a number.
 constexpr float PG_NOTHING = -1e30f;
+// fp16 weights are 2^7 times what the reference maximum makes of them, so that those of 2^-31 of it and more are not
+// lost; with ATT_LAZY_RESCALE they stay below 2^15.
+constexpr float PG_FP16_UP = 7.0f, PG_FP16_SCALE = 0x1p7f;
 
 // What a CTA of the first launch leaves for the second one: the unit that it found begun, if there is one.
 struct PagedPiece {
@@ -202,7 +206,8 @@ __device__ __forceinline__ void paged_emit(const PagedParams& p, int b, int head
         l == 0.0f ? -INFINITY : (mx + log2f(l)) * 0.6931471805599453f;
 }
 
-template <int D, bool BF16, bool FOUR, int NT>
+// TWICE: at most four rows, which have two of the tile's eight columns each (see the weights below).
+template <int D, bool BF16, bool FOUR, int NT, bool TWICE>
 __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     attn_paged_kernel(const __grid_constant__ PagedParams p) {
   using L = PgShape<D, FOUR, NT>;
@@ -428,6 +433,9 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
   };
   auto tiles_of = [&](const Unit& u) { return u.valid ? max(0, (u.t1 - u.t0 - warp + PG_WARPS - 1) / PG_WARPS) : 0; };
 
+  // (the sum of 4 bits goes by 1 / step_v, which has the factor)
+  constexpr bool FP16_WEIGHTS = FOUR || !BF16;
+  constexpr float O_DOWN = FP16_WEIGHTS ? 1.0f / PG_FP16_SCALE : 1.0f, L_DOWN = FOUR ? 1.0f : O_DOWN;
   const float sl2 = p.scale_log2;
   const bool has_alibi = p.slopes != nullptr;
   const int key_of_row = FOUR ? (g8 >> 1) + ((g8 & 1) << 2) : g8;  // 4 bits: 0, 4, 1, 5, 2, 6, 3, 7
@@ -465,7 +473,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
     int row_at[NT][2];                                 // their positions
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = u.r0 + 8 * n + g8;
+      const int r = u.r0 + 8 * n + (TWICE ? g8 & 3 : g8);
       const bool live = r < rows;
       const int rr = live ? r : rows - 1, token = paged_token(p, rr);
       const int h = u.head * p.group + rr - token * p.group;
@@ -602,7 +610,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
               const float v_step = fmaxf(vs.x, PG_LEAST_STEP);
               float log_step;
               asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(log_step) : "f"(v_step));
-              asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inv[k][e]) : "f"(v_step));
+              asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inv[k][e]) : "f"(v_step * PG_FP16_SCALE));
               v_low[k][e] = vs.y;
 #pragma unroll
               for (int n = 0; n < NT; ++n)
@@ -672,11 +680,13 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
               }
             }
         }
-        uint32_t pf[SUBS][NT][2];
-        // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there. What the
-        // rounding takes off a weight goes in with the code 8: only codes' distances from that, their spread, meet the
-        // rounded weight. (Without, the roundings count with the codes' mean: fp16, 24 x 5 rows behind 46 to 3001 keys
-        // 3.3e-4 off the definition instead of 2.5e-4, of which the output's own type is 2.1e-4.)
+        // The weights of the second product, and what their rounding takes off them, in a product of its own, or, where
+        // a row has two columns, in the second one: the two together are within 2^-16 (fp16: 2^-22) of the fp32
+        // weight, which the sum has whole. (64 sequences, 4 bits: 44.7 us with two columns to a row, 47.3 with a second
+        // product, 44.4 with rounded weights alone; 48 sequences of 16 bits 71.8, 71.2, 70.6. Rounded weights alone are
+        // up to a third farther off the definition than the output's own type.)
+        // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there.
+        uint32_t pf[SUBS][NT][2], pr[SUBS][NT][2];
         auto weigh = [&](auto masked) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -684,13 +694,20 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
             for (int k = 0; k < SUBS; ++k)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                float w[2];
+                float w[2], r[2];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) w[c] = fast_exp2(x[k][n][2 * e + c] - m_run[n][c]);
-                const uint32_t rounded = pack16<BF16 && !FOUR>(w[0], w[1]);
-                pf[k][n][e] = transpose_8x8(rounded);
-                float r[2] = {0.0f, 0.0f};
-                if constexpr (FOUR) Pack<__half>::unpack2(rounded, r[0], r[1]);
+                for (int c = 0; c < 2; ++c)
+                  w[c] = fast_exp2(x[k][n][2 * e + c] - (FP16_WEIGHTS ? m_run[n][c] - PG_FP16_UP : m_run[n][c]));
+                const uint32_t rounded = pack16<!FP16_WEIGHTS>(w[0], w[1]);
+                if constexpr (FP16_WEIGHTS) {
+                  Pack<__half>::unpack2(rounded, r[0], r[1]);
+                } else {
+                  r[0] = __uint_as_float(rounded << 16);
+                  r[1] = __uint_as_float(rounded & 0xffff0000u);
+                }
+                const uint32_t rest = pack16<!FP16_WEIGHTS>(w[0] - r[0], w[1] - r[1]);
+                pf[k][n][e] = transpose_8x8(TWICE && t4 >= 2 ? rest : rounded);
+                if constexpr (!TWICE) pr[k][n][e] = transpose_8x8(rest);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                   if constexpr (FOUR) {
@@ -699,7 +716,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
                     if constexpr (decltype(masked)::value)
                       if (x[k][n][2 * e + c] == -INFINITY) low = 0.0f;
                     l_run[n][c] += prob;
-                    low_run[n][c] = fmaf(8.0f, w[c] - r[c], fmaf(prob, low, low_run[n][c]));
+                    low_run[n][c] = fmaf(prob, low, low_run[n][c]);
                   } else {
                     l_run[n][c] += w[c];
                   }
@@ -729,6 +746,7 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     mma_16816<false>(o[4 * w + 2 * half + i][n], f, pf[k][n][0], pf[k][n][1]);
+                    if constexpr (!TWICE) mma_16816<false>(o[4 * w + 2 * half + i][n], f, pr[k][n][0], pr[k][n][1]);
                   }
                   a >>= 8;
                   c >>= 8;
@@ -753,7 +771,10 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 #pragma unroll
               for (int i = 0; i < 4; ++i) f[i] &= keep[i >> 1];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816<BF16>(o[m][n], f, pf[0][n][0], pf[0][n][1]);
+            for (int n = 0; n < NT; ++n) {
+              mma_16816<BF16>(o[m][n], f, pf[0][n][0], pf[0][n][1]);
+              if constexpr (!TWICE) mma_16816<BF16>(o[m][n], f, pr[0][n][0], pr[0][n][1]);
+            }
           }
         }
       }
@@ -785,19 +806,20 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
           l += __shfl_xor_sync(0xffffffffu, l, w);
           if constexpr (FOUR) low += __shfl_xor_sync(0xffffffffu, low, w);
         }
+        if (TWICE && t4 >= 2) low = 0.0f;  // the row's other column has it
         if (g8 == 0) {
           ml[warp * L::ROWS + 8 * n + r] = m_run[n][c];
-          ml[(PG_WARPS + warp) * L::ROWS + 8 * n + r] = l;
+          ml[(PG_WARPS + warp) * L::ROWS + 8 * n + r] = l * L_DOWN;
         }
         if (ok)
 #pragma unroll
           for (int m = 0; m < MTILES; ++m) {
             if constexpr (FOUR) {  // columns 2 m, 2 m + 1 of this lane's D / 8
               *reinterpret_cast<float2*>(ow + r * D + ((g8 * (D / 8) + 2 * m) ^ swap)) =
-                  make_float2(fmaf(o[m][n][c], 0x1p24f, low), fmaf(o[m][n][2 + c], 0x1p20f, low));
+                  make_float2(fmaf(o[m][n][c], 0x1p24f * O_DOWN, low), fmaf(o[m][n][2 + c], 0x1p20f * O_DOWN, low));
             } else {
-              ow[r * D + ((16 * m + g8) ^ swap)] = o[m][n][c];
-              ow[r * D + ((16 * m + 8 + g8) ^ swap)] = o[m][n][2 + c];
+              ow[r * D + ((16 * m + g8) ^ swap)] = o[m][n][c] * O_DOWN;
+              ow[r * D + ((16 * m + 8 + g8) ^ swap)] = o[m][n][2 + c] * O_DOWN;
             }
           }
       }
@@ -821,9 +843,12 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 #pragma unroll
       for (int w = 0; w < PG_WARPS; ++w) {
         const float f = fast_exp2(ml[w * L::ROWS + r] - top);
-        const float4 v = *reinterpret_cast<const float4*>(
-            reinterpret_cast<const float*>(smem + o_at[w * NT + (r >> 3)]) + (r & 7) * D +
-            ((4 * c4) ^ (((r & 7) >> 1) << 3)));
+        const float* from = reinterpret_cast<const float*>(smem + o_at[w * NT + (r >> 3)]);
+        float4 v = *reinterpret_cast<const float4*>(from + (r & 7) * D + ((4 * c4) ^ (((r & 7) >> 1) << 3)));
+        if constexpr (TWICE) {
+          const float4 rest = *reinterpret_cast<const float4*>(from + (r + 4) * D + ((4 * c4) ^ (((r + 4) >> 1) << 3)));
+          v = make_float4(v.x + rest.x, v.y + rest.y, v.z + rest.z, v.w + rest.w);
+        }
         l = fmaf(f, ml[(PG_WARPS + w) * L::ROWS + r], l);
         acc.x = fmaf(f, v.x, acc.x);
         acc.y = fmaf(f, v.y, acc.y);
@@ -1030,10 +1055,10 @@ static PagedPlan paged_plan(int64_t units, int64_t keys) {
   return plan;
 }
 
-template <int D, bool BF16, bool FOUR, int NT>
+template <int D, bool BF16, bool FOUR, int NT, bool TWICE>
 static int launch_paged(PagedParams& p, const PagedPlan& plan, cudaStream_t stream) {
   using L = PgShape<D, FOUR, NT>;
-  auto kernel = attn_paged_kernel<D, BF16, FOUR, NT>;
+  auto kernel = attn_paged_kernel<D, BF16, FOUR, NT, TWICE>;
   static std::atomic<bool> configured[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return TRX_ERR_CUDA;
