@@ -138,14 +138,18 @@ class PagedKVCache:
     def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, window: Optional[Tuple[int, int]] = None,
                alibi_slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of the last tokens q (batch, S, heads, head_dim) over the cache: `ops.attention_paged`
-        for few of them, else the cache's rows packed (`ops.gather_paged`) and `ops.attention_packed`."""
+        for few of them, else the cache's rows packed (`ops.gather_paged`) and `ops.attention_packed`. Captured in a
+        graph, the latter packs all that the batch may ever hold, since its replays may find more pages in use."""
         B, S, Hq, D = q.shape
         if S <= self.LONG:
             return ops.attention_paged(q, self.k_pages, self.v_pages, self.block_table, self.lengths, scale=scale,
                                        window=window, alibi_slopes=alibi_slopes, **self._scales())
         starts = self._starts()
         # room for all that the sequences' pages hold, whatever the host has seen of the lengths
-        k, v = self._gather(starts, sum(len(p) for p in self._pages) * self.page_size)
+        pages = sum(len(p) for p in self._pages)
+        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+            pages = min(self.k_pages.shape[0], self.batch_size * self.max_pages)
+        k, v = self._gather(starts, pages * self.page_size)
         rows = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=q.device)
         out = ops.attention_packed(q.reshape(B * S, Hq, D), k, v, rows, starts, causal=True, scale=scale,
                                    window=None if window is None else (window[0], 0), alibi_slopes=alibi_slopes)
