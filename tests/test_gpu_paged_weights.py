@@ -77,3 +77,49 @@ def test_many_small_weights_count(cuda, dtype, bits):
     allowed = (want.to(dtype).double() - want).abs() + 2 * y * want.abs() + n * 2.0 ** -32 * 1024.0
     off = (out.double() - want).abs()
     assert not (off > allowed).any(), float((off / allowed).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("window", [None, (5, 0)], ids=str)
+@pytest.mark.parametrize("Sq,heads,dim", [(3, 1, 64), (4, 2, 128), (9, 4, 64), (2, 4, 128), (5, 6, 128)])
+def test_values_that_a_query_does_not_see_may_be_anything(cuda, Sq, heads, dim, window, dtype):
+    """16 bits: an infinite value or one that is not a number counts for the queries that see its key, and for no other
+    one of the same tile: those of earlier drafted tokens, those that a window has left it behind."""
+    lengths, page = [50, 37, 16, 400], 16
+    c = make_cache(lengths, 1, page, dim, 16, dtype, cuda)
+    q = torch.randn(len(lengths), Sq, heads, dim, generator=torch.Generator(device=cuda).manual_seed(1), device=cuda).to(dtype)
+    call = dict(lengths=i32(lengths, cuda), window=window)
+    want = T.attention_paged(q, **c, **call)
+    rows = torch.arange(Sq)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        for back in (1, 2, Sq + 4):  # the last key, the one before it, one that a window of 5 has left behind for the last query
+            now = {n: t.clone() for n, t in c.items()}
+            for b, n in enumerate(lengths):
+                at = n - back
+                now["v_pages"][int(c["block_table"][b, at // page]), 0, at % page, 3] = bad
+            got = T.attention_paged(q, **now, **call)
+            for b, n in enumerate(lengths):
+                here = rows + n - Sq
+                sees = (n - back <= here) & ((n - back >= here - 5) if window else True)
+                assert torch.equal(got[b, ~sees], want[b, ~sees])
+                assert torch.equal(got[b, sees][..., :3], want[b, sees][..., :3])
+                hit = got[b, sees][..., 3]
+                assert hit.isnan().all() if bad != bad else (hit == bad).all()
+    assert T.attention_status(cuda) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("heads,n", [(1, 5), (4, 300), (7, 300), (24, 300), (4, 20000), (7, 20000)])
+def test_infinite_values_stay_infinite(cuda, heads, n, dtype):
+    c = make_cache([n], 1, 16, 64, 16, dtype, cuda)
+    q = torch.randn(1, 1, heads, 64, generator=torch.Generator(device=cuda).manual_seed(1), device=cuda).to(dtype) / 8
+    want = T.attention_paged(q, **c, lengths=i32([n], cuda))
+    for bad, at in ((float("inf"), 0), (float("-inf"), n - 1), (float("inf"), n // 2)):
+        v = c["v_pages"][int(c["block_table"][0, at // 16]), 0, at % 16]
+        held = v.clone()
+        v[7] = bad
+        got = T.attention_paged(q, **c, lengths=i32([n], cuda))
+        v.copy_(held)
+        assert (got[..., 7] == bad).all()
+        got[..., 7] = want[..., 7]
+        assert torch.equal(got, want)

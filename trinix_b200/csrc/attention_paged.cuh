@@ -145,6 +145,14 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
+// (lo, hi) as 16-bit numbers that are not larger, for those that are not negative.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16_below(float lo, float hi) {
+  if constexpr (BF16) return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+  uint32_t d;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
 template <int WORDS>
 __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[WORDS]) {
   static_assert(WORDS == 1 || WORDS == 2 || WORDS == 4, "one load");
@@ -685,6 +693,8 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
         // weight, which the sum has whole. (64 sequences, 4 bits: 44.7 us with two columns to a row, 47.3 with a second
         // product, 44.4 with rounded weights alone; 48 sequences of 16 bits 71.8, 71.2, 70.6. Rounded weights alone are
         // up to a third farther off the definition than the output's own type.)
+        // 16 bits: both are above 0, so that an infinite value stays infinite (down to weights of 2^-10, in fp16, where
+        // the second one may be 0).
         // 4 bits: a key that a row does not see may be anything, behind the last one there is what was there.
         uint32_t pf[SUBS][NT][2], pr[SUBS][NT][2];
         auto weigh = [&](auto masked) {
@@ -698,15 +708,17 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
                   w[c] = fast_exp2(x[k][n][2 * e + c] - (FP16_WEIGHTS ? m_run[n][c] - PG_FP16_UP : m_run[n][c]));
-                const uint32_t rounded = pack16<!FP16_WEIGHTS>(w[0], w[1]);
+                const uint32_t first = FOUR ? pack16<false>(w[0], w[1]) : pack16_below<BF16>(w[0], w[1]);
                 if constexpr (FP16_WEIGHTS) {
-                  Pack<__half>::unpack2(rounded, r[0], r[1]);
+                  Pack<__half>::unpack2(first, r[0], r[1]);
                 } else {
-                  r[0] = __uint_as_float(rounded << 16);
-                  r[1] = __uint_as_float(rounded & 0xffff0000u);
+                  r[0] = __uint_as_float(first << 16);
+                  r[1] = __uint_as_float(first & 0xffff0000u);
                 }
-                const uint32_t rest = pack16<!FP16_WEIGHTS>(w[0] - r[0], w[1] - r[1]);
-                pf[k][n][e] = transpose_8x8(TWICE && t4 >= 2 ? rest : rounded);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) r[c] = FOUR ? w[c] - r[c] : fmaxf(w[c] - r[c], w[c] * 0x1p-22f);
+                const uint32_t rest = pack16<!FP16_WEIGHTS>(r[0], r[1]);
+                pf[k][n][e] = transpose_8x8(TWICE && t4 >= 2 ? rest : first);
                 if constexpr (!TWICE) pr[k][n][e] = transpose_8x8(rest);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -754,27 +766,70 @@ __global__ void __launch_bounds__(PG_THREADS, PgShape<D, FOUR, NT>::CTAS_PER_SM)
               }
           }
         } else {
-          // V behind the sequence's last key may be anything: keys 2 t4, 2 t4 + 1 of either half, if they are its
-          uint32_t keep[2];
+          // V of keys that no row sees may be anything: of keys 2 t4, 2 t4 + 1 of either half, those that `first` to
+          // `last` has
+          auto seen = [&](int first, int last, uint32_t (&keep)[2]) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int left = u.sk - c0 - 8 * e - 2 * t4;
-            keep[e] = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
-          }
+            for (int e = 0; e < 2; ++e) {
+              const int j = c0 + 8 * e + 2 * t4;
+              keep[e] = (j >= first && j <= last ? 0xffffu : 0u) | (j + 1 >= first && j < last ? 0xffff0000u : 0u);
+            }
+          };
           const int key = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
-#pragma unroll
-          for (int m = 0; m < MTILES; ++m) {
-            uint32_t f[4];
+          auto values = [&](int m, const uint32_t (&keep)[2], uint32_t (&f)[4]) {
             const int col = (m % 4) * 2 + half;
             ldsm_x4_trans(tile + L::HALF_BYTES + (m / 4) * L::CHUNK_BYTES + key * 128 + ((col ^ (lane & 7)) << 4), f);
             if (need_mask)
 #pragma unroll
               for (int i = 0; i < 4; ++i) f[i] &= keep[i >> 1];
+          };
+          uint32_t keep[2];
+          if (need_mask) seen(p.win_left >= 0 ? u.hi_min - p.win_left : 0, u.hi, keep);
+          // where rows see different keys, a value that is not finite would reach those that do not see it, as 0 times it
+          bool odd = false;
+          if (need_mask && u.hi != u.hi_min) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma_16816<BF16>(o[m][n], f, pf[0][n][0], pf[0][n][1]);
-              if constexpr (!TWICE) mma_16816<BF16>(o[m][n], f, pr[0][n][0], pr[0][n][1]);
+            for (int m = 0; m < MTILES; ++m) {
+              constexpr uint32_t EXPONENT = BF16 ? 0x7F80u : 0x7C00u;
+              uint32_t f[4];
+              values(m, keep, f);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                odd = odd || (f[i] & EXPONENT) == EXPONENT || (f[i] >> 16 & EXPONENT) == EXPONENT;
             }
+            odd = __any_sync(0xffffffffu, odd);
+          }
+          if (!odd) {
+#pragma unroll
+            for (int m = 0; m < MTILES; ++m) {
+              uint32_t f[4];
+              values(m, keep, f);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma_16816<BF16>(o[m][n], f, pf[0][n][0], pf[0][n][1]);
+                if constexpr (!TWICE) mma_16816<BF16>(o[m][n], f, pr[0][n][0], pr[0][n][1]);
+              }
+            }
+          } else {  // a row at a time, with the values that it sees
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll 1
+              for (int r = 0; r < 8; ++r) {
+                const int at = __shfl_sync(0xffffffffu, r & 1 ? row_at[n][1] : row_at[n][0], r >> 1);
+                seen(p.win_left >= 0 ? at - p.win_left : 0, at, keep);
+                const bool mine = t4 == r >> 1;
+#pragma unroll
+                for (int m = 0; m < MTILES; ++m) {
+                  uint32_t f[4];
+                  float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                  values(m, keep, f);
+                  mma_16816<BF16>(d, f, pf[0][n][0], pf[0][n][1]);
+                  if constexpr (!TWICE) mma_16816<BF16>(d, f, pr[0][n][0], pr[0][n][1]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (mine && (i & 1) == (r & 1)) o[m][n][i] += d[i];
+                }
+              }
           }
         }
       }
