@@ -54,3 +54,74 @@ def test_captured_pieces_behind_pages_reserved_later(cuda, bits):
         assert torch.equal(a.lengths, b.lengths)
         assert torch.equal(out, want), i
     assert T.attention_status(cuda) == 0
+
+
+def step(c, t, S=1):
+    q, k, v = (x[:, :S] for x in t)
+    c.append(k, v)
+    return c.attend(q)
+
+
+@pytest.mark.parametrize("S", [1, 3, 40])
+def test_an_idle_place_takes_no_part(cuda, S):
+    """The others' steps are what they were; its own queries see nothing; it costs no pages."""
+    a, b = T.PagedKVCache(20, 16, HK, D, 3), T.PagedKVCache(18, 16, HK, D, 2)
+    first = tokens(cuda, 3, 20)
+    step(a, first, 20)
+    step(b, [x[::2] for x in first], 20)
+    a.release(1, idle=True)
+    for i in range(3):
+        t = tokens(cuda, 3, S, seed=i + 1)
+        got, want = step(a, t, S), step(b, [x[::2] for x in t], S)
+        assert torch.equal(got[::2], want) and not got[1].any()
+    assert a.lengths.tolist() == [20 + 3 * S, 0, 20 + 3 * S]
+    assert all(torch.equal(x, y) for x, y in zip(a.gather(), b.gather()))
+    a.reserve([0, 1, 0])
+    assert step(a, first).shape == (3, 1, HQ, D) and a.lengths.tolist()[1] == 1
+
+
+def test_replays_pass_a_released_place_over(cuda):
+    """Its length stays 0, what the next sequence there sees is its own."""
+    a, b = (T.PagedKVCache(12, 16, HK, D, 2) for _ in range(2))
+    t = tokens(cuda, 2, 1)
+    step(T.PagedKVCache(4, 16, HK, D, 2), t)
+    b.reserve(40)
+    graph, out = captured(lambda: step(b, t))
+
+    def both(seed):
+        for x, y in zip(t, tokens(cuda, 2, 1, seed=seed)):
+            x.copy_(y)
+        graph.replay()
+        return step(a, t)
+
+    for i in range(5):
+        assert torch.equal(out, both(i))
+    for c in (a, b):
+        c.release(0, idle=True)
+    for i in range(5, 10):
+        want = both(i)
+        assert torch.equal(out, want) and not out[0].any()
+        assert a.lengths.tolist() == b.lengths.tolist() == [0, i + 1]
+    for c in (a, b):
+        c.reserve([20, 20])
+    for i in range(10, 14):
+        assert torch.equal(out, both(i))
+    assert a.lengths.tolist() == b.lengths.tolist() == [4, 14]
+    assert all(torch.equal(x, y) for x, y in zip(a.gather(), b.gather()))
+
+
+def test_replays_behind_what_was_reserved_are_told(cuda):
+    c = T.PagedKVCache(4, 16, HK, D, 1)
+    t = tokens(cuda, 1, 1)
+    step(T.PagedKVCache(4, 16, HK, D, 1), t)
+    c.reserve(16)
+    graph, _ = captured(lambda: step(c, t))
+    for _ in range(17):
+        graph.replay()
+    for call in (c.sync, lambda: c.reserve(1), lambda: step(c, t)):
+        with pytest.raises(RuntimeError, match="lost"):
+            call()
+    c.lengths.fill_(16)
+    step(c, t)
+    assert c.lengths.tolist() == [17]
+    assert T.attention_status(cuda) == 0

@@ -22,7 +22,8 @@ class PagedKVCache:
     and the lengths that the kernels read are on the device, so that a step (`reserve` aside) may be captured in a
     CUDA graph and replayed: reserve the steps' tokens first. What replays append the host does not see: from the
     first capture on, `reserve` and an `append` that is not captured read the lengths from the device before they
-    look for room. bits=4 holds each row of head_dim values in head_dim / 2 + 8 bytes.
+    look for room. A place of the batch without pages takes no tokens: its length stays 0, nothing of it is written,
+    and its queries get 0. bits=4 holds each row of head_dim values in head_dim / 2 + 8 bytes.
     """
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, batch_size: int = 1, *,
@@ -45,12 +46,16 @@ class PagedKVCache:
             self.k_scales, self.v_scales = (torch.zeros((*shape[:3], 2), dtype=torch.float32, device=device)
                                             for _ in range(2))
         self.max_pages = num_pages if max_pages is None else max_pages
-        self.block_table = torch.full((batch_size, self.max_pages), -1, dtype=torch.int32, device=device)
+        # a place's row: whether it has pages, then which
+        self._table = torch.full((batch_size, 1 + self.max_pages), -1, dtype=torch.int32, device=device)
+        self._table[:, 0] = 0
+        self._in_use, self.block_table = self._table[:, 0], self._table[:, 1:]
         self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(batch_size)]
         self._tokens = [0] * batch_size  # that there is room for
         self._held = [0] * batch_size    # that have been appended, as far as the host has seen to it
+        self._idle = [False] * batch_size
         self._captured = False           # a graph may append too
 
     @property
@@ -65,10 +70,11 @@ class PagedKVCache:
     # -- pages ----------------------------------------------------------------------------------
     def reserve(self, tokens: Union[int, Sequence[int]]) -> None:
         """Make sure that every sequence (or each by its own number) has pages for so many tokens more than it
-        holds. Raises, with nothing changed, if the pool or the table's rows have too few."""
+        holds. Raises, with nothing changed, if the pool or the table's rows have too few. One number for all leaves
+        idle places out; one of its own, above 0, ends a place's being idle."""
         if self._captured:
             self.sync()
-        more = [tokens] * self.batch_size if isinstance(tokens, int) else list(tokens)
+        more = [0 if i else tokens for i in self._idle] if isinstance(tokens, int) else list(tokens)
         if len(more) != self.batch_size or min(more) < 0:
             raise ValueError(f"expected {self.batch_size} numbers of tokens, none negative")
         want = [max(t, h + n) for t, h, n in zip(self._tokens, self._held, more)]
@@ -78,6 +84,7 @@ class PagedKVCache:
             raise RuntimeError(f"{missing} pages more are needed and {max(need)} for one sequence: the cache has "
                                f"{len(self._free)} free ones and room for {self.max_pages}")
         self._tokens = want
+        self._idle = [i and n == 0 for i, n in zip(self._idle, more)]
         if missing:
             for p, n in zip(self._pages, need):
                 while len(p) < n:
@@ -86,21 +93,29 @@ class PagedKVCache:
 
     def sync(self) -> None:
         """Read from the device how many tokens the sequences hold (after replays of captured steps, or a change of
-        `lengths` from outside)."""
-        self._held = self.lengths.tolist()
+        `lengths` from outside). Raises for one that is longer than its pages: tokens of it have been lost."""
+        held = self.lengths.tolist()
+        over = [b for b, (h, p) in enumerate(zip(held, self._pages)) if h > len(p) * self.page_size]
+        if over:
+            raise RuntimeError(f"sequences {over} have more tokens than their pages hold: replays went on behind what was "
+                               "reserved, and those tokens are lost; set `lengths` back, or release the sequences")
+        self._held = held
         self._tokens = [max(t, h) for t, h in zip(self._tokens, self._held)]
 
-    def release(self, sequence: int) -> None:
-        """Forget a sequence: its pages are free, its place in the batch is empty."""
+    def release(self, sequence: int, *, idle: bool = False) -> None:
+        """Forget a sequence: its pages are free, and its place in the batch is empty. The next `append` (or `reserve`)
+        begins another sequence there; with `idle`, `append` passes the place over until `reserve` is given a number
+        of its own for it. Replays of captured steps pass over every place that has no pages."""
         self._free.extend(reversed(self._pages[sequence]))
         self._pages[sequence] = []
         self._tokens[sequence] = self._held[sequence] = 0
+        self._idle[sequence] = idle
         self.lengths[sequence] = 0
         self._write_table()
 
     def _write_table(self) -> None:
-        rows = [p + [-1] * (self.max_pages - len(p)) for p in self._pages]
-        self.block_table.copy_(torch.tensor(rows, dtype=torch.int32))
+        rows = [[int(bool(p)), *p] + [-1] * (self.max_pages - len(p)) for p in self._pages]
+        self._table.copy_(torch.tensor(rows, dtype=torch.int32))
 
     # -- kernels ----------------------------------------------------------------------------------
     def _scales(self) -> dict:
@@ -109,7 +124,8 @@ class PagedKVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor] = None,
                sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """`ops.append_paged` of k / v (batch, S, heads, head_dim) behind what the sequences hold; pages are
-        reserved for them if they have not been (not while a graph is captured). Returns the rotated queries."""
+        reserved for them if they have not been (not while a graph is captured). Rows of idle places are passed over.
+        Returns the rotated queries."""
         if k.dim() != 4 or k.shape[0] != self.batch_size:
             raise ValueError(f"expected k ({self.batch_size}, tokens, heads, head_dim), got {tuple(k.shape)}")
         if k.dtype != self.dtype:
@@ -117,17 +133,17 @@ class PagedKVCache:
         new, capturing = k.shape[1], k.is_cuda and torch.cuda.is_current_stream_capturing()
         if self._captured and not capturing:
             self.sync()
-        held = [h + new for h in self._held]
+        held = [h if i else h + new for h, i in zip(self._held, self._idle)]
         if any(h > t for h, t in zip(held, self._tokens)):
             if capturing:
                 raise RuntimeError("a captured step finds no room: reserve its replays' tokens before the capture")
             self.reserve(new)
-        self.lengths.add_(new)
+        self.lengths.add_(self._in_use, alpha=new)
         try:
             out = ops.append_paged(k, v, self.k_pages, self.v_pages, self.block_table, self.lengths, cos=cos,
                                    sin=sin, q=q, **self._scales())
         except Exception:
-            self.lengths.sub_(new)
+            self.lengths.sub_(self._in_use, alpha=new)
             raise
         if capturing:
             self._captured = True  # nothing has run
