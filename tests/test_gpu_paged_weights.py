@@ -123,3 +123,13 @@ def test_infinite_values_stay_infinite(cuda, heads, n, dtype):
         assert (got[..., 7] == bad).all()
         got[..., 7] = want[..., 7]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_window_beyond_all_keys(cuda, bits):
+    lengths = [9000, 3, 700]
+    c = make_cache(lengths, 2, 64, 64, bits, torch.float16, cuda)
+    q = torch.randn(3, 2, 4, 64, device=cuda).half()
+    want = T.attention_paged(q, **c, lengths=i32(lengths, cuda))
+    for left in (1 << 20, 1 << 40, 2 ** 63 - 1):
+        assert torch.equal(T.attention_paged(q, **c, lengths=i32(lengths, cuda), window=(left, 0)), want)

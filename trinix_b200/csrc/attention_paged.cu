@@ -19,7 +19,7 @@ static auto paged_shape(int64_t D, bool four, int64_t rows, F&& f) {
 static PagedPlan plan_of(int64_t B, int64_t Sq, int64_t Hq, int64_t Hk, int64_t D, int64_t keys, int64_t window_left,
                          bool four) {
   const int64_t rows = Sq * (Hq / Hk), tile = rows > 8 ? 16 : 8;
-  if (window_left >= 0 && Sq + window_left < keys) keys = Sq + window_left;
+  if (window_left >= 0 && window_left < keys - Sq) keys = Sq + window_left;
   return paged_shape(D, four, rows, [&](auto d, auto bits, auto nt) {
     return paged_plan<decltype(d)::value, decltype(bits)::value, decltype(nt)::value>(
         B * Hk * ((rows + tile - 1) / tile), keys);
