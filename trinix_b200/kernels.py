@@ -199,8 +199,7 @@ class _QKNormRoPEFn(torch.autograd.Function):
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, q_bias, k_bias, eps, norm, norm_first, positions):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.how = (eps, norm, norm_first)
-        ctx.dtypes = (k_weight.dtype, None if q_bias is None else q_bias.dtype,
-                      None if k_bias is None else k_bias.dtype)
+        ctx.like = tuple(None if t is None else (t.dtype, t.shape) for t in (q_weight, k_weight, q_bias, k_bias))
         return ops.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, q_bias=q_bias, k_bias=k_bias, eps=eps,
                                 norm=norm, norm_first=norm_first, positions=positions)
 
@@ -212,13 +211,16 @@ class _QKNormRoPEFn(torch.autograd.Function):
         grads = list(ops.qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, eps=eps,
                                                norm=norm, norm_first=norm_first, positions=positions,
                                                need_dw=need[2] or need[3], need_db=need[6] or need[7]))
-        # those of another dtype than q's weight were summed in its dtype
-        for i, dtype in zip((3, 4, 5), ctx.dtypes):
-            if grads[i] is not None and grads[i].dtype != dtype:
-                grads[i] = None if dtype is None else grads[i].to(dtype)
-        for i, w in ((2, q_weight), (3, k_weight)):
-            if grads[i] is not None and w.dim() != 1:
-                grads[i] = grads[i].view(w.shape)
+        # those of another dtype than q's weight were summed in its dtype; all as rows of head_dim
+        for i, like in enumerate(ctx.like, 2):
+            if grads[i] is None or like is None:
+                grads[i] = None
+                continue
+            dtype, shape = like
+            if grads[i].dtype != dtype:
+                grads[i] = grads[i].to(dtype)
+            if len(shape) != 1:
+                grads[i] = grads[i].view(shape)
         dq, dk, dqw, dkw, dqb, dkb = grads
         return dq, dk, dqw, dkw, None, None, dqb, dkb, None, None, None, None
 
