@@ -208,10 +208,12 @@ class _QKNormRoPEFn(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         need, (eps, norm, norm_first) = ctx.needs_input_grad, ctx.how
-        grads = list(ops.qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, eps=eps,
+        dtypes = {like[0] for like in ctx.like if like is not None}
+        qw = q_weight if len(dtypes) == 1 else q_weight.float()  # sums in fp32, for parameters of several types
+        grads = list(ops.qk_norm_rope_backward(dq_out, dk_out, q, k, qw, k_weight, cos, sin, eps=eps,
                                                norm=norm, norm_first=norm_first, positions=positions,
                                                need_dw=need[2] or need[3], need_db=need[6] or need[7]))
-        # those of another dtype than q's weight were summed in its dtype; all as rows of head_dim
+        # as rows of head_dim, of one type
         for i, like in enumerate(ctx.like, 2):
             if grads[i] is None or like is None:
                 grads[i] = None

@@ -395,6 +395,15 @@ def _head_param(t: torch.Tensor, D: int, dtype: torch.dtype) -> torch.Tensor:
     return t if t.is_contiguous() else t.detach().contiguous()
 
 
+def _param_dtype(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.dtype:
+    """The type that weights and biases are read in: their own, or float32 where they differ."""
+    dtype = first.dtype
+    for t in others:
+        if t is not None and t.dtype != dtype:
+            return torch.float32
+    return dtype
+
+
 def _qk_inputs(dev, q, k, cos, sin, norm: str, positions):
     """What the forward and the backward pass of qk_norm_rope check and take: q, k, the tables, the sizes, the
     positions' address, strides and type, the norm's number, the types' of the tables and of q."""
@@ -438,7 +447,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     dev = _same_device(q, k, q_weight, k_weight, cos, sin, positions, q_bias, k_bias)
     q, k, cos, sin, sizes, (pos, pb, ps, wide), how, table_code, code = _qk_inputs(dev, q, k, cos, sin, norm,
                                                                                    positions)
-    D, kind = sizes[4], q_weight.dtype
+    D, kind = sizes[4], _param_dtype(q_weight, k_weight, q_bias, k_bias)
     qw, kw = _head_param(q_weight, D, kind), _head_param(k_weight, D, kind)
     qb = kb = None
     if q_bias is not None or k_bias is not None:
@@ -462,7 +471,8 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
                           need_dw: bool = True, need_db: bool = False):
     """(dq, dk, dq_weight, dk_weight, dq_bias, dk_bias) of qk_norm_rope given the gradients of its two
     outputs; those of the weights are None unless need_dw, those of the biases unless need_db ("layernorm"
-    only). They have the dtype of q_weight and are summed in fp32 in a fixed order."""
+    only). They have the dtype of the weights (float32 where the two differ) and are summed in fp32 in a fixed
+    order."""
     if need_db and norm != "layernorm":
         raise ValueError("only layernorm has biases")
     dev = _same_device(q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out)
@@ -470,7 +480,7 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
                                                                                    positions)
     if dq_out.shape != q.shape or dk_out.shape != k.shape or dq_out.dtype != q.dtype or dk_out.dtype != q.dtype:
         raise ValueError("gradients must have the shape and dtype of the outputs")
-    D, kind = sizes[4], q_weight.dtype
+    D, kind = sizes[4], _param_dtype(q_weight, k_weight)
     dq_out, dk_out = _bshd(dq_out), _bshd(dk_out)
     qw, kw = _head_param(q_weight, D, kind), _head_param(k_weight, D, kind)
     dq, dk = _new(q), _new(k)
