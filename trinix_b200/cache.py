@@ -16,7 +16,8 @@ from . import ops
 
 class PagedKVCache:
     """`num_pages` pages of `page_size` tokens for `num_kv_heads` heads of `head_dim`, shared by `batch_size`
-    sequences of up to `max_pages` pages each (default: all of them).
+    sequences of up to `max_pages` pages each (default: all of them; attention modules with rotation keep tables of so
+    many positions).
 
     Which page is whose is kept on the host, with the lengths that the host has reserved room for; the block table
     and the lengths that the kernels read are on the device, so that a step (`reserve` aside) may be captured in a

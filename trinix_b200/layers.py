@@ -14,6 +14,7 @@ package's kernels the names "triton" and "flash" both mean the sm_100a backend.
 from __future__ import annotations
 
 import math
+import weakref
 from typing import Optional, Tuple, Union
 
 import torch
@@ -309,6 +310,16 @@ class FastReGLU(_FastGLU):
 
 
 # ----------------------------------------------------------------------------- position
+class _RotationTables:
+    """(cos, sin) that modules of one base and dim share, as long as one of them lives."""
+
+    def __init__(self, pair):
+        self.pair = pair
+
+
+_rotation_tables: "weakref.WeakValueDictionary" = weakref.WeakValueDictionary()
+
+
 class FastRoPEPositionEmbedding(nn.Module):
     """Mirror of trinix/layers/embeddings/rope.py:13-134.
 
@@ -341,32 +352,40 @@ class FastRoPEPositionEmbedding(nn.Module):
             self._table_key = key
         return self._tables
 
-    def _build(self, rows: int, device: torch.device, dtype: torch.dtype):
+    def _build(self, rows: int, device: torch.device, dtype: torch.dtype, half: bool = False):
         inv_freq = 1.0 / self.base ** (
             torch.arange(0, self.dim, 2, device=device, dtype=torch.float32) / self.dim)
         pos = torch.arange(rows, device=device, dtype=torch.float32)
         angles = torch.outer(pos, inv_freq)
-        table = torch.cat((angles, angles), dim=-1)
+        table = angles if half else torch.cat((angles, angles), dim=-1)
         return table.cos().to(dtype), table.sin().to(dtype)
 
-    def tables(self, seq_len: int, device: torch.device):
+    def tables(self, seq_len: int, device: torch.device, half: bool = False):
         """(cos, sin) of forward in fp32, of at least max_position_embeddings positions: what the kernels that
-        look a token's position up take. Kept as long as the module, since a captured graph may read them; longer
-        ones are of a power of two, so that they are few."""
+        look a token's position up take; half: the dim / 2 columns of them that these read. Kept as long as the module,
+        since a captured graph may read them, once for all modules of the same base and dim; longer ones are of a power
+        of two, so that they are few."""
         rows = max(seq_len, self.max_position_embeddings)
+        columns = self.dim // 2 if half else self.dim
         for kept in self._wide_tables:
-            if kept[0].device == device and kept[0].shape[0] >= rows:
-                return kept
-        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            return self._build(rows, device, torch.float32)  # the graph's own: there is nothing in them yet
+            cos = kept.pair[0]
+            if cos.device == device and cos.shape[0] >= rows and cos.shape[1] == columns:
+                return kept.pair
         if rows > self.max_position_embeddings:
             rows = 1 << (rows - 1).bit_length()
-        with torch.inference_mode(False), torch.no_grad():  # a training step may save them
-            made = self._build(rows, device, torch.float32)
-        if device.type == "cuda":
-            torch.cuda.current_stream(device).synchronize()  # the next call may be on another stream
+        key = (self.dim, float(self.base), rows, columns, device)
+        made = _rotation_tables.get(key)
+        if made is None:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                # the graph's own: there is nothing in them yet
+                return self._build(max(seq_len, self.max_position_embeddings), device, torch.float32, half)
+            with torch.inference_mode(False), torch.no_grad():  # a training step may save them
+                made = _RotationTables(self._build(rows, device, torch.float32, half))
+            if device.type == "cuda":
+                torch.cuda.current_stream(device).synchronize()  # the next call may be on another stream
+            _rotation_tables[key] = made
         self._wide_tables.append(made)
-        return made
+        return made.pair
 
     @staticmethod
     def _rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -493,7 +512,7 @@ class FastBaseAttention(nn.Module):
         """Rotation, then the q / k norms, as one kernel with fp32 in between (the modules round to the activation's
         type in between): with fused_qk, position_method="rope" and qk_norm, on the kernel path. positions are
         below max_seq_len, or `most`."""
-        cos, sin = self.position_embedding.tables(max(most, q.shape[1]), q.device)
+        cos, sin = self.position_embedding.tables(max(most, q.shape[1]), q.device, half=True)
         return QKNormRoPEKernel.apply(
             q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, getattr(self.q_norm, "bias", None),
             getattr(self.k_norm, "bias", None), self.q_norm.eps,
@@ -643,7 +662,7 @@ class FastGroupedQueryAttention(FastBaseAttention):
             cache.append(k, v)
         else:
             most = cache.max_pages * cache.page_size
-            q = cache.append(k, v, *self.position_embedding.tables(most, q.device), q=q)
+            q = cache.append(k, v, *self.position_embedding.tables(most, q.device, half=True), q=q)
         window = (self.sliding_window_size, 0) if self.use_sliding_window else None
         slopes = self.position_embedding.slopes if self.position_method == "alibi" else None
         return cache.attend(q, scale=self.scale, window=window, alibi_slopes=slopes)
