@@ -125,3 +125,18 @@ def test_replays_behind_what_was_reserved_are_told(cuda):
     step(c, t)
     assert c.lengths.tolist() == [17]
     assert T.attention_status(cuda) == 0
+
+
+def test_a_module_with_dropout(cuda):
+    """Refused while it trains, with the cache as it was; eval() does what a module without does."""
+    torch.manual_seed(0)
+    kw = dict(kernel_type="triton", causal=True, position_method="rope", head_dim=D)
+    a, b = (T.FastGroupedQueryAttention(512, HQ, HK, dropout=p, **kw).to(cuda).bfloat16() for p in (0.0, 0.25))
+    b.load_state_dict(a.state_dict())
+    x = torch.randn(1, 3, 512, device=cuda).bfloat16()
+    c, other = (T.PagedKVCache(2, 16, HK, D) for _ in range(2))
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="eval"):
+            b(x, past_key_value=c)
+        assert c.lengths.tolist() == [0] and not c.k_pages.any()
+        assert torch.equal(b.eval()(x, past_key_value=c)[0], a(x, past_key_value=other)[0])

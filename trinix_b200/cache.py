@@ -3,7 +3,7 @@
 The reference's attention modules keep past keys and values by concatenation
 (trinix/layers/attention/grouped_query_attention.py:178-184): every step copies the whole cache. Here it is a pool of
 pages of fixed size, in the activation's 16 bits or in 4 bits (`ops.append_paged`), of which each sequence of the
-batch owns some; the attention modules take one as `past_key_value`.
+batch owns some; FastGroupedQueryAttention and FastMultiQueryAttention take one as `past_key_value`.
 """
 from __future__ import annotations
 

@@ -647,6 +647,8 @@ class FastGroupedQueryAttention(FastBaseAttention):
         """Append to the cache, attend over it. A token's position is its place in its sequence."""
         if not (self.causal and self._uses_kernel(q)):
             raise ValueError("a paged cache needs causal=True and the kernel path")
+        if self.training and self.dropout > 0.0:
+            raise ValueError("attention over a paged cache drops nothing: call eval() on a module with dropout")
         if position_ids is not None:
             raise ValueError("behind a paged cache a token's position is its place in its sequence")
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
