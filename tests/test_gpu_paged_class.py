@@ -140,3 +140,32 @@ def test_a_module_with_dropout(cuda):
             b(x, past_key_value=c)
         assert c.lengths.tolist() == [0] and not c.k_pages.any()
         assert torch.equal(b.eval()(x, past_key_value=c)[0], a(x, past_key_value=other)[0])
+
+
+def test_pages_do_not_change_hands_in_a_capture(cuda):
+    """Refused, with the host's lists as they were: it would hold pages for given that the table never names."""
+    c = T.PagedKVCache(4, 16, HK, D, 1)
+    t = tokens(cuda, 1, 1)
+    step(c, t)
+
+    def try_all():
+        for call in (lambda: c.reserve(30), lambda: c.release(0), c.sync):
+            with pytest.raises(RuntimeError, match="capture"):
+                call()
+        return t[0] + 1
+
+    graph, out = captured(try_all)
+    graph.replay()
+    assert torch.equal(out, t[0] + 1)
+    assert "free=3" in repr(c) and c._tokens == [1] and c.lengths.tolist() == [1]
+    c.reserve(30)
+    assert (c.block_table >= 0).sum() == 2
+
+
+def test_long_steps_of_idle_places_alone(cuda):
+    c = T.PagedKVCache(4, 16, HK, D, 2)
+    for b in range(2):
+        c.release(b, idle=True)
+    for S in (1, 40):
+        assert not step(c, tokens(cuda, 2, S), S).any()
+    assert c.lengths.tolist() == [0, 0] and "free=4" in repr(c)

@@ -73,6 +73,7 @@ class PagedKVCache:
         """Make sure that every sequence (or each by its own number) has pages for so many tokens more than it
         holds. Raises, with nothing changed, if the pool or the table's rows have too few. One number for all leaves
         idle places out; one of its own, above 0, ends a place's being idle."""
+        self._refuse_capture("reserve")
         if self._captured:
             self.sync()
         more = [0 if i else tokens for i in self._idle] if isinstance(tokens, int) else list(tokens)
@@ -95,6 +96,7 @@ class PagedKVCache:
     def sync(self) -> None:
         """Read from the device how many tokens the sequences hold (after replays of captured steps, or a change of
         `lengths` from outside). Raises for one that is longer than its pages: tokens of it have been lost."""
+        self._refuse_capture("sync")
         held = self.lengths.tolist()
         over = [b for b, (h, p) in enumerate(zip(held, self._pages)) if h > len(p) * self.page_size]
         if over:
@@ -107,6 +109,7 @@ class PagedKVCache:
         """Forget a sequence: its pages are free, and its place in the batch is empty. The next `append` (or `reserve`)
         begins another sequence there; with `idle`, `append` passes the place over until `reserve` is given a number
         of its own for it. Replays of captured steps pass over every place that has no pages."""
+        self._refuse_capture("release")
         self._free.extend(reversed(self._pages[sequence]))
         self._pages[sequence] = []
         self._tokens[sequence] = self._held[sequence] = 0
@@ -117,6 +120,14 @@ class PagedKVCache:
     def _write_table(self) -> None:
         rows = [[int(bool(p)), *p] + [-1] * (self.max_pages - len(p)) for p in self._pages]
         self._table.copy_(torch.tensor(rows, dtype=torch.int32))
+
+    def _capturing(self) -> bool:
+        return self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()
+
+    def _refuse_capture(self, what: str) -> None:
+        """Before anything has changed: what the host does of it would be done, what the device does would not."""
+        if self._capturing():
+            raise RuntimeError(f"PagedKVCache.{what}() is not for a graph's capture: call it before")
 
     # -- kernels ----------------------------------------------------------------------------------
     def _scales(self) -> dict:
@@ -131,7 +142,7 @@ class PagedKVCache:
             raise ValueError(f"expected k ({self.batch_size}, tokens, heads, head_dim), got {tuple(k.shape)}")
         if k.dtype != self.dtype:
             raise TypeError(f"the cache is for {self.dtype}, got {k.dtype}")
-        new, capturing = k.shape[1], k.is_cuda and torch.cuda.is_current_stream_capturing()
+        new, capturing = k.shape[1], self._capturing()
         if self._captured and not capturing:
             self.sync()
         held = [h if i else h + new for h, i in zip(self._held, self._idle)]
@@ -164,7 +175,7 @@ class PagedKVCache:
         starts = self._starts()
         # room for all that the sequences' pages hold, whatever the host has seen of the lengths
         pages = sum(len(p) for p in self._pages)
-        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             pages = min(self.k_pages.shape[0], self.batch_size * self.max_pages)
         k, v = self._gather(starts, pages * self.page_size)
         rows = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=q.device)
