@@ -183,7 +183,12 @@ class PagedKVCache:
                                    window=None if window is None else (window[0], 0), alibi_slopes=alibi_slopes)
         return out.view(B, S, Hq, D)
 
-    # Tokens to a sequence from which on the cache is read back for the kernel of packed sequences.
+    # Tokens to a sequence from which on the cache is read back for the kernel of packed sequences. attention_paged reads
+    # the keys once for every 16 rows, tokens x query heads to a kv head; reading back costs the pages of all sequences,
+    # in a captured step those of the pool. attention_paged / read back, us, 8 kv heads x 128 in 16 bits, 8 sequences of
+    # 16000 keys: 1 query head to each, 16 tokens 97 / 361, 32 179 / 363, 64 339 / 366, 128 631 / 369; 4 heads, 8 tokens
+    # 179 / 362, 16 338 / 369, 32 632 / 374; 64 sequences of 1000, 4 heads, 8 tokens 104 / 159, 16 184 / 161, 32 339 / 177;
+    # one of 2000, 4 heads, 32 tokens 18 / 40, 64 32 / 43, 128 51 / 43.
     LONG = 32
 
     def gather(self) -> Tuple[torch.Tensor, torch.Tensor]:

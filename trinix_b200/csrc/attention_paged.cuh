@@ -38,11 +38,11 @@
 //     are.
 // Scores, sums and O are fp32.
 //
-// Measured (32 / 8 heads x 128, one token to a sequence): 48 sequences of 128 to 8192 keys, 16 bits, 385 MB: 70.5 us,
-// 5.5 TB/s; 64 of 4 bits, 143 MB: 44.3 us; 2 x 131072 and fewer keys of 4 bits, 155 MB: 43.9 us, 3.5 TB/s. What bounds
+// Measured (32 / 8 heads x 128, one token to a sequence): 48 sequences of 128 to 8192 keys, 16 bits, 385 MB: 72 us,
+// 5.3 TB/s; 64 of 4 bits, 143 MB: 44.7 us; 2 x 131072 and fewer keys of 4 bits, 155 MB: 44.2 us, 3.5 TB/s. What bounds
 // it: 16 bits, the memory (without the arithmetic 67.7 us). 4 bits, both: loads alone would take 36 us, arithmetic
 // alone 37 (500 instructions to 32 keys of a warp, 176 of them the shifts, ANDs and permutes that make operands of
-// codes; three CTAs of 166 registers issue 45 % of the time), 8 of either the call's start, the cuts and the parts.
+// codes; three CTAs of 168 registers issue 46 % of the time), 8 of either the call's start, the cuts and the parts.
 // Tried: 16 keys at a time as in attention_decode.cuh and clusters of fixed splits, 4 bits 100 and 109 us; tiles of
 // 32 keys 48 and 47 us; four CTAs to an SM 64 to 67 (registers); two sums for a run's products, or two steps of 32
 // keys unrolled: nothing.
@@ -123,9 +123,13 @@ struct PgShape {
   static constexpr int ALIGN = FOUR ? 128 : 1024;
   static constexpr int DYN_BYTES = TOTAL + ALIGN;
   static constexpr int PART_FLOATS = ROWS * (D + 2);  // of one part in memory
-  // What a unit costs beside its tiles, in tiles, and what a piece of the line has at least. Of tiles of 32 keys of 4
-  // bits 2, 4, 8, 12, 16 for a unit made 64 sequences of 128 to 8192 keys take 71, 61, 49, 48, 50 us (tiles are now 64);
-  // of 16 bits, 48 sequences 86, 83, 73, 71, 72 us.
+  // What a unit costs beside its tiles, in tiles. 4 bits 2, 3, 4, 6, 8, 12: 64 sequences of 128 to 8192 keys 54.0, 49.5,
+  // 47.4, 44.5, 45.8, 47.6 us, 256 of up to 600 46.7, 43.2, 43.5, 39.9, 39.7, 41.4; 16 bits 4, 6, 8, 12, 16, 24: 48
+  // sequences 80.9, 73.6, 71.6, 71.8, 71.3, 72.9, 256 of up to 600 60.2, 53.4, 50.5, 45.1, 45.1, 48.4.
+  // What a piece of the line has at least, so that a CTA that has one works longer than it takes to start and to hand
+  // its part over. It matters to lines of few tiles alone: 4 bits, 2 to 8 alike, 16: 24 x 5 rows of up to 3001 keys 29.3
+  // instead of 26.0 us, 16 sequences of up to 8000 23.1 instead of 21.9, one of 32768 21.2 instead of 23.3; 16 bits, 4 to
+  // 32 alike.
   static constexpr int UNIT_COST = FOUR ? 6 : 12;
   static constexpr int LEAST_PIECE = FOUR ? 8 : 16;
   static_assert(RING_BYTES >= PG_THREADS * 8, "the sums of the lengths");
@@ -1097,9 +1101,15 @@ static PagedPlan paged_plan(int64_t units, int64_t keys) {
   int n = 1;
   while (n < PG_MOST_SPLITS && units * 2 * n <= slots && tiles >= 2 * n * PG_WARPS * (FOUR ? 1 : 2)) n *= 2;
   const int64_t chain = (tiles + n * PG_WARPS - 1) / (n * PG_WARPS);
-  // More than a few tiles to a warp, or units that do not all run at once: the line. Line / clusters, 16 bits and 4:
-  // 4 sequences of up to 1000 keys, 16 / 2 heads 13.7 / 9.6 us, 14.4 / 10.3; 4 of up to 8000, 32 / 8 heads 23.4 / 20.4,
-  // 18.3 / 15.1; 64 of up to 500 17.3 / 19.8 and, 4 bits, 20.5 / 14.9.
+  // More than a few tiles to a warp, or units that do not all run at once: the line. Line / clusters, us, 16 bits and 4,
+  // 32 / 8 heads x 128, sequences of up to so many keys; first units that run at once (so many tiles to a warp):
+  //   16 bits: 1 of 600 (3) 11.7 / 8.9, 16 of 500 (4) 12.6 / 9.6, 1 of 4096 (8) 12.3 / 13.0, 16 of 2000 (16) 15.2 / 19.9, 1
+  //   of 32768 (64) 32.1 / 55.3. 4 bits: 1 of 600 (2) 13.0 / 10.4, 16 of 500 (1) 15.1 / 9.7, 16 of 2000 (4) 16.4 / 15.3,
+  //   16 of 8000 (16) 21.9 / 38.8.
+  // and the others: 16 bits: 64 of 100 (2) 14.4 / 11.2, 64 of 500 (8) 17.8 / 15.8, 256 of 250 (4) 36.0 / 40.5, 64 of 1000
+  //   (16) 22.5 / 23.2. 4 bits: 64 of 250 (1) 16.6 / 13.5, 64 of 500 (2) 17.6 / 15.1, 64 of 1000 (4) 19.7 / 18.1, 256 of
+  //   600 (3) 40.3 / 39.8, 64 of 2048 (8) 25.3 / 27.1.
+  // `keys` is what the block table has room for: the lengths are the device's.
   const bool line = chain > (units * n <= slots ? (FOUR ? 5 : 16) : (FOUR ? 2 : 3));
   plan.splits = line ? 0 : n;
   plan.ctas = !line ? units * n : slots < PG_MOST_CTAS ? slots : PG_MOST_CTAS;

@@ -9,11 +9,14 @@
 //             dw = sum g n,  db = sum g,  d = g w,  dz = rstd (d - n mean(d n) [- mean d])
 //             dx = dz or R^T dz
 // All in fp32, one rounding at the end; row statistics are recomputed in the backward pass, where the row is in
-// registers anyway. Memory bounds both: a row is read once and stays with its few lanes (head_rows.cuh), no barrier
-// in the loop, arithmetic in packed pairs (a half as many instructions as without: 119 us instead of 92 at a training
-// step of 8192 tokens, 32 / 8 heads x 128 bf16, which now is 79.6). There: forward 168 MB in 31.5 us, 5.3 TB/s;
-// backward, with the sums of the weight gradients, 252 MB in 48, 5.2 TB/s: three CTAs to an SM, as the sums of a
-// thread's columns leave registers for, issue 38 % of what they could and wait for rows the rest.
+// registers anyway. A row is read once and stays with its few lanes (head_rows.cuh), no barrier in the loop,
+// arithmetic in packed pairs (a half as many instructions as without: 119 us instead of 92 at a training step of 8192
+// tokens, 32 / 8 heads x 128 bf16, which now is 79.6). There: forward 168 MB in 31.5 us, 5.3 TB/s; backward, with the sums
+// of the weight gradients, 252 MB in 48, 5.2 TB/s. Neither the memory (47 and 60 % of its peak with cold caches) nor the
+// issue slots (44 and 49 %) are full: at four and three CTAs to an SM, as registers leave room for, rows are waited for.
+// Other shapes, 4096 tokens, forward, and forward and backward (floors at 6.55 TB/s): fp32 32 / 8 x 128 28.8 us (25.8),
+// 74.5 (51.4); bf16 16 / 4 x 256 16.0 (13.1), 49.6 (25.9); 8 / 2 x 512 18.5 (13.5), 56.2 (26.3); rows that cannot be read
+// in 16-byte vectors: 32 / 8 x 126 26.7 (12.8), 163 (25.4), 16 / 4 x 258 41.3 (13.2), 148 (26.1).
 #include "head_rows.cuh"
 
 namespace trx {
