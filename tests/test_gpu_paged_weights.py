@@ -5,6 +5,7 @@ import torch
 
 import trinix_b200 as T
 from tests.paged_ref import make_cache
+from tests.test_gpu_paged import check_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +134,23 @@ def test_a_window_beyond_all_keys(cuda, bits):
     want = T.attention_paged(q, **c, lengths=i32(lengths, cuda))
     for left in (1 << 20, 1 << 40, 2 ** 63 - 1):
         assert torch.equal(T.attention_paged(q, **c, lengths=i32(lengths, cuda), window=(left, 0)), want)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("Sq,heads,dtype", [(1, 8, torch.bfloat16), (3, 12, torch.float16)], ids=str)
+@pytest.mark.parametrize("B,width", [(3, 30), (3, 700), (3, 1 << 16), (16, 40), (16, 200), (16, 1000), (64, 60), (64, 512)])
+def test_tables_wider_than_the_sequences(cuda, B, width, Sq, heads, dtype, bits):
+    """How a call is cut goes by what the table has room for: short sequences in tables of all widths."""
+    g = torch.Generator().manual_seed(B + width)
+    lengths = torch.randint(0, 400, (B,), generator=g).tolist()
+    lengths[1], lengths[2] = 0, 470
+    c = make_cache(lengths, 2, 16, 64, bits, dtype, cuda)
+    narrow = c["block_table"]
+    c["block_table"] = torch.full((B, width), -1, dtype=torch.int32, device=cuda)
+    c["block_table"][:, : narrow.shape[1]] = narrow
+    q = torch.randn(B, Sq, heads, 64, generator=torch.Generator(device=cuda).manual_seed(2), device=cuda).to(dtype)
+    out, lse = T.attention_paged(q, **c, lengths=i32(lengths, cuda), return_lse=True)
+    some = [0, 1, 2, B - 1]
+    few = {**c, "block_table": narrow[some]}
+    check_attention(out[some], lse[some], q[some], few, [lengths[b] for b in some], bits)
+    assert T.attention_status(cuda) == 0
