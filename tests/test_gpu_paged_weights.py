@@ -132,7 +132,7 @@ def test_a_window_beyond_all_keys(cuda, bits):
     c = make_cache(lengths, 2, 64, 64, bits, torch.float16, cuda)
     q = torch.randn(3, 2, 4, 64, device=cuda).half()
     want = T.attention_paged(q, **c, lengths=i32(lengths, cuda))
-    for left in (1 << 20, 1 << 40, 2 ** 63 - 1):
+    for left in (1 << 20, 1 << 40, 2 ** 63 - 1, 2 ** 64, 2 ** 64 + 1):
         assert torch.equal(T.attention_paged(q, **c, lengths=i32(lengths, cuda), window=(left, 0)), want)
 
 

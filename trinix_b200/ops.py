@@ -1212,7 +1212,8 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     q (B, Sq, Hq, D): the last Sq tokens of each sequence, whose keys are among its lengths[b] (int32 on the
     device) in the cache; Hq % Hk == 0. Query i stands at position lengths[b] - Sq + i and sees the keys up to
     there, with window = (left, right) no more than left of them before its own; alibi_slopes (Hq,) add -slope *
-    distance. A query without a key (a padded sequence of length 0) is 0. Pages as in append_paged, of 16 bits
+    distance. A query without a key (a padded sequence of length 0) is 0; keys that a query does not see do not reach
+    it, finite or not. Pages as in append_paged, of 16 bits
     or, with scales, of 4; a page number outside the cache reads as zeros (pages that the window has left behind
     may be given away). With return_lse also the fp32 (B, Hq, Sq) log-sum-exp.
 
@@ -1235,7 +1236,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"lengths must be an int32 tensor of {B} entries")
     left = -1
     if window is not None:
-        left = int(window[0])
+        left = min(int(window[0]), (1 << 63) - 1)
         if left < 0 or int(window[1]) < 0:
             raise ValueError("window sizes must be >= 0")
     slopes = _slopes(alibi_slopes, Hq)
